@@ -422,6 +422,80 @@ TraceaStatus tracea_conv_params_pack(int32_t n, int32_t h, int32_t w, int32_t c,
 TraceaStatus tracea_conv_coords_device(const TraceaConvParamsBlock *p, int32_t *rows,
                                        int64_t *base_off, int32_t *cols, void *stream);
 
+/* ======================================================================== */
+/* Training a block of attention.  None of these has a counterpart in the   */
+/* reference, whose attention is forward only.                              */
+/* ======================================================================== */
+
+/* Attention whose forward pass keeps each row's log-sum-exp, and its backward pass, which recomputes the probabilities.
+ *   q, o, d_o, dq [B,Hq,Sq,D]   k, v, dk, dv [B,Hk,Sk,D]   Hq a multiple of Hk: query head h reads key/value head
+ *   h / (Hq / Hk), and dk, dv are sums over the query heads that read them   lse [B,Hq,Sq] f32
+ *   q_lengths, k_lengths: optional [B] i32, contiguous, on the device: batch entry b has the first q_lengths[b] queries
+ *   and k_lengths[b] keys (clamped to 0..Sq, 0..Sk); absent: all.  What lies behind them is never used, whatever it holds.
+ * Query i of b sees keys j < k_lengths[b]; with params.causal, of those j <= i + k_lengths[b] - q_lengths[b] (the
+ * last query sees every key).  lse = log of the sum of exp(scale q.k) over them; a query that sees none, or lies
+ * behind its sequence's length, has o = 0, lse = -inf and gradient 0, keys behind the length have gradient 0.
+ * All tensors but lse share one type, f16 or bf16, D from 1 to 128; sums, statistics and probabilities are fp32,
+ * probabilities and their gradients are rounded once to the operand type for the matrix products.  scale 0 selects
+ * 1/sqrt(D); softmax_mode is ignored.  The same call on the same inputs gives the same bits.
+ * Read and written in place: D a multiple of 8 and contiguous, other strides multiples of 8 elements (rows and heads not
+ * descending), bases on 16 bytes, no result over an operand.  Anything else runs from copies in the padded road's
+ * per-(device, stream) buffer (at most 1 GiB, not grown under capture).  Both calls take a workspace per (device,
+ * stream), grown on demand, never under capture and never freed: 8 bytes per row for the backward pass; for a forward
+ * pass of few rows over many keys, which is split along the keys, the partial results. */
+TraceaStatus tracea_attention_forward(TraceaTensorView q, TraceaTensorView k, TraceaTensorView v,
+                                      const TraceaTensorView *q_lengths, const TraceaTensorView *k_lengths,
+                                      TraceaTensorView *o, TraceaTensorView *lse, TraceaAttentionParams params);
+TraceaStatus tracea_attention_backward(TraceaTensorView q, TraceaTensorView k, TraceaTensorView v, TraceaTensorView o,
+                                       TraceaTensorView lse, TraceaTensorView d_o, const TraceaTensorView *q_lengths,
+                                       const TraceaTensorView *k_lengths, TraceaTensorView *dq, TraceaTensorView *dk,
+                                       TraceaTensorView *dv, TraceaAttentionParams params);
+
+/* Rotary positions on 1 to TRACEA_MAX_ROTARY_AXES axes (text: one; images: row, column; video: frame, row, column).
+ *   q [B,Hq,S,D], k [B,Hk,S,D] (optional) and their results, f32, f16 or bf16, D contiguous, any other strides
+ *   positions [B,S,A] or [1,S,A] (one for the whole batch), i32, A contiguous   inv_freq [P] f32, contiguous, P <= D/2
+ * Pair p belongs to the axis whose section it lies in (sections[0] pairs of axis 0, then sections[1] of axis 1, ...;
+ * their sum is P) and is turned by positions[..., axis] * inv_freq[p], worked out exactly before it is reduced, so that long
+ * positions lose nothing.  Pair p is columns p and p + P, or 2p and 2p + 1 with `adjacent`; columns from 2P on are
+ * copied.  `inverse` turns back: the gradient of the rotation.  A result may be its own operand (the same view), and
+ * may not otherwise overlap one. */
+#define TRACEA_MAX_ROTARY_AXES 4
+typedef struct {
+  uint32_t axes;
+  uint32_t sections[TRACEA_MAX_ROTARY_AXES];
+  uint8_t adjacent;
+  uint8_t inverse;
+  void *stream;
+} TraceaRotaryParams;
+TraceaStatus tracea_rotary(TraceaTensorView q, const TraceaTensorView *k, TraceaTensorView positions, TraceaTensorView inv_freq,
+                           TraceaTensorView *q_out, TraceaTensorView *k_out, TraceaRotaryParams params);
+
+/* What stands between two blocks of a network with a norm behind each block and one in front of it:
+ *   n = h * rsqrt(mean(h^2) + eps) * w_post      x_out = residual_scale * x + gate * n
+ *   y = x_out * rsqrt(mean(x_out^2) + eps) * w_pre                       (means over the channels)
+ *   x, h, x_out, y [B,T,C], C contiguous, up to 8192, one type of f32, f16, bf16
+ *   w_post, w_pre [C], gate [G,C] with G = 1 or B (absent: 1), contiguous, f32
+ * h, w_post, gate and x_out go together: without h (first norm of a network) x_out is x itself, passed as NULL, and
+ * residual_scale is not used.  Without y and w_pre (behind the last block) there is no second norm.  x_out may be x or h, y may be
+ * h, as the same view; otherwise results overlap no operand and not each other.
+ * The backward pass reads x_out (x where there is no h) and h as the forward pass left them and works out both norms
+ * again: dx_out (optional: absent is 0) and dy are the gradients of x_out and y; dx, dh have the type of h, dw_post, dgate
+ * [G,C], dw_pre are f32 and are summed in an order that does not change.  Gradients that are not wanted are NULL (dx is
+ * required).  It takes a workspace per (device, stream) of at most 16 MiB + 8 bytes per channel and batch entry, grown on demand, never under capture. */
+typedef struct {
+  float eps;
+  float residual_scale;
+  void *stream;
+} TraceaNormParams;
+TraceaStatus tracea_norm_gate_residual(TraceaTensorView x, const TraceaTensorView *h, const TraceaTensorView *w_post,
+                                       const TraceaTensorView *gate, const TraceaTensorView *w_pre, TraceaTensorView *x_out,
+                                       TraceaTensorView *y, TraceaNormParams params);
+TraceaStatus tracea_norm_gate_residual_backward(const TraceaTensorView *dx_out, const TraceaTensorView *dy, TraceaTensorView x_out,
+                                                const TraceaTensorView *h, const TraceaTensorView *w_post,
+                                                const TraceaTensorView *gate, const TraceaTensorView *w_pre, TraceaTensorView *dx,
+                                                TraceaTensorView *dh, TraceaTensorView *dw_post, TraceaTensorView *dgate,
+                                                TraceaTensorView *dw_pre, TraceaNormParams params);
+
 #ifdef __cplusplus
 }
 #endif

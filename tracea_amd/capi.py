@@ -61,6 +61,18 @@ class EpilogueOp(C.Structure):
                 ("p2", C.c_void_p), ("p3", C.c_void_p), ("epsilon", C.c_float), ("ld", C.c_int64)]
 
 
+MAX_ROTARY_AXES = 4
+
+
+class RotaryParams(C.Structure):
+    _fields_ = [("axes", C.c_uint32), ("sections", C.c_uint32 * MAX_ROTARY_AXES), ("adjacent", C.c_uint8),
+                ("inverse", C.c_uint8), ("stream", C.c_void_p)]
+
+
+class NormParams(C.Structure):
+    _fields_ = [("eps", C.c_float), ("residual_scale", C.c_float), ("stream", C.c_void_p)]
+
+
 class ConvParamsBlock(C.Structure):
     _fields_ = [(n, C.c_int32) for n in
                 ("batch", "h_in", "w_in", "c_in", "k_out", "h_out", "w_out", "r_sz", "s_sz",
@@ -138,6 +150,15 @@ SIGNATURES = {
                                   C.POINTER(TensorView), GemmParams, C.c_void_p]),
     "tracea_gemm_ttg_ex": (C.c_int, [TensorView, TensorView, C.POINTER(TensorView), GemmParams,
                                      C.POINTER(EpilogueOp), C.c_uint32, C.c_void_p]),
+    "tracea_attention_forward": (C.c_int, [TensorView, TensorView, TensorView, C.POINTER(TensorView),
+                                           C.POINTER(TensorView), C.POINTER(TensorView), C.POINTER(TensorView),
+                                           AttentionParams]),
+    "tracea_attention_backward": (C.c_int, [TensorView] * 6 + [C.POINTER(TensorView)] * 5 + [AttentionParams]),
+    "tracea_rotary": (C.c_int, [TensorView, C.POINTER(TensorView), TensorView, TensorView, C.POINTER(TensorView),
+                                C.POINTER(TensorView), RotaryParams]),
+    "tracea_norm_gate_residual": (C.c_int, [TensorView] + [C.POINTER(TensorView)] * 6 + [NormParams]),
+    "tracea_norm_gate_residual_backward": (C.c_int, [C.POINTER(TensorView)] * 2 + [TensorView] +
+                                           [C.POINTER(TensorView)] * 9 + [NormParams]),
     "tracea_set_split_k": (None, [C.c_int32]),
     "tracea_set_split_k_one_launch": (None, [C.c_int32]),
     "tracea_last_split_k_launches": (C.c_int32, []),

@@ -155,6 +155,38 @@ TraceaStatus tracea_attention(TraceaTensorView q, TraceaTensorView k, TraceaTens
   TRACEA_GUARDED(dispatch_attention(q, k, v, o, params))
 }
 
+TraceaStatus tracea_attention_forward(TraceaTensorView q, TraceaTensorView k, TraceaTensorView v,
+                                      const TraceaTensorView *q_lengths, const TraceaTensorView *k_lengths,
+                                      TraceaTensorView *o, TraceaTensorView *lse, TraceaAttentionParams params) {
+  TRACEA_GUARDED(dispatch_attention_forward(q, k, v, q_lengths, k_lengths, o, lse, params))
+}
+
+TraceaStatus tracea_attention_backward(TraceaTensorView q, TraceaTensorView k, TraceaTensorView v, TraceaTensorView o,
+                                       TraceaTensorView lse, TraceaTensorView d_o, const TraceaTensorView *q_lengths,
+                                       const TraceaTensorView *k_lengths, TraceaTensorView *dq, TraceaTensorView *dk,
+                                       TraceaTensorView *dv, TraceaAttentionParams params) {
+  TRACEA_GUARDED(dispatch_attention_backward(q, k, v, o, lse, d_o, q_lengths, k_lengths, dq, dk, dv, params))
+}
+
+TraceaStatus tracea_rotary(TraceaTensorView q, const TraceaTensorView *k, TraceaTensorView positions, TraceaTensorView inv_freq,
+                           TraceaTensorView *q_out, TraceaTensorView *k_out, TraceaRotaryParams params) {
+  TRACEA_GUARDED(dispatch_rotary(q, k, positions, inv_freq, q_out, k_out, params))
+}
+
+TraceaStatus tracea_norm_gate_residual(TraceaTensorView x, const TraceaTensorView *h, const TraceaTensorView *w_post,
+                                       const TraceaTensorView *gate, const TraceaTensorView *w_pre, TraceaTensorView *x_out,
+                                       TraceaTensorView *y, TraceaNormParams params) {
+  TRACEA_GUARDED(dispatch_norm(x, h, w_post, gate, w_pre, x_out, y, params))
+}
+
+TraceaStatus tracea_norm_gate_residual_backward(const TraceaTensorView *dx_out, const TraceaTensorView *dy, TraceaTensorView x_out,
+                                                const TraceaTensorView *h, const TraceaTensorView *w_post,
+                                                const TraceaTensorView *gate, const TraceaTensorView *w_pre, TraceaTensorView *dx,
+                                                TraceaTensorView *dh, TraceaTensorView *dw_post, TraceaTensorView *dgate,
+                                                TraceaTensorView *dw_pre, TraceaNormParams params) {
+  TRACEA_GUARDED(dispatch_norm_backward(dx_out, dy, x_out, h, w_post, gate, w_pre, dx, dh, dw_post, dgate, dw_pre, params))
+}
+
 void tracea_set_split_k(int32_t enabled) { set_split_k_enabled(enabled != 0); }
 void tracea_set_split_k_one_launch(int32_t enabled) { set_split_k_one_launch(enabled != 0); }
 int32_t tracea_last_split_k_launches(void) { return last_split_k_launches(); }

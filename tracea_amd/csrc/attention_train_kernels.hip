@@ -1,0 +1,877 @@
+// Attention for training, gfx950: a forward pass that keeps each row's log-sum-exp and a backward pass that recomputes the
+// probabilities from it.
+//
+//   s_ij = scale q_i . k_j  over the keys a row sees (j < its sequence's key length; causal: j <= i + keys - queries)
+//   lse_i = log sum_j exp(s_ij)      o_i = sum_j exp(s_ij - lse_i) v_j        (no key: lse -inf, o 0)
+//   P_ij = exp(s_ij - lse_i)   delta_i = dO_i . O_i   dS_ij = P_ij (dO_i . v_j - delta_i)
+//   dV_j = sum_i P_ij dO_i     dK_j = scale sum_i dS_ij q_i     dQ_i = scale sum_j dS_ij k_j
+//
+// Three kernels of one shape.  A wave owns 32 columns whose operand fragments stay in registers and streams the other
+// side in tiles of 64 through LDS; every product is v_mfma_f32_16x16x32 with fp32 sums.  In the result of a 16x16 block
+// lane l holds column l & 15 and rows 4 (l >> 4) + 0..3; two blocks one above the other, converted to 16 bits, are the
+// second operand of the next product over those 32 rows (k slots 0-3: rows 4 g + e, slots 4-7: rows 16 + 4 g + e,
+// g = l >> 4), whose first operand enumerates the same rows: two transposing reads of the tile.
+//   forward  columns = query rows, stream K and V:    S^T = K Q^T, O^T += V^T P^T
+//   dQ       columns = query rows, stream K and V:    S^T, dP^T = V dO^T, dQ^T += K^T dS^T
+//   dK, dV   columns = keys, stream Q and dO:         S = Q K^T, dP = dO V^T, dV^T += dO^T P, dK^T += Q^T dS
+// dQ has a kernel of its own although that computes S and dP twice (7 products instead of 5): sums over the keys of a
+// row would otherwise meet from different workgroups, in an order that changes from run to run.
+#include <type_traits>
+
+#include "contraction_kernel.hpp"
+#include "train.hpp"
+
+namespace tracea_amd {
+
+namespace {
+
+constexpr int TILE = 64;  // rows of a streamed tile
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+// Probabilities and their gradients become 16-bit operands.  f16 has no range for either: a row over thousands of keys has
+// probabilities below its smallest normal number.  P is kept as 2^14 P, dS scaled by a power of two from the largest
+// |dP - delta| there can be (see ds_scale); both factors leave with the results.  bf16 needs neither.
+constexpr float F16_P_SHIFT = 14.0f;
+
+template <int DT>
+__device__ __forceinline__ u32x4 pack_operand(const f32x4 &lo, const f32x4 &hi) {
+  if constexpr (DT == DT_F16) {
+    f16x8 h = {(_Float16)lo[0], (_Float16)lo[1], (_Float16)lo[2], (_Float16)lo[3],
+               (_Float16)hi[0], (_Float16)hi[1], (_Float16)hi[2], (_Float16)hi[3]};
+    return __builtin_bit_cast(u32x4, h);
+  } else {
+    bf16x8 h = {(__bf16)lo[0], (__bf16)lo[1], (__bf16)lo[2], (__bf16)lo[3],
+                (__bf16)hi[0], (__bf16)hi[1], (__bf16)hi[2], (__bf16)hi[3]};
+    return __builtin_bit_cast(u32x4, h);
+  }
+}
+template <int DT>
+__device__ __forceinline__ u32x2 pack_result(const f32x4 &x, float f) {
+  if constexpr (DT == DT_F16) {
+    f16x4 h = {(_Float16)(x[0] * f), (_Float16)(x[1] * f), (_Float16)(x[2] * f), (_Float16)(x[3] * f)};
+    return __builtin_bit_cast(u32x2, h);
+  } else {
+    bf16x4 h = {(__bf16)(x[0] * f), (__bf16)(x[1] * f), (__bf16)(x[2] * f), (__bf16)(x[3] * f)};
+    return __builtin_bit_cast(u32x2, h);
+  }
+}
+template <int DT>
+__device__ __forceinline__ void unpack8(u32x4 w, float (&x)[8]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (DT == DT_F16) {
+      x[2 * e] = (float)__builtin_bit_cast(_Float16, (unsigned short)(w[e] & 0xffffu));
+      x[2 * e + 1] = (float)__builtin_bit_cast(_Float16, (unsigned short)(w[e] >> 16));
+    } else {
+      x[2 * e] = __builtin_bit_cast(float, w[e] << 16);
+      x[2 * e + 1] = __builtin_bit_cast(float, w[e] & 0xffff0000u);
+    }
+  }
+}
+
+// A tile in LDS: 64 rows of DL elements, the 16-byte column XOR-ed with a number made of the row.  It serves both ways a
+// tile is read.  Row fragments (16 rows x one column per 16 lanes) need 16 different bank groups from 16 rows: the numbers of
+// rows 0..15 differ (with DL = 64 two rows share a 256-byte line, and those of a pair are alike).  Transposing reads take 8 rows x 2
+// columns per half-wave: all but the lowest bit of the numbers of 8 rows differ.  A rotation by one bit of the row has both.
+template <int DL>
+struct Tile {
+  static constexpr int ROW_BYTES = DL * 2, CH = DL / 8, RP = 256 / ROW_BYTES, BYTES = TILE * ROW_BYTES;
+  static __device__ __forceinline__ int swz(int row) {
+    const int k = (row / RP) & (CH - 1);
+    return ((k << 1) | (k / (CH / 2))) & (CH - 1);
+  }
+};
+
+// A direct-to-LDS load: lane l's bytes from its offset land at lds + l * size.  Written as instructions: behind the builtin
+// the compiler, which cannot tell the buffers of a ring apart, waits for all requests in front of the next LDS read.  The
+// kernels wait for a tile themselves (vmcnt(0) and a barrier) before they read it.  (s_nop: m0 is read by the load behind it.)
+__device__ __forceinline__ void dma16(u32x4 rsrc, unsigned offset, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(rsrc) : "memory");
+}
+__device__ __forceinline__ void dma4(u32x4 rsrc, unsigned offset, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(rsrc) : "memory");
+}
+__device__ __forceinline__ u32x4 resource(const void *base, unsigned bytes) {
+  const unsigned long long at = (unsigned long long)base;
+  return u32x4{(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)at),
+               (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(at >> 32)) & 0xffffu, bytes, 0x00020000u};
+}
+__device__ __forceinline__ unsigned lds_address(const void *p) {
+  return (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(unsigned long long)(__attribute__((address_space(3))) const void *)p);
+}
+
+// Requests 64 rows of a tensor into LDS (16 bytes per lane, 1 KB per wave and request).  offset(row) is the byte offset
+// of a row from `base`, below 2^31, or BEYOND for a row that reads as zeros; columns from D on read as zeros too.
+constexpr unsigned BEYOND = 0x80000000u;
+template <int DL, int WAVES, typename F>
+__device__ __forceinline__ void load_tile(const void *base, const unsigned char *dst, int D, int lane, int wave_u, F &&offset) {
+  using T = Tile<DL>;
+  constexpr int RPI = 64 / T::CH;             // rows per request
+  constexpr int NI = TILE / (RPI * WAVES);
+  const u32x4 rsrc = resource(base, BEYOND);
+  const unsigned lds = lds_address(dst);
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int first = (i * WAVES + wave_u) * RPI, row = first + lane / T::CH;
+    const int col = ((lane % T::CH) ^ T::swz(row)) << 3;
+    const unsigned off = offset(row);
+    dma16(rsrc, (off == BEYOND || col >= D) ? BEYOND : off + (unsigned)(col * 2), lds + (unsigned)(first * T::ROW_BYTES));
+  }
+}
+
+// First operand of a product over the head dimension: rows 16 rb .. + 15 of the tile, columns 32 ks .. + 31.
+template <int DL>
+__device__ __forceinline__ u32x4 read_rows(const unsigned char *tile, int rb, int ks, int r16, int g4) {
+  using T = Tile<DL>;
+  return *(const u32x4 *)(tile + rb * 16 * T::ROW_BYTES + r16 * T::ROW_BYTES + (((ks * 4 + g4) ^ T::swz(r16)) << 4));
+}
+// First operand of a product over the rows 32 s .. + 31: columns 16 db .. + 15 of the tile, transposed.
+template <int DL>
+__device__ __forceinline__ u32x4 read_columns(const unsigned char *tile, int s, int db, int r16, int g4) {
+  using T = Tile<DL>;
+  const int row = g4 * 4 + (r16 >> 2);
+  const int at = row * T::ROW_BYTES + (((((r16 & 3) >> 1) ^ T::swz(row)) ^ (db << 1)) << 4) + (r16 & 1) * 8;
+  const unsigned char *p = tile + s * 32 * T::ROW_BYTES + at;
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p);
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(p + 16 * T::ROW_BYTES));
+  const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
+  return u32x4{a[0], a[1], b[0], b[1]};
+}
+
+// Nothing is scheduled across: the compiler otherwise hoists the reads of several phases and runs out of registers.
+__device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
+
+// max / sum over the four 16-lane groups
+__device__ __forceinline__ float groups_max(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16, 64));
+  return fmaxf(x, __shfl_xor(x, 32, 64));
+}
+__device__ __forceinline__ float groups_sum(float x) {
+  x += __shfl_xor(x, 16, 64);
+  return x + __shfl_xor(x, 32, 64);
+}
+
+// Consecutive workgroups go to the 8 XCDs in turn; handing each XCD a run of blocks brings a head's tiles into one L2.
+__device__ __forceinline__ int xcd_run(int id, int total) {
+  const int q = total >> 3, rem = total & 7, x = id & 7, i = id >> 3;
+  return x * q + (x < rem ? x : rem) + i;
+}
+
+struct Rows {  // of one batch entry and key/value head
+  int b, hk, lq, lk, off;  // lengths; a causal row of query i sees keys up to i + off
+};
+__device__ __forceinline__ Rows rows_of(const AttentionTrainArgs &a, int bh) {
+  Rows r;
+  r.b = bh / a.Hk;
+  r.hk = bh - r.b * a.Hk;
+  r.lq = a.Sq;
+  r.lk = a.Sk;
+  if (a.q_len != nullptr) r.lq = min(max(a.q_len[r.b], 0), a.Sq);
+  if (a.k_len != nullptr) r.lk = min(max(a.k_len[r.b], 0), a.Sk);
+  r.off = r.lk - r.lq;
+  return r;
+}
+__device__ __forceinline__ int query_of(const AttentionTrainArgs &a, int r) {
+  return a.G == 1 ? r : (int)__umulhi((unsigned)r, a.g_magic);
+}
+__device__ __forceinline__ long long row_at(const AttentionTrainArgs &a, const HeadView &t, const Rows &w, int r) {
+  const int i = query_of(a, r);
+  return (long long)w.b * t.sb + (long long)(w.hk * a.G + (r - i * a.G)) * t.sh + (long long)i * t.ss;
+}
+__device__ __forceinline__ const unsigned short *slice(const HeadView &t, int b, int h) {
+  return (const unsigned short *)t.p + (long long)b * t.sb + (long long)h * t.sh;
+}
+
+// Fragment of 16 resident rows for the k-step ks: lane l holds row l & 15, columns 32 ks + 8 (l >> 4) .. + 7.
+__device__ __forceinline__ u32x4 resident(const unsigned short *row, bool there, int col, int D) {
+  u32x4 z = {0, 0, 0, 0};
+  return there && col < D ? *(const u32x4 *)(row + col) : z;
+}
+
+// The power of two that dS is multiplied by before it becomes an f16 operand: |dP - delta| <= 2 max|dO| max|V|
+// (delta is a mean of the dP of its row), and P <= 1.
+__device__ __forceinline__ float ds_scale(const AttentionTrainArgs &a, int bh, int lane) {
+  const float *n = a.norms + (long long)bh * a.norm_blocks;
+  const int of_rows = a.rows_pad / TILE;
+  float mo = 0.0f, mv = 0.0f;
+  for (int i = lane; i < a.norm_blocks; i += 64) {
+    const float x = n[i];
+    if (i < of_rows) mo = fmaxf(mo, x);
+    else mv = fmaxf(mv, x);
+  }
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    mo = fmaxf(mo, __shfl_xor(mo, m, 64));
+    mv = fmaxf(mv, __shfl_xor(mv, m, 64));
+  }
+  const float bound = 2.0f * sqrtf(mo) * sqrtf(mv);
+  if (!(bound > 0.0f) || !(bound < 3.0e38f)) return 1.0f;
+  int e;
+  (void)frexpf(bound, &e);  // bound < 2^e
+  e = 14 - e;
+  e = e < -100 ? -100 : e > 100 ? 100 : e;
+  return __builtin_bit_cast(float, (unsigned)(127 + e) << 23);
+}
+
+// ---- forward --------------------------------------------------------------------------------------------------
+
+// The running maximum moves only when a tile exceeds it by more than this many powers of two: a row needs one reference for
+// all its keys, not the largest score, and 2^8 is far inside the range of the 16-bit operands.
+constexpr float LAZY_MAX = 8.0f;
+
+template <int DT, int DL, int DU, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
+attention_train_forward_kernel(const AttentionTrainArgs a) {
+  using T = Tile<DL>;
+  constexpr int BR = 32 * WAVES, KS = DU / 32, DB = DU / 16, KB = TILE / 16;
+  __shared__ __attribute__((aligned(1024))) unsigned char sK[2 * T::BYTES], sV[2 * T::BYTES];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r16 = lane & 15, g4 = lane >> 4;
+  const int blocks = (a.G * a.Sq + BR - 1) / BR;
+  const int vid = xcd_run(blockIdx.x, gridDim.x);
+  const int bh = vid / blocks, blk = blocks - 1 - (vid - bh * blocks);  // most keys under a causal mask first
+  const Rows w = rows_of(a, bh);
+  const int rows = a.G * w.lq;
+  const int r_wave = blk * BR + wave * 32;
+
+  const int last_row = min(blk * BR + BR, rows) - 1;
+  int keys = 0;  // that any row of the block sees
+  if (last_row >= blk * BR) keys = a.causal ? min(w.lk, query_of(a, last_row) + w.off + 1) : w.lk;
+  int tiles = keys > 0 ? (keys + TILE - 1) / TILE : 0;
+  int t0 = 0;
+  if (a.splits > 1) {
+    t0 = (int)blockIdx.y * a.tiles_per_split;
+    tiles = min(tiles, t0 + a.tiles_per_split);
+  }
+
+  int q_last[2];  // the last key that the lane's queries see
+  u32x4 qf[2][KS];
+#pragma unroll
+  for (int qb = 0; qb < 2; ++qb) {
+    const int r = r_wave + qb * 16 + r16;
+    const bool there = r < rows;
+    q_last[qb] = !there ? -1 : a.causal ? min(w.lk - 1, query_of(a, r) + w.off) : w.lk - 1;
+    const unsigned short *p = (const unsigned short *)a.q.p + (there ? row_at(a, a.q, w, r) : 0);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qf[qb][ks] = resident(p, there, ks * 32 + g4 * 8, a.D);
+      if (a.negate) qf[qb][ks] ^= 0x80008000u;
+    }
+  }
+  // of the wave: keys that some row sees, and the first that not every row sees
+  int wave_keys = 0, wave_full = 0;
+  if (r_wave < rows) {
+    const int r_end = min(r_wave + 32, rows) - 1;
+    wave_keys = a.causal ? min(w.lk, query_of(a, r_end) + w.off + 1) : w.lk;
+    wave_full = r_wave + 32 > rows ? 0 : a.causal ? min(w.lk, query_of(a, r_wave) + w.off + 1) : w.lk;
+  }
+
+  const unsigned short *Kg = slice(a.k, w.b, w.hk), *Vg = slice(a.v, w.b, w.hk);
+  auto request = [&](int t) __attribute__((always_inline)) {
+    const int left = w.lk - t * TILE, at = (t & 1) * T::BYTES;
+    const unsigned kss = (unsigned)a.k.ss * 2u, vss = (unsigned)a.v.ss * 2u;
+    load_tile<DL, WAVES>(Kg + (long long)t * TILE * a.k.ss, sK + at, a.D, lane, wave, [&](int row) { return row < left ? row * kss : BEYOND; });
+    load_tile<DL, WAVES>(Vg + (long long)t * TILE * a.v.ss, sV + at, a.D, lane, wave, [&](int row) { return row < left ? row * vss : BEYOND; });
+  };
+
+  f32x4 o[2][DB];
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};  // reference (log2 units) and sum of the lane's keys
+#pragma unroll
+  for (int qb = 0; qb < 2; ++qb)
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[qb][d] = f32x4{0, 0, 0, 0};
+
+  auto compute = [&](int t, auto edge_tag) __attribute__((always_inline)) {
+    constexpr bool EDGE = decltype(edge_tag)::value;
+    const unsigned char *tK = sK + (t & 1) * T::BYTES, *tV = sV + (t & 1) * T::BYTES;
+    f32x4 z[2][KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb) z[qb][kb] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const u32x4 kf = read_rows<DL>(tK, kb, ks, r16, g4);
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) z[qb][kb] = Mfma16<DT>::run(kf, qf[qb][ks], z[qb][kb]);
+      }
+    fence();
+    bool moved = false;
+    float alpha[2];
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (EDGE) z[qb][kb][e] = t * TILE + kb * 16 + g4 * 4 + e > q_last[qb] ? -INFINITY : z[qb][kb][e];
+          mx = fmaxf(mx, z[qb][kb][e]);
+        }
+      mx = groups_max(mx) * a.scale_log2;
+      const bool mv = mx > m[qb] + LAZY_MAX;  // (a first score above -inf always moves it)
+      const float mn = mv ? mx : m[qb];
+      alpha[qb] = mv ? __builtin_amdgcn_exp2f(m[qb] - mn) : 1.0f;
+      m[qb] = mn;
+      moved |= mv;
+    }
+    if (__any(moved)) {
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb) {
+        l[qb] *= alpha[qb];
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[qb][d] *= alpha[qb];
+      }
+    }
+    u32x4 pf[2][2];
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+      const float ref = m[qb] == -INFINITY ? 0.0f : m[qb];  // (nothing visible yet: exp2(-inf) = 0)
+      float sum = 0.0f;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          z[qb][kb][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[qb][kb][e], a.scale_log2, -ref));
+          sum += z[qb][kb][e];
+        }
+      l[qb] += sum;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) pf[qb][s] = pack_operand<DT>(z[qb][2 * s], z[qb][2 * s + 1]);
+    }
+    fence();
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const u32x4 vf = read_columns<DL>(tV, s, d, r16, g4);
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) o[qb][d] = Mfma16<DT>::run(vf, pf[qb][s], o[qb][d]);
+      }
+  };
+  auto head = [&](int t) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this tile
+    __syncthreads();
+    if (t + 1 < tiles) request(t + 1);
+  };
+  // tiles that every row of the wave sees whole, then the others (a wave takes part in the loads of tiles that none sees)
+  int t = t0;
+  if (t < tiles) request(t);
+  for (const int end = min(tiles, wave_full / TILE); t < end; ++t) {
+    head(t);
+    compute(t, std::false_type{});
+  }
+  for (; t < tiles; ++t) {
+    head(t);
+    if (t * TILE < wave_keys) compute(t, std::true_type{});
+  }
+
+#pragma unroll
+  for (int qb = 0; qb < 2; ++qb) {
+    const int r = r_wave + qb * 16 + r16;
+    const float sum = groups_sum(l[qb]);
+    if (r >= a.G * a.Sq) continue;
+    if (a.splits > 1) {
+      const long long at = ((long long)blockIdx.y * a.B * a.Hk + bh) * a.rows_pad + r;
+      if (g4 == 0) {
+        a.part_ml[2 * at] = m[qb];
+        a.part_ml[2 * at + 1] = sum;
+      }
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+        if (d * 16 + g4 * 4 < a.D) *(f32x4 *)(a.part_o + at * DU + d * 16 + g4 * 4) = o[qb][d];
+      continue;
+    }
+    const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;  // (NaN stays)
+    unsigned short *p = (unsigned short *)a.o.p + row_at(a, a.o, w, r);
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+      if (d * 16 + g4 * 4 < a.D) *(u32x2 *)(p + d * 16 + g4 * 4) = pack_result<DT>(o[qb][d], inv);
+    if (g4 == 0) {
+      const int i = query_of(a, r);
+      a.lse[(long long)w.b * a.lse_sb + (long long)(w.hk * a.G + r - i * a.G) * a.lse_sh + (long long)i * a.lse_ss] =
+          sum == 0.0f ? -INFINITY : (m[qb] + __builtin_amdgcn_logf(sum)) * LN2;
+    }
+  }
+}
+
+// Joins the partial results of a split key axis: one row per DU / 4 lanes.
+template <int DT, int DU>
+__global__ void __launch_bounds__(256) attention_train_join_kernel(const AttentionTrainArgs a) {
+  constexpr int LPR = 32;  // lanes per row, 4 columns each
+  const long long id = ((long long)blockIdx.x * 256 + threadIdx.x) / LPR;
+  const int c = (threadIdx.x % LPR) * 4;
+  const int per = a.G * a.Sq;
+  if (id >= (long long)a.B * a.Hk * per) return;
+  const int bh = (int)(id / per), r = (int)(id - (long long)bh * per);
+  const Rows w = rows_of(a, bh);
+  const long long plane = (long long)a.B * a.Hk * a.rows_pad, at = (long long)bh * a.rows_pad + r;
+  float m = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[2 * (s * plane + at)]);
+  const float ref = m == -INFINITY ? 0.0f : m;
+  float sum = 0.0f;
+  f32x4 o = {0, 0, 0, 0};
+  for (int s = 0; s < a.splits; ++s) {
+    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * (s * plane + at)] - ref);
+    sum += f * a.part_ml[2 * (s * plane + at) + 1];
+    if (c < a.D) o += f * *(const f32x4 *)(a.part_o + (s * plane + at) * DU + c);
+  }
+  const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
+  if (c < a.D) *(u32x2 *)((unsigned short *)a.o.p + row_at(a, a.o, w, r) + c) = pack_result<DT>(o, inv);
+  if (c == 0) {
+    const int i = query_of(a, r);
+    a.lse[(long long)w.b * a.lse_sb + (long long)(w.hk * a.G + r - i * a.G) * a.lse_sh + (long long)i * a.lse_ss] =
+        sum == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(sum)) * LN2;
+  }
+}
+
+// ---- backward ---------------------------------------------------------------------------------------------------
+
+// Per packed row -lse log2(e) and -(dO . O); f16: the largest squared norms of 64 rows of dO, and of 64 keys of V.
+template <int DT>
+__global__ void __launch_bounds__(256) attention_train_rows_kernel(const AttentionTrainArgs a) {
+  constexpr int LPR = 16;  // lanes per row, 8 columns each
+  __shared__ float s_max[4];
+  const int c = (threadIdx.x % LPR) * 8, row_blocks = a.rows_pad / TILE;
+  const int bh = blockIdx.y, blk = blockIdx.x;
+  const Rows w = rows_of(a, bh);
+  float big = 0.0f;
+#pragma unroll
+  for (int it = 0; it < TILE / 16; ++it) {
+    const int row = it * 16 + (int)threadIdx.x / LPR;
+    float dot = 0.0f, norm = 0.0f;
+    if (blk < row_blocks) {
+      const int r = blk * TILE + row;
+      const bool there = r < a.G * w.lq;
+      if (there && c < a.D) {
+        float x[8], y[8];
+        unpack8<DT>(*(const u32x4 *)((const unsigned short *)a.d_o.p + row_at(a, a.d_o, w, r) + c), x);
+        unpack8<DT>(*(const u32x4 *)((const unsigned short *)a.o.p + row_at(a, a.o, w, r) + c), y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          dot = __builtin_fmaf(x[e], y[e], dot);
+          norm = __builtin_fmaf(x[e], x[e], norm);
+        }
+      }
+#pragma unroll
+      for (int s = 1; s < LPR; s <<= 1) dot += __shfl_xor(dot, s, 64);
+      if (c == 0) {
+        float nl = -INFINITY;
+        if (there) {
+          const int i = query_of(a, r);
+          const float lse = a.lse[(long long)w.b * a.lse_sb + (long long)(w.hk * a.G + r - i * a.G) * a.lse_sh + (long long)i * a.lse_ss];
+          if (lse != -INFINITY) nl = (DT == DT_F16 ? F16_P_SHIFT : 0.0f) - lse * LOG2E;
+        }
+        a.neg_lse2[(long long)bh * a.rows_pad + r] = nl;
+        a.neg_delta[(long long)bh * a.rows_pad + r] = nl == -INFINITY ? 0.0f : -dot;
+      }
+    } else {
+      const int j = (blk - row_blocks) * TILE + row;
+      if (j < w.lk && c < a.D) {
+        float x[8];
+        unpack8<DT>(*(const u32x4 *)(slice(a.v, w.b, w.hk) + (long long)j * a.v.ss + c), x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) norm = __builtin_fmaf(x[e], x[e], norm);
+      }
+    }
+    if constexpr (DT == DT_F16) {
+#pragma unroll
+      for (int s = 1; s < LPR; s <<= 1) norm += __shfl_xor(norm, s, 64);
+      big = fmaxf(big, norm);
+    }
+  }
+  if constexpr (DT == DT_F16) {
+    big = groups_max(big);
+    if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = big;
+    __syncthreads();
+    if (threadIdx.x == 0) a.norms[(long long)bh * a.norm_blocks + blk] = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+  }
+}
+
+template <int DT, int DL, int DU, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
+attention_train_dq_kernel(const AttentionTrainArgs a) {
+  using T = Tile<DL>;
+  constexpr int BR = 32 * WAVES, KS = DU / 32, DB = DU / 16;
+  __shared__ __attribute__((aligned(1024))) unsigned char sK[2 * T::BYTES], sV[2 * T::BYTES];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r16 = lane & 15, g4 = lane >> 4;
+  const int blocks = (a.G * a.Sq + BR - 1) / BR;
+  const int vid = xcd_run(blockIdx.x, gridDim.x);
+  const int bh = vid / blocks, blk = blocks - 1 - (vid - bh * blocks);
+  const Rows w = rows_of(a, bh);
+  const int rows = a.G * w.lq;
+  const int r_wave = blk * BR + wave * 32;
+  const int last_row = min(blk * BR + BR, rows) - 1;
+  int keys = 0;
+  if (last_row >= blk * BR) keys = a.causal ? min(w.lk, query_of(a, last_row) + w.off + 1) : w.lk;
+  const int tiles = keys > 0 ? (keys + TILE - 1) / TILE : 0;
+
+  int q_last[2];
+  float nl[2], nd[2];
+  u32x4 qf[2][KS], of[2][KS];
+#pragma unroll
+  for (int qb = 0; qb < 2; ++qb) {
+    const int r = r_wave + qb * 16 + r16;
+    const bool there = r < rows;
+    q_last[qb] = !there ? -1 : a.causal ? min(w.lk - 1, query_of(a, r) + w.off) : w.lk - 1;
+    const unsigned short *p = (const unsigned short *)a.q.p + (there ? row_at(a, a.q, w, r) : 0);
+    const unsigned short *g = (const unsigned short *)a.d_o.p + (there ? row_at(a, a.d_o, w, r) : 0);
+    nl[qb] = there ? a.neg_lse2[(long long)bh * a.rows_pad + r] : -INFINITY;
+    nd[qb] = there ? a.neg_delta[(long long)bh * a.rows_pad + r] : 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qf[qb][ks] = resident(p, there, ks * 32 + g4 * 8, a.D);
+      if (a.negate) qf[qb][ks] ^= 0x80008000u;
+      of[qb][ks] = resident(g, there, ks * 32 + g4 * 8, a.D);
+    }
+  }
+  int wave_keys = 0, wave_full = 0;
+  if (r_wave < rows) {
+    const int r_end = min(r_wave + 32, rows) - 1;
+    wave_keys = a.causal ? min(w.lk, query_of(a, r_end) + w.off + 1) : w.lk;
+    wave_full = a.causal ? min(w.lk, query_of(a, r_wave) + w.off + 1) : w.lk;  // (rows past the end have P = 0)
+  }
+  float dsc = 1.0f, dsp = 1.0f;  // dS operand = P' (dP - delta) dsp = dS dsc
+  if constexpr (DT == DT_F16) {
+    dsc = ds_scale(a, bh, lane);
+    dsp = dsc * (1.0f / 16384.0f);
+  }
+
+  const unsigned short *Kg = slice(a.k, w.b, w.hk), *Vg = slice(a.v, w.b, w.hk);
+  auto request = [&](int t) __attribute__((always_inline)) {
+    const int left = w.lk - t * TILE, at = (t & 1) * T::BYTES;
+    const unsigned kss = (unsigned)a.k.ss * 2u, vss = (unsigned)a.v.ss * 2u;
+    load_tile<DL, WAVES>(Kg + (long long)t * TILE * a.k.ss, sK + at, a.D, lane, wave, [&](int row) { return row < left ? row * kss : BEYOND; });
+    load_tile<DL, WAVES>(Vg + (long long)t * TILE * a.v.ss, sV + at, a.D, lane, wave, [&](int row) { return row < left ? row * vss : BEYOND; });
+  };
+
+  f32x4 acc[2][DB];
+#pragma unroll
+  for (int qb = 0; qb < 2; ++qb)
+#pragma unroll
+    for (int d = 0; d < DB; ++d) acc[qb][d] = f32x4{0, 0, 0, 0};
+
+  auto compute = [&](int t, auto edge_tag) __attribute__((always_inline)) {
+    constexpr bool EDGE = decltype(edge_tag)::value;
+    const unsigned char *tK = sK + (t & 1) * T::BYTES, *tV = sV + (t & 1) * T::BYTES;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      f32x4 z[2][2], g[2][2];  // [qb][block of 16 keys]
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) {
+          z[qb][kb] = f32x4{0, 0, 0, 0};
+          g[qb][kb] = f32x4{nd[qb], nd[qb], nd[qb], nd[qb]};
+        }
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          const u32x4 kf = read_rows<DL>(tK, 2 * s + kb, ks, r16, g4);
+#pragma unroll
+          for (int qb = 0; qb < 2; ++qb) z[qb][kb] = Mfma16<DT>::run(kf, qf[qb][ks], z[qb][kb]);
+        }
+      fence();
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          const u32x4 vf = read_rows<DL>(tV, 2 * s + kb, ks, r16, g4);
+#pragma unroll
+          for (int qb = 0; qb < 2; ++qb) g[qb][kb] = Mfma16<DT>::run(vf, of[qb][ks], g[qb][kb]);
+        }
+      fence();
+      u32x4 df[2];
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z[qb][kb][e], a.scale_log2, nl[qb]));
+            // (a row that sees one key has P = 1 whatever the score: no gradient, not the rounding of O in delta)
+            if constexpr (EDGE) p = t * TILE + s * 32 + kb * 16 + g4 * 4 + e > q_last[qb] || q_last[qb] == 0 ? 0.0f : p;
+            if constexpr (DT == DT_F16) p *= dsp;
+            z[qb][kb][e] = p * g[qb][kb][e];
+          }
+        df[qb] = pack_operand<DT>(z[qb][0], z[qb][1]);
+      }
+      fence();
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const u32x4 kf = read_columns<DL>(tK, s, d, r16, g4);
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) acc[qb][d] = Mfma16<DT>::run(kf, df[qb], acc[qb][d]);
+      }
+      fence();
+    }
+  };
+  auto head = [&](int t) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this tile
+    __syncthreads();
+    if (t + 1 < tiles) request(t + 1);
+  };
+  // tiles that every row of the wave sees whole, then the others (a wave takes part in the loads of tiles that none sees)
+  int t = 0;
+  if (t < tiles) request(t);
+  for (const int end = min(tiles, wave_full / TILE); t < end; ++t) {
+    head(t);
+    compute(t, std::false_type{});
+  }
+  for (; t < tiles; ++t) {
+    head(t);
+    if (t * TILE < wave_keys) compute(t, std::true_type{});
+  }
+
+  const float f = (a.negate ? -a.scale : a.scale) / dsc;
+#pragma unroll
+  for (int qb = 0; qb < 2; ++qb) {
+    const int r = r_wave + qb * 16 + r16;
+    if (r >= a.G * a.Sq) continue;
+    unsigned short *p = (unsigned short *)a.dq.p + row_at(a, a.dq, w, r);
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+      if (d * 16 + g4 * 4 < a.D) *(u32x2 *)(p + d * 16 + g4 * 4) = pack_result<DT>(acc[qb][d], f);
+  }
+}
+
+template <int DT, int DL, int DU, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DU == 128 ? 1 : 2, DU == 128 ? 1 : 2)))
+attention_train_dkv_kernel(const AttentionTrainArgs a) {
+  using T = Tile<DL>;
+  constexpr int BC = 32 * WAVES, KS = DU / 32, DB = DU / 16;
+  __shared__ __attribute__((aligned(1024))) unsigned char sQ[2 * T::BYTES], sO[2 * T::BYTES];
+  __shared__ __attribute__((aligned(16))) float sL[2 * TILE], sD[2 * TILE];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r16 = lane & 15, g4 = lane >> 4;
+  const int blocks = (a.Sk + BC - 1) / BC;
+  const int vid = xcd_run(blockIdx.x, gridDim.x);
+  const int bh = vid / blocks, blk = vid - bh * blocks;  // (under a causal mask the first keys have most rows)
+  const Rows w = rows_of(a, bh);
+  const int rows = a.G * w.lq;
+  const int k_blk = blk * BC, k_wave = k_blk + wave * 32;
+
+  // tiles of packed rows that see a key of the block, from the first one on
+  int t_begin = 0;
+  const int t_end = k_blk < w.lk ? (rows + TILE - 1) / TILE : 0;
+  if (a.causal) t_begin = (int)(((long long)max(0, k_blk - w.off) * a.G) / TILE);
+
+  u32x4 kf[2][KS], vf[2][KS];
+#pragma unroll
+  for (int nb = 0; nb < 2; ++nb) {
+    const int j = k_wave + nb * 16 + r16;
+    const bool there = j < w.lk;
+    const unsigned short *kp = slice(a.k, w.b, w.hk) + (there ? (long long)j * a.k.ss : 0);
+    const unsigned short *vp = slice(a.v, w.b, w.hk) + (there ? (long long)j * a.v.ss : 0);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      kf[nb][ks] = resident(kp, there, ks * 32 + g4 * 8, a.D);
+      if (a.negate) kf[nb][ks] ^= 0x80008000u;
+      vf[nb][ks] = resident(vp, there, ks * 32 + g4 * 8, a.D);
+    }
+  }
+  // of the wave: rows from here on see some of its keys / all of them (rows past the end have P = 0)
+  const bool live = k_wave < w.lk;
+  long long row_some = 0, row_all = 0;
+  if (a.causal) {
+    row_some = (long long)max(0, k_wave - w.off) * a.G;
+    row_all = (long long)max(0, k_wave + 31 - w.off) * a.G;
+  }
+  if (w.lk == 1) row_all = 0x7fffffff;
+  float dsc = 1.0f, dsp = 1.0f;
+  if constexpr (DT == DT_F16) {
+    dsc = ds_scale(a, bh, lane);
+    dsp = dsc * (1.0f / 16384.0f);
+  }
+
+  const unsigned short *Qg = slice(a.q, w.b, w.hk * a.G), *Og = slice(a.d_o, w.b, w.hk * a.G);
+  const float *nl = a.neg_lse2 + (long long)bh * a.rows_pad, *nd = a.neg_delta + (long long)bh * a.rows_pad;
+  auto request = [&](int t) __attribute__((always_inline)) {
+    const int r0 = t * TILE, i0 = query_of(a, r0), at = (t & 1) * T::BYTES;
+    auto offset = [&](const HeadView &v, int row) __attribute__((always_inline)) -> unsigned {
+      const int r = r0 + row, i = query_of(a, r);
+      return r < rows ? (unsigned)(i - i0) * ((unsigned)v.ss * 2u) + (unsigned)(r - i * a.G) * ((unsigned)v.sh * 2u) : BEYOND;
+    };
+    load_tile<DL, WAVES>(Qg + (long long)i0 * a.q.ss, sQ + at, a.D, lane, wave, [&](int row) { return offset(a.q, row); });
+    load_tile<DL, WAVES>(Og + (long long)i0 * a.d_o.ss, sO + at, a.D, lane, wave, [&](int row) { return offset(a.d_o, row); });
+    if (wave < 2) {  // (rows_pad is a multiple of the tile)
+      dma4(resource((wave == 0 ? nl : nd) + r0, TILE * 4), lane * 4, lds_address((wave == 0 ? sL : sD) + (t & 1) * TILE));
+    }
+  };
+
+  f32x4 dk[2][DB], dv[2][DB];
+#pragma unroll
+  for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+    for (int d = 0; d < DB; ++d) dk[nb][d] = dv[nb][d] = f32x4{0, 0, 0, 0};
+
+  auto compute = [&](int t, auto edge_tag) __attribute__((always_inline)) {
+    constexpr bool EDGE = decltype(edge_tag)::value;
+    const unsigned char *tQ = sQ + (t & 1) * T::BYTES, *tO = sO + (t & 1) * T::BYTES;
+    const float *tL = sL + (t & 1) * TILE, *tD = sD + (t & 1) * TILE;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      f32x4 z[2][2], g[2][2];  // [block of 16 rows][nb]
+#pragma unroll
+      for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb) z[rb][nb] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb) {
+          const u32x4 qf = read_rows<DL>(tQ, 2 * s + rb, ks, r16, g4);
+#pragma unroll
+          for (int nb = 0; nb < 2; ++nb) z[rb][nb] = Mfma16<DT>::run(qf, kf[nb][ks], z[rb][nb]);
+        }
+      fence();
+#pragma unroll
+      for (int rb = 0; rb < 2; ++rb) {
+        const f32x4 l4 = *(const f32x4 *)(tL + s * 32 + rb * 16 + g4 * 4);
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z[rb][nb][e], a.scale_log2, l4[e]));
+            if constexpr (EDGE) {
+              const int i = query_of(a, t * TILE + s * 32 + rb * 16 + g4 * 4 + e);
+              p = a.causal && k_wave + nb * 16 + r16 > i + w.off ? 0.0f : p;
+            }
+            z[rb][nb][e] = p;
+          }
+      }
+      u32x4 pf[2];
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb) pf[nb] = pack_operand<DT>(z[0][nb], z[1][nb]);
+      fence();
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const u32x4 of = read_columns<DL>(tO, s, d, r16, g4);
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb) dv[nb][d] = Mfma16<DT>::run(of, pf[nb], dv[nb][d]);
+      }
+      fence();
+#pragma unroll
+      for (int rb = 0; rb < 2; ++rb) {
+        const f32x4 d4 = *(const f32x4 *)(tD + s * 32 + rb * 16 + g4 * 4);
+        g[rb][0] = g[rb][1] = d4;
+      }
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb) {
+          const u32x4 of = read_rows<DL>(tO, 2 * s + rb, ks, r16, g4);
+#pragma unroll
+          for (int nb = 0; nb < 2; ++nb) g[rb][nb] = Mfma16<DT>::run(of, vf[nb][ks], g[rb][nb]);
+        }
+#pragma unroll
+      for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float x = z[rb][nb][e] * g[rb][nb][e];
+            if constexpr (DT == DT_F16) x *= dsp;
+            if constexpr (EDGE) {  // (a row that sees one key has P = 1 whatever the score)
+              const int i = query_of(a, t * TILE + s * 32 + rb * 16 + g4 * 4 + e);
+              x = w.lk == 1 || (a.causal && i + w.off == 0) ? 0.0f : x;
+            }
+            z[rb][nb][e] = x;
+          }
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb) pf[nb] = pack_operand<DT>(z[0][nb], z[1][nb]);
+      fence();
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const u32x4 qf = read_columns<DL>(tQ, s, d, r16, g4);
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb) dk[nb][d] = Mfma16<DT>::run(qf, pf[nb], dk[nb][d]);
+      }
+      fence();
+    }
+  };
+  auto head = [&](int t) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this tile
+    __syncthreads();
+    if (t + 1 < t_end) request(t + 1);
+  };
+  // tiles with rows that see some of the wave's keys, then those whose rows see all
+  int t = t_begin;
+  if (t < t_end) request(t);
+  for (; t < t_end && t * TILE < row_all; ++t) {
+    head(t);
+    if (live && t * TILE + TILE > row_some) compute(t, std::true_type{});
+  }
+  for (; t < t_end; ++t) {
+    head(t);
+    if (live) compute(t, std::false_type{});
+  }
+
+  const float fk = (a.negate ? -a.scale : a.scale) / dsc, fv = DT == DT_F16 ? 1.0f / 16384.0f : 1.0f;
+#pragma unroll
+  for (int nb = 0; nb < 2; ++nb) {
+    const int j = k_wave + nb * 16 + r16;
+    if (j >= a.Sk) continue;
+    unsigned short *kp = (unsigned short *)slice(a.dk, w.b, w.hk) + (long long)j * a.dk.ss;
+    unsigned short *vp = (unsigned short *)slice(a.dv, w.b, w.hk) + (long long)j * a.dv.ss;
+    const bool there = j < w.lk;  // (a key past the end was read as zeros, its P is not)
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+      if (d * 16 + g4 * 4 < a.D) {
+        u32x2 x = pack_result<DT>(dk[nb][d], fk), y = pack_result<DT>(dv[nb][d], fv);
+        *(u32x2 *)(kp + d * 16 + g4 * 4) = there ? x : u32x2{0, 0};
+        *(u32x2 *)(vp + d * 16 + g4 * 4) = there ? y : u32x2{0, 0};
+      }
+  }
+}
+
+template <int DT, int DL, int DU>
+int forward(const AttentionTrainArgs &a, hipStream_t stream) {
+  constexpr int W = 4;
+  const unsigned blocks = (unsigned)((a.G * a.Sq + 32 * W - 1) / (32 * W)) * (unsigned)(a.B * a.Hk);
+  hipLaunchKernelGGL((attention_train_forward_kernel<DT, DL, DU, W>), dim3(blocks, (unsigned)a.splits), dim3(W * 64), 0, stream, a);
+  if (a.splits > 1) {
+    const long long rows = (long long)a.B * a.Hk * a.G * a.Sq;
+    hipLaunchKernelGGL((attention_train_join_kernel<DT, DU>), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, stream, a);
+  }
+  return (int)hipGetLastError();
+}
+
+template <int DT, int DL, int DU>
+int backward(const AttentionTrainArgs &a, hipStream_t stream) {
+  constexpr int W = 4;
+  const unsigned bh = (unsigned)(a.B * a.Hk);
+  const unsigned row_blocks = (unsigned)(DT == DT_F16 ? a.norm_blocks : a.rows_pad / TILE);
+  if (row_blocks > 0) hipLaunchKernelGGL((attention_train_rows_kernel<DT>), dim3(row_blocks, bh), dim3(256), 0, stream, a);
+  const unsigned kb = (unsigned)((a.Sk + 32 * W - 1) / (32 * W)) * bh;
+  if (kb > 0) hipLaunchKernelGGL((attention_train_dkv_kernel<DT, DL, DU, W>), dim3(kb), dim3(W * 64), 0, stream, a);
+  const unsigned qb = (unsigned)((a.G * a.Sq + 32 * W - 1) / (32 * W)) * bh;
+  if (qb > 0) hipLaunchKernelGGL((attention_train_dq_kernel<DT, DL, DU, W>), dim3(qb), dim3(W * 64), 0, stream, a);
+  return (int)hipGetLastError();
+}
+
+template <int DT>
+int forward_any(const AttentionTrainArgs &a, hipStream_t stream) {
+  return a.D <= 64 ? forward<DT, 64, 64>(a, stream) : a.D <= 96 ? forward<DT, 128, 96>(a, stream) : forward<DT, 128, 128>(a, stream);
+}
+template <int DT>
+int backward_any(const AttentionTrainArgs &a, hipStream_t stream) {
+  return a.D <= 64 ? backward<DT, 64, 64>(a, stream) : a.D <= 96 ? backward<DT, 128, 96>(a, stream) : backward<DT, 128, 128>(a, stream);
+}
+
+}  // namespace
+
+int launch_attention_train_forward(const AttentionTrainArgs &a, int dtype, hipStream_t stream) {
+  return dtype == DT_F16 ? forward_any<DT_F16>(a, stream) : forward_any<DT_BF16>(a, stream);
+}
+int launch_attention_train_backward(const AttentionTrainArgs &a, int dtype, hipStream_t stream) {
+  return dtype == DT_F16 ? backward_any<DT_F16>(a, stream) : backward_any<DT_BF16>(a, stream);
+}
+
+}  // namespace tracea_amd

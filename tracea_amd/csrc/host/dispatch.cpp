@@ -17,124 +17,11 @@
 
 #include "tuner.hpp"
 #include "tuning_cache.hpp"
+#include "views.hpp"
 
 namespace tracea_amd {
 
 namespace {
-
-struct View {
-  void *ptr = nullptr;
-  int rank = 0;
-  long long shape[4] = {0, 0, 0, 0};
-  long long stride[4] = {0, 0, 0, 0};
-  int dtype = 0;
-  int device = -1;
-};
-
-// Copies a TraceaTensorView; a NULL stride array means contiguous row-major.
-TraceaStatus read_view(const char *what, const TraceaTensorView &t, int want_rank, View *v) {
-  if (t.ptr == nullptr) return fail(TRACEA_INVALID_PARAMS, "%s: data pointer is NULL", what);
-  if (t.shape == nullptr) return fail(TRACEA_INVALID_PARAMS, "%s: shape pointer is NULL", what);
-  if ((int)t.rank != want_rank)
-    return fail(TRACEA_INVALID_PARAMS, "%s: expected rank %d, got %u", what, want_rank, t.rank);
-  v->ptr = t.ptr;
-  v->rank = (int)t.rank;
-  for (int i = 0; i < want_rank; ++i) v->shape[i] = (long long)t.shape[i];
-  if (t.stride != nullptr) {
-    for (int i = 0; i < want_rank; ++i) v->stride[i] = (long long)t.stride[i];
-  } else {
-    long long s = 1;
-    for (int i = want_rank - 1; i >= 0; --i) {
-      v->stride[i] = s;
-      s *= v->shape[i];
-    }
-  }
-  v->dtype = (int)t.dtype;
-  v->device = t.device_id;
-  return TRACEA_SUCCESS;
-}
-
-bool is_half(int dt) { return dt == TRACEA_DTYPE_FLOAT16 || dt == TRACEA_DTYPE_BFLOAT16; }
-bool is_float_type(int dt) { return dt == TRACEA_DTYPE_FLOAT32 || is_half(dt); }
-int elem_size(int dt) { return dt == TRACEA_DTYPE_FLOAT32 ? 4 : 2; }
-bool aligned(const void *p, size_t a) { return (((uintptr_t)p) & (a - 1)) == 0; }
-
-// Rows of equal length on one pitch, the form of most views: element rows `pitch` apart, `len` elements of each used.
-bool row_form(const View &v, long long *pitch, long long *len) {
-  if (v.rank < 2 || v.stride[v.rank - 1] != 1) return false;
-  // the pitch is the stride of the last dim but one; a [B,H,S,D] view of [B,S,H,D] storage has its heads inside the row
-  *pitch = v.stride[v.rank - 2];
-  *len = v.shape[v.rank - 1];
-  if (*pitch < *len) return false;
-  for (int i = v.rank - 3; i >= 0; --i) {
-    if (v.shape[i] == 1 || v.stride[i] % *pitch == 0) continue;
-    if (v.stride[i] < *len || (*len += (v.shape[i] - 1) * v.stride[i]) > *pitch) return false;
-  }
-  return true;
-}
-
-// Whether two views may share an element (columns of one buffer side by side, a query tensor inside a packed
-// [Q K V] row and the like are told apart).
-bool may_overlap(const View &a, const View &b) {
-  auto span = [](const View &v, uintptr_t *lo, uintptr_t *hi) {
-    long long first = 0, last = 0;
-    for (int i = 0; i < v.rank; ++i) {
-      if (v.shape[i] <= 0) return false;
-      (v.stride[i] < 0 ? first : last) += (v.shape[i] - 1) * v.stride[i];
-    }
-    *lo = (uintptr_t)v.ptr + (uintptr_t)(first * elem_size(v.dtype));
-    *hi = (uintptr_t)v.ptr + (uintptr_t)((last + 1) * elem_size(v.dtype));
-    return true;
-  };
-  uintptr_t alo, ahi, blo, bhi;
-  if (!span(a, &alo, &ahi) || !span(b, &blo, &bhi) || ahi <= blo || bhi <= alo) return false;
-  long long pa, la, pb, lb;
-  if (!row_form(a, &pa, &la) || !row_form(b, &pb, &lb)) return true;
-  pa *= elem_size(a.dtype); la *= elem_size(a.dtype); pb *= elem_size(b.dtype); lb *= elem_size(b.dtype);
-  if (pa != pb) return true;
-  long long d = ((long long)((intptr_t)b.ptr - (intptr_t)a.ptr)) % pa;
-  if (d < 0) d += pa;
-  return d < la || d + lb > pa;
-}
-
-const char *dtype_name(int dt) {
-  switch (dt) {
-    case TRACEA_DTYPE_FLOAT32: return "f32";
-    case TRACEA_DTYPE_FLOAT16: return "f16";
-    case TRACEA_DTYPE_BFLOAT16: return "bf16";
-    case TRACEA_DTYPE_INT32: return "i32";
-    case TRACEA_DTYPE_INT8: return "i8";
-    default: return "?";
-  }
-}
-
-TraceaStatus check_device(const char *what, int device) {
-  if (device < 0)
-    return fail(TRACEA_CPU_ERROR,
-                "%s: host memory (device_id -1) is not supported; this library has no CPU arm",
-                what);
-  if (device >= runtime_device_count())
-    return fail(TRACEA_INVALID_PARAMS, "%s: device_id %d out of range (%d devices)", what, device,
-                runtime_device_count());
-  return TRACEA_SUCCESS;
-}
-
-// Makes `device` current for the lifetime of the object.
-struct DeviceScope {
-  int prev = -1;
-  bool switched = false;
-  hipError_t err = hipSuccess;
-  explicit DeviceScope(int device) {
-    err = hipGetDevice(&prev);
-    if (err == hipSuccess && prev != device) {
-      err = hipSetDevice(device);
-      switched = err == hipSuccess;
-    }
-  }
-  ~DeviceScope() {
-    if (switched) (void)hipSetDevice(prev);
-  }
-};
 
 // ---- epilogue chains ---------------------------------------------------------
 
@@ -295,11 +182,6 @@ std::atomic<bool> g_conv_transpose_by_phase{true};
 thread_local int t_last_contraction = -1, t_last_conv = -1, t_last_attention = -1;
 thread_local int t_last_splits = 1;  // K ranges of the calling thread's latest gemm / conv2d launch
 thread_local int t_last_split_launches = 1;  // kernels that launch took: 2 when a reduction kernel followed
-
-TraceaStatus hip_status(const char *what, int e) {
-  if (e == 0) return TRACEA_SUCCESS;
-  return fail(TRACEA_CUDA_ERROR, "%s: %s", what, hipGetErrorString((hipError_t)e));
-}
 
 }  // namespace
 
@@ -679,10 +561,10 @@ void *splitk_scratch(int device, hipStream_t stream, size_t bytes) {
 // rules: grows on demand up to a cap, never while its stream is being captured, never freed.
 constexpr size_t kPadScratchCap = 1u << 30;
 std::map<std::pair<int, void *>, std::pair<void *, size_t>> g_pad_scratch;
-void *pad_scratch(int device, hipStream_t stream, size_t bytes) {
-  if (bytes > kPadScratchCap) return nullptr;
+std::map<std::pair<int, void *>, std::pair<void *, size_t>> g_train_scratch;  // workspaces of the operators for training
+void *keep_scratch(std::map<std::pair<int, void *>, std::pair<void *, size_t>> &all, int device, hipStream_t stream, size_t bytes) {
   std::lock_guard<std::mutex> lock(g_scratch_mu);
-  auto &slot = g_pad_scratch[{device, (void *)stream}];
+  auto &slot = all[{device, (void *)stream}];
   if (slot.second >= bytes) return slot.first;
   hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
   if (hipStreamIsCapturing(stream, &cap) != hipSuccess || cap != hipStreamCaptureStatusNone) {
@@ -698,6 +580,9 @@ void *pad_scratch(int device, hipStream_t stream, size_t bytes) {
   }
   slot = {p, want};
   return p;
+}
+void *pad_scratch(int device, hipStream_t stream, size_t bytes) {
+  return bytes > kPadScratchCap ? nullptr : keep_scratch(g_pad_scratch, device, stream, bytes);
 }
 
 // Ticket counters of the one-launch split, one per tile, kept per (device, stream) like the scratch
@@ -2993,6 +2878,9 @@ TraceaStatus dispatch_attention(const TraceaTensorView &tq, const TraceaTensorVi
   return hip_status("attention launch",
                     attention_variant(vi).launch(a, q.dtype, (hipStream_t)params.stream));
 }
+
+void *padded_scratch(int device, hipStream_t stream, size_t bytes) { return pad_scratch(device, stream, bytes); }
+void *train_scratch(int device, hipStream_t stream, size_t bytes) { return keep_scratch(g_train_scratch, device, stream, bytes); }
 
 TraceaStatus dispatch_clock_probe(void *out, int32_t samples, int32_t gap, void *stream) {
   if (!runtime_ready()) return fail(TRACEA_UNKNOWN_ERROR, "tracea_init has not been called");

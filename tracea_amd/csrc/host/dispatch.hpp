@@ -110,6 +110,30 @@ TraceaStatus dispatch_attention(const TraceaTensorView &q, const TraceaTensorVie
                                 const TraceaTensorView &v, TraceaTensorView *o,
                                 const TraceaAttentionParams &params);
 
+TraceaStatus dispatch_attention_forward(const TraceaTensorView &q, const TraceaTensorView &k, const TraceaTensorView &v,
+                                        const TraceaTensorView *q_lengths, const TraceaTensorView *k_lengths,
+                                        TraceaTensorView *o, TraceaTensorView *lse, const TraceaAttentionParams &params);
+TraceaStatus dispatch_attention_backward(const TraceaTensorView &q, const TraceaTensorView &k, const TraceaTensorView &v,
+                                         const TraceaTensorView &o, const TraceaTensorView &lse, const TraceaTensorView &d_o,
+                                         const TraceaTensorView *q_lengths, const TraceaTensorView *k_lengths,
+                                         TraceaTensorView *dq, TraceaTensorView *dk, TraceaTensorView *dv,
+                                         const TraceaAttentionParams &params);
+TraceaStatus dispatch_rotary(const TraceaTensorView &q, const TraceaTensorView *k, const TraceaTensorView &positions,
+                             const TraceaTensorView &inv_freq, TraceaTensorView *q_out, TraceaTensorView *k_out,
+                             const TraceaRotaryParams &params);
+TraceaStatus dispatch_norm(const TraceaTensorView &x, const TraceaTensorView *h, const TraceaTensorView *w_post,
+                           const TraceaTensorView *gate, const TraceaTensorView *w_pre, TraceaTensorView *x_out,
+                           TraceaTensorView *y, const TraceaNormParams &params);
+TraceaStatus dispatch_norm_backward(const TraceaTensorView *dx_out, const TraceaTensorView *dy, const TraceaTensorView &x_out,
+                                    const TraceaTensorView *h, const TraceaTensorView *w_post, const TraceaTensorView *gate,
+                                    const TraceaTensorView *w_pre, TraceaTensorView *dx, TraceaTensorView *dh,
+                                    TraceaTensorView *dw_post, TraceaTensorView *dgate, TraceaTensorView *dw_pre,
+                                    const TraceaNormParams &params);
+// Device memory kept per (device, stream): grows on demand, never while the stream is being captured (null then), is never
+// freed.  The first holds padded copies of operands (at most 1 GiB), the second workspaces of the operators for training.
+void *padded_scratch(int device, hipStream_t stream, size_t bytes);
+void *train_scratch(int device, hipStream_t stream, size_t bytes);
+
 // Shader-clock probe (tracea_clock_probe): argument checks, then the one-wave sampling kernel on `stream`.
 TraceaStatus dispatch_clock_probe(void *out, int32_t samples, int32_t gap, void *stream);
 

@@ -1,0 +1,110 @@
+// Rotary positions on several axes, gfx950: pair p of every head of a token is turned by the angle position[axis of p] * freq[p].
+//   (u, v) -> (u cos - v sin, v cos + u sin)      inverse: the angle's other sign (the rotation's transpose, its gradient)
+//
+// Bound by memory: every element is read once and written once.  A thread takes 16 bytes of u and 16 bytes of v of one token
+// through the heads, so that the sine and cosine of a pair, and the position behind them, are worked out once
+// per group of heads instead of once per element.
+#include "contraction_kernel.hpp"
+#include "train.hpp"
+
+namespace tracea_amd {
+
+namespace {
+
+template <typename T, int E>
+struct alignas(sizeof(T) * E) Piece {
+  T x[E];
+};
+
+// The angle is formed and reduced in 64 bits: the product of a 31-bit position and a 24-bit frequency has up to 55 bits,
+// and what counts is its remainder of a whole turn.  32 bits would be off by 2^-24 of the ANGLE: 0.004 rad at position 65536.
+// The sine and cosine of the remainder are fp32.
+__device__ __forceinline__ void turn(int position, float freq, float sign, float &c, float &s) {
+  const double turns = (double)position * (double)freq * 0.15915494309189535;
+  sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
+  s *= sign;
+}
+
+template <typename T, int E, bool ADJ>
+__device__ __forceinline__ void rotate(const T *in, T *out, int at_u, int at_v, const float (&c)[E], const float (&s)[E]) {
+  using P = Piece<T, E>;
+  const P u = *(const P *)(in + at_u), v = *(const P *)(in + at_v);
+  P a, b;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    if constexpr (ADJ && E > 1) {  // pairs side by side: the first half of them in u, the second in v
+      const P &w = e < E / 2 ? u : v;
+      P &r = e < E / 2 ? a : b;
+      const int i = 2 * (e % (E / 2));
+      const float x = (float)w.x[i], y = (float)w.x[i + 1];
+      r.x[i] = (T)(x * c[e] - y * s[e]);
+      r.x[i + 1] = (T)(y * c[e] + x * s[e]);
+    } else {
+      const float x = (float)u.x[e], y = (float)v.x[e];
+      a.x[e] = (T)(x * c[e] - y * s[e]);
+      b.x[e] = (T)(y * c[e] + x * s[e]);
+    }
+  }
+  *(P *)(out + at_u) = a;
+  *(P *)(out + at_v) = b;
+}
+
+template <typename T, int E, bool ADJ>
+__global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
+  using P = Piece<T, E>;
+  // pieces of a token: those with E pairs, then those of the columns that are copied
+  const int turned = a.P / E, all = turned + (a.D - 2 * a.P) / E;
+  const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
+  const long long token = id / all;
+  const int piece = (int)(id - token * all);
+  if (token >= (long long)a.B * a.S) return;
+  const int b = (int)(token / a.S), i = (int)(token - (long long)b * a.S);
+  const int h0 = blockIdx.y * a.heads_per_group, h1 = min(h0 + a.heads_per_group, a.Hq + a.Hk);
+  auto heads = [&](auto &&body) __attribute__((always_inline)) {
+    for (int h = h0; h < h1; ++h) {
+      const bool is_q = h < a.Hq;
+      const HeadView &in = is_q ? a.q : a.k, &out = is_q ? a.q_out : a.k_out;
+      const int hh = is_q ? h : h - a.Hq;
+      body((const T *)in.p + (long long)b * in.sb + (long long)hh * in.sh + (long long)i * in.ss,
+           (T *)out.p + (long long)b * out.sb + (long long)hh * out.sh + (long long)i * out.ss);
+    }
+  };
+  if (piece >= turned) {
+    const int at = 2 * a.P + (piece - turned) * E;
+    heads([&](const T *in, T *out) {
+      if (in != out) *(P *)(out + at) = *(const P *)(in + at);
+    });
+    return;
+  }
+  float c[E], s[E];
+  const int *pos = a.positions + (long long)b * a.pos_sb + (long long)i * a.pos_ss;
+  const float sign = a.inverse ? -1.0f : 1.0f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int p = piece * E + e;
+    int axis = 0;
+    for (int x = 1; x < a.axes; ++x) axis += p >= a.first[x];
+    turn(pos[axis], a.inv_freq[p], sign, c[e], s[e]);
+  }
+  const int at_u = ADJ ? 2 * piece * E : piece * E, at_v = ADJ ? at_u + E : at_u + a.P;
+  heads([&](const T *in, T *out) __attribute__((always_inline)) { rotate<T, E, ADJ>(in, out, at_u, at_v, c, s); });
+}
+
+template <typename T, int E>
+int launch(const RotaryArgs &a, hipStream_t stream) {
+  const long long threads = (long long)a.B * a.S * (a.P / E + (a.D - 2 * a.P) / E);
+  const dim3 grid((unsigned)((threads + 255) / 256), (unsigned)((a.Hq + a.Hk + a.heads_per_group - 1) / a.heads_per_group));
+  if (a.adjacent) hipLaunchKernelGGL((rotary_kernel<T, E, true>), grid, dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((rotary_kernel<T, E, false>), grid, dim3(256), 0, stream, a);
+  return (int)hipGetLastError();
+}
+
+}  // namespace
+
+int launch_rotary(const RotaryArgs &a, int dtype, hipStream_t stream) {
+  if (dtype == DT_F32) return a.vec ? launch<float, 4>(a, stream) : launch<float, 1>(a, stream);
+  if (dtype == DT_F16) return a.vec ? launch<_Float16, 8>(a, stream) : launch<_Float16, 1>(a, stream);
+  return a.vec ? launch<__bf16, 8>(a, stream) : launch<__bf16, 1>(a, stream);
+}
+
+}  // namespace tracea_amd

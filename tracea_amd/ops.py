@@ -336,3 +336,111 @@ def attention(q, k, v, causal=False, scale=0.0, out=None):
     st = capi.lib().tracea_attention(vq.c, vk.c, vv.c, C.byref(vo.c), params)
     capi.check("tracea_attention", st)
     return out
+
+
+_LAYOUTS = {}
+
+
+def _plain_view(t):
+    """capi.TensorView of a tensor, and what it borrows.  The extent and stride arrays are kept by layout (shape and
+    strides), never by a tensor's address."""
+    shape, stride = t.shape, t.stride()
+    arrays = _LAYOUTS.get((shape, stride))
+    if arrays is None:
+        if len(_LAYOUTS) >= 1024:
+            _LAYOUTS.clear()
+        v = capi.View(None, shape, stride, 0, 0)
+        arrays = _LAYOUTS[(shape, stride)] = (v._shape, v._stride)
+    dtype = _DTYPES.get(t.dtype)
+    if dtype is None:
+        raise TypeError("unsupported dtype %s" % t.dtype)
+    return capi.TensorView(t.data_ptr(), len(shape), arrays[0], arrays[1], dtype, t.get_device())
+
+
+def _ref(t):
+    return None if t is None else C.byref(_plain_view(t))
+
+
+def attention_forward(q, k, v, causal=False, scale=0.0, q_lengths=None, k_lengths=None, out=None, lse=None):
+    """(o, lse) of softmax(scale q k^T) v, with lse [B,Hq,Sq] the log-sum-exp of each row's scores, for
+    :func:`attention_backward`.  q [B,Hq,Sq,D], k and v [B,Hk,Sk,D] with Hq a multiple of Hk; q_lengths, k_lengths [B] int32:
+    the queries and keys that each sequence of a padded batch has; causal: the last query sees every key, the one before it all
+    but one, and so on.  scale 0 means 1/sqrt(D).  Rows that see no key: o 0, lse -inf."""
+    if out is None:
+        out = torch.empty_like(q)
+    if lse is None:
+        lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
+    params = capi.AttentionParams(1 if causal else 0, 0, float(scale), _stream(q))
+    st = capi.lib().tracea_attention_forward(_plain_view(q), _plain_view(k), _plain_view(v), _ref(q_lengths), _ref(k_lengths),
+                                             _ref(out), _ref(lse), params)
+    capi.check("tracea_attention_forward", st)
+    return out, lse
+
+
+def attention_backward(q, k, v, o, lse, d_o, causal=False, scale=0.0, q_lengths=None, k_lengths=None, dq=None, dk=None,
+                       dv=None):
+    """(dq, dk, dv) for the gradient d_o of :func:`attention_forward`'s o, from its operands and results."""
+    dq = torch.empty_like(q) if dq is None else dq
+    dk = torch.empty_like(k) if dk is None else dk
+    dv = torch.empty_like(v) if dv is None else dv
+    params = capi.AttentionParams(1 if causal else 0, 0, float(scale), _stream(q))
+    st = capi.lib().tracea_attention_backward(_plain_view(q), _plain_view(k), _plain_view(v), _plain_view(o),
+                                              _plain_view(lse), _plain_view(d_o), _ref(q_lengths), _ref(k_lengths), _ref(dq),
+                                              _ref(dk), _ref(dv), params)
+    capi.check("tracea_attention_backward", st)
+    return dq, dk, dv
+
+
+def rotary(q, k, positions, inv_freq, sections=None, adjacent=False, inverse=False, q_out=None, k_out=None):
+    """(q, k) with every pair of columns turned by positions[..., axis] * inv_freq[pair].  q [B,Hq,S,D], k [B,Hk,S,D] or
+    None; positions [B or 1,S,axes] int32 (or [B or 1,S]: one axis); inv_freq [P] float32, P <= D/2; sections: pairs of
+    each axis, together P (default: one axis).  Pair p is columns p and p + P, or 2p and 2p + 1 with ``adjacent``; columns from 2P
+    on stay.  ``inverse`` turns back, which is the gradient: rotary(dq, dk, ..., inverse=True).  q_out may be q, k_out k."""
+    if positions.dim() == 2:
+        positions = positions.unsqueeze(-1)
+    sections = [inv_freq.shape[0]] if sections is None else list(sections)
+    if len(sections) > capi.MAX_ROTARY_AXES or any(n < 0 for n in sections):
+        raise ValueError("sections: the pairs of 1 to %d axes, got %r" % (capi.MAX_ROTARY_AXES, sections))
+    q_out = torch.empty_like(q) if q_out is None else q_out
+    if k is not None:
+        k_out = torch.empty_like(k) if k_out is None else k_out
+    params = capi.RotaryParams(len(sections), (C.c_uint32 * capi.MAX_ROTARY_AXES)(*sections), 1 if adjacent else 0,
+                               1 if inverse else 0, _stream(q))
+    st = capi.lib().tracea_rotary(_plain_view(q), _ref(k), _plain_view(positions), _plain_view(inv_freq), _ref(q_out),
+                                  _ref(k_out), params)
+    capi.check("tracea_rotary", st)
+    return q_out, k_out
+
+
+def norm_gate_residual(x, h=None, w_post=None, gate=None, w_pre=None, residual_scale=1.0, eps=1e-6, x_out=None, y=None):
+    """(x_out, y) of the sum between two blocks: x_out = residual_scale x + gate norm(h) w_post, y = norm(x_out) w_pre, with
+    norm(t) = t / sqrt(mean(t^2) + eps) over the channels.  x, h [B,T,C]; w_post, w_pre [C], gate [1,C] or [B,C], float32.
+    Without h (a network's first norm) x_out is x; without w_pre (behind its last block) y is None."""
+    if h is not None:
+        x_out = torch.empty_like(x) if x_out is None else x_out
+    if w_pre is not None:
+        y = torch.empty_like(x) if y is None else y
+    params = capi.NormParams(float(eps), float(residual_scale), _stream(x))
+    st = capi.lib().tracea_norm_gate_residual(_plain_view(x), _ref(h), _ref(w_post), _ref(gate), _ref(w_pre), _ref(x_out),
+                                              _ref(y), params)
+    capi.check("tracea_norm_gate_residual", st)
+    return (x if h is None else x_out), y
+
+
+def norm_gate_residual_backward(dx_out, dy, x_out, h=None, w_post=None, gate=None, w_pre=None, residual_scale=1.0, eps=1e-6,
+                                dx=None, dh=None):
+    """(dx, dh, dw_post, dgate, dw_pre) for the gradients dx_out (None: zero) and dy of :func:`norm_gate_residual`'s results, from
+    its x_out (x where there is no h) and h; None for what the call has not."""
+    f32 = dict(dtype=torch.float32, device=x_out.device)
+    dx = torch.empty_like(x_out) if dx is None else dx
+    if h is not None:
+        dh = torch.empty_like(h) if dh is None else dh
+    dw_post = None if w_post is None else torch.empty(w_post.shape, **f32)
+    dgate = None if gate is None else torch.empty(gate.shape, **f32)
+    dw_pre = None if w_pre is None else torch.empty(w_pre.shape, **f32)
+    params = capi.NormParams(float(eps), float(residual_scale), _stream(x_out))
+    st = capi.lib().tracea_norm_gate_residual_backward(_ref(dx_out), _ref(dy), _plain_view(x_out), _ref(h), _ref(w_post),
+                                                       _ref(gate), _ref(w_pre), _ref(dx), _ref(dh), _ref(dw_post),
+                                                       _ref(dgate), _ref(dw_pre), params)
+    capi.check("tracea_norm_gate_residual_backward", st)
+    return dx, dh, dw_post, dgate, dw_pre
