@@ -95,9 +95,10 @@ __device__ __forceinline__ u32x4 resource(const void *base, unsigned bytes) {
   return u32x4{(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)at),
                (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(at >> 32)) & 0xffffu, bytes, 0x00020000u};
 }
-__device__ __forceinline__ unsigned lds_address(const void *p) {
-  return (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(unsigned long long)(__attribute__((address_space(3))) const void *)p);
+__device__ __forceinline__ unsigned lds_offset(const void *p) {
+  return (unsigned)(unsigned long long)(__attribute__((address_space(3))) const void *)p;
 }
+__device__ __forceinline__ unsigned lds_address(const void *p) { return (unsigned)__builtin_amdgcn_readfirstlane((int)lds_offset(p)); }
 
 // Requests 64 rows of a tensor into LDS (16 bytes per lane, 1 KB per wave and request).  offset(row) is the byte offset
 // of a row from `base`, below 2^31, or BEYOND for a row that reads as zeros; columns from D on read as zeros too.
@@ -118,27 +119,45 @@ __device__ __forceinline__ void load_tile(const void *base, const unsigned char 
   }
 }
 
+// Where a lane reads a tile, as LDS addresses: everything but the constant part of a fragment's place, which is XOR-ed in (it
+// shares no bit with the row, and the bits that it shares with the swizzle are what the swizzle is for).
+template <int DL>
+__device__ __forceinline__ unsigned rows_base(const unsigned char *tile, int r16, int g4) {
+  using T = Tile<DL>;
+  return lds_offset(tile) + (unsigned)(r16 * T::ROW_BYTES + ((g4 ^ T::swz(r16)) << 4));
+}
+template <int DL>
+__device__ __forceinline__ unsigned columns_base(const unsigned char *tile, int r16, int g4) {
+  using T = Tile<DL>;
+  const int row = g4 * 4 + (r16 >> 2);
+  return lds_offset(tile) + (unsigned)(row * T::ROW_BYTES + ((((r16 & 3) >> 1) ^ T::swz(row)) << 4) + (r16 & 1) * 8);
+}
+typedef __attribute__((address_space(3))) const u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 // First operand of a product over the head dimension: rows 16 rb .. + 15 of the tile, columns 32 ks .. + 31.
 template <int DL>
-__device__ __forceinline__ u32x4 read_rows(const unsigned char *tile, int rb, int ks, int r16, int g4) {
-  using T = Tile<DL>;
-  return *(const u32x4 *)(tile + rb * 16 * T::ROW_BYTES + r16 * T::ROW_BYTES + (((ks * 4 + g4) ^ T::swz(r16)) << 4));
+__device__ __forceinline__ u32x4 read_rows(unsigned base, unsigned side, int rb, int ks) {
+  return *(lds_u32x4 *)(uintptr_t)((base ^ (unsigned)(ks << 6)) + side + (unsigned)(rb * 16 * Tile<DL>::ROW_BYTES));
 }
 // First operand of a product over the rows 32 s .. + 31: columns 16 db .. + 15 of the tile, transposed.
 template <int DL>
-__device__ __forceinline__ u32x4 read_columns(const unsigned char *tile, int s, int db, int r16, int g4) {
-  using T = Tile<DL>;
-  const int row = g4 * 4 + (r16 >> 2);
-  const int at = row * T::ROW_BYTES + (((((r16 & 3) >> 1) ^ T::swz(row)) ^ (db << 1)) << 4) + (r16 & 1) * 8;
-  const unsigned char *p = tile + s * 32 * T::ROW_BYTES + at;
-  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p);
-  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(p + 16 * T::ROW_BYTES));
+__device__ __forceinline__ u32x4 read_columns(unsigned base, unsigned side, int s, int db) {
+  const unsigned at = (base ^ (unsigned)(db << 5)) + side + (unsigned)(s * 32 * Tile<DL>::ROW_BYTES);
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(uintptr_t)at);
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(uintptr_t)(at + 16 * Tile<DL>::ROW_BYTES));
   const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
   return u32x4{a[0], a[1], b[0], b[1]};
 }
 
 // Nothing is scheduled across: the compiler otherwise hoists the reads of several phases and runs out of registers.
 __device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
+
+// A value that the compiler takes for a new one: what follows from it is worked out again where it is used, in an instruction
+// or two, instead of being held in registers all through a loop that has none to spare.
+__device__ __forceinline__ unsigned fresh(unsigned x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
 
 // max / sum over the four 16-lane groups
 __device__ __forceinline__ float groups_max(float x) {
@@ -204,12 +223,11 @@ __device__ __forceinline__ float ds_scale(const AttentionTrainArgs &a, int bh, i
     mv = fmaxf(mv, __shfl_xor(mv, m, 64));
   }
   const float bound = 2.0f * sqrtf(mo) * sqrtf(mv);
-  if (!(bound > 0.0f) || !(bound < 3.0e38f)) return 1.0f;
-  int e;
-  (void)frexpf(bound, &e);  // bound < 2^e
+  int e = 14;
+  if (bound > 0.0f && bound < 3.0e38f) (void)frexpf(bound, &e);  // bound < 2^e
   e = 14 - e;
   e = e < -100 ? -100 : e > 100 ? 100 : e;
-  return __builtin_bit_cast(float, (unsigned)(127 + e) << 23);
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane((127 + e) << 23));
 }
 
 // ---- forward --------------------------------------------------------------------------------------------------
@@ -223,7 +241,8 @@ __global__ void __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu
 attention_train_forward_kernel(const AttentionTrainArgs a) {
   using T = Tile<DL>;
   constexpr int BR = 32 * WAVES, KS = DU / 32, DB = DU / 16, KB = TILE / 16;
-  __shared__ __attribute__((aligned(1024))) unsigned char sK[2 * T::BYTES], sV[2 * T::BYTES];
+  __shared__ __attribute__((aligned(1024))) unsigned char sK[4 * T::BYTES];  // two tiles of K, two of V
+  constexpr unsigned V_AT = 2 * T::BYTES;
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, g4 = lane >> 4;
@@ -271,7 +290,7 @@ attention_train_forward_kernel(const AttentionTrainArgs a) {
     const int left = w.lk - t * TILE, at = (t & 1) * T::BYTES;
     const unsigned kss = (unsigned)a.k.ss * 2u, vss = (unsigned)a.v.ss * 2u;
     load_tile<DL, WAVES>(Kg + (long long)t * TILE * a.k.ss, sK + at, a.D, lane, wave, [&](int row) { return row < left ? row * kss : BEYOND; });
-    load_tile<DL, WAVES>(Vg + (long long)t * TILE * a.v.ss, sV + at, a.D, lane, wave, [&](int row) { return row < left ? row * vss : BEYOND; });
+    load_tile<DL, WAVES>(Vg + (long long)t * TILE * a.v.ss, sK + V_AT + at, a.D, lane, wave, [&](int row) { return row < left ? row * vss : BEYOND; });
   };
 
   f32x4 o[2][DB];
@@ -281,9 +300,10 @@ attention_train_forward_kernel(const AttentionTrainArgs a) {
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[qb][d] = f32x4{0, 0, 0, 0};
 
+  const unsigned rows0 = rows_base<DL>(sK, r16, g4), cols0 = columns_base<DL>(sK, r16, g4);
   auto compute = [&](int t, auto edge_tag) __attribute__((always_inline)) {
     constexpr bool EDGE = decltype(edge_tag)::value;
-    const unsigned char *tK = sK + (t & 1) * T::BYTES, *tV = sV + (t & 1) * T::BYTES;
+    const unsigned rows_at = rows0 + (unsigned)(t & 1) * T::BYTES, cols_at = cols0 + (unsigned)(t & 1) * T::BYTES;
     f32x4 z[2][KB];
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
@@ -293,7 +313,7 @@ attention_train_forward_kernel(const AttentionTrainArgs a) {
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
-        const u32x4 kf = read_rows<DL>(tK, kb, ks, r16, g4);
+        const u32x4 kf = read_rows<DL>(rows_at, 0, kb, ks);
 #pragma unroll
         for (int qb = 0; qb < 2; ++qb) z[qb][kb] = Mfma16<DT>::run(kf, qf[qb][ks], z[qb][kb]);
       }
@@ -346,7 +366,7 @@ attention_train_forward_kernel(const AttentionTrainArgs a) {
     for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int d = 0; d < DB; ++d) {
-        const u32x4 vf = read_columns<DL>(tV, s, d, r16, g4);
+        const u32x4 vf = read_columns<DL>(cols_at, V_AT, s, d);
 #pragma unroll
         for (int qb = 0; qb < 2; ++qb) o[qb][d] = Mfma16<DT>::run(vf, pf[qb][s], o[qb][d]);
       }
@@ -495,7 +515,8 @@ __global__ void __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu
 attention_train_dq_kernel(const AttentionTrainArgs a) {
   using T = Tile<DL>;
   constexpr int BR = 32 * WAVES, KS = DU / 32, DB = DU / 16;
-  __shared__ __attribute__((aligned(1024))) unsigned char sK[2 * T::BYTES], sV[2 * T::BYTES];
+  __shared__ __attribute__((aligned(1024))) unsigned char sK[4 * T::BYTES];  // two tiles of K, two of V
+  constexpr unsigned V_AT = 2 * T::BYTES;
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, g4 = lane >> 4;
@@ -518,6 +539,8 @@ attention_train_dq_kernel(const AttentionTrainArgs a) {
     const int r = r_wave + qb * 16 + r16;
     const bool there = r < rows;
     q_last[qb] = !there ? -1 : a.causal ? min(w.lk - 1, query_of(a, r) + w.off) : w.lk - 1;
+    // (a row that sees one key has P = 1 whatever the score: no gradient, not the rounding of O in delta)
+    if (q_last[qb] == 0) q_last[qb] = -1;
     const unsigned short *p = (const unsigned short *)a.q.p + (there ? row_at(a, a.q, w, r) : 0);
     const unsigned short *g = (const unsigned short *)a.d_o.p + (there ? row_at(a, a.d_o, w, r) : 0);
     nl[qb] = there ? a.neg_lse2[(long long)bh * a.rows_pad + r] : -INFINITY;
@@ -546,7 +569,7 @@ attention_train_dq_kernel(const AttentionTrainArgs a) {
     const int left = w.lk - t * TILE, at = (t & 1) * T::BYTES;
     const unsigned kss = (unsigned)a.k.ss * 2u, vss = (unsigned)a.v.ss * 2u;
     load_tile<DL, WAVES>(Kg + (long long)t * TILE * a.k.ss, sK + at, a.D, lane, wave, [&](int row) { return row < left ? row * kss : BEYOND; });
-    load_tile<DL, WAVES>(Vg + (long long)t * TILE * a.v.ss, sV + at, a.D, lane, wave, [&](int row) { return row < left ? row * vss : BEYOND; });
+    load_tile<DL, WAVES>(Vg + (long long)t * TILE * a.v.ss, sK + V_AT + at, a.D, lane, wave, [&](int row) { return row < left ? row * vss : BEYOND; });
   };
 
   f32x4 acc[2][DB];
@@ -555,9 +578,10 @@ attention_train_dq_kernel(const AttentionTrainArgs a) {
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[qb][d] = f32x4{0, 0, 0, 0};
 
+  const unsigned rows0 = rows_base<DL>(sK, r16, g4), cols0 = columns_base<DL>(sK, r16, g4);
   auto compute = [&](int t, auto edge_tag) __attribute__((always_inline)) {
     constexpr bool EDGE = decltype(edge_tag)::value;
-    const unsigned char *tK = sK + (t & 1) * T::BYTES, *tV = sV + (t & 1) * T::BYTES;
+    const unsigned rows_at = rows0 + (unsigned)(t & 1) * T::BYTES, cols_at = cols0 + (unsigned)(t & 1) * T::BYTES;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       f32x4 z[2][2], g[2][2];  // [qb][block of 16 keys]
@@ -572,7 +596,7 @@ attention_train_dq_kernel(const AttentionTrainArgs a) {
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
-          const u32x4 kf = read_rows<DL>(tK, 2 * s + kb, ks, r16, g4);
+          const u32x4 kf = read_rows<DL>(rows_at, 0, 2 * s + kb, ks);
 #pragma unroll
           for (int qb = 0; qb < 2; ++qb) z[qb][kb] = Mfma16<DT>::run(kf, qf[qb][ks], z[qb][kb]);
         }
@@ -581,7 +605,7 @@ attention_train_dq_kernel(const AttentionTrainArgs a) {
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
-          const u32x4 vf = read_rows<DL>(tV, 2 * s + kb, ks, r16, g4);
+          const u32x4 vf = read_rows<DL>(rows_at, V_AT, 2 * s + kb, ks);
 #pragma unroll
           for (int qb = 0; qb < 2; ++qb) g[qb][kb] = Mfma16<DT>::run(vf, of[qb][ks], g[qb][kb]);
         }
@@ -594,8 +618,7 @@ attention_train_dq_kernel(const AttentionTrainArgs a) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z[qb][kb][e], a.scale_log2, nl[qb]));
-            // (a row that sees one key has P = 1 whatever the score: no gradient, not the rounding of O in delta)
-            if constexpr (EDGE) p = t * TILE + s * 32 + kb * 16 + g4 * 4 + e > q_last[qb] || q_last[qb] == 0 ? 0.0f : p;
+            if constexpr (EDGE) p = t * TILE + s * 32 + kb * 16 + g4 * 4 + e > q_last[qb] ? 0.0f : p;
             if constexpr (DT == DT_F16) p *= dsp;
             z[qb][kb][e] = p * g[qb][kb][e];
           }
@@ -604,7 +627,7 @@ attention_train_dq_kernel(const AttentionTrainArgs a) {
       fence();
 #pragma unroll
       for (int d = 0; d < DB; ++d) {
-        const u32x4 kf = read_columns<DL>(tK, s, d, r16, g4);
+        const u32x4 kf = read_columns<DL>(cols_at, 0, s, d);
 #pragma unroll
         for (int qb = 0; qb < 2; ++qb) acc[qb][d] = Mfma16<DT>::run(kf, df[qb], acc[qb][d]);
       }
@@ -641,11 +664,12 @@ attention_train_dq_kernel(const AttentionTrainArgs a) {
 }
 
 template <int DT, int DL, int DU, int WAVES>
-__global__ void __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(DU == 128 ? 1 : 2, DU == 128 ? 1 : 2)))
+__global__ void __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 attention_train_dkv_kernel(const AttentionTrainArgs a) {
   using T = Tile<DL>;
   constexpr int BC = 32 * WAVES, KS = DU / 32, DB = DU / 16;
-  __shared__ __attribute__((aligned(1024))) unsigned char sQ[2 * T::BYTES], sO[2 * T::BYTES];
+  __shared__ __attribute__((aligned(1024))) unsigned char sQ[4 * T::BYTES];  // two tiles of Q, two of dO
+  constexpr unsigned O_AT = 2 * T::BYTES;
   __shared__ __attribute__((aligned(16))) float sL[2 * TILE], sD[2 * TILE];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -684,6 +708,10 @@ attention_train_dkv_kernel(const AttentionTrainArgs a) {
     row_all = (long long)max(0, k_wave + 31 - w.off) * a.G;
   }
   if (w.lk == 1) row_all = 0x7fffffff;
+  // The first packed row that sees the lane's key of block 0 (block 1: first_step further); and the first row that sees more than
+  // one key: a row that sees one has P = 1 whatever the score, and no gradient (not the rounding of O in delta).
+  const int first_row = a.causal ? (k_wave + r16 - w.off) * a.G : 0, first_step = a.causal ? 16 * a.G : 0;
+  const int two_keys = w.lk == 1 ? 0x7fffffff : a.causal ? (1 - w.off) * a.G : 0;
   float dsc = 1.0f, dsp = 1.0f;
   if constexpr (DT == DT_F16) {
     dsc = ds_scale(a, bh, lane);
@@ -693,13 +721,13 @@ attention_train_dkv_kernel(const AttentionTrainArgs a) {
   const unsigned short *Qg = slice(a.q, w.b, w.hk * a.G), *Og = slice(a.d_o, w.b, w.hk * a.G);
   const float *nl = a.neg_lse2 + (long long)bh * a.rows_pad, *nd = a.neg_delta + (long long)bh * a.rows_pad;
   auto request = [&](int t) __attribute__((always_inline)) {
-    const int r0 = t * TILE, i0 = query_of(a, r0), at = (t & 1) * T::BYTES;
+    const int r0 = t * TILE, i0 = query_of(a, r0), at = (t & 1) * T::BYTES, lane_ = fresh(lane);
     auto offset = [&](const HeadView &v, int row) __attribute__((always_inline)) -> unsigned {
       const int r = r0 + row, i = query_of(a, r);
       return r < rows ? (unsigned)(i - i0) * ((unsigned)v.ss * 2u) + (unsigned)(r - i * a.G) * ((unsigned)v.sh * 2u) : BEYOND;
     };
-    load_tile<DL, WAVES>(Qg + (long long)i0 * a.q.ss, sQ + at, a.D, lane, wave, [&](int row) { return offset(a.q, row); });
-    load_tile<DL, WAVES>(Og + (long long)i0 * a.d_o.ss, sO + at, a.D, lane, wave, [&](int row) { return offset(a.d_o, row); });
+    load_tile<DL, WAVES>(Qg + (long long)i0 * a.q.ss, sQ + at, a.D, lane_, wave, [&](int row) { return offset(a.q, row); });
+    load_tile<DL, WAVES>(Og + (long long)i0 * a.d_o.ss, sQ + O_AT + at, a.D, lane_, wave, [&](int row) { return offset(a.d_o, row); });
     if (wave < 2) {  // (rows_pad is a multiple of the tile)
       dma4(resource((wave == 0 ? nl : nd) + r0, TILE * 4), lane * 4, lds_address((wave == 0 ? sL : sD) + (t & 1) * TILE));
     }
@@ -711,13 +739,15 @@ attention_train_dkv_kernel(const AttentionTrainArgs a) {
 #pragma unroll
     for (int d = 0; d < DB; ++d) dk[nb][d] = dv[nb][d] = f32x4{0, 0, 0, 0};
 
+  const unsigned rows0 = rows_base<DL>(sQ, r16, g4), cols0 = columns_base<DL>(sQ, r16, g4);
   auto compute = [&](int t, auto edge_tag) __attribute__((always_inline)) {
     constexpr bool EDGE = decltype(edge_tag)::value;
-    const unsigned char *tQ = sQ + (t & 1) * T::BYTES, *tO = sO + (t & 1) * T::BYTES;
+    const unsigned rows_at = rows0 + (unsigned)(t & 1) * T::BYTES, cols_at = cols0 + (unsigned)(t & 1) * T::BYTES;
     const float *tL = sL + (t & 1) * TILE, *tD = sD + (t & 1) * TILE;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       f32x4 z[2][2], g[2][2];  // [block of 16 rows][nb]
+      const unsigned at_s = fresh(rows_at);
 #pragma unroll
       for (int rb = 0; rb < 2; ++rb)
 #pragma unroll
@@ -726,7 +756,7 @@ attention_train_dkv_kernel(const AttentionTrainArgs a) {
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int rb = 0; rb < 2; ++rb) {
-          const u32x4 qf = read_rows<DL>(tQ, 2 * s + rb, ks, r16, g4);
+          const u32x4 qf = read_rows<DL>(at_s, 0, 2 * s + rb, ks);
 #pragma unroll
           for (int nb = 0; nb < 2; ++nb) z[rb][nb] = Mfma16<DT>::run(qf, kf[nb][ks], z[rb][nb]);
         }
@@ -739,10 +769,7 @@ attention_train_dkv_kernel(const AttentionTrainArgs a) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z[rb][nb][e], a.scale_log2, l4[e]));
-            if constexpr (EDGE) {
-              const int i = query_of(a, t * TILE + s * 32 + rb * 16 + g4 * 4 + e);
-              p = a.causal && k_wave + nb * 16 + r16 > i + w.off ? 0.0f : p;
-            }
+            if constexpr (EDGE) p = t * TILE + s * 32 + rb * 16 + g4 * 4 + e < (int)fresh(first_row) + nb * first_step ? 0.0f : p;
             z[rb][nb][e] = p;
           }
       }
@@ -750,11 +777,13 @@ attention_train_dkv_kernel(const AttentionTrainArgs a) {
 #pragma unroll
       for (int nb = 0; nb < 2; ++nb) pf[nb] = pack_operand<DT>(z[0][nb], z[1][nb]);
       fence();
+      const unsigned at_v = fresh(cols_at);
 #pragma unroll
       for (int d = 0; d < DB; ++d) {
-        const u32x4 of = read_columns<DL>(tO, s, d, r16, g4);
+        const u32x4 of = read_columns<DL>(at_v, O_AT, s, d);
 #pragma unroll
         for (int nb = 0; nb < 2; ++nb) dv[nb][d] = Mfma16<DT>::run(of, pf[nb], dv[nb][d]);
+        if (d == DB / 2) fence();
       }
       fence();
 #pragma unroll
@@ -762,13 +791,15 @@ attention_train_dkv_kernel(const AttentionTrainArgs a) {
         const f32x4 d4 = *(const f32x4 *)(tD + s * 32 + rb * 16 + g4 * 4);
         g[rb][0] = g[rb][1] = d4;
       }
+      const unsigned at_p = fresh(rows_at);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int rb = 0; rb < 2; ++rb) {
-          const u32x4 of = read_rows<DL>(tO, 2 * s + rb, ks, r16, g4);
+          const u32x4 of = read_rows<DL>(at_p, O_AT, 2 * s + rb, ks);
 #pragma unroll
           for (int nb = 0; nb < 2; ++nb) g[rb][nb] = Mfma16<DT>::run(of, vf[nb][ks], g[rb][nb]);
+          if (ks == KS / 2 && rb == 0) fence();
         }
 #pragma unroll
       for (int rb = 0; rb < 2; ++rb)
@@ -778,18 +809,16 @@ attention_train_dkv_kernel(const AttentionTrainArgs a) {
           for (int e = 0; e < 4; ++e) {
             float x = z[rb][nb][e] * g[rb][nb][e];
             if constexpr (DT == DT_F16) x *= dsp;
-            if constexpr (EDGE) {  // (a row that sees one key has P = 1 whatever the score)
-              const int i = query_of(a, t * TILE + s * 32 + rb * 16 + g4 * 4 + e);
-              x = w.lk == 1 || (a.causal && i + w.off == 0) ? 0.0f : x;
-            }
+            if constexpr (EDGE) x = t * TILE + s * 32 + rb * 16 + g4 * 4 + e < max((int)fresh(first_row) + nb * first_step, two_keys) ? 0.0f : x;
             z[rb][nb][e] = x;
           }
 #pragma unroll
       for (int nb = 0; nb < 2; ++nb) pf[nb] = pack_operand<DT>(z[0][nb], z[1][nb]);
       fence();
+      const unsigned at_k = fresh(cols_at);
 #pragma unroll
       for (int d = 0; d < DB; ++d) {
-        const u32x4 qf = read_columns<DL>(tQ, s, d, r16, g4);
+        const u32x4 qf = read_columns<DL>(at_k, 0, s, d);
 #pragma unroll
         for (int nb = 0; nb < 2; ++nb) dk[nb][d] = Mfma16<DT>::run(qf, pf[nb], dk[nb][d]);
       }
