@@ -175,6 +175,22 @@ __device__ __forceinline__ int xcd_run(int id, int total) {
   return x * q + (x < rem ? x : rem) + i;
 }
 
+// The block and the (batch, key/value head) of workgroup `id` of blocks * B * Hk, blocks numbered from the one with most work.
+// Dense: an XCD has a run of them.  Causal: the heaviest blocks of all heads first; a head stays on one XCD where their number is a
+// multiple of 8.  With lengths a head's blocks go round the XCDs, which otherwise would get sequences of unequal lengths.
+struct Slot {
+  int blk, bh;
+};
+__device__ __forceinline__ Slot slot_of(const AttentionTrainArgs &a, int id, int blocks) {
+  const int heads = a.B * a.Hk;
+  if (a.order == 0) {
+    const int vid = xcd_run(id, heads * blocks), bh = vid / blocks;
+    return {vid - bh * blocks, bh};
+  }
+  const int blk = id / heads, bh = id - blk * heads;
+  return {blk, a.order == 1 ? bh : (bh + blk) % heads};
+}
+
 struct Rows {  // of one batch entry and key/value head
   int b, hk, lq, lk, off;  // lengths; a causal row of query i sees keys up to i + off
 };
@@ -204,6 +220,22 @@ __device__ __forceinline__ const unsigned short *slice(const HeadView &t, int b,
 __device__ __forceinline__ u32x4 resident(const unsigned short *row, bool there, int col, int D) {
   u32x4 z = {0, 0, 0, 0};
   return there && col < D ? *(const u32x4 *)(row + col) : z;
+}
+
+// Adds the accumulators of the second of two waves that share columns to the first's, through LDS (the tiles are done with).
+template <int N, typename F>
+__device__ __forceinline__ void join_halves(unsigned char *lds, int group, int half, int lane, F &&acc) {
+  f32x4 *at = (f32x4 *)lds + group * N * 64 + lane;
+  __syncthreads();
+  if (half == 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) at[i * 64] = acc(i);
+  }
+  __syncthreads();
+  if (half == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc(i) += at[i * 64];
+  }
 }
 
 // The power of two that dS is multiplied by before it becomes an f16 operand: |dP - delta| <= 2 max|dO| max|V|
@@ -247,8 +279,8 @@ attention_train_forward_kernel(const AttentionTrainArgs a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, g4 = lane >> 4;
   const int blocks = (a.G * a.Sq + BR - 1) / BR;
-  const int vid = xcd_run(blockIdx.x, gridDim.x);
-  const int bh = vid / blocks, blk = blocks - 1 - (vid - bh * blocks);  // most keys under a causal mask first
+  const Slot slot = slot_of(a, blockIdx.x, blocks);
+  const int bh = slot.bh, blk = blocks - 1 - slot.blk;  // most keys under a causal mask first
   const Rows w = rows_of(a, bh);
   const int rows = a.G * w.lq;
   const int r_wave = blk * BR + wave * 32;
@@ -510,22 +542,21 @@ __global__ void __launch_bounds__(256) attention_train_rows_kernel(const Attenti
   }
 }
 
-template <int DT, int DL, int DU, int WAVES>
-__global__ void __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
-attention_train_dq_kernel(const AttentionTrainArgs a) {
+// dQ of a block of packed rows.  SG = 2: two waves share 32 rows, each takes half of every tile of keys.
+template <int DT, int DL, int DU, int WAVES, int SG>
+__device__ __forceinline__ void dq_block(const AttentionTrainArgs &a, int id, unsigned char *sK) {
   using T = Tile<DL>;
-  constexpr int BR = 32 * WAVES, KS = DU / 32, DB = DU / 16;
-  __shared__ __attribute__((aligned(1024))) unsigned char sK[4 * T::BYTES];  // two tiles of K, two of V
-  constexpr unsigned V_AT = 2 * T::BYTES;
+  constexpr int BR = 32 * WAVES / SG, KS = DU / 32, DB = DU / 16;
+  constexpr unsigned V_AT = 2 * T::BYTES;  // two tiles of K, two of V
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int r16 = lane & 15, g4 = lane >> 4;
+  const int r16 = lane & 15, g4 = lane >> 4, group = wave / SG, half = wave % SG;
   const int blocks = (a.G * a.Sq + BR - 1) / BR;
-  const int vid = xcd_run(blockIdx.x, gridDim.x);
-  const int bh = vid / blocks, blk = blocks - 1 - (vid - bh * blocks);
+  const Slot slot = slot_of(a, id, blocks);
+  const int bh = slot.bh, blk = blocks - 1 - slot.blk;
   const Rows w = rows_of(a, bh);
   const int rows = a.G * w.lq;
-  const int r_wave = blk * BR + wave * 32;
+  const int r_wave = blk * BR + group * 32;
   const int last_row = min(blk * BR + BR, rows) - 1;
   int keys = 0;
   if (last_row >= blk * BR) keys = a.causal ? min(w.lk, query_of(a, last_row) + w.off + 1) : w.lk;
@@ -583,7 +614,8 @@ attention_train_dq_kernel(const AttentionTrainArgs a) {
     constexpr bool EDGE = decltype(edge_tag)::value;
     const unsigned rows_at = rows0 + (unsigned)(t & 1) * T::BYTES, cols_at = cols0 + (unsigned)(t & 1) * T::BYTES;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
+    for (int n = 0; n < 2 / SG; ++n) {
+      const int s = SG == 1 ? n : half;
       f32x4 z[2][2], g[2][2];  // [qb][block of 16 keys]
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
@@ -651,6 +683,8 @@ attention_train_dq_kernel(const AttentionTrainArgs a) {
     if (t * TILE < wave_keys) compute(t, std::true_type{});
   }
 
+  if constexpr (SG == 2) join_halves<2 * DB>(sK, group, half, lane, [&](int i) -> f32x4 & { return acc[i / DB][i % DB]; });
+  if (half != 0) return;
   const float f = (a.negate ? -a.scale : a.scale) / dsc;
 #pragma unroll
   for (int qb = 0; qb < 2; ++qb) {
@@ -663,28 +697,31 @@ attention_train_dq_kernel(const AttentionTrainArgs a) {
   }
 }
 
-template <int DT, int DL, int DU, int WAVES>
-__global__ void __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
-attention_train_dkv_kernel(const AttentionTrainArgs a) {
+// dK and dV of a block of keys, or of a part of the rows that see them.  SG = 2: two waves share 32 keys, each takes half of
+// every tile of rows.
+template <int DT, int DL, int DU, int WAVES, int SG>
+__device__ __forceinline__ void dkv_block(const AttentionTrainArgs &a, int id, unsigned char *sQ, float *sL, float *sD) {
   using T = Tile<DL>;
-  constexpr int BC = 32 * WAVES, KS = DU / 32, DB = DU / 16;
-  __shared__ __attribute__((aligned(1024))) unsigned char sQ[4 * T::BYTES];  // two tiles of Q, two of dO
-  constexpr unsigned O_AT = 2 * T::BYTES;
-  __shared__ __attribute__((aligned(16))) float sL[2 * TILE], sD[2 * TILE];
+  constexpr int BC = 32 * WAVES / SG, KS = DU / 32, DB = DU / 16;
+  constexpr unsigned O_AT = 2 * T::BYTES;  // two tiles of Q, two of dO
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int r16 = lane & 15, g4 = lane >> 4;
+  const int r16 = lane & 15, g4 = lane >> 4, group = wave / SG, half = wave % SG;
   const int blocks = (a.Sk + BC - 1) / BC;
-  const int vid = xcd_run(blockIdx.x, gridDim.x);
-  const int bh = vid / blocks, blk = vid - bh * blocks;  // (under a causal mask the first keys have most rows)
+  const Slot slot = slot_of(a, id, blocks * a.row_splits);
+  const int bh = slot.bh, blk = slot.blk / a.row_splits, part = slot.blk - blk * a.row_splits;  // (causal: the first keys have most rows)
   const Rows w = rows_of(a, bh);
   const int rows = a.G * w.lq;
-  const int k_blk = blk * BC, k_wave = k_blk + wave * 32;
+  const int k_blk = blk * BC, k_wave = k_blk + group * 32;
 
   // tiles of packed rows that see a key of the block, from the first one on
-  int t_begin = 0;
-  const int t_end = k_blk < w.lk ? (rows + TILE - 1) / TILE : 0;
-  if (a.causal) t_begin = (int)(((long long)max(0, k_blk - w.off) * a.G) / TILE);
+  int t_begin = a.causal ? (int)(((long long)max(0, k_blk - w.off) * a.G) / TILE) : 0;
+  int t_end = k_blk < w.lk ? (rows + TILE - 1) / TILE : 0;
+  if (a.row_splits > 1) {
+    const int n = max(0, t_end - t_begin), from = t_begin;
+    t_begin = from + n * part / a.row_splits;
+    t_end = from + n * (part + 1) / a.row_splits;
+  }
 
   u32x4 kf[2][KS], vf[2][KS];
 #pragma unroll
@@ -745,7 +782,8 @@ attention_train_dkv_kernel(const AttentionTrainArgs a) {
     const unsigned rows_at = rows0 + (unsigned)(t & 1) * T::BYTES, cols_at = cols0 + (unsigned)(t & 1) * T::BYTES;
     const float *tL = sL + (t & 1) * TILE, *tD = sD + (t & 1) * TILE;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
+    for (int n = 0; n < 2 / SG; ++n) {
+      const int s = SG == 1 ? n : half;
       f32x4 z[2][2], g[2][2];  // [block of 16 rows][nb]
       const unsigned at_s = fresh(rows_at);
 #pragma unroll
@@ -842,6 +880,9 @@ attention_train_dkv_kernel(const AttentionTrainArgs a) {
     if (live) compute(t, std::false_type{});
   }
 
+  if constexpr (SG == 2)
+    join_halves<4 * DB>(sQ, group, half, lane, [&](int i) -> f32x4 & { return i < 2 * DB ? dk[i / DB][i % DB] : dv[i / DB - 2][i % DB]; });
+  if (half != 0) return;
   const float fk = (a.negate ? -a.scale : a.scale) / dsc, fv = DT == DT_F16 ? 1.0f / 16384.0f : 1.0f;
 #pragma unroll
   for (int nb = 0; nb < 2; ++nb) {
@@ -850,6 +891,16 @@ attention_train_dkv_kernel(const AttentionTrainArgs a) {
     unsigned short *kp = (unsigned short *)slice(a.dk, w.b, w.hk) + (long long)j * a.dk.ss;
     unsigned short *vp = (unsigned short *)slice(a.dv, w.b, w.hk) + (long long)j * a.dv.ss;
     const bool there = j < w.lk;  // (a key past the end was read as zeros, its P is not)
+    if (a.row_splits > 1) {
+      float *at = a.part_dkv + (((long long)part * a.B * a.Hk + bh) * a.Sk + j) * 2 * DU + g4 * 4;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+        if (d * 16 + g4 * 4 < a.D) {
+          *(f32x4 *)(at + d * 16) = there ? dk[nb][d] * fk : f32x4{0, 0, 0, 0};
+          *(f32x4 *)(at + DU + d * 16) = there ? dv[nb][d] * fv : f32x4{0, 0, 0, 0};
+        }
+      continue;
+    }
 #pragma unroll
     for (int d = 0; d < DB; ++d)
       if (d * 16 + g4 * 4 < a.D) {
@@ -858,6 +909,33 @@ attention_train_dkv_kernel(const AttentionTrainArgs a) {
         *(u32x2 *)(vp + d * 16 + g4 * 4) = there ? y : u32x2{0, 0};
       }
   }
+}
+
+// The workgroups of dK and dV first, then those of dQ: one launch, so that neither waits for the other's last ones.
+template <int DT, int DL, int DU, int WAVES, int SG>
+__global__ void __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
+attention_train_backward_kernel(const AttentionTrainArgs a, int dkv_blocks) {
+  __shared__ __attribute__((aligned(1024))) unsigned char tiles[4 * Tile<DL>::BYTES];
+  __shared__ __attribute__((aligned(16))) float sL[2 * TILE], sD[2 * TILE];
+  if ((int)blockIdx.x < dkv_blocks) dkv_block<DT, DL, DU, WAVES, SG>(a, blockIdx.x, tiles, sL, sD);
+  else dq_block<DT, DL, DU, WAVES, SG>(a, blockIdx.x - dkv_blocks, tiles);
+}
+
+// Adds up the parts of dK and dV where the rows are split over workgroups: 4 columns per thread.
+template <int DT, int DU>
+__global__ void __launch_bounds__(256) attention_train_sum_kernel(const AttentionTrainArgs a) {
+  constexpr int PER = 2 * DU / 4;
+  const long long id = (long long)blockIdx.x * 256 + threadIdx.x, key = id / PER;
+  const int piece = (int)(id - key * PER), c = (piece % (DU / 4)) * 4;
+  const bool is_v = piece >= DU / 4;
+  if (key >= (long long)a.B * a.Hk * a.Sk || c >= a.D) return;
+  const long long plane = (long long)a.B * a.Hk * a.Sk * 2 * DU;
+  const float *at = a.part_dkv + key * 2 * DU + piece * 4;
+  f32x4 x = *(const f32x4 *)at;
+  for (int r = 1; r < a.row_splits; ++r) x += *(const f32x4 *)(at + r * plane);
+  const int bh = (int)(key / a.Sk), j = (int)(key - (long long)bh * a.Sk), b = bh / a.Hk;
+  const HeadView &out = is_v ? a.dv : a.dk;
+  *(u32x2 *)((unsigned short *)slice(out, b, bh - b * a.Hk) + (long long)j * out.ss + c) = pack_result<DT>(x, 1.0f);
 }
 
 template <int DT, int DL, int DU>
@@ -878,10 +956,16 @@ int backward(const AttentionTrainArgs &a, hipStream_t stream) {
   const unsigned bh = (unsigned)(a.B * a.Hk);
   const unsigned row_blocks = (unsigned)(DT == DT_F16 ? a.norm_blocks : a.rows_pad / TILE);
   if (row_blocks > 0) hipLaunchKernelGGL((attention_train_rows_kernel<DT>), dim3(row_blocks, bh), dim3(256), 0, stream, a);
-  const unsigned kb = (unsigned)((a.Sk + 32 * W - 1) / (32 * W)) * bh;
-  if (kb > 0) hipLaunchKernelGGL((attention_train_dkv_kernel<DT, DL, DU, W>), dim3(kb), dim3(W * 64), 0, stream, a);
-  const unsigned qb = (unsigned)((a.G * a.Sq + 32 * W - 1) / (32 * W)) * bh;
-  if (qb > 0) hipLaunchKernelGGL((attention_train_dq_kernel<DT, DL, DU, W>), dim3(qb), dim3(W * 64), 0, stream, a);
+  auto blocks = [&](int n) { return (unsigned)((n + a.block - 1) / a.block) * bh; };
+  const unsigned kb = blocks(a.Sk) * (unsigned)a.row_splits, qb = blocks(a.G * a.Sq);
+  if (kb + qb > 0) {
+    if (a.block == 32 * W) hipLaunchKernelGGL((attention_train_backward_kernel<DT, DL, DU, W, 1>), dim3(kb + qb), dim3(W * 64), 0, stream, a, (int)kb);
+    else hipLaunchKernelGGL((attention_train_backward_kernel<DT, DL, DU, W, 2>), dim3(kb + qb), dim3(W * 64), 0, stream, a, (int)kb);
+  }
+  if (a.row_splits > 1 && a.Sk > 0) {
+    const long long pieces = (long long)a.B * a.Hk * a.Sk * 2 * DU / 4;
+    hipLaunchKernelGGL((attention_train_sum_kernel<DT, DU>), dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, stream, a);
+  }
   return (int)hipGetLastError();
 }
 

@@ -178,6 +178,8 @@ TraceaStatus run_attention(const Attention &c, bool from_copies) {
   a.scale_log2 = a.scale * 1.4426950408889634f;
   a.causal = c.causal;
   a.rows_pad = (int)rows_pad;
+  a.order = c.q_len != nullptr || c.k_len != nullptr ? 2 : c.causal ? 1 : 0;
+  if (getenv("TM")) a.order = atoi(getenv("TM"));
   a.splits = 1;
   const int cus = (int)device_limits().cus;
   if (!c.backward) {
@@ -205,13 +207,22 @@ TraceaStatus run_attention(const Attention &c, bool from_copies) {
   a.d_o = head_view(c.d_o); a.dq = head_view(c.dq); a.dk = head_view(c.dk); a.dv = head_view(c.dv);
   const size_t stats = (size_t)(B * Hk * rows_pad);
   a.norm_blocks = c.q.dtype == TRACEA_DTYPE_FLOAT16 ? (int)(rows_pad / 64 + (Sk + 63) / 64) : 0;
-  float *ws = (float *)train_scratch(c.q.device, c.stream, (2 * stats + (size_t)(B * Hk) * a.norm_blocks + 1) * 4);
+  const long long tiles_q = rows_pad / 64;
+  a.block = 128;
+  a.row_splits = 1;
+  if (getenv("TB")) a.block = atoi(getenv("TB"));
+  if (getenv("TR")) a.row_splits = atoi(getenv("TR"));
+  (void)tiles_q;
+  const size_t width = D <= 64 ? 64 : D <= 96 ? 96 : 128;
+  const size_t norms = ((size_t)(B * Hk) * a.norm_blocks + 3) / 4 * 4, parts = a.row_splits > 1 ? (size_t)a.row_splits * B * Hk * Sk * 2 * width : 0;
+  float *ws = (float *)train_scratch(c.q.device, c.stream, (2 * stats + norms + parts + 1) * 4);
   if (ws == nullptr)
     return fail(TRACEA_UNSUPPORTED_CONFIG, "%s: no workspace can be had (a stream under capture that made no such call before, or out of "
                                            "memory)", c.op);
   a.neg_lse2 = ws;
   a.neg_delta = ws + stats;
   a.norms = ws + 2 * stats;
+  a.part_dkv = a.norms + norms;
   return hip_status("attention backward launch", launch_attention_train_backward(a, c.q.dtype, c.stream));
 }
 

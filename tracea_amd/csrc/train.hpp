@@ -24,9 +24,13 @@ struct AttentionTrainArgs {
   unsigned g_magic;   // ceil(2^32 / G) (G > 1): r / G = umulhi(r, g_magic) while G * G * Sq < 2^32
   float scale, scale_log2;  // magnitudes; negate: the caller's scale is below zero
   int negate, causal;
+  int order;  // of the workgroups: 0 runs of heads, 1 heaviest blocks first, 2 those going round the XCDs
   // backward: per packed row -lse * log2(e) (-inf: nothing visible) and -(dO . O), [B * Hk][rows_pad] each
   float *neg_lse2, *neg_delta;
   int rows_pad;  // G * Sq up to a multiple of 64
+  int block;       // columns (keys, packed rows) of a workgroup: 128, or 64 with two waves on 32 columns
+  int row_splits;  // parts of the rows for dK and dV, each with a workgroup of its own
+  float *part_dkv; // [row_splits][B * Hk][Sk][dK, dV][width], row_splits > 1
   // f16 only: largest squared row norms of dO and V, [B * Hk][norm_blocks] (64 rows of dO or 64 keys of V each)
   float *norms;
   int norm_blocks;
