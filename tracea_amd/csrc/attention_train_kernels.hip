@@ -68,16 +68,19 @@ __device__ __forceinline__ void unpack8(u32x4 w, float (&x)[8]) {
   }
 }
 
-// A tile in LDS: 64 rows of DL elements, the 16-byte column XOR-ed with a number made of the row.  It serves both ways a
-// tile is read.  Row fragments (16 rows x one column per 16 lanes) need 16 different bank groups from 16 rows: the numbers of
-// rows 0..15 differ (with DL = 64 two rows share a 256-byte line, and those of a pair are alike).  Transposing reads take 8 rows x 2
-// columns per half-wave: all but the lowest bit of the numbers of 8 rows differ.  A rotation by one bit of the row has both.
+// A tile in LDS: 64 rows of DL elements, the 16-byte column XOR-ed with a number f made of the row; 64 banks of 4 bytes, 16 lanes of
+// 16 bytes or 32 of 8 at a time.  f serves both ways a tile is read:
+//   row fragments (16 rows, four columns one apart): the hardware takes rows 0-3 and 12-15 of one column together with
+//   rows 4-11 of the next, so that f of the former must be whole pairs {2n, 2n + 1};
+//   transposing reads (8 rows x 2 columns): f / 2 must differ between rows 0-7, and between rows 8-15.
+// (A plain rotation of the row has the second only: 128 of 368 LDS cycles of a pair of half-tiles were conflicts.)  With DL = 64
+// two rows share a line of 256 bytes, and k is the line.
 template <int DL>
 struct Tile {
   static constexpr int ROW_BYTES = DL * 2, CH = DL / 8, RP = 256 / ROW_BYTES, BYTES = TILE * ROW_BYTES;
   static __device__ __forceinline__ int swz(int row) {
-    const int k = (row / RP) & (CH - 1);
-    return ((k << 1) | (k / (CH / 2))) & (CH - 1);
+    const int k = (row / RP) & (CH - 1), upper = k / (CH / 2);
+    return (((k & (CH / 2 - 1)) ^ (upper * (CH / 4))) << 1) | upper;
   }
 };
 
@@ -100,14 +103,25 @@ __device__ __forceinline__ unsigned lds_offset(const void *p) {
 }
 __device__ __forceinline__ unsigned lds_address(const void *p) { return (unsigned)__builtin_amdgcn_readfirstlane((int)lds_offset(p)); }
 
-// Requests 64 rows of a tensor into LDS (16 bytes per lane, 1 KB per wave and request).  offset(row) is the byte offset
-// of a row from `base`, below 2^31, or BEYOND for a row that reads as zeros; columns from D on read as zeros too.
-constexpr unsigned BEYOND = 0x80000000u;
+// Requests 64 rows of a tensor into LDS, 16 bytes per lane and 1 KB per wave and request; a wave's requests are 16 (DL = 128) or 32 rows
+// apart.  Columns from D on read as zeros.
+constexpr unsigned BEYOND = 0x80000000u;  // an offset that no tile has: out of the resource's range, reads as zeros
+// ... where the offset of row r + 16 is that of row r and a step, for whole tiles: offset(row) the byte offset of row 0..15 / 0..31 from `base`.
 template <int DL, int WAVES, typename F>
-__device__ __forceinline__ void load_tile(const void *base, const unsigned char *dst, int D, int lane, int wave_u, F &&offset) {
+__device__ __forceinline__ void load_tile(const void *base, long long step, const unsigned char *dst, int D, int lane, int wave_u, F &&offset) {
   using T = Tile<DL>;
-  constexpr int RPI = 64 / T::CH;             // rows per request
-  constexpr int NI = TILE / (RPI * WAVES);
+  constexpr int RPI = 64 / T::CH, NI = TILE / (RPI * WAVES);
+  const int first = wave_u * RPI, row = first + lane / T::CH;
+  const int col = ((lane % T::CH) ^ T::swz(row)) << 3;
+  const unsigned at = col >= D ? BEYOND : offset(row) + (unsigned)(col * 2), lds = lds_address(dst) + (unsigned)(first * T::ROW_BYTES);
+#pragma unroll
+  for (int i = 0; i < NI; ++i) dma16(resource((const char *)base + i * step, BEYOND), at, lds + (unsigned)(i * WAVES * RPI * T::ROW_BYTES));
+}
+// ... any rows: offset(row) is below 2^31, or BEYOND for a row that reads as zeros.
+template <int DL, int WAVES, typename F>
+__device__ __forceinline__ void load_tile_any(const void *base, const unsigned char *dst, int D, int lane, int wave_u, F &&offset) {
+  using T = Tile<DL>;
+  constexpr int RPI = 64 / T::CH, NI = TILE / (RPI * WAVES);
   const u32x4 rsrc = resource(base, BEYOND);
   const unsigned lds = lds_address(dst);
 #pragma unroll
@@ -319,10 +333,17 @@ attention_train_forward_kernel(const AttentionTrainArgs a) {
 
   const unsigned short *Kg = slice(a.k, w.b, w.hk), *Vg = slice(a.v, w.b, w.hk);
   auto request = [&](int t) __attribute__((always_inline)) {
-    const int left = w.lk - t * TILE, at = (t & 1) * T::BYTES;
+    const int left = w.lk - t * TILE, at = (t & 1) * T::BYTES, lane_ = fresh(lane);
     const unsigned kss = (unsigned)a.k.ss * 2u, vss = (unsigned)a.v.ss * 2u;
-    load_tile<DL, WAVES>(Kg + (long long)t * TILE * a.k.ss, sK + at, a.D, lane, wave, [&](int row) { return row < left ? row * kss : BEYOND; });
-    load_tile<DL, WAVES>(Vg + (long long)t * TILE * a.v.ss, sK + V_AT + at, a.D, lane, wave, [&](int row) { return row < left ? row * vss : BEYOND; });
+    const unsigned short *kt = Kg + (long long)t * TILE * a.k.ss, *vt = Vg + (long long)t * TILE * a.v.ss;
+    if (left >= TILE) {
+      constexpr int STEP = WAVES * 64 / T::CH;
+      load_tile<DL, WAVES>(kt, (long long)kss * STEP, sK + at, a.D, lane_, wave, [&](int row) { return row * kss; });
+      load_tile<DL, WAVES>(vt, (long long)vss * STEP, sK + V_AT + at, a.D, lane_, wave, [&](int row) { return row * vss; });
+    } else {
+      load_tile_any<DL, WAVES>(kt, sK + at, a.D, lane_, wave, [&](int row) { return row < left ? row * kss : BEYOND; });
+      load_tile_any<DL, WAVES>(vt, sK + V_AT + at, a.D, lane_, wave, [&](int row) { return row < left ? row * vss : BEYOND; });
+    }
   };
 
   f32x4 o[2][DB];
@@ -597,10 +618,17 @@ __device__ __forceinline__ void dq_block(const AttentionTrainArgs &a, int id, un
 
   const unsigned short *Kg = slice(a.k, w.b, w.hk), *Vg = slice(a.v, w.b, w.hk);
   auto request = [&](int t) __attribute__((always_inline)) {
-    const int left = w.lk - t * TILE, at = (t & 1) * T::BYTES;
+    const int left = w.lk - t * TILE, at = (t & 1) * T::BYTES, lane_ = fresh(lane);
     const unsigned kss = (unsigned)a.k.ss * 2u, vss = (unsigned)a.v.ss * 2u;
-    load_tile<DL, WAVES>(Kg + (long long)t * TILE * a.k.ss, sK + at, a.D, lane, wave, [&](int row) { return row < left ? row * kss : BEYOND; });
-    load_tile<DL, WAVES>(Vg + (long long)t * TILE * a.v.ss, sK + V_AT + at, a.D, lane, wave, [&](int row) { return row < left ? row * vss : BEYOND; });
+    const unsigned short *kt = Kg + (long long)t * TILE * a.k.ss, *vt = Vg + (long long)t * TILE * a.v.ss;
+    if (left >= TILE) {
+      constexpr int STEP = WAVES * 64 / T::CH;
+      load_tile<DL, WAVES>(kt, (long long)kss * STEP, sK + at, a.D, lane_, wave, [&](int row) { return row * kss; });
+      load_tile<DL, WAVES>(vt, (long long)vss * STEP, sK + V_AT + at, a.D, lane_, wave, [&](int row) { return row * vss; });
+    } else {
+      load_tile_any<DL, WAVES>(kt, sK + at, a.D, lane_, wave, [&](int row) { return row < left ? row * kss : BEYOND; });
+      load_tile_any<DL, WAVES>(vt, sK + V_AT + at, a.D, lane_, wave, [&](int row) { return row < left ? row * vss : BEYOND; });
+    }
   };
 
   f32x4 acc[2][DB];
@@ -610,61 +638,72 @@ __device__ __forceinline__ void dq_block(const AttentionTrainArgs &a, int id, un
     for (int d = 0; d < DB; ++d) acc[qb][d] = f32x4{0, 0, 0, 0};
 
   const unsigned rows0 = rows_base<DL>(sK, r16, g4), cols0 = columns_base<DL>(sK, r16, g4);
+  // A tile's first-operand fragments in the order of their use, for half-tiles s = 0, 1: S, dP (under it the exponentials of S),
+  // then S of the other half (under it this half's dS), its dP, and dQ of both.  One chunk per fragment: the read of the fragment AHEAD chunks
+  // on, the two products of this one, a share of the vector work.
   auto compute = [&](int t, auto edge_tag) __attribute__((always_inline)) {
     constexpr bool EDGE = decltype(edge_tag)::value;
-    const unsigned rows_at = rows0 + (unsigned)(t & 1) * T::BYTES, cols_at = cols0 + (unsigned)(t & 1) * T::BYTES;
-#pragma unroll
-    for (int n = 0; n < 2 / SG; ++n) {
-      const int s = SG == 1 ? n : half;
-      f32x4 z[2][2], g[2][2];  // [qb][block of 16 keys]
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int qb = 0; qb < 2; ++qb) {
-          z[qb][kb] = f32x4{0, 0, 0, 0};
-          g[qb][kb] = f32x4{nd[qb], nd[qb], nd[qb], nd[qb]};
-        }
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          const u32x4 kf = read_rows<DL>(rows_at, 0, 2 * s + kb, ks);
-#pragma unroll
-          for (int qb = 0; qb < 2; ++qb) z[qb][kb] = Mfma16<DT>::run(kf, qf[qb][ks], z[qb][kb]);
-        }
-      fence();
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          const u32x4 vf = read_rows<DL>(rows_at, V_AT, 2 * s + kb, ks);
-#pragma unroll
-          for (int qb = 0; qb < 2; ++qb) g[qb][kb] = Mfma16<DT>::run(vf, of[qb][ks], g[qb][kb]);
-        }
-      fence();
-      u32x4 df[2];
+    constexpr int AHEAD = 2, PER = (16 + DB - 1) / DB, H = 2 / SG, N = 3 * DB * H;
+    const unsigned at_r = rows0 + (unsigned)(t & 1) * T::BYTES, at_c = cols0 + (unsigned)(t & 1) * T::BYTES;
+    f32x4 z[H][2][2], g[2][2];  // [half][qb][block of 16 keys]
+    u32x4 df[2], frag[AHEAD + 1];
+    // phase of chunk i: S 0, dP 1, dQ 2 of half h
+    auto phase = [](int i) constexpr { return H == 1 ? i / DB : (i / DB == 0 || i / DB == 2) ? 0 : (i / DB == 1 || i / DB == 3) ? 1 : 2; };
+    auto half_of = [](int i) constexpr { return H == 1 ? 0 : i / DB < 2 ? 0 : i / DB < 4 ? 1 : i / DB - 4; };
+    auto read = [&](auto tag) __attribute__((always_inline)) {
+      constexpr int i = decltype(tag)::value, j = i % DB;
+      if constexpr (i < N) {
+        const int s = SG == 1 ? half_of(i) : half;
+        if constexpr (phase(i) == 0) frag[i % (AHEAD + 1)] = read_rows<DL>(at_r, 0, 2 * s + j % 2, j / 2);
+        else if constexpr (phase(i) == 1) frag[i % (AHEAD + 1)] = read_rows<DL>(at_r, V_AT, 2 * s + j % 2, j / 2);
+        else frag[i % (AHEAD + 1)] = read_columns<DL>(at_c, 0, s, j);
+      }
+    };
+    auto probability = [&](int h, int v) __attribute__((always_inline)) {
+      const int qb = v >> 3, kb = (v >> 2) & 1, e = v & 3, s = SG == 1 ? h : half;
+      float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z[h][qb][kb][e], a.scale_log2, nl[qb]));
+      if constexpr (EDGE) p = t * TILE + s * 32 + kb * 16 + g4 * 4 + e > q_last[qb] ? 0.0f : p;
+      if constexpr (DT == DT_F16) p *= dsp;
+      z[h][qb][kb][e] = p;
+    };
+    auto gradient = [&](int h, int v) __attribute__((always_inline)) {
+      const int qb = v >> 3, kb = (v >> 2) & 1, e = v & 3;
+      z[h][qb][kb][e] *= g[qb][kb][e];
+    };
+    u32x4 df1[2];  // of half 0 while half 1 is under way
+    static_for<0, AHEAD>([&](auto tag) __attribute__((always_inline)) { read(tag); });
+    static_for<0, N>([&](auto tag) __attribute__((always_inline)) {
+      constexpr int i = decltype(tag)::value, j = i % DB, kb = j % 2, ks = j / 2, h = half_of(i), ph = phase(i);
+      const u32x4 &f = frag[i % (AHEAD + 1)];
+      read(std::integral_constant<int, i + AHEAD>{});
 #pragma unroll
       for (int qb = 0; qb < 2; ++qb) {
+        if constexpr (ph == 0) z[h][qb][kb] = Mfma16<DT>::run(f, qf[qb][ks], ks == 0 ? f32x4{0, 0, 0, 0} : z[h][qb][kb]);
+        else if constexpr (ph == 1) g[qb][kb] = Mfma16<DT>::run(f, of[qb][ks], ks == 0 ? f32x4{nd[qb], nd[qb], nd[qb], nd[qb]} : g[qb][kb]);
+        else acc[qb][j] = Mfma16<DT>::run(f, H == 2 && h == 0 ? df1[qb] : df[qb], acc[qb][j]);
+      }
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+      for (int v = j * PER; v < j * PER + PER && v < 16; ++v) {
+        if constexpr (ph == 1) probability(h, v);
+        if constexpr (H == 2 && i / DB == 2) gradient(0, v);
+        if constexpr (H == 2 && i / DB == 4) gradient(1, v);
+      }
+      if constexpr (H == 2 && i == 3 * DB - 1) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z[qb][kb][e], a.scale_log2, nl[qb]));
-            if constexpr (EDGE) p = t * TILE + s * 32 + kb * 16 + g4 * 4 + e > q_last[qb] ? 0.0f : p;
-            if constexpr (DT == DT_F16) p *= dsp;
-            z[qb][kb][e] = p * g[qb][kb][e];
-          }
-        df[qb] = pack_operand<DT>(z[qb][0], z[qb][1]);
+        for (int qb = 0; qb < 2; ++qb) df1[qb] = pack_operand<DT>(z[0][qb][0], z[0][qb][1]);
+      }
+      if constexpr (H == 2 && i == 5 * DB - 1) {
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) df[qb] = pack_operand<DT>(z[H - 1][qb][0], z[H - 1][qb][1]);
+      }
+      if constexpr (H == 1 && i == 2 * DB - 1) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) gradient(0, v);
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) df[qb] = pack_operand<DT>(z[0][qb][0], z[0][qb][1]);
       }
       fence();
-#pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        const u32x4 kf = read_columns<DL>(cols_at, 0, s, d);
-#pragma unroll
-        for (int qb = 0; qb < 2; ++qb) acc[qb][d] = Mfma16<DT>::run(kf, df[qb], acc[qb][d]);
-      }
-      fence();
-    }
+    });
   };
   auto head = [&](int t) __attribute__((always_inline)) {
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this tile
@@ -700,7 +739,7 @@ __device__ __forceinline__ void dq_block(const AttentionTrainArgs &a, int id, un
 // dK and dV of a block of keys, or of a part of the rows that see them.  SG = 2: two waves share 32 keys, each takes half of
 // every tile of rows.
 template <int DT, int DL, int DU, int WAVES, int SG>
-__device__ __forceinline__ void dkv_block(const AttentionTrainArgs &a, int id, unsigned char *sQ, float *sL, float *sD) {
+__device__ __forceinline__ void dkv_block(const AttentionTrainArgs &a, int id, unsigned char *sQ, float *sL, float *sD, u32x4 *parked) {
   using T = Tile<DL>;
   constexpr int BC = 32 * WAVES / SG, KS = DU / 32, DB = DU / 16;
   constexpr unsigned O_AT = 2 * T::BYTES;  // two tiles of Q, two of dO
@@ -737,6 +776,14 @@ __device__ __forceinline__ void dkv_block(const AttentionTrainArgs &a, int id, u
       vf[nb][ks] = resident(vp, there, ks * 32 + g4 * 8, a.D);
     }
   }
+  // (D = 128 is some registers short: three fragments wait in LDS; a fourth would cost the second workgroup of a CU)
+  constexpr bool PARK = DU == 128;
+  auto own = [&](int i) -> u32x4 & { return parked[(wave * 3 + i) * 64 + (int)fresh(lane)]; };
+  if constexpr (PARK) {
+    own(0) = vf[0][KS - 1];
+    own(1) = vf[1][KS - 1];
+    own(2) = kf[1][KS - 1];
+  }
   // of the wave: rows from here on see some of its keys / all of them (rows past the end have P = 0)
   const bool live = k_wave < w.lk;
   long long row_some = 0, row_all = 0;
@@ -759,12 +806,19 @@ __device__ __forceinline__ void dkv_block(const AttentionTrainArgs &a, int id, u
   const float *nl = a.neg_lse2 + (long long)bh * a.rows_pad, *nd = a.neg_delta + (long long)bh * a.rows_pad;
   auto request = [&](int t) __attribute__((always_inline)) {
     const int r0 = t * TILE, i0 = query_of(a, r0), at = (t & 1) * T::BYTES, lane_ = fresh(lane);
+    const unsigned short *qt = Qg + (long long)i0 * a.q.ss, *ot = Og + (long long)i0 * a.d_o.ss;
     auto offset = [&](const HeadView &v, int row) __attribute__((always_inline)) -> unsigned {
       const int r = r0 + row, i = query_of(a, r);
-      return r < rows ? (unsigned)(i - i0) * ((unsigned)v.ss * 2u) + (unsigned)(r - i * a.G) * ((unsigned)v.sh * 2u) : BEYOND;
+      return (unsigned)(i - i0) * ((unsigned)v.ss * 2u) + (unsigned)(r - i * a.G) * ((unsigned)v.sh * 2u);
     };
-    load_tile<DL, WAVES>(Qg + (long long)i0 * a.q.ss, sQ + at, a.D, lane_, wave, [&](int row) { return offset(a.q, row); });
-    load_tile<DL, WAVES>(Og + (long long)i0 * a.d_o.ss, sQ + O_AT + at, a.D, lane_, wave, [&](int row) { return offset(a.d_o, row); });
+    constexpr int STEP = WAVES * 64 / T::CH;
+    if (r0 + TILE <= rows && 16 % a.G == 0) {  // (a power of two: rows 16 apart are 16 / G queries apart)
+      load_tile<DL, WAVES>(qt, (long long)(STEP / a.G) * a.q.ss * 2, sQ + at, a.D, lane_, wave, [&](int row) { return offset(a.q, row); });
+      load_tile<DL, WAVES>(ot, (long long)(STEP / a.G) * a.d_o.ss * 2, sQ + O_AT + at, a.D, lane_, wave, [&](int row) { return offset(a.d_o, row); });
+    } else {
+      load_tile_any<DL, WAVES>(qt, sQ + at, a.D, lane_, wave, [&](int row) { return r0 + row < rows ? offset(a.q, row) : BEYOND; });
+      load_tile_any<DL, WAVES>(ot, sQ + O_AT + at, a.D, lane_, wave, [&](int row) { return r0 + row < rows ? offset(a.d_o, row) : BEYOND; });
+    }
     if (wave < 2) {  // (rows_pad is a multiple of the tile)
       dma4(resource((wave == 0 ? nl : nd) + r0, TILE * 4), lane * 4, lds_address((wave == 0 ? sL : sD) + (t & 1) * TILE));
     }
@@ -776,91 +830,74 @@ __device__ __forceinline__ void dkv_block(const AttentionTrainArgs &a, int id, u
 #pragma unroll
     for (int d = 0; d < DB; ++d) dk[nb][d] = dv[nb][d] = f32x4{0, 0, 0, 0};
 
-  const unsigned rows0 = rows_base<DL>(sQ, r16, g4), cols0 = columns_base<DL>(sQ, r16, g4);
   auto compute = [&](int t, auto edge_tag) __attribute__((always_inline)) {
     constexpr bool EDGE = decltype(edge_tag)::value;
-    const unsigned rows_at = rows0 + (unsigned)(t & 1) * T::BYTES, cols_at = cols0 + (unsigned)(t & 1) * T::BYTES;
+    const int lane_ = fresh(lane);
+    const unsigned rows_at = rows_base<DL>(sQ, lane_ & 15, lane_ >> 4) + (unsigned)(t & 1) * T::BYTES;
+    const unsigned cols_at = columns_base<DL>(sQ, lane_ & 15, lane_ >> 4) + (unsigned)(t & 1) * T::BYTES;
     const float *tL = sL + (t & 1) * TILE, *tD = sD + (t & 1) * TILE;
 #pragma unroll
     for (int n = 0; n < 2 / SG; ++n) {
       const int s = SG == 1 ? n : half;
-      f32x4 z[2][2], g[2][2];  // [block of 16 rows][nb]
-      const unsigned at_s = fresh(rows_at);
-#pragma unroll
-      for (int rb = 0; rb < 2; ++rb)
-#pragma unroll
-        for (int nb = 0; nb < 2; ++nb) z[rb][nb] = f32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int rb = 0; rb < 2; ++rb) {
-          const u32x4 qf = read_rows<DL>(at_s, 0, 2 * s + rb, ks);
-#pragma unroll
-          for (int nb = 0; nb < 2; ++nb) z[rb][nb] = Mfma16<DT>::run(qf, kf[nb][ks], z[rb][nb]);
+      // S; dP with the exponentials of S under it; dV with dS under it; dK.  One chunk per first-operand fragment: the read of the
+      // fragment AHEAD chunks on, the two products of this one, a share of the vector work.
+      constexpr int AHEAD = DU == 128 ? 1 : 2, PER = (16 + DB - 1) / DB, N = 4 * DB;
+      f32x4 z[2][2], g[2][2], l4, d4[2];  // [block of 16 rows][nb]
+      u32x4 pf[2], frag[AHEAD + 1];  // (dS takes P's place once dV has it)
+      const unsigned at_r = fresh(rows_at), at_c = fresh(cols_at);
+      auto read = [&](auto tag) __attribute__((always_inline)) {
+        constexpr int i = decltype(tag)::value, j = i % DB;
+        if constexpr (i < DB) frag[i % (AHEAD + 1)] = read_rows<DL>(at_r, 0, 2 * s + j % 2, j / 2);
+        else if constexpr (i < 2 * DB) frag[i % (AHEAD + 1)] = read_rows<DL>(at_r, O_AT, 2 * s + j % 2, j / 2);
+        else if constexpr (i < 3 * DB) frag[i % (AHEAD + 1)] = read_columns<DL>(at_c, O_AT, s, j);
+        else if constexpr (i < N) frag[i % (AHEAD + 1)] = read_columns<DL>(at_c, 0, s, j);
+      };
+      static_for<0, AHEAD>([&](auto tag) __attribute__((always_inline)) { read(tag); });
+      static_for<0, N>([&](auto tag) __attribute__((always_inline)) {
+        constexpr int i = decltype(tag)::value, phase = i / DB, j = i % DB, rb = j % 2, ks = j / 2;
+        const u32x4 &f = frag[i % (AHEAD + 1)];
+        read(std::integral_constant<int, i + AHEAD>{});
+        if constexpr (i == DB - 1) {
+          d4[0] = *(const f32x4 *)(tD + s * 32 + g4 * 4);
+          d4[1] = *(const f32x4 *)(tD + s * 32 + 16 + g4 * 4);
+          l4 = *(const f32x4 *)(tL + s * 32 + g4 * 4);
         }
-      fence();
 #pragma unroll
-      for (int rb = 0; rb < 2; ++rb) {
-        const f32x4 l4 = *(const f32x4 *)(tL + s * 32 + rb * 16 + g4 * 4);
+        for (int nb = 0; nb < 2; ++nb) {
+          if constexpr (phase == 0) z[rb][nb] = Mfma16<DT>::run(f, PARK && nb == 1 && ks == KS - 1 ? own(2) : kf[nb][ks], ks == 0 ? f32x4{0, 0, 0, 0} : z[rb][nb]);
+          else if constexpr (phase == 1) g[rb][nb] = Mfma16<DT>::run(f, PARK && ks == KS - 1 ? own(nb) : vf[nb][ks], ks == 0 ? d4[rb] : g[rb][nb]);
+          else if constexpr (phase == 2) dv[nb][j] = Mfma16<DT>::run(f, pf[nb], dv[nb][j]);
+          else dk[nb][j] = Mfma16<DT>::run(f, pf[nb], dk[nb][j]);
+        }
+        int limit[2];  // of the lane's key: rows of this half-tile below it do not count
+        if constexpr (EDGE) {
 #pragma unroll
-        for (int nb = 0; nb < 2; ++nb)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z[rb][nb][e], a.scale_log2, l4[e]));
-            if constexpr (EDGE) p = t * TILE + s * 32 + rb * 16 + g4 * 4 + e < (int)fresh(first_row) + nb * first_step ? 0.0f : p;
-            z[rb][nb][e] = p;
+          for (int nb = 0; nb < 2; ++nb) {
+            const int from = (int)fresh(first_row) + nb * first_step;
+            limit[nb] = (phase == 2 ? max(from, two_keys) : from) - (t * TILE + s * 32 + g4 * 4);
           }
-      }
-      u32x4 pf[2];
-#pragma unroll
-      for (int nb = 0; nb < 2; ++nb) pf[nb] = pack_operand<DT>(z[0][nb], z[1][nb]);
-      fence();
-      const unsigned at_v = fresh(cols_at);
-#pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        const u32x4 of = read_columns<DL>(at_v, O_AT, s, d);
-#pragma unroll
-        for (int nb = 0; nb < 2; ++nb) dv[nb][d] = Mfma16<DT>::run(of, pf[nb], dv[nb][d]);
-        if (d == DB / 2) fence();
-      }
-      fence();
-#pragma unroll
-      for (int rb = 0; rb < 2; ++rb) {
-        const f32x4 d4 = *(const f32x4 *)(tD + s * 32 + rb * 16 + g4 * 4);
-        g[rb][0] = g[rb][1] = d4;
-      }
-      const unsigned at_p = fresh(rows_at);
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int rb = 0; rb < 2; ++rb) {
-          const u32x4 of = read_rows<DL>(at_p, O_AT, 2 * s + rb, ks);
-#pragma unroll
-          for (int nb = 0; nb < 2; ++nb) g[rb][nb] = Mfma16<DT>::run(of, vf[nb][ks], g[rb][nb]);
-          if (ks == KS / 2 && rb == 0) fence();
         }
 #pragma unroll
-      for (int rb = 0; rb < 2; ++rb)
-#pragma unroll
-        for (int nb = 0; nb < 2; ++nb)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float x = z[rb][nb][e] * g[rb][nb][e];
+        for (int v = j * PER; v < j * PER + PER && v < 16; ++v) {
+          const int vr = v >> 3, nb = (v >> 2) & 1, e = v & 3;
+          if constexpr (phase == 1) {
+            if (v == 8) l4 = *(const f32x4 *)(tL + s * 32 + 16 + g4 * 4);
+            float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z[vr][nb][e], a.scale_log2, l4[e]));
+            if constexpr (EDGE) p = vr * 16 + e < limit[nb] ? 0.0f : p;
+            z[vr][nb][e] = p;
+          } else if constexpr (phase == 2) {
+            float x = z[vr][nb][e] * g[vr][nb][e];
             if constexpr (DT == DT_F16) x *= dsp;
-            if constexpr (EDGE) x = t * TILE + s * 32 + rb * 16 + g4 * 4 + e < max((int)fresh(first_row) + nb * first_step, two_keys) ? 0.0f : x;
-            z[rb][nb][e] = x;
+            if constexpr (EDGE) x = vr * 16 + e < limit[nb] ? 0.0f : x;
+            z[vr][nb][e] = x;
           }
+        }
+        if constexpr (i == 2 * DB - 1 || i == 3 * DB - 1) {
 #pragma unroll
-      for (int nb = 0; nb < 2; ++nb) pf[nb] = pack_operand<DT>(z[0][nb], z[1][nb]);
-      fence();
-      const unsigned at_k = fresh(cols_at);
-#pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        const u32x4 qf = read_columns<DL>(at_k, 0, s, d);
-#pragma unroll
-        for (int nb = 0; nb < 2; ++nb) dk[nb][d] = Mfma16<DT>::run(qf, pf[nb], dk[nb][d]);
-      }
-      fence();
+          for (int nb = 0; nb < 2; ++nb) pf[nb] = pack_operand<DT>(z[0][nb], z[1][nb]);
+        }
+        fence();
+      });
     }
   };
   auto head = [&](int t) __attribute__((always_inline)) {
@@ -917,7 +954,8 @@ __global__ void __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu
 attention_train_backward_kernel(const AttentionTrainArgs a, int dkv_blocks) {
   __shared__ __attribute__((aligned(1024))) unsigned char tiles[4 * Tile<DL>::BYTES];
   __shared__ __attribute__((aligned(16))) float sL[2 * TILE], sD[2 * TILE];
-  if ((int)blockIdx.x < dkv_blocks) dkv_block<DT, DL, DU, WAVES, SG>(a, blockIdx.x, tiles, sL, sD);
+  __shared__ u32x4 parked[DU == 128 ? WAVES * 3 * 64 : 1];
+  if ((int)blockIdx.x < dkv_blocks) dkv_block<DT, DL, DU, WAVES, SG>(a, blockIdx.x, tiles, sL, sD, parked);
   else dq_block<DT, DL, DU, WAVES, SG>(a, blockIdx.x - dkv_blocks, tiles);
 }
 
