@@ -5,10 +5,12 @@
 //             A_b = sum over b's rows of dt h^: dgate_b = A_b w_post, dw_post = sum_b gate_b A_b; dw_pre = sum dy x^
 //
 // Bound by memory: one pass, each row read once and written once.  A row is held in registers by the threads of a
-// workgroup (or, up to 256 channels in 16 bits, by some lanes of a wave), 8 channels each; a workgroup takes a run of rows of one batch entry, with the
-// weights and, backward, the column sums in registers all along.  The backward pass needs six sums over a row; all are linear in what is loaded, so
+// workgroup (up to 256 channels: by some lanes of a wave), 8 channels each; a workgroup takes a run of rows of one batch entry,
+// the next one requested ahead, with the weights and, backward, the column sums in registers all along.  The backward pass needs six sums over a row; all are linear in what is loaded, so
 // that they are taken in one go and the threads meet once per row.  Column sums leave as one partial row per workgroup and a second
 // kernel adds these up in their order: no atomics.
+// Measured (GPU time, a large copy reaches 4.8 TB/s): forward C2048 T24960 bf16 89 us = 4.6 TB/s, C4096 T8192 48 us (5.6 TB/s, partly from
+// the memory-side cache), 16 rows of 4096 4.6 us; backward C2048 T24960 118 us = 5.2 TB/s with its column sums.
 #include "contraction_kernel.hpp"
 #include "train.hpp"
 
@@ -28,25 +30,28 @@ template <bool VEC>
 __device__ __forceinline__ int channel(int e, int lane, int lanes) {
   return VEC ? lane * V + e : e * lanes + lane;
 }
+// A thread's channels of a row as they lie in memory: the next row's are requested before this one's are worked on.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load(const T *row, int lane, int lanes, int C, float (&x)[V]) {
+__device__ __forceinline__ Eight<T> request(const T *row, int lane, int lanes, int C) {
+  Eight<T> p;
   if constexpr (VEC) {
     const int c = channel<VEC>(0, lane, lanes);
-    if (c < C) {
-      const Eight<T> p = *(const Eight<T> *)(row + c);
+    if (c < C) return *(const Eight<T> *)(row + c);
 #pragma unroll
-      for (int e = 0; e < V; ++e) x[e] = (float)p.x[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < V; ++e) x[e] = 0.0f;
-    }
+    for (int e = 0; e < V; ++e) p.x[e] = (T)0.0f;
   } else {
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       const int c = channel<VEC>(e, lane, lanes);
-      x[e] = c < C ? (float)row[c] : 0.0f;
+      p.x[e] = c < C ? row[c] : (T)0.0f;
     }
   }
+  return p;
+}
+template <typename T>
+__device__ __forceinline__ void widen(const Eight<T> &p, float (&x)[V]) {
+#pragma unroll
+  for (int e = 0; e < V; ++e) x[e] = (float)p.x[e];
 }
 template <typename T, bool VEC>
 __device__ __forceinline__ void store(T *row, int lane, int lanes, int C, const float (&x)[V]) {
@@ -66,14 +71,15 @@ __device__ __forceinline__ void store(T *row, int lane, int lanes, int C, const 
     }
   }
 }
-// fp32 vectors of C channels (alignment unknown)
+// fp32 vectors of C channels, on 16 bytes where the rows are; absent: ones
 template <bool VEC>
 __device__ __forceinline__ void load_weights(const float *w, int lane, int lanes, int C, float (&x)[V]) {
+  if (w == nullptr) {
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
-    const int c = channel<VEC>(e, lane, lanes);
-    x[e] = w == nullptr ? 1.0f : c < C ? w[c] : 0.0f;
+    for (int e = 0; e < V; ++e) x[e] = 1.0f;
+    return;
   }
+  widen(request<float, VEC>(w, lane, lanes, C), x);
 }
 
 // Sums of N values over the threads that share a row: `lanes` lanes of a wave (a power of two up to 64), then the waves of
@@ -131,6 +137,14 @@ __global__ void __launch_bounds__(1024) norm_forward_kernel(const NormArgs a, in
   const Place p = place(a, lanes);
   const int waves = blockDim.x >> 6;
   RowSum<1> row_sum{buf};
+  if (p.first >= p.end) return;
+  Eight<T> next_x, next_h;
+  auto fetch = [&](int t) __attribute__((always_inline)) {
+    const int tt = t < p.end ? t : p.first;
+    next_x = request<T, VEC>(row_of<const T>(a.x, p.b, tt), p.lane, lanes, a.C);
+    if constexpr (POST) next_h = request<T, VEC>(row_of<const T>(a.h, p.b, tt), p.lane, lanes, a.C);
+  };
+  fetch(p.first + p.slot);
   float gw[V], wp[V];  // gate * w_post, w_pre
   if constexpr (POST) {
     float gate[V];
@@ -142,14 +156,14 @@ __global__ void __launch_bounds__(1024) norm_forward_kernel(const NormArgs a, in
   if constexpr (PRE) load_weights<VEC>(a.w_pre, p.lane, lanes, a.C, wp);
   const float per_c = 1.0f / (float)a.C;
   for (int t0 = p.first; t0 < p.end; t0 += p.slots) {  // (every thread takes every turn: there is a barrier in it)
-    const int t = t0 + p.slot;
-    const bool there = t < p.end;
-    const int tt = there ? t : p.first;
-    float x[V];
-    load<T, VEC>(row_of<const T>(a.x, p.b, tt), p.lane, lanes, a.C, x);
+    const int tt = t0 + p.slot;
+    const bool there = tt < p.end;
+    float x[V], h[V];
+    widen(next_x, x);
+    if constexpr (POST) widen(next_h, h);
+    if (t0 + p.slots < p.end) fetch(tt + p.slots);
     if constexpr (POST) {
-      float h[V], sum[1] = {0.0f};
-      load<T, VEC>(row_of<const T>(a.h, p.b, tt), p.lane, lanes, a.C, h);
+      float sum[1] = {0.0f};
 #pragma unroll
       for (int e = 0; e < V; ++e) sum[0] = __builtin_fmaf(h[e], h[e], sum[0]);
       row_sum(sum, lanes, waves);
@@ -177,6 +191,21 @@ __global__ void __launch_bounds__(1024) norm_backward_kernel(const NormArgs a, i
   const Place p = place(a, lanes);
   const int waves = blockDim.x >> 6;
   RowSum<6> row_sum{buf};
+  const bool has_dx = a.dx_out.p != nullptr;
+  constexpr bool AHEAD = VEC && sizeof(T) == 2;  // (else a row more takes the registers beyond the 128 that 1024 threads have)
+  Eight<T> next_x, next_g, next_h, next_d;
+  auto fetch = [&](int t) __attribute__((always_inline)) {
+    const int tt = t < p.end ? t : p.first;
+    if constexpr (PRE) {
+      next_x = request<T, VEC>(row_of<const T>(a.x_out, p.b, tt), p.lane, lanes, a.C);
+      next_g = request<T, VEC>(row_of<const T>(a.dy, p.b, tt), p.lane, lanes, a.C);
+    }
+    if constexpr (POST) next_h = request<T, VEC>(row_of<const T>(a.h, p.b, tt), p.lane, lanes, a.C);
+    if (has_dx) next_d = request<T, VEC>(row_of<const T>(a.dx_out, p.b, tt), p.lane, lanes, a.C);
+  };
+#pragma unroll
+  for (int e = 0; e < V; ++e) next_d.x[e] = (T)0.0f;
+  if (AHEAD && p.first < p.end) fetch(p.first + p.slot);
   float gw[V], wp[V], sa[V], sp[V];
   if constexpr (POST) {
     float gate[V];
@@ -189,22 +218,18 @@ __global__ void __launch_bounds__(1024) norm_backward_kernel(const NormArgs a, i
 #pragma unroll
   for (int e = 0; e < V; ++e) sa[e] = sp[e] = 0.0f;
   const float per_c = 1.0f / (float)a.C;
-  const bool has_dx = a.dx_out.p != nullptr;
   for (int t0 = p.first; t0 < p.end; t0 += p.slots) {
-    const int t = t0 + p.slot;
-    const bool there = t < p.end;
-    const int tt = there ? t : p.first;
+    const int tt = t0 + p.slot;
+    const bool there = tt < p.end;
     float x[V], g[V], h[V], d[V];
+    if constexpr (!AHEAD) fetch(tt);
     if constexpr (PRE) {
-      load<T, VEC>(row_of<const T>(a.x_out, p.b, tt), p.lane, lanes, a.C, x);
-      load<T, VEC>(row_of<const T>(a.dy, p.b, tt), p.lane, lanes, a.C, g);
+      widen(next_x, x);
+      widen(next_g, g);
     }
-    if constexpr (POST) load<T, VEC>(row_of<const T>(a.h, p.b, tt), p.lane, lanes, a.C, h);
-    if (has_dx) load<T, VEC>(row_of<const T>(a.dx_out, p.b, tt), p.lane, lanes, a.C, d);
-    else {
-#pragma unroll
-      for (int e = 0; e < V; ++e) d[e] = 0.0f;
-    }
+    if constexpr (POST) widen(next_h, h);
+    widen(next_d, d);
+    if (AHEAD && t0 + p.slots < p.end) fetch(tt + p.slots);
     // x'.x', g.x', h.h, and (gate w_post h).dx', .g, .x': mean(a h^) follows from the last three
     float s[6] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -274,42 +299,38 @@ __global__ void __launch_bounds__(1024) norm_backward_kernel(const NormArgs a, i
   }
 }
 
-// Adds up the partial rows: one thread per channel of 64, 16 groups of rows side by side.
+// Adds up the partial rows: a workgroup takes 16 channels of one sum (blockIdx.y: dw_post and the shared dgate, dw_pre, then dgate of each batch
+// entry), 64 groups of threads a 64th of the rows each, in an order that does not change.
 __global__ void __launch_bounds__(1024) norm_columns_kernel(const NormArgs a) {
-  __shared__ float s_sum[16][64];
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), group = threadIdx.x >> 6;
-  const long long plane = (long long)a.B * a.chunks * a.C;
+  __shared__ float s_sum[64][16];
+  const int cl = threadIdx.x & 15, group = threadIdx.x >> 4, c = blockIdx.x * 16 + cl, task = blockIdx.y;
   const int cc = min(c, a.C - 1);
-  auto join = [&](float x) __attribute__((always_inline)) -> float {
-    s_sum[group][threadIdx.x & 63] = x;
-    __syncthreads();
-    float t = 0.0f;
-    if (group == 0)
-      for (int g = 0; g < 16; ++g) t += s_sum[g][threadIdx.x & 63];
-    __syncthreads();
-    return t;
-  };
-  const bool write = group == 0 && c < a.C;
-  if (a.dw_post != nullptr || a.dgate != nullptr) {
-    float dw = 0.0f, all = 0.0f;
-    const float w = a.w_post[cc];
-    for (int b = 0; b < a.B; ++b) {
-      float x = 0.0f;
-      for (int k = group; k < a.chunks; k += 16) x += a.partial[((long long)b * a.chunks + k) * a.C + cc];
-      x = join(x);
-      const float gate = a.gate == nullptr ? 1.0f : a.gate[b * a.gate_sb + cc];
-      dw = __builtin_fmaf(gate, x, dw);
-      all += x;
-      if (write && a.dgate != nullptr && a.gate_sb != 0) a.dgate[(long long)b * a.gate_sb + c] = x * w;
-    }
-    if (write && a.dgate != nullptr && a.gate_sb == 0) a.dgate[c] = all * w;
-    if (write && a.dw_post != nullptr) a.dw_post[c] = dw;
+  const bool shared_gate = a.gate_sb == 0;
+  if (task == 0 ? a.dw_post == nullptr && (a.dgate == nullptr || !shared_gate) : task == 1 && a.dw_pre == nullptr) return;
+  const float *rows = a.partial;
+  long long n = (long long)a.B * a.chunks;
+  if (task == 1) rows += n * a.C;
+  if (task > 1) {
+    rows += (long long)(task - 2) * a.chunks * a.C;
+    n = a.chunks;
   }
-  if (a.dw_pre != nullptr) {
-    float x = 0.0f;
-    for (int k = group; k < a.B * a.chunks; k += 16) x += a.partial[plane + (long long)k * a.C + cc];
-    x = join(x);
-    if (write) a.dw_pre[c] = x;
+  const bool weigh = task == 0 && a.gate != nullptr && !shared_gate;  // dw_post = sum over b of gate_b A_b
+  float x = 0.0f;
+  for (long long k = group; k < n; k += 64) {
+    const float v = rows[k * a.C + cc];
+    x = weigh ? __builtin_fmaf(a.gate[k / a.chunks * a.gate_sb + cc], v, x) : x + v;
+  }
+  s_sum[group][cl] = x;
+  __syncthreads();
+  if (group != 0 || c >= a.C) return;
+  for (int g = 1; g < 64; ++g) x += s_sum[g][cl];
+  if (task == 0) {
+    if (a.dw_post != nullptr) a.dw_post[c] = a.gate != nullptr && shared_gate ? x * a.gate[c] : x;
+    if (a.dgate != nullptr && shared_gate) a.dgate[c] = x * a.w_post[c];
+  } else if (task == 1) {
+    a.dw_pre[c] = x;
+  } else {
+    a.dgate[(long long)(task - 2) * a.gate_sb + c] = x * a.w_post[c];
   }
 }
 
@@ -344,7 +365,10 @@ int backward(const NormArgs &a, hipStream_t stream) {
   if (a.h.p != nullptr && a.dy.p != nullptr) hipLaunchKernelGGL((norm_backward_kernel<T, VEC, true, true>), grid, block, 0, stream, a, s.lanes);
   else if (a.h.p != nullptr) hipLaunchKernelGGL((norm_backward_kernel<T, VEC, true, false>), grid, block, 0, stream, a, s.lanes);
   else hipLaunchKernelGGL((norm_backward_kernel<T, VEC, false, true>), grid, block, 0, stream, a, s.lanes);
-  if (a.partial != nullptr) hipLaunchKernelGGL(norm_columns_kernel, dim3((unsigned)((a.C + 63) / 64)), dim3(1024), 0, stream, a);
+  if (a.partial != nullptr) {
+    const unsigned tasks = 2 + (a.dgate != nullptr && a.gate_sb != 0 ? (unsigned)a.B : 0);
+    hipLaunchKernelGGL(norm_columns_kernel, dim3((unsigned)((a.C + 15) / 16), tasks), dim3(1024), 0, stream, a);
+  }
   return (int)hipGetLastError();
 }
 template <typename T>
@@ -355,15 +379,17 @@ int any(const NormArgs &a, bool back, hipStream_t stream) {
 
 }  // namespace
 
+// Workgroups per batch entry: one round of them.  Of waves on a CU, forward 20 (C1152 T8192 f16 19.5 us; 16 20.8, 32 26.8, with 12 23.8),
+// backward 12 where a row takes up to four waves, 16 beyond (C2048 T24960 bf16 118 us; with 16 124, with 8 127; C1152
+// 41; with 16, a round and a bit, 53; C4096 T8192 88; with 12 97).  Backward a workgroup has at least four rows, or its partial
+// column sums are a good part of what it moves (C1001 T999 f32 18 us; one row each 23).
 int norm_chunks(int B, int T, int C, int cus, bool backward) {
   const Shape s = shape_of(C);
   const int slots = s.threads / s.lanes;  // rows a workgroup has at a time
-  const long long waves = s.threads / 64;
-  // waves in flight that fill the device (backward: half, a partial row each is paid for)
-  const long long want = (long long)cus * (backward ? 16 : 32) / waves;
-  long long chunks = (want + B - 1) / B;
-  const long long most = (T + slots - 1) / slots;
-  if (chunks > most) chunks = most;
+  const int waves = s.threads / 64, on_cu = (backward ? (waves <= 4 ? 12 : 16) : 20) / waves;
+  const long long want = (long long)cus * (on_cu > 1 ? on_cu : 1) / B;
+  const long long least_rows = backward ? 4ll * slots : slots, most = (T + least_rows - 1) / least_rows;
+  const long long chunks = want < most ? want : most;
   return chunks < 1 ? 1 : (int)chunks;
 }
 
