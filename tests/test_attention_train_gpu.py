@@ -306,3 +306,14 @@ def test_refusals(tracea_gpu):
     refused(capi.INVALID_PARAMS, bwd, q, k, k, q, lse, q, dk=both, dv=both)
     with pytest.raises(TypeError):
         fwd(q.long(), k, k)
+
+
+def test_the_road_a_call_takes(tracea_gpu):
+    """Launches of a call: the forward pass alone, or with the join of a split key axis; backward the row statistics and the gradients,
+    or with the sums of dK and dV from parts of the rows.  Either road against the formulas."""
+    from helpers import launches
+    for b, hq, hk, sq, sk, d, fwd, bwd in ((1, 2, 1, 1, 4000, 128, 2, 2), (1, 12, 12, 256, 256, 64, 1, 2), (1, 16, 1, 500, 500, 64, 1, 3),
+                                           (1, 20, 1, 300, 300, 128, 1, 3)):
+        q, k, v, do, o, lse, dq, dk, dv = check(tracea_gpu, b, hq, hk, sq, sk, d)
+        assert launches(lambda: tracea_gpu.attention_forward(q, k, v, out=o, lse=lse)) == fwd, (hq, hk, sq, sk, d)
+        assert launches(lambda: tracea_gpu.attention_backward(q, k, v, o, lse, do, dq=dq, dk=dk, dv=dv)) == bwd, (hq, hk, sq, sk, d)

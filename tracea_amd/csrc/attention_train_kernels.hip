@@ -173,7 +173,7 @@ __device__ __forceinline__ unsigned fresh(unsigned x) {
   return x;
 }
 
-// max / sum over the four 16-lane groups
+// max / sum over the four 16-lane groups, through LDS
 __device__ __forceinline__ float groups_max(float x) {
   x = fmaxf(x, __shfl_xor(x, 16, 64));
   return fmaxf(x, __shfl_xor(x, 32, 64));
@@ -282,31 +282,44 @@ __device__ __forceinline__ float ds_scale(const AttentionTrainArgs &a, int bh, i
 // all its keys, not the largest score, and 2^8 is far inside the range of the 16-bit operands.
 constexpr float LAZY_MAX = 8.0f;
 
-template <int DT, int DL, int DU, int WAVES>
+// Over a lane's own value and those of the other three 16-lane groups, by exchanges in the vector ALU: v_permlane16_swap trades the
+// odd 16-lane rows of its first operand for the even ones of its second, v_permlane32_swap the halves; given one value
+// twice, the two results are a lane's own and its partner's, in one order or the other.  (As instructions: the builtin hands back its first
+// result twice.  The s_nop covers the wait between a vector-ALU write and the swap.)
+__device__ __forceinline__ float groups_max_valu(float x) {
+  float a0 = x, a1 = x;
+  asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a0), "+v"(a1));
+  float b0 = fmaxf(a0, a1), b1 = b0;
+  asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(b0), "+v"(b1));
+  return fmaxf(b0, b1);
+}
+
+// A wave's scores of tile t + 1 are computed under the exponentials of tile t, and P V of tile t under the maximum over t + 1, so
+// that K is a tile ahead of V.  SG = 2: two waves share 32 rows and walk every other tile of 64 keys; their states are joined at the end.
+template <int DT, int DL, int DU, int WAVES, int SG>
 __global__ void __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 attention_train_forward_kernel(const AttentionTrainArgs a) {
   using T = Tile<DL>;
-  constexpr int BR = 32 * WAVES, KS = DU / 32, DB = DU / 16, KB = TILE / 16;
-  __shared__ __attribute__((aligned(1024))) unsigned char sK[4 * T::BYTES];  // two tiles of K, two of V
-  constexpr unsigned V_AT = 2 * T::BYTES;
+  constexpr int BR = 32 * WAVES / SG, KS = DU / 32, DB = DU / 16, KB = TILE / 16, STEP = SG * TILE;  // keys of a step
+  constexpr unsigned SIDE = SG * T::BYTES, V_AT = 2 * SIDE;  // two steps of K, two of V
+  __shared__ __attribute__((aligned(1024))) unsigned char sK[4 * SIDE];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int r16 = lane & 15, g4 = lane >> 4;
+  const int r16 = lane & 15, g4 = lane >> 4, group = wave / SG, kg = wave % SG;
   const int blocks = (a.G * a.Sq + BR - 1) / BR;
   const Slot slot = slot_of(a, blockIdx.x, blocks);
   const int bh = slot.bh, blk = blocks - 1 - slot.blk;  // most keys under a causal mask first
   const Rows w = rows_of(a, bh);
   const int rows = a.G * w.lq;
-  const int r_wave = blk * BR + wave * 32;
+  const int r_wave = blk * BR + group * 32;
 
   const int last_row = min(blk * BR + BR, rows) - 1;
   int keys = 0;  // that any row of the block sees
   if (last_row >= blk * BR) keys = a.causal ? min(w.lk, query_of(a, last_row) + w.off + 1) : w.lk;
-  int tiles = keys > 0 ? (keys + TILE - 1) / TILE : 0;
-  int t0 = 0;
+  int steps = keys > 0 ? (keys + STEP - 1) / STEP : 0, s0 = 0;
   if (a.splits > 1) {
-    t0 = (int)blockIdx.y * a.tiles_per_split;
-    tiles = min(tiles, t0 + a.tiles_per_split);
+    s0 = (int)blockIdx.y * a.steps_per_split;
+    steps = min(steps, s0 + a.steps_per_split);
   }
 
   int q_last[2];  // the last key that the lane's queries see
@@ -323,28 +336,33 @@ attention_train_forward_kernel(const AttentionTrainArgs a) {
       if (a.negate) qf[qb][ks] ^= 0x80008000u;
     }
   }
-  // of the wave: keys that some row sees, and the first that not every row sees
+  // of the wave: keys that some row sees, and the first that not every row sees; as steps: those with a tile of its own that some row
+  // sees, and those whose tile every row sees whole
   int wave_keys = 0, wave_full = 0;
   if (r_wave < rows) {
     const int r_end = min(r_wave + 32, rows) - 1;
     wave_keys = a.causal ? min(w.lk, query_of(a, r_end) + w.off + 1) : w.lk;
-    wave_full = r_wave + 32 > rows ? 0 : a.causal ? min(w.lk, query_of(a, r_wave) + w.off + 1) : w.lk;
+    wave_full = a.causal ? min(w.lk, query_of(a, r_wave) + w.off + 1) : w.lk;  // (what rows past the end hold is dropped)
   }
+  const int wave_steps = wave_keys > kg * TILE ? min(steps, (wave_keys - kg * TILE + STEP - 1) / STEP) : 0;
+  const int full_steps = wave_full >= (kg + 1) * TILE ? min(wave_steps, (wave_full - kg * TILE) / TILE / SG + ((wave_full - kg * TILE) / TILE % SG != 0)) : 0;
 
   const unsigned short *Kg = slice(a.k, w.b, w.hk), *Vg = slice(a.v, w.b, w.hk);
-  auto request = [&](int t) __attribute__((always_inline)) {
-    const int left = w.lk - t * TILE, at = (t & 1) * T::BYTES, lane_ = fresh(lane);
-    const unsigned kss = (unsigned)a.k.ss * 2u, vss = (unsigned)a.v.ss * 2u;
-    const unsigned short *kt = Kg + (long long)t * TILE * a.k.ss, *vt = Vg + (long long)t * TILE * a.v.ss;
-    if (left >= TILE) {
-      constexpr int STEP = WAVES * 64 / T::CH;
-      load_tile<DL, WAVES>(kt, (long long)kss * STEP, sK + at, a.D, lane_, wave, [&](int row) { return row * kss; });
-      load_tile<DL, WAVES>(vt, (long long)vss * STEP, sK + V_AT + at, a.D, lane_, wave, [&](int row) { return row * vss; });
-    } else {
-      load_tile_any<DL, WAVES>(kt, sK + at, a.D, lane_, wave, [&](int row) { return row < left ? row * kss : BEYOND; });
-      load_tile_any<DL, WAVES>(vt, sK + V_AT + at, a.D, lane_, wave, [&](int row) { return row < left ? row * vss : BEYOND; });
+  auto request = [&](const unsigned short *base, long long ss, int step, unsigned side) __attribute__((always_inline)) {
+    const int lane_ = fresh(lane);
+    const unsigned bytes = (unsigned)ss * 2u;
+#pragma unroll
+    for (int g = 0; g < SG; ++g) {
+      const int tile = step * SG + g, left = w.lk - tile * TILE;
+      const unsigned char *dst = sK + side + (unsigned)(step & 1) * SIDE + g * T::BYTES;
+      const unsigned short *at = base + (long long)tile * TILE * ss;
+      constexpr int APART = WAVES * 64 / T::CH;
+      if (left >= TILE) load_tile<DL, WAVES>(at, (long long)bytes * APART, dst, a.D, lane_, wave, [&](int row) { return row * bytes; });
+      else load_tile_any<DL, WAVES>(at, dst, a.D, lane_, wave, [&](int row) { return row < left ? row * bytes : BEYOND; });
     }
   };
+  auto request_k = [&](int step) __attribute__((always_inline)) { request(Kg, a.k.ss, step, 0); };
+  auto request_v = [&](int step) __attribute__((always_inline)) { request(Vg, a.v.ss, step, V_AT); };
 
   f32x4 o[2][DB];
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};  // reference (log2 units) and sum of the lane's keys
@@ -353,39 +371,23 @@ attention_train_forward_kernel(const AttentionTrainArgs a) {
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[qb][d] = f32x4{0, 0, 0, 0};
 
-  const unsigned rows0 = rows_base<DL>(sK, r16, g4), cols0 = columns_base<DL>(sK, r16, g4);
-  auto compute = [&](int t, auto edge_tag) __attribute__((always_inline)) {
-    constexpr bool EDGE = decltype(edge_tag)::value;
-    const unsigned rows_at = rows0 + (unsigned)(t & 1) * T::BYTES, cols_at = cols0 + (unsigned)(t & 1) * T::BYTES;
-    f32x4 z[2][KB];
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-      for (int qb = 0; qb < 2; ++qb) z[qb][kb] = f32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        const u32x4 kf = read_rows<DL>(rows_at, 0, kb, ks);
-#pragma unroll
-        for (int qb = 0; qb < 2; ++qb) z[qb][kb] = Mfma16<DT>::run(kf, qf[qb][ks], z[qb][kb]);
-      }
-    fence();
+  const unsigned rows0 = rows_base<DL>(sK, r16, g4) + kg * T::BYTES, cols0 = columns_base<DL>(sK, r16, g4) + kg * T::BYTES;
+  // What a row does not see becomes -inf; the largest score of the lane's in tile `step`, one value at a time.
+  auto take_max = [&](int step, int v, f32x4 (&z)[2][KB], float (&mx)[2], auto edge_tag) __attribute__((always_inline)) {
+    const int qb = v >> 4, kb = (v >> 2) & 3, e = v & 3;
+    if constexpr (decltype(edge_tag)::value)
+      z[qb][kb][e] = (step * SG + kg) * TILE + kb * 16 + g4 * 4 + e > q_last[qb] ? -INFINITY : z[qb][kb][e];
+    mx[qb] = fmaxf(mx[qb], z[qb][kb][e]);
+  };
+  // A row needs one reference for all its keys, not the largest score: it moves when a tile exceeds it by LAZY_MAX powers of two.
+  auto move_reference = [&](const float (&mx)[2]) __attribute__((always_inline)) {
     bool moved = false;
     float alpha[2];
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) {
-      float mx = -INFINITY;
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if constexpr (EDGE) z[qb][kb][e] = t * TILE + kb * 16 + g4 * 4 + e > q_last[qb] ? -INFINITY : z[qb][kb][e];
-          mx = fmaxf(mx, z[qb][kb][e]);
-        }
-      mx = groups_max(mx) * a.scale_log2;
-      const bool mv = mx > m[qb] + LAZY_MAX;  // (a first score above -inf always moves it)
-      const float mn = mv ? mx : m[qb];
+      const float top = groups_max_valu(mx[qb]) * a.scale_log2;
+      const bool mv = top > m[qb] + LAZY_MAX;  // (a first score above -inf always moves it)
+      const float mn = mv ? top : m[qb];
       alpha[qb] = mv ? __builtin_amdgcn_exp2f(m[qb] - mn) : 1.0f;
       m[qb] = mn;
       moved |= mv;
@@ -398,54 +400,151 @@ attention_train_forward_kernel(const AttentionTrainArgs a) {
         for (int d = 0; d < DB; ++d) o[qb][d] *= alpha[qb];
       }
     }
-    u32x4 pf[2][2];
+  };
+
+  // One step: P of the scores `z` of step t, its P V, and, unless LAST, the scores `zn` of step t + 1 (EDGE: masked) and their maximum.
+  // One chunk per first-operand fragment, read AHEAD chunks before.
+  constexpr int AHEAD = 2;
+  auto iterate = [&](int t, f32x4 (&z)[2][KB], f32x4 (&zn)[2][KB], auto edge_tag, auto last_tag) __attribute__((always_inline)) {
+    constexpr bool LAST = decltype(last_tag)::value;
+    constexpr int N1 = LAST ? 0 : KB * KS, N2 = 2 * DB, N = N1 + N2;
+    const unsigned at_k = fresh(rows0) + (unsigned)((t + 1) & 1) * SIDE, at_v = fresh(cols0) + (unsigned)(t & 1) * SIDE;
+    u32x4 frag[AHEAD + 1], pf[2][2];
+    float mx[2] = {-INFINITY, -INFINITY}, ref[2], sum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) ref[qb] = m[qb] == -INFINITY ? 0.0f : m[qb];  // (nothing visible yet: exp2(-inf) = 0)
+    auto read = [&](auto tag) __attribute__((always_inline)) {
+      constexpr int i = decltype(tag)::value;
+      if constexpr (i < N1) frag[i % (AHEAD + 1)] = read_rows<DL>(at_k, 0, i % KB, i / KB);
+      else if constexpr (i < N) frag[i % (AHEAD + 1)] = read_columns<DL>(at_v, V_AT, (i - N1) / DB, (i - N1) % DB);
+    };
+    auto probability = [&](int v) __attribute__((always_inline)) {
+      const int qb = v >> 4, kb = (v >> 2) & 3, e = v & 3;
+      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z[qb][kb][e], a.scale_log2, -ref[qb]));
+      sum[qb] += p;
+      z[qb][kb][e] = p;
+      if ((v & 7) == 7) pf[qb][kb >> 1] = pack_operand<DT>(z[qb][kb - 1], z[qb][kb]);
+    };
+    static_for<0, AHEAD>([&](auto tag) __attribute__((always_inline)) { read(tag); });
+    if constexpr (LAST) {
+#pragma unroll
+      for (int v = 0; v < 32; ++v) probability(v);
+    }
+    static_for<0, N>([&](auto tag) __attribute__((always_inline)) {
+      constexpr int i = decltype(tag)::value;
+      const u32x4 &f = frag[i % (AHEAD + 1)];
+      read(std::integral_constant<int, i + AHEAD>{});
+      if constexpr (i < N1) {
+        constexpr int kb = i % KB, ks = i / KB, PER = (32 + N1 - 1) / (LAST ? 1 : N1);
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) zn[qb][kb] = Mfma16<DT>::run(f, qf[qb][ks], ks == 0 ? f32x4{0, 0, 0, 0} : zn[qb][kb]);
+#pragma unroll
+        for (int v = i * PER; v < (i + 1) * PER && v < 32; ++v) probability(v);
+      } else {
+        constexpr int j = i - N1, s = j / DB, d = j % DB, PER = (32 + N2 - 1) / N2;
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) o[qb][d] = Mfma16<DT>::run(f, pf[qb][s], o[qb][d]);
+        if constexpr (!LAST) {
+#pragma unroll
+          for (int v = j * PER; v < (j + 1) * PER && v < 32; ++v) take_max(t + 1, v, zn, mx, edge_tag);
+        }
+      }
+      fence();
+    });
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) l[qb] += sum[qb];
+    if constexpr (!LAST) move_reference(mx);
+  };
+  // Step t: the scores of t are there; K of t + 1 and V of t have arrived, K of t + 2 and V of t + 1 go out.
+  auto head = [&](int t) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    __syncthreads();
+    if (t + 2 < steps) request_k(t + 2);
+    if (t + 1 < steps) request_v(t + 1);
+  };
+
+  f32x4 za[2][KB], zb[2][KB];
+  int t = s0;
+  if (t < steps) {
+    request_k(t);
+    request_v(t);
+    if (t + 1 < steps) request_k(t + 1);
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    __syncthreads();
+    if (t < wave_steps) {  // the first scores, on their own
+      const unsigned at_k = fresh(rows0) + (unsigned)(t & 1) * SIDE;
+      float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          const u32x4 kf = read_rows<DL>(at_k, 0, kb, ks);
+#pragma unroll
+          for (int qb = 0; qb < 2; ++qb) za[qb][kb] = Mfma16<DT>::run(kf, qf[qb][ks], ks == 0 ? f32x4{0, 0, 0, 0} : za[qb][kb]);
+        }
+#pragma unroll
+      for (int v = 0; v < 32; ++v) take_max(t, v, za, mx, std::true_type{});
+      move_reference(mx);
+    }
+  }
+  const int whole = full_steps - 1, last = wave_steps - 1;  // steps whose next one is whole; the wave's last
+  auto back = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) za[qb][kb] = zb[qb][kb];
+  };
+  for (; t + 1 < whole; t += 2) {
+    head(t);
+    iterate(t, za, zb, std::false_type{}, std::false_type{});
+    head(t + 1);
+    iterate(t + 1, zb, za, std::false_type{}, std::false_type{});
+  }
+  for (; t < last; ++t) {
+    head(t);
+    iterate(t, za, zb, std::true_type{}, std::false_type{});
+    back();
+  }
+  if (t == last && t >= s0) {
+    head(t);
+    iterate(t, za, zb, std::true_type{}, std::true_type{});
+    ++t;
+  }
+  for (; t < steps; ++t) head(t);  // (tiles that only other waves see)
+
+  if constexpr (SG == 2) {  // the second wave's state to the first
+    f32x4 *const at = (f32x4 *)sK + group * (2 * DB + 1) * 64 + lane;
+    __syncthreads();
+    if (kg == 1) {
+#pragma unroll
+      for (int i = 0; i < 2 * DB; ++i) at[i * 64] = o[i / DB][i % DB];
+      at[2 * DB * 64] = f32x4{m[0], m[1], l[0], l[1]};
+    }
+    __syncthreads();
+    if (kg == 1) return;
+    const f32x4 ml = at[2 * DB * 64];
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) {
-      const float ref = m[qb] == -INFINITY ? 0.0f : m[qb];  // (nothing visible yet: exp2(-inf) = 0)
-      float sum = 0.0f;
+      const float top = fmaxf(m[qb], ml[qb]), ref = top == -INFINITY ? 0.0f : top;
+      const float f0 = __builtin_amdgcn_exp2f(m[qb] - ref), f1 = __builtin_amdgcn_exp2f(ml[qb] - ref);
+      m[qb] = top;
+      l[qb] = f0 * l[qb] + f1 * ml[2 + qb];
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          z[qb][kb][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[qb][kb][e], a.scale_log2, -ref));
-          sum += z[qb][kb][e];
-        }
-      l[qb] += sum;
-#pragma unroll
-      for (int s = 0; s < 2; ++s) pf[qb][s] = pack_operand<DT>(z[qb][2 * s], z[qb][2 * s + 1]);
+      for (int d = 0; d < DB; ++d) o[qb][d] = f0 * o[qb][d] + f1 * at[(qb * DB + d) * 64];
     }
-    fence();
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        const u32x4 vf = read_columns<DL>(cols_at, V_AT, s, d);
-#pragma unroll
-        for (int qb = 0; qb < 2; ++qb) o[qb][d] = Mfma16<DT>::run(vf, pf[qb][s], o[qb][d]);
-      }
-  };
-  auto head = [&](int t) __attribute__((always_inline)) {
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this tile
-    __syncthreads();
-    if (t + 1 < tiles) request(t + 1);
-  };
-  // tiles that every row of the wave sees whole, then the others (a wave takes part in the loads of tiles that none sees)
-  int t = t0;
-  if (t < tiles) request(t);
-  for (const int end = min(tiles, wave_full / TILE); t < end; ++t) {
-    head(t);
-    compute(t, std::false_type{});
-  }
-  for (; t < tiles; ++t) {
-    head(t);
-    if (t * TILE < wave_keys) compute(t, std::true_type{});
   }
 
 #pragma unroll
   for (int qb = 0; qb < 2; ++qb) {
     const int r = r_wave + qb * 16 + r16;
-    const float sum = groups_sum(l[qb]);
+    float sum = groups_sum(l[qb]);
     if (r >= a.G * a.Sq) continue;
+    if (r >= rows) {  // a query behind its sequence's length
+      m[qb] = -INFINITY;
+      sum = 0.0f;
+#pragma unroll
+      for (int d = 0; d < DB; ++d) o[qb][d] = f32x4{0, 0, 0, 0};
+    }
     if (a.splits > 1) {
       const long long at = ((long long)blockIdx.y * a.B * a.Hk + bh) * a.rows_pad + r;
       if (g4 == 0) {
@@ -470,27 +569,29 @@ attention_train_forward_kernel(const AttentionTrainArgs a) {
   }
 }
 
-// Joins the partial results of a split key axis: one row per DU / 4 lanes.
+// Joins the partial results of a split key axis: a row per 32 lanes, which load one part's reference and sum each (at most 32
+// parts) and 4 columns of every part's o.
 template <int DT, int DU>
 __global__ void __launch_bounds__(256) attention_train_join_kernel(const AttentionTrainArgs a) {
-  constexpr int LPR = 32;  // lanes per row, 4 columns each
-  const long long id = ((long long)blockIdx.x * 256 + threadIdx.x) / LPR;
-  const int c = (threadIdx.x % LPR) * 4;
-  const int per = a.G * a.Sq;
+  const long long id = ((long long)blockIdx.x * 256 + threadIdx.x) / 32;
+  const int lane = threadIdx.x & 31, c = lane * 4, per = a.G * a.Sq;
   if (id >= (long long)a.B * a.Hk * per) return;
   const int bh = (int)(id / per), r = (int)(id - (long long)bh * per);
   const Rows w = rows_of(a, bh);
   const long long plane = (long long)a.B * a.Hk * a.rows_pad, at = (long long)bh * a.rows_pad + r;
-  float m = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[2 * (s * plane + at)]);
-  const float ref = m == -INFINITY ? 0.0f : m;
-  float sum = 0.0f;
+  const float own_m = lane < a.splits ? a.part_ml[2 * (lane * plane + at)] : -INFINITY;
+  const float own_l = lane < a.splits ? a.part_ml[2 * (lane * plane + at) + 1] : 0.0f;
+  float m = own_m;
+#pragma unroll
+  for (int s = 1; s < 32; s <<= 1) m = fmaxf(m, __shfl_xor(m, s, 32));
+  const float own_f = __builtin_amdgcn_exp2f(own_m - (m == -INFINITY ? 0.0f : m));
+  float sum = own_f * own_l;
+#pragma unroll
+  for (int s = 1; s < 32; s <<= 1) sum += __shfl_xor(sum, s, 32);
   f32x4 o = {0, 0, 0, 0};
-  for (int s = 0; s < a.splits; ++s) {
-    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * (s * plane + at)] - ref);
-    sum += f * a.part_ml[2 * (s * plane + at) + 1];
-    if (c < a.D) o += f * *(const f32x4 *)(a.part_o + (s * plane + at) * DU + c);
-  }
+  const float *from = a.part_o + at * DU + (c < a.D ? c : 0);
+#pragma unroll 8
+  for (int s = 0; s < a.splits; ++s) o += __shfl(own_f, s, 32) * *(const f32x4 *)(from + s * plane * DU);
   const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
   if (c < a.D) *(u32x2 *)((unsigned short *)a.o.p + row_at(a, a.o, w, r) + c) = pack_result<DT>(o, inv);
   if (c == 0) {
@@ -979,8 +1080,9 @@ __global__ void __launch_bounds__(256) attention_train_sum_kernel(const Attentio
 template <int DT, int DL, int DU>
 int forward(const AttentionTrainArgs &a, hipStream_t stream) {
   constexpr int W = 4;
-  const unsigned blocks = (unsigned)((a.G * a.Sq + 32 * W - 1) / (32 * W)) * (unsigned)(a.B * a.Hk);
-  hipLaunchKernelGGL((attention_train_forward_kernel<DT, DL, DU, W>), dim3(blocks, (unsigned)a.splits), dim3(W * 64), 0, stream, a);
+  const dim3 grid((unsigned)((a.G * a.Sq + a.block - 1) / a.block) * (unsigned)(a.B * a.Hk), (unsigned)a.splits);
+  if (a.block == 32 * W) hipLaunchKernelGGL((attention_train_forward_kernel<DT, DL, DU, W, 1>), grid, dim3(W * 64), 0, stream, a);
+  else hipLaunchKernelGGL((attention_train_forward_kernel<DT, DL, DU, W, 2>), grid, dim3(W * 64), 0, stream, a);
   if (a.splits > 1) {
     const long long rows = (long long)a.B * a.Hk * a.G * a.Sq;
     hipLaunchKernelGGL((attention_train_join_kernel<DT, DU>), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, stream, a);

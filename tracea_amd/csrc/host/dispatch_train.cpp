@@ -95,6 +95,36 @@ bool rows_in_place(const View &t, long long D) {
          t.stride[1] >= 0 && t.stride[2] >= 0 && aligned(t.ptr, 16);
 }
 
+// Rows of a workgroup and parts of the keys for the forward pass, by the least of this estimate (us) over the candidates, in the terms of
+// plan_backward: few rows over many keys leave CUs idle unless the keys are shared, by two waves of a workgroup (blocks of 64 rows) or by
+// workgroups, whose results a second launch joins.  Fitted to 25 shapes with every candidate timed; its choice is 1 % behind the best on
+// average and 5 % at worst.  Best / unsplit blocks of 128, us: B1 H12 S1024 D64 causal 15.4 / 21.9 (blocks of 64), B8 H32:8 one query over 8192 keys
+// 49 / 180 (8 parts), B1 H8 1000 queries over 5000 keys D64 30 / 63 (4 parts).
+struct ForwardPlan {
+  int block, splits;
+};
+ForwardPlan plan_forward(long long heads, long long rows, long long keys, int width, bool half, int cus) {
+  ForwardPlan best{128, 1};
+  double least = 1e300;
+  const double f = width / 128.0, tiles = (double)((keys + 63) / 64), seen = half ? 0.5 : 1.0;
+  for (int block : {128, 64})
+    for (int splits : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+      const int step = block == 64 ? 2 : 1;  // tiles
+      const double bytes = 2.0 * splits * heads * rows * width * 4;
+      if (tiles < step || (splits > 1 && (tiles < step * splits || bytes > (1 << 30)))) continue;
+      const double lat = (block == 128 ? 1.26 : 0.85) * (0.24 + 0.76 * f), thr = (block == 128 ? 0.72 : 0.89) * f / cus;
+      const double walk = tiles / splits, fill = rows < block ? 0.3 + 0.7 * rows / block : 1.0;
+      const double total = thr * fill * ((rows + block - 1) / block) * heads * splits * (walk * seen + 3);
+      const double longest = std::max(lat * (walk + 3), 4.0 * heads * keys * width * seen / 6.1e6);
+      const double time = std::max(total, longest) + 0.42 * std::min(total, longest) + (splits > 1 ? 3.3 + bytes / 5.5e6 : 0.0);
+      if (time < least) {
+        least = time;
+        best = {block, splits};
+      }
+    }
+  return best;
+}
+
 // Columns of a workgroup and parts of the rows for dK and dV, by the least of this estimate (us) over the candidates.  A tile of 64 costs a
 // workgroup of four waves `lat` while it walks and a CU `thr` of its throughput; blocks of 64 columns, two waves on 32, do half the
 // work of blocks of 128 in 0.72 of the time.  The device is busy for the sum of all walks, but no shorter than the longest.  Parts are written and read as
@@ -211,25 +241,20 @@ TraceaStatus run_attention(const Attention &c, bool from_copies) {
   a.rows_pad = (int)rows_pad;
   a.order = c.q_len != nullptr || c.k_len != nullptr ? 2 : c.causal ? 1 : 0;
   a.splits = 1;
-  const int cus = (int)device_limits().cus;
   if (!c.backward) {
     if (Sq == 0) return TRACEA_SUCCESS;
-    // Few rows over many keys leave most CUs idle: the keys are split over workgroups and a second kernel joins the parts.
-    const long long blocks = (G * Sq + 127) / 128 * B * Hk, tiles = (Sk + 63) / 64;
-    if (blocks < cus && tiles >= 8) {
-      long long splits = 2 * cus / blocks;
-      if (splits > tiles / 4) splits = tiles / 4;
-      const long long per = (tiles + splits - 1) / splits;
-      splits = (tiles + per - 1) / per;
-      const long long width = D <= 64 ? 64 : D <= 96 ? 96 : 128;
-      const size_t rows = (size_t)(splits * B * Hk * rows_pad);
-      if (splits > 1) {
-        a.part_o = (float *)train_scratch(c.q.device, c.stream, rows * (size_t)(width + 2) * 4);
-        if (a.part_o != nullptr) {  // (else unsplit: slower, the same result to rounding)
-          a.part_ml = a.part_o + rows * width;
-          a.splits = (int)splits;
-          a.tiles_per_split = (int)per;
-        }
+    const int width = D <= 64 ? 64 : D <= 96 ? 96 : 128;
+    const ForwardPlan plan = plan_forward(B * Hk, G * Sq, Sk, width, a.causal && Sq == Sk, (int)device_limits().cus);
+    a.block = plan.block;
+    if (plan.splits > 1) {
+      const long long keys = a.block == 64 ? 128 : 64, steps = (Sk + keys - 1) / keys, per = (steps + plan.splits - 1) / plan.splits;
+      const long long splits = (steps + per - 1) / per;
+      const size_t n = (size_t)(splits * B * Hk * rows_pad);
+      a.part_o = (float *)train_scratch(c.q.device, c.stream, n * (size_t)(width + 2) * 4);
+      if (a.part_o != nullptr) {  // (else unsplit: slower, the same result to rounding)
+        a.part_ml = a.part_o + n * width;
+        a.splits = (int)splits;
+        a.steps_per_split = (int)per;
       }
     }
     return hip_status("attention forward launch", launch_attention_train_forward(a, c.q.dtype, c.stream));
