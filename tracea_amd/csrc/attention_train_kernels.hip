@@ -295,12 +295,13 @@ __device__ __forceinline__ float groups_max_valu(float x) {
 }
 
 // A wave's scores of tile t + 1 are computed under the exponentials of tile t, and P V of tile t under the maximum over t + 1, so
-// that K is a tile ahead of V.  SG = 2: two waves share 32 rows and walk every other tile of 64 keys; their states are joined at the end.
-template <int DT, int DL, int DU, int WAVES, int SG>
+// that K is a tile ahead of V.  SG = 2: two waves share their rows and walk every other tile of 64 keys; their states are joined at the end.  A wave has 16 NQ rows:
+// 32, or 16 for a token or two of some heads, where the empty half would be most of what it waits for.
+template <int DT, int DL, int DU, int WAVES, int SG, int NQ>
 __global__ void __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 attention_train_forward_kernel(const AttentionTrainArgs a) {
   using T = Tile<DL>;
-  constexpr int BR = 32 * WAVES / SG, KS = DU / 32, DB = DU / 16, KB = TILE / 16, STEP = SG * TILE;  // keys of a step
+  constexpr int WR = 16 * NQ, BR = WR * WAVES / SG, KS = DU / 32, DB = DU / 16, KB = TILE / 16, STEP = SG * TILE;  // keys of a step
   constexpr unsigned SIDE = SG * T::BYTES, V_AT = 2 * SIDE;  // two steps of K, two of V
   __shared__ __attribute__((aligned(1024))) unsigned char sK[4 * SIDE];
 
@@ -311,7 +312,7 @@ attention_train_forward_kernel(const AttentionTrainArgs a) {
   const int bh = slot.bh, blk = blocks - 1 - slot.blk;  // most keys under a causal mask first
   const Rows w = rows_of(a, bh);
   const int rows = a.G * w.lq;
-  const int r_wave = blk * BR + group * 32;
+  const int r_wave = blk * BR + group * WR;
 
   const int last_row = min(blk * BR + BR, rows) - 1;
   int keys = 0;  // that any row of the block sees
@@ -322,10 +323,10 @@ attention_train_forward_kernel(const AttentionTrainArgs a) {
     steps = min(steps, s0 + a.steps_per_split);
   }
 
-  int q_last[2];  // the last key that the lane's queries see
-  u32x4 qf[2][KS];
+  int q_last[NQ];  // the last key that the lane's queries see
+  u32x4 qf[NQ][KS];
 #pragma unroll
-  for (int qb = 0; qb < 2; ++qb) {
+  for (int qb = 0; qb < NQ; ++qb) {
     const int r = r_wave + qb * 16 + r16;
     const bool there = r < rows;
     q_last[qb] = !there ? -1 : a.causal ? min(w.lk - 1, query_of(a, r) + w.off) : w.lk - 1;
@@ -340,7 +341,7 @@ attention_train_forward_kernel(const AttentionTrainArgs a) {
   // sees, and those whose tile every row sees whole
   int wave_keys = 0, wave_full = 0;
   if (r_wave < rows) {
-    const int r_end = min(r_wave + 32, rows) - 1;
+    const int r_end = min(r_wave + WR, rows) - 1;
     wave_keys = a.causal ? min(w.lk, query_of(a, r_end) + w.off + 1) : w.lk;
     wave_full = a.causal ? min(w.lk, query_of(a, r_wave) + w.off + 1) : w.lk;  // (what rows past the end hold is dropped)
   }
@@ -364,27 +365,30 @@ attention_train_forward_kernel(const AttentionTrainArgs a) {
   auto request_k = [&](int step) __attribute__((always_inline)) { request(Kg, a.k.ss, step, 0); };
   auto request_v = [&](int step) __attribute__((always_inline)) { request(Vg, a.v.ss, step, V_AT); };
 
-  f32x4 o[2][DB];
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};  // reference (log2 units) and sum of the lane's keys
+  f32x4 o[NQ][DB];
+  float m[NQ], l[NQ];  // reference (log2 units) and sum of the lane's keys
 #pragma unroll
-  for (int qb = 0; qb < 2; ++qb)
+  for (int qb = 0; qb < NQ; ++qb) {
+    m[qb] = -INFINITY;
+    l[qb] = 0.0f;
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[qb][d] = f32x4{0, 0, 0, 0};
+  }
 
   const unsigned rows0 = rows_base<DL>(sK, r16, g4) + kg * T::BYTES, cols0 = columns_base<DL>(sK, r16, g4) + kg * T::BYTES;
   // What a row does not see becomes -inf; the largest score of the lane's in tile `step`, one value at a time.
-  auto take_max = [&](int step, int v, f32x4 (&z)[2][KB], float (&mx)[2], auto edge_tag) __attribute__((always_inline)) {
+  auto take_max = [&](int step, int v, f32x4 (&z)[NQ][KB], float (&mx)[NQ], auto edge_tag) __attribute__((always_inline)) {
     const int qb = v >> 4, kb = (v >> 2) & 3, e = v & 3;
     if constexpr (decltype(edge_tag)::value)
       z[qb][kb][e] = (step * SG + kg) * TILE + kb * 16 + g4 * 4 + e > q_last[qb] ? -INFINITY : z[qb][kb][e];
     mx[qb] = fmaxf(mx[qb], z[qb][kb][e]);
   };
   // A row needs one reference for all its keys, not the largest score: it moves when a tile exceeds it by LAZY_MAX powers of two.
-  auto move_reference = [&](const float (&mx)[2]) __attribute__((always_inline)) {
+  auto move_reference = [&](const float (&mx)[NQ]) __attribute__((always_inline)) {
     bool moved = false;
-    float alpha[2];
+    float alpha[NQ];
 #pragma unroll
-    for (int qb = 0; qb < 2; ++qb) {
+    for (int qb = 0; qb < NQ; ++qb) {
       const float top = groups_max_valu(mx[qb]) * a.scale_log2;
       const bool mv = top > m[qb] + LAZY_MAX;  // (a first score above -inf always moves it)
       const float mn = mv ? top : m[qb];
@@ -394,7 +398,7 @@ attention_train_forward_kernel(const AttentionTrainArgs a) {
     }
     if (__any(moved)) {
 #pragma unroll
-      for (int qb = 0; qb < 2; ++qb) {
+      for (int qb = 0; qb < NQ; ++qb) {
         l[qb] *= alpha[qb];
 #pragma unroll
         for (int d = 0; d < DB; ++d) o[qb][d] *= alpha[qb];
@@ -405,14 +409,18 @@ attention_train_forward_kernel(const AttentionTrainArgs a) {
   // One step: P of the scores `z` of step t, its P V, and, unless LAST, the scores `zn` of step t + 1 (EDGE: masked) and their maximum.
   // One chunk per first-operand fragment, read AHEAD chunks before.
   constexpr int AHEAD = 2;
-  auto iterate = [&](int t, f32x4 (&z)[2][KB], f32x4 (&zn)[2][KB], auto edge_tag, auto last_tag) __attribute__((always_inline)) {
+  auto iterate = [&](int t, f32x4 (&z)[NQ][KB], f32x4 (&zn)[NQ][KB], auto edge_tag, auto last_tag) __attribute__((always_inline)) {
     constexpr bool LAST = decltype(last_tag)::value;
     constexpr int N1 = LAST ? 0 : KB * KS, N2 = 2 * DB, N = N1 + N2;
     const unsigned at_k = fresh(rows0) + (unsigned)((t + 1) & 1) * SIDE, at_v = fresh(cols0) + (unsigned)(t & 1) * SIDE;
-    u32x4 frag[AHEAD + 1], pf[2][2];
-    float mx[2] = {-INFINITY, -INFINITY}, ref[2], sum[2] = {0.0f, 0.0f};
+    u32x4 frag[AHEAD + 1], pf[NQ][2];
+    float mx[NQ], ref[NQ], sum[NQ];
 #pragma unroll
-    for (int qb = 0; qb < 2; ++qb) ref[qb] = m[qb] == -INFINITY ? 0.0f : m[qb];  // (nothing visible yet: exp2(-inf) = 0)
+    for (int qb = 0; qb < NQ; ++qb) {
+      mx[qb] = -INFINITY;
+      ref[qb] = m[qb] == -INFINITY ? 0.0f : m[qb];  // (nothing visible yet: exp2(-inf) = 0)
+      sum[qb] = 0.0f;
+    }
     auto read = [&](auto tag) __attribute__((always_inline)) {
       constexpr int i = decltype(tag)::value;
       if constexpr (i < N1) frag[i % (AHEAD + 1)] = read_rows<DL>(at_k, 0, i % KB, i / KB);
@@ -428,31 +436,31 @@ attention_train_forward_kernel(const AttentionTrainArgs a) {
     static_for<0, AHEAD>([&](auto tag) __attribute__((always_inline)) { read(tag); });
     if constexpr (LAST) {
 #pragma unroll
-      for (int v = 0; v < 32; ++v) probability(v);
+      for (int v = 0; v < 16 * NQ; ++v) probability(v);
     }
     static_for<0, N>([&](auto tag) __attribute__((always_inline)) {
       constexpr int i = decltype(tag)::value;
       const u32x4 &f = frag[i % (AHEAD + 1)];
       read(std::integral_constant<int, i + AHEAD>{});
       if constexpr (i < N1) {
-        constexpr int kb = i % KB, ks = i / KB, PER = (32 + N1 - 1) / (LAST ? 1 : N1);
+        constexpr int kb = i % KB, ks = i / KB, PER = (16 * NQ + N1 - 1) / (LAST ? 1 : N1);
 #pragma unroll
-        for (int qb = 0; qb < 2; ++qb) zn[qb][kb] = Mfma16<DT>::run(f, qf[qb][ks], ks == 0 ? f32x4{0, 0, 0, 0} : zn[qb][kb]);
+        for (int qb = 0; qb < NQ; ++qb) zn[qb][kb] = Mfma16<DT>::run(f, qf[qb][ks], ks == 0 ? f32x4{0, 0, 0, 0} : zn[qb][kb]);
 #pragma unroll
-        for (int v = i * PER; v < (i + 1) * PER && v < 32; ++v) probability(v);
+        for (int v = i * PER; v < (i + 1) * PER && v < 16 * NQ; ++v) probability(v);
       } else {
-        constexpr int j = i - N1, s = j / DB, d = j % DB, PER = (32 + N2 - 1) / N2;
+        constexpr int j = i - N1, s = j / DB, d = j % DB, PER = (16 * NQ + N2 - 1) / N2;
 #pragma unroll
-        for (int qb = 0; qb < 2; ++qb) o[qb][d] = Mfma16<DT>::run(f, pf[qb][s], o[qb][d]);
+        for (int qb = 0; qb < NQ; ++qb) o[qb][d] = Mfma16<DT>::run(f, pf[qb][s], o[qb][d]);
         if constexpr (!LAST) {
 #pragma unroll
-          for (int v = j * PER; v < (j + 1) * PER && v < 32; ++v) take_max(t + 1, v, zn, mx, edge_tag);
+          for (int v = j * PER; v < (j + 1) * PER && v < 16 * NQ; ++v) take_max(t + 1, v, zn, mx, edge_tag);
         }
       }
       fence();
     });
 #pragma unroll
-    for (int qb = 0; qb < 2; ++qb) l[qb] += sum[qb];
+    for (int qb = 0; qb < NQ; ++qb) l[qb] += sum[qb];
     if constexpr (!LAST) move_reference(mx);
   };
   // Step t: the scores of t are there; K of t + 1 and V of t have arrived, K of t + 2 and V of t + 1 go out.
@@ -463,7 +471,7 @@ attention_train_forward_kernel(const AttentionTrainArgs a) {
     if (t + 1 < steps) request_v(t + 1);
   };
 
-  f32x4 za[2][KB], zb[2][KB];
+  f32x4 za[NQ][KB], zb[NQ][KB];
   int t = s0;
   if (t < steps) {
     request_k(t);
@@ -473,24 +481,26 @@ attention_train_forward_kernel(const AttentionTrainArgs a) {
     __syncthreads();
     if (t < wave_steps) {  // the first scores, on their own
       const unsigned at_k = fresh(rows0) + (unsigned)(t & 1) * SIDE;
-      float mx[2] = {-INFINITY, -INFINITY};
+      float mx[NQ];
+#pragma unroll
+      for (int qb = 0; qb < NQ; ++qb) mx[qb] = -INFINITY;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
           const u32x4 kf = read_rows<DL>(at_k, 0, kb, ks);
 #pragma unroll
-          for (int qb = 0; qb < 2; ++qb) za[qb][kb] = Mfma16<DT>::run(kf, qf[qb][ks], ks == 0 ? f32x4{0, 0, 0, 0} : za[qb][kb]);
+          for (int qb = 0; qb < NQ; ++qb) za[qb][kb] = Mfma16<DT>::run(kf, qf[qb][ks], ks == 0 ? f32x4{0, 0, 0, 0} : za[qb][kb]);
         }
 #pragma unroll
-      for (int v = 0; v < 32; ++v) take_max(t, v, za, mx, std::true_type{});
+      for (int v = 0; v < 16 * NQ; ++v) take_max(t, v, za, mx, std::true_type{});
       move_reference(mx);
     }
   }
   const int whole = full_steps - 1, last = wave_steps - 1;  // steps whose next one is whole; the wave's last
   auto back = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int qb = 0; qb < 2; ++qb)
+    for (int qb = 0; qb < NQ; ++qb)
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) za[qb][kb] = zb[qb][kb];
   };
@@ -513,18 +523,18 @@ attention_train_forward_kernel(const AttentionTrainArgs a) {
   for (; t < steps; ++t) head(t);  // (tiles that only other waves see)
 
   if constexpr (SG == 2) {  // the second wave's state to the first
-    f32x4 *const at = (f32x4 *)sK + group * (2 * DB + 1) * 64 + lane;
+    f32x4 *const at = (f32x4 *)sK + group * (NQ * DB + 1) * 64 + lane;
     __syncthreads();
     if (kg == 1) {
 #pragma unroll
-      for (int i = 0; i < 2 * DB; ++i) at[i * 64] = o[i / DB][i % DB];
-      at[2 * DB * 64] = f32x4{m[0], m[1], l[0], l[1]};
+      for (int i = 0; i < NQ * DB; ++i) at[i * 64] = o[i / DB][i % DB];
+      at[NQ * DB * 64] = f32x4{m[0], m[NQ - 1], l[0], l[NQ - 1]};
     }
     __syncthreads();
     if (kg == 1) return;
-    const f32x4 ml = at[2 * DB * 64];
+    const f32x4 ml = at[NQ * DB * 64];
 #pragma unroll
-    for (int qb = 0; qb < 2; ++qb) {
+    for (int qb = 0; qb < NQ; ++qb) {
       const float top = fmaxf(m[qb], ml[qb]), ref = top == -INFINITY ? 0.0f : top;
       const float f0 = __builtin_amdgcn_exp2f(m[qb] - ref), f1 = __builtin_amdgcn_exp2f(ml[qb] - ref);
       m[qb] = top;
@@ -535,7 +545,7 @@ attention_train_forward_kernel(const AttentionTrainArgs a) {
   }
 
 #pragma unroll
-  for (int qb = 0; qb < 2; ++qb) {
+  for (int qb = 0; qb < NQ; ++qb) {
     const int r = r_wave + qb * 16 + r16;
     float sum = groups_sum(l[qb]);
     if (r >= a.G * a.Sq) continue;
@@ -1081,8 +1091,9 @@ template <int DT, int DL, int DU>
 int forward(const AttentionTrainArgs &a, hipStream_t stream) {
   constexpr int W = 4;
   const dim3 grid((unsigned)((a.G * a.Sq + a.block - 1) / a.block) * (unsigned)(a.B * a.Hk), (unsigned)a.splits);
-  if (a.block == 32 * W) hipLaunchKernelGGL((attention_train_forward_kernel<DT, DL, DU, W, 1>), grid, dim3(W * 64), 0, stream, a);
-  else hipLaunchKernelGGL((attention_train_forward_kernel<DT, DL, DU, W, 2>), grid, dim3(W * 64), 0, stream, a);
+  if (a.block == 32 * W) hipLaunchKernelGGL((attention_train_forward_kernel<DT, DL, DU, W, 1, 2>), grid, dim3(W * 64), 0, stream, a);
+  else if (a.block == 16 * W) hipLaunchKernelGGL((attention_train_forward_kernel<DT, DL, DU, W, 2, 2>), grid, dim3(W * 64), 0, stream, a);
+  else hipLaunchKernelGGL((attention_train_forward_kernel<DT, DL, DU, W, 2, 1>), grid, dim3(W * 64), 0, stream, a);
   if (a.splits > 1) {
     const long long rows = (long long)a.B * a.Hk * a.G * a.Sq;
     hipLaunchKernelGGL((attention_train_join_kernel<DT, DU>), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, stream, a);

@@ -96,10 +96,11 @@ bool rows_in_place(const View &t, long long D) {
 }
 
 // Rows of a workgroup and parts of the keys for the forward pass, by the least of this estimate (us) over the candidates, in the terms of
-// plan_backward: few rows over many keys leave CUs idle unless the keys are shared, by two waves of a workgroup (blocks of 64 rows) or by
-// workgroups, whose results a second launch joins.  Fitted to 25 shapes with every candidate timed; its choice is 1 % behind the best on
-// average and 5 % at worst.  Best / unsplit blocks of 128, us: B1 H12 S1024 D64 causal 15.4 / 21.9 (blocks of 64), B8 H32:8 one query over 8192 keys
-// 49 / 180 (8 parts), B1 H8 1000 queries over 5000 keys D64 30 / 63 (4 parts).
+// plan_backward and of how fast the keys can arrive: few rows over many keys leave CUs idle unless the keys are shared, by two waves of a
+// workgroup (blocks of 64 rows, of 32 for at most 16 rows) or by workgroups, whose results a second launch joins.  Fitted to 34 shapes with every
+// candidate timed; its choice is 2 % behind the best on average and 16 % at worst (of 6 us).  Best / unsplit blocks of 128, us: B1 H12 S1024
+// D64 causal 15.4 / 21.9 (blocks of 64), B8 H32:8 one query over up to 8192 keys 37 / 165 (8 parts of blocks of 128, or 4 of 32), B1 H40:8
+// one query over 32768 keys 34 / 642 (24 parts of blocks of 32), B1 H8 1000 queries over 5000 keys D64 30 / 63 (4 parts).
 struct ForwardPlan {
   int block, splits;
 };
@@ -107,16 +108,18 @@ ForwardPlan plan_forward(long long heads, long long rows, long long keys, int wi
   ForwardPlan best{128, 1};
   double least = 1e300;
   const double f = width / 128.0, tiles = (double)((keys + 63) / 64), seen = half ? 0.5 : 1.0;
-  for (int block : {128, 64})
+  for (int block : {128, rows > 16 ? 64 : 32})
     for (int splits : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
-      const int step = block == 64 ? 2 : 1;  // tiles
+      const int step = block < 128 ? 2 : 1;  // tiles
       const double bytes = 2.0 * splits * heads * rows * width * 4;
       if (tiles < step || (splits > 1 && (tiles < step * splits || bytes > (1 << 30)))) continue;
-      const double lat = (block == 128 ? 1.26 : 0.85) * (0.24 + 0.76 * f), thr = (block == 128 ? 0.72 : 0.89) * f / cus;
-      const double walk = tiles / splits, fill = rows < block ? 0.3 + 0.7 * rows / block : 1.0;
-      const double total = thr * fill * ((rows + block - 1) / block) * heads * splits * (walk * seen + 3);
-      const double longest = std::max(lat * (walk + 3), 4.0 * heads * keys * width * seen / 6.1e6);
-      const double time = std::max(total, longest) + 0.42 * std::min(total, longest) + (splits > 1 ? 3.3 + bytes / 5.5e6 : 0.0);
+      const double lat = (block == 128 ? 1.37 : block == 64 ? 0.88 : 0.72) * (0.14 + 0.86 * f);
+      const double thr = (block == 128 ? 0.81 : block == 64 ? 0.94 : 0.68) * f / cus, fill = rows < block ? 0.22 + 0.78 * rows / block : 1.0;
+      const double n = (double)((rows + block - 1) / block) * heads * splits, walk = tiles / splits;
+      const double slots = cus * (block == 128 || width == 64 ? 2.0 : 1.0);
+      const double arrive = 4.0 * heads * keys * width * seen / 6e6 * std::max(1.0, 0.34 * slots / n);
+      const double total = thr * fill * n * (walk * seen + 2.2), longest = std::max(lat * (walk + 2.2), arrive);
+      const double time = std::max(total, longest) + 0.42 * std::min(total, longest) + (splits > 1 ? 3.5 + bytes / 5.3e6 : 0.0);
       if (time < least) {
         least = time;
         best = {block, splits};
@@ -247,7 +250,7 @@ TraceaStatus run_attention(const Attention &c, bool from_copies) {
     const ForwardPlan plan = plan_forward(B * Hk, G * Sq, Sk, width, a.causal && Sq == Sk, (int)device_limits().cus);
     a.block = plan.block;
     if (plan.splits > 1) {
-      const long long keys = a.block == 64 ? 128 : 64, steps = (Sk + keys - 1) / keys, per = (steps + plan.splits - 1) / plan.splits;
+      const long long keys = a.block < 128 ? 128 : 64, steps = (Sk + keys - 1) / keys, per = (steps + plan.splits - 1) / plan.splits;
       const long long splits = (steps + per - 1) / per;
       const size_t n = (size_t)(splits * B * Hk * rows_pad);
       a.part_o = (float *)train_scratch(c.q.device, c.stream, n * (size_t)(width + 2) * 4);

@@ -28,14 +28,14 @@ struct AttentionTrainArgs {
   // backward: per packed row -lse * log2(e) (-inf: nothing visible) and -(dO . O), [B * Hk][rows_pad] each
   float *neg_lse2, *neg_delta;
   int rows_pad;  // G * Sq up to a multiple of 64
-  int block;       // columns (packed rows, keys) of a workgroup: 128, or 64 with two waves on 32 columns
+  int block;       // columns (packed rows, keys) of a workgroup: 128; 64, two waves on 32 columns; forward only: 32, two waves on 16 rows
   int row_splits;  // parts of the rows for dK and dV, each with a workgroup of its own
   float *part_dkv; // [row_splits][B * Hk][Sk][dK, dV][width], row_splits > 1
   // f16 only: largest squared row norms of dO and V, [B * Hk][norm_blocks] (64 rows of dO or 64 keys of V each)
   float *norms;
   int norm_blocks;
   // forward over a split key axis: partial results (o in fp32 unnormalised, running maximum and sum per row)
-  int splits, steps_per_split;  // steps: 64 keys, or 128 with two waves on 32 rows
+  int splits, steps_per_split;  // steps: 64 keys, or 128 with two waves on the same rows
   float *part_o, *part_ml;
 };
 
