@@ -1043,9 +1043,9 @@ __device__ __forceinline__ void dkv_block(const AttentionTrainArgs &a, int id, u
       float *at = a.part_dkv + (((long long)part * a.B * a.Hk + bh) * a.Sk + j) * 2 * DU + g4 * 4;
 #pragma unroll
       for (int d = 0; d < DB; ++d)
-        if (d * 16 + g4 * 4 < a.D) {
-          *(f32x4 *)(at + d * 16) = there ? dk[nb][d] * fk : f32x4{0, 0, 0, 0};
-          *(f32x4 *)(at + DU + d * 16) = there ? dv[nb][d] * fv : f32x4{0, 0, 0, 0};
+        if (there && d * 16 + g4 * 4 < a.D) {  // (what lies behind the length is not read)
+          *(f32x4 *)(at + d * 16) = dk[nb][d] * fk;
+          *(f32x4 *)(at + DU + d * 16) = dv[nb][d] * fv;
         }
       continue;
     }
@@ -1078,11 +1078,14 @@ __global__ void __launch_bounds__(256) attention_train_sum_kernel(const Attentio
   const int piece = (int)(id - key * PER), c = (piece % (DU / 4)) * 4;
   const bool is_v = piece >= DU / 4;
   if (key >= (long long)a.B * a.Hk * a.Sk || c >= a.D) return;
+  const int bh = (int)(key / a.Sk), j = (int)(key - (long long)bh * a.Sk), b = bh / a.Hk;
   const long long plane = (long long)a.B * a.Hk * a.Sk * 2 * DU;
   const float *at = a.part_dkv + key * 2 * DU + piece * 4;
-  f32x4 x = *(const f32x4 *)at;
-  for (int r = 1; r < a.row_splits; ++r) x += *(const f32x4 *)(at + r * plane);
-  const int bh = (int)(key / a.Sk), j = (int)(key - (long long)bh * a.Sk), b = bh / a.Hk;
+  f32x4 x = {0, 0, 0, 0};
+  if (j < rows_of(a, bh).lk) {
+    x = *(const f32x4 *)at;
+    for (int r = 1; r < a.row_splits; ++r) x += *(const f32x4 *)(at + r * plane);
+  }
   const HeadView &out = is_v ? a.dv : a.dk;
   *(u32x2 *)((unsigned short *)slice(out, b, bh - b * a.Hk) + (long long)j * out.ss + c) = pack_result<DT>(x, 1.0f);
 }

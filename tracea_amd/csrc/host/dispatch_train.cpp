@@ -99,12 +99,12 @@ bool rows_in_place(const View &t, long long D) {
 // plan_backward and of how fast the keys can arrive: few rows over many keys leave CUs idle unless the keys are shared, by two waves of a
 // workgroup (blocks of 64 rows, of 32 for at most 16 rows) or by workgroups, whose results a second launch joins.  Fitted to 34 shapes with every
 // candidate timed; its choice is 2 % behind the best on average and 16 % at worst (of 6 us).  Best / unsplit blocks of 128, us: B1 H12 S1024
-// D64 causal 15.4 / 21.9 (blocks of 64), B8 H32:8 one query over up to 8192 keys 37 / 165 (8 parts of blocks of 128, or 4 of 32), B1 H40:8
-// one query over 32768 keys 34 / 642 (24 parts of blocks of 32), B1 H8 1000 queries over 5000 keys D64 30 / 63 (4 parts).
+// D64 causal 15.4 / 21.9 (blocks of 64), B8 H32:8 one query over up to 8192 keys 46 / 167 (8 parts of blocks of 128; 4 of 32: 52; keys
+// from HBM), B1 H40:8 one query over 32768 keys 34 / 642 (24 parts of blocks of 32), B1 H8 1000 queries over 5000 keys D64 30 / 63 (4 parts).
 struct ForwardPlan {
   int block, splits;
 };
-ForwardPlan plan_forward(long long heads, long long rows, long long keys, int width, bool half, int cus) {
+ForwardPlan plan_forward(long long heads, long long rows, long long keys, int width, bool half, bool lengths, int cus) {
   ForwardPlan best{128, 1};
   double least = 1e300;
   const double f = width / 128.0, tiles = (double)((keys + 63) / 64), seen = half ? 0.5 : 1.0;
@@ -117,7 +117,8 @@ ForwardPlan plan_forward(long long heads, long long rows, long long keys, int wi
       const double thr = (block == 128 ? 0.81 : block == 64 ? 0.94 : 0.68) * f / cus, fill = rows < block ? 0.22 + 0.78 * rows / block : 1.0;
       const double n = (double)((rows + block - 1) / block) * heads * splits, walk = tiles / splits;
       const double slots = cus * (block == 128 || width == 64 ? 2.0 : 1.0);
-      const double arrive = 4.0 * heads * keys * width * seen / 6e6 * std::max(1.0, 0.34 * slots / n);
+      const double arrive = 4.0 * heads * keys * width * seen / 6e6 * std::max(1.0, 0.34 * slots / n) *
+                            (lengths && block == 32 && width > 64 ? 1.2 : 1.0);  // (one workgroup on a CU: idle where its sequence has ended)
       const double total = thr * fill * n * (walk * seen + 2.2), longest = std::max(lat * (walk + 2.2), arrive);
       const double time = std::max(total, longest) + 0.42 * std::min(total, longest) + (splits > 1 ? 3.5 + bytes / 5.3e6 : 0.0);
       if (time < least) {
@@ -247,7 +248,7 @@ TraceaStatus run_attention(const Attention &c, bool from_copies) {
   if (!c.backward) {
     if (Sq == 0) return TRACEA_SUCCESS;
     const int width = D <= 64 ? 64 : D <= 96 ? 96 : 128;
-    const ForwardPlan plan = plan_forward(B * Hk, G * Sq, Sk, width, a.causal && Sq == Sk, (int)device_limits().cus);
+    const ForwardPlan plan = plan_forward(B * Hk, G * Sq, Sk, width, a.causal && Sq == Sk, c.k_len != nullptr, (int)device_limits().cus);
     a.block = plan.block;
     if (plan.splits > 1) {
       const long long keys = a.block < 128 ? 128 : 64, steps = (Sk + keys - 1) / keys, per = (steps + plan.splits - 1) / plan.splits;

@@ -435,13 +435,12 @@ def norm_gate_residual_backward(dx_out, dy, x_out, h=None, w_post=None, gate=Non
                                 dx=None, dh=None):
     """(dx, dh, dw_post, dgate, dw_pre) for the gradients dx_out (None: zero) and dy of :func:`norm_gate_residual`'s results, from
     its x_out (x where there is no h) and h; None for what the call has not."""
-    f32 = dict(dtype=torch.float32, device=x_out.device)
     dx = torch.empty_like(x_out) if dx is None else dx
     if h is not None:
         dh = torch.empty_like(h) if dh is None else dh
-    dw_post = None if w_post is None else torch.empty(w_post.shape, **f32)
-    dgate = None if gate is None else torch.empty(gate.shape, **f32)
-    dw_pre = None if w_pre is None else torch.empty(w_pre.shape, **f32)
+    dw_post = None if w_post is None else torch.empty_like(w_post)
+    dgate = None if gate is None else torch.empty_like(gate)
+    dw_pre = None if w_pre is None else torch.empty_like(w_pre)
     params = capi.NormParams(float(eps), float(residual_scale), _stream(x_out))
     st = capi.lib().tracea_norm_gate_residual_backward(_ref(dx_out), _ref(dy), _plain_view(x_out), _ref(h), _ref(w_post),
                                                        _ref(gate), _ref(w_pre), _ref(dx), _ref(dh), _ref(dw_post),
