@@ -435,6 +435,8 @@ TraceaStatus tracea_conv_coords_device(const TraceaConvParamsBlock *p, int32_t *
  * Query i of b sees keys j < k_lengths[b]; with params.causal, of those j <= i + k_lengths[b] - q_lengths[b] (the
  * last query sees every key).  lse = log of the sum of exp(scale q.k) over them; a query that sees none, or lies
  * behind its sequence's length, has o = 0, lse = -inf and gradient 0, keys behind the length have gradient 0.
+ * (Infinities and NaN within the lengths spread as 0 * inf does: from a key that a causal mask hides, also to queries up to 63
+ * positions in front of it.)
  * All tensors but lse share one type, f16 or bf16, D from 1 to 128; sums, statistics and probabilities are fp32,
  * probabilities and their gradients are rounded once to the operand type for the matrix products.  scale 0 selects
  * 1/sqrt(D); softmax_mode is ignored.  The same call on the same inputs gives the same bits.
@@ -481,7 +483,8 @@ TraceaStatus tracea_rotary(TraceaTensorView q, const TraceaTensorView *k, Tracea
  * The backward pass reads x_out (x where there is no h) and h as the forward pass left them and works out both norms
  * again: dx_out (optional: absent is 0) and dy are the gradients of x_out and y; dx, dh have the type of h, dw_post, dgate
  * [G,C], dw_pre are f32 and are summed in an order that does not change.  Gradients that are not wanted are NULL (dx is
- * required).  It takes a workspace per (device, stream) of at most 16 MiB + 8 bytes per channel and batch entry, grown on demand, never under capture. */
+ * required).  It takes a workspace per (device,
+ * stream), at most 16 MiB and 8 bytes per channel and batch entry, grown on demand, never under capture. */
 typedef struct {
   float eps;
   float residual_scale;

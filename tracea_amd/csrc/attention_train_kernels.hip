@@ -86,7 +86,8 @@ struct Tile {
 
 // A direct-to-LDS load: lane l's bytes from its offset land at lds + l * size.  Written as instructions: behind the builtin
 // the compiler, which cannot tell the buffers of a ring apart, waits for all requests in front of the next LDS read.  The
-// kernels wait for a tile themselves (vmcnt(0) and a barrier) before they read it.  (s_nop: m0 is read by the load behind it.)
+// kernels wait for a tile themselves (vmcnt(0) and a barrier) before they read it.  (s_nop: m0 is read by the load behind it; m0 is
+// reserved, the compiler writes it in front of each use of its own.)
 __device__ __forceinline__ void dma16(u32x4 rsrc, unsigned offset, unsigned lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(rsrc) : "memory");
 }

@@ -1,6 +1,7 @@
 // Argument checks and launches of the operators for training: attention with row statistics and its backward pass, rotary
 // positions, the norm / gate / residual sum.  Status codes as in dispatch.cpp.
 #include <cmath>
+#include <mutex>
 
 #include "../train.hpp"
 #include "views.hpp"
@@ -8,6 +9,9 @@
 namespace tracea_amd {
 
 namespace {
+
+// The launches of a call that pass something on in a workspace stay together on their stream, whichever threads use it.
+std::mutex g_launches;
 
 TraceaStatus ready(const char *what) {
   return runtime_ready() ? TRACEA_SUCCESS : fail(TRACEA_UNKNOWN_ERROR, "%s: tracea_init has not been called", what);
@@ -354,6 +358,7 @@ TraceaStatus dispatch_attention_forward(const TraceaTensorView &q, const TraceaT
   if (folds(c.o) || folds(c.lse)) return overlapping(op, "elements of a result share an address");
   if (may_overlap(c.lse, c.q) || may_overlap(c.lse, c.k) || may_overlap(c.lse, c.v) || may_overlap(c.lse, c.o))
     return overlapping(op, "lse overlaps another tensor");
+  std::lock_guard<std::mutex> together(g_launches);
   return run_attention(c, false);
 }
 
@@ -383,6 +388,7 @@ TraceaStatus dispatch_attention_backward(const TraceaTensorView &q, const Tracea
     for (int j = 0; j < i; ++j)
       if (may_overlap(*results[i], *results[j])) return overlapping(op, "results overlap each other");
   }
+  std::lock_guard<std::mutex> together(g_launches);
   return run_attention(c, false);
 }
 
@@ -676,6 +682,7 @@ TraceaStatus dispatch_norm_backward(const TraceaTensorView *dx_out, const Tracea
     return TRACEA_SUCCESS;
   }
   finish(c, tensors, n, true, params, &a);
+  std::lock_guard<std::mutex> together(g_launches);
   if (columns) {
     a.partial = (float *)train_scratch(c.device, stream, (size_t)2 * a.B * a.chunks * a.C * 4);
     if (a.partial == nullptr)
