@@ -324,6 +324,28 @@ attention_train_forward_kernel(const AttentionTrainArgs a) {
     steps = min(steps, s0 + a.steps_per_split);
   }
 
+  const unsigned short *Kg = slice(a.k, w.b, w.hk), *Vg = slice(a.v, w.b, w.hk);
+  auto request = [&](const unsigned short *base, long long ss, int step, unsigned side) __attribute__((always_inline)) {
+    const int lane_ = fresh(lane);
+    const unsigned bytes = (unsigned)ss * 2u;
+#pragma unroll
+    for (int g = 0; g < SG; ++g) {
+      const int tile = step * SG + g, left = w.lk - tile * TILE;
+      const unsigned char *dst = sK + side + (unsigned)(step & 1) * SIDE + g * T::BYTES;
+      const unsigned short *at = base + (long long)tile * TILE * ss;
+      constexpr int APART = WAVES * 64 / T::CH;
+      if (left >= TILE) load_tile<DL, WAVES>(at, (long long)bytes * APART, dst, a.D, lane_, wave, [&](int row) { return row * bytes; });
+      else load_tile_any<DL, WAVES>(at, dst, a.D, lane_, wave, [&](int row) { return row < left ? row * bytes : BEYOND; });
+    }
+  };
+  auto request_k = [&](int step) __attribute__((always_inline)) { request(Kg, a.k.ss, step, 0); };
+  auto request_v = [&](int step) __attribute__((always_inline)) { request(Vg, a.v.ss, step, V_AT); };
+  if (s0 < steps) {  // (in flight while the rest is set up)
+    request_k(s0);
+    request_v(s0);
+    if (s0 + 1 < steps) request_k(s0 + 1);
+  }
+
   int q_last[NQ];  // the last key that the lane's queries see
   u32x4 qf[NQ][KS];
 #pragma unroll
@@ -349,22 +371,6 @@ attention_train_forward_kernel(const AttentionTrainArgs a) {
   const int wave_steps = wave_keys > kg * TILE ? min(steps, (wave_keys - kg * TILE + STEP - 1) / STEP) : 0;
   const int full_steps = wave_full >= (kg + 1) * TILE ? min(wave_steps, (wave_full - kg * TILE) / TILE / SG + ((wave_full - kg * TILE) / TILE % SG != 0)) : 0;
 
-  const unsigned short *Kg = slice(a.k, w.b, w.hk), *Vg = slice(a.v, w.b, w.hk);
-  auto request = [&](const unsigned short *base, long long ss, int step, unsigned side) __attribute__((always_inline)) {
-    const int lane_ = fresh(lane);
-    const unsigned bytes = (unsigned)ss * 2u;
-#pragma unroll
-    for (int g = 0; g < SG; ++g) {
-      const int tile = step * SG + g, left = w.lk - tile * TILE;
-      const unsigned char *dst = sK + side + (unsigned)(step & 1) * SIDE + g * T::BYTES;
-      const unsigned short *at = base + (long long)tile * TILE * ss;
-      constexpr int APART = WAVES * 64 / T::CH;
-      if (left >= TILE) load_tile<DL, WAVES>(at, (long long)bytes * APART, dst, a.D, lane_, wave, [&](int row) { return row * bytes; });
-      else load_tile_any<DL, WAVES>(at, dst, a.D, lane_, wave, [&](int row) { return row < left ? row * bytes : BEYOND; });
-    }
-  };
-  auto request_k = [&](int step) __attribute__((always_inline)) { request(Kg, a.k.ss, step, 0); };
-  auto request_v = [&](int step) __attribute__((always_inline)) { request(Vg, a.v.ss, step, V_AT); };
 
   f32x4 o[NQ][DB];
   float m[NQ], l[NQ];  // reference (log2 units) and sum of the lane's keys
@@ -475,9 +481,6 @@ attention_train_forward_kernel(const AttentionTrainArgs a) {
   f32x4 za[NQ][KB], zb[NQ][KB];
   int t = s0;
   if (t < steps) {
-    request_k(t);
-    request_v(t);
-    if (t + 1 < steps) request_k(t + 1);
     __builtin_amdgcn_s_waitcnt(0x0f70);
     __syncthreads();
     if (t < wave_steps) {  // the first scores, on their own
@@ -695,6 +698,22 @@ __device__ __forceinline__ void dq_block(const AttentionTrainArgs &a, int id, un
   if (last_row >= blk * BR) keys = a.causal ? min(w.lk, query_of(a, last_row) + w.off + 1) : w.lk;
   const int tiles = keys > 0 ? (keys + TILE - 1) / TILE : 0;
 
+  const unsigned short *Kg = slice(a.k, w.b, w.hk), *Vg = slice(a.v, w.b, w.hk);
+  auto request = [&](int t) __attribute__((always_inline)) {
+    const int left = w.lk - t * TILE, at = (t & 1) * T::BYTES, lane_ = fresh(lane);
+    const unsigned kss = (unsigned)a.k.ss * 2u, vss = (unsigned)a.v.ss * 2u;
+    const unsigned short *kt = Kg + (long long)t * TILE * a.k.ss, *vt = Vg + (long long)t * TILE * a.v.ss;
+    if (left >= TILE) {
+      constexpr int STEP = WAVES * 64 / T::CH;
+      load_tile<DL, WAVES>(kt, (long long)kss * STEP, sK + at, a.D, lane_, wave, [&](int row) { return row * kss; });
+      load_tile<DL, WAVES>(vt, (long long)vss * STEP, sK + V_AT + at, a.D, lane_, wave, [&](int row) { return row * vss; });
+    } else {
+      load_tile_any<DL, WAVES>(kt, sK + at, a.D, lane_, wave, [&](int row) { return row < left ? row * kss : BEYOND; });
+      load_tile_any<DL, WAVES>(vt, sK + V_AT + at, a.D, lane_, wave, [&](int row) { return row < left ? row * vss : BEYOND; });
+    }
+  };
+  if (tiles > 0) request(0);  // (in flight while the rest is set up)
+
   int q_last[2];
   float nl[2], nd[2];
   u32x4 qf[2][KS], of[2][KS];
@@ -728,20 +747,6 @@ __device__ __forceinline__ void dq_block(const AttentionTrainArgs &a, int id, un
     dsp = dsc * (1.0f / 16384.0f);
   }
 
-  const unsigned short *Kg = slice(a.k, w.b, w.hk), *Vg = slice(a.v, w.b, w.hk);
-  auto request = [&](int t) __attribute__((always_inline)) {
-    const int left = w.lk - t * TILE, at = (t & 1) * T::BYTES, lane_ = fresh(lane);
-    const unsigned kss = (unsigned)a.k.ss * 2u, vss = (unsigned)a.v.ss * 2u;
-    const unsigned short *kt = Kg + (long long)t * TILE * a.k.ss, *vt = Vg + (long long)t * TILE * a.v.ss;
-    if (left >= TILE) {
-      constexpr int STEP = WAVES * 64 / T::CH;
-      load_tile<DL, WAVES>(kt, (long long)kss * STEP, sK + at, a.D, lane_, wave, [&](int row) { return row * kss; });
-      load_tile<DL, WAVES>(vt, (long long)vss * STEP, sK + V_AT + at, a.D, lane_, wave, [&](int row) { return row * vss; });
-    } else {
-      load_tile_any<DL, WAVES>(kt, sK + at, a.D, lane_, wave, [&](int row) { return row < left ? row * kss : BEYOND; });
-      load_tile_any<DL, WAVES>(vt, sK + V_AT + at, a.D, lane_, wave, [&](int row) { return row < left ? row * vss : BEYOND; });
-    }
-  };
 
   f32x4 acc[2][DB];
 #pragma unroll
@@ -824,7 +829,6 @@ __device__ __forceinline__ void dq_block(const AttentionTrainArgs &a, int id, un
   };
   // tiles that every row of the wave sees whole, then the others (a wave takes part in the loads of tiles that none sees)
   int t = 0;
-  if (t < tiles) request(t);
   for (const int end = min(tiles, wave_full / TILE); t < end; ++t) {
     head(t);
     compute(t, std::false_type{});
@@ -874,6 +878,29 @@ __device__ __forceinline__ void dkv_block(const AttentionTrainArgs &a, int id, u
     t_end = from + n * (part + 1) / a.row_splits;
   }
 
+  const unsigned short *Qg = slice(a.q, w.b, w.hk * a.G), *Og = slice(a.d_o, w.b, w.hk * a.G);
+  const float *nl = a.neg_lse2 + (long long)bh * a.rows_pad, *nd = a.neg_delta + (long long)bh * a.rows_pad;
+  auto request = [&](int t) __attribute__((always_inline)) {
+    const int r0 = t * TILE, i0 = query_of(a, r0), at = (t & 1) * T::BYTES, lane_ = fresh(lane);
+    const unsigned short *qt = Qg + (long long)i0 * a.q.ss, *ot = Og + (long long)i0 * a.d_o.ss;
+    auto offset = [&](const HeadView &v, int row) __attribute__((always_inline)) -> unsigned {
+      const int r = r0 + row, i = query_of(a, r);
+      return (unsigned)(i - i0) * ((unsigned)v.ss * 2u) + (unsigned)(r - i * a.G) * ((unsigned)v.sh * 2u);
+    };
+    constexpr int STEP = WAVES * 64 / T::CH;
+    if (r0 + TILE <= rows && 16 % a.G == 0) {  // (a power of two: rows 16 apart are 16 / G queries apart)
+      load_tile<DL, WAVES>(qt, (long long)(STEP / a.G) * a.q.ss * 2, sQ + at, a.D, lane_, wave, [&](int row) { return offset(a.q, row); });
+      load_tile<DL, WAVES>(ot, (long long)(STEP / a.G) * a.d_o.ss * 2, sQ + O_AT + at, a.D, lane_, wave, [&](int row) { return offset(a.d_o, row); });
+    } else {
+      load_tile_any<DL, WAVES>(qt, sQ + at, a.D, lane_, wave, [&](int row) { return r0 + row < rows ? offset(a.q, row) : BEYOND; });
+      load_tile_any<DL, WAVES>(ot, sQ + O_AT + at, a.D, lane_, wave, [&](int row) { return r0 + row < rows ? offset(a.d_o, row) : BEYOND; });
+    }
+    if (wave < 2) {  // (rows_pad is a multiple of the tile)
+      dma4(resource((wave == 0 ? nl : nd) + r0, TILE * 4), lane * 4, lds_address((wave == 0 ? sL : sD) + (t & 1) * TILE));
+    }
+  };
+  if (t_begin < t_end) request(t_begin);  // (in flight while the rest is set up)
+
   u32x4 kf[2][KS], vf[2][KS];
 #pragma unroll
   for (int nb = 0; nb < 2; ++nb) {
@@ -914,27 +941,6 @@ __device__ __forceinline__ void dkv_block(const AttentionTrainArgs &a, int id, u
     dsp = dsc * (1.0f / 16384.0f);
   }
 
-  const unsigned short *Qg = slice(a.q, w.b, w.hk * a.G), *Og = slice(a.d_o, w.b, w.hk * a.G);
-  const float *nl = a.neg_lse2 + (long long)bh * a.rows_pad, *nd = a.neg_delta + (long long)bh * a.rows_pad;
-  auto request = [&](int t) __attribute__((always_inline)) {
-    const int r0 = t * TILE, i0 = query_of(a, r0), at = (t & 1) * T::BYTES, lane_ = fresh(lane);
-    const unsigned short *qt = Qg + (long long)i0 * a.q.ss, *ot = Og + (long long)i0 * a.d_o.ss;
-    auto offset = [&](const HeadView &v, int row) __attribute__((always_inline)) -> unsigned {
-      const int r = r0 + row, i = query_of(a, r);
-      return (unsigned)(i - i0) * ((unsigned)v.ss * 2u) + (unsigned)(r - i * a.G) * ((unsigned)v.sh * 2u);
-    };
-    constexpr int STEP = WAVES * 64 / T::CH;
-    if (r0 + TILE <= rows && 16 % a.G == 0) {  // (a power of two: rows 16 apart are 16 / G queries apart)
-      load_tile<DL, WAVES>(qt, (long long)(STEP / a.G) * a.q.ss * 2, sQ + at, a.D, lane_, wave, [&](int row) { return offset(a.q, row); });
-      load_tile<DL, WAVES>(ot, (long long)(STEP / a.G) * a.d_o.ss * 2, sQ + O_AT + at, a.D, lane_, wave, [&](int row) { return offset(a.d_o, row); });
-    } else {
-      load_tile_any<DL, WAVES>(qt, sQ + at, a.D, lane_, wave, [&](int row) { return r0 + row < rows ? offset(a.q, row) : BEYOND; });
-      load_tile_any<DL, WAVES>(ot, sQ + O_AT + at, a.D, lane_, wave, [&](int row) { return r0 + row < rows ? offset(a.d_o, row) : BEYOND; });
-    }
-    if (wave < 2) {  // (rows_pad is a multiple of the tile)
-      dma4(resource((wave == 0 ? nl : nd) + r0, TILE * 4), lane * 4, lds_address((wave == 0 ? sL : sD) + (t & 1) * TILE));
-    }
-  };
 
   f32x4 dk[2][DB], dv[2][DB];
 #pragma unroll
@@ -1019,7 +1025,6 @@ __device__ __forceinline__ void dkv_block(const AttentionTrainArgs &a, int id, u
   };
   // tiles with rows that see some of the wave's keys, then those whose rows see all
   int t = t_begin;
-  if (t < t_end) request(t);
   for (; t < t_end && t * TILE < row_all; ++t) {
     head(t);
     if (live && t * TILE + TILE > row_some) compute(t, std::true_type{});
