@@ -209,6 +209,17 @@ def test_empty(tracea_gpu):
     assert (dw_post == 0).all() and (dw_pre == 0).all() and dgate is None
 
 
+@pytest.mark.parametrize("gates", [None, 0, 1])
+def test_a_batch_without_entries_has_zero_weight_gradients(tracea_gpu, gates):
+    w = torch.ones(72, device="cuda")
+    x = torch.empty(0, 3, 72, device="cuda", dtype=torch.bfloat16)
+    gate = None if gates is None else torch.ones(gates, 72, device="cuda")
+    dx, dh, dw_post, dgate, dw_pre = tracea_gpu.norm_gate_residual_backward(x, x, x, x, w, gate, w)
+    assert dx.shape == dh.shape == x.shape
+    assert (dw_post == 0).all() and (dw_pre == 0).all()
+    assert (dgate is None) == (gates is None) and (gates is None or (dgate.shape == gate.shape and (dgate == 0).all()))
+
+
 def test_refusals(tracea_gpu):
     from tracea_amd import capi
     x = torch.randn(2, 5, 64, device="cuda")

@@ -672,14 +672,18 @@ TraceaStatus dispatch_norm_backward(const TraceaTensorView *dx_out, const Tracea
       if (o != nullptr && may_overlap(*r, *o)) return overlapping(op, "results overlap each other");
     }
   }
-  if (c.B == 0) c.T = 0;
   DeviceScope scope(c.device);
   if (scope.err != hipSuccess) return hip_status("hipSetDevice", (int)scope.err);
   hipStream_t stream = (hipStream_t)params.stream;
   const bool columns = dw_post != nullptr || dgate != nullptr || dw_pre != nullptr;
-  if (c.B == 0 || (c.T == 0 && !columns)) {
-    if (c.B == 0 && columns) return fail(TRACEA_UNSUPPORTED_CONFIG, "%s: weight gradients of an empty batch", op);
-    return TRACEA_SUCCESS;
+  if ((c.B == 0 || c.T == 0) && !columns) return TRACEA_SUCCESS;
+  if (c.B == 0) {  // (no batch entry: sums over one of no rows, without the gates that no entry has)
+    c.B = 1;
+    c.T = 0;
+    if (gates == 0) {
+      a.gate = a.dgate = nullptr;
+      a.gate_sb = 0;
+    }
   }
   finish(c, tensors, n, true, params, &a);
   std::lock_guard<std::mutex> together(g_launches);
