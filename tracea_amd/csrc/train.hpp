@@ -50,7 +50,7 @@ struct RotaryArgs {
   int first[TRACEA_MAX_ROTARY_AXES];  // first pair of the axis
   int adjacent, inverse;
   int vec;  // 16-byte pieces: columns, strides and bases allow it
-  int heads_per_group;
+  int heads_per_group, beside;  // a workgroup has a group of heads of its tokens; `beside` threads next to each other take them in turn
 };
 int launch_rotary(const RotaryArgs &a, int dtype, hipStream_t stream);
 
