@@ -6,16 +6,20 @@
 //   P_ij = exp(s_ij - lse_i)   delta_i = dO_i . O_i   dS_ij = P_ij (dO_i . v_j - delta_i)
 //   dV_j = sum_i P_ij dO_i     dK_j = scale sum_i dS_ij q_i     dQ_i = scale sum_j dS_ij k_j
 //
-// Three kernels of one shape.  A wave owns 32 columns whose operand fragments stay in registers and streams the other
-// side in tiles of 64 through LDS; every product is v_mfma_f32_16x16x32 with fp32 sums.  In the result of a 16x16 block
+// Three walks of one shape.  A wave owns 32 columns whose operand fragments stay in registers and streams the other
+// side in tiles of 64 through LDS (32: with D = 128 the sums of dK and dV are half of the 256 registers that leave room for two
+// waves on a SIMD, and the products of one fill the gaps of the other); every product is v_mfma_f32_16x16x32 with fp32 sums.  In the result of a 16x16 block
 // lane l holds column l & 15 and rows 4 (l >> 4) + 0..3; two blocks one above the other, converted to 16 bits, are the
 // second operand of the next product over those 32 rows (k slots 0-3: rows 4 g + e, slots 4-7: rows 16 + 4 g + e,
 // g = l >> 4), whose first operand enumerates the same rows: two transposing reads of the tile.
 //   forward  columns = query rows, stream K and V:    S^T = K Q^T, O^T += V^T P^T
 //   dQ       columns = query rows, stream K and V:    S^T, dP^T = V dO^T, dQ^T += K^T dS^T
 //   dK, dV   columns = keys, stream Q and dO:         S = Q K^T, dP = dO V^T, dV^T += dO^T P, dK^T += Q^T dS
-// dQ has a kernel of its own although that computes S and dP twice (7 products instead of 5): sums over the keys of a
-// row would otherwise meet from different workgroups, in an order that changes from run to run.
+// dQ has a walk of its own although that computes S and dP twice (7 products instead of 5): sums over the keys of a
+// row would otherwise meet from different workgroups, in an order that changes from run to run.  Both walks are one launch.
+//
+// The rows of a head that shares its keys with G - 1 others are packed, r = query G + head of the group: a tile of K and V is read
+// once for all of them, and the sums over the heads of a group in dK and dV are sums over rows.
 #include <type_traits>
 
 #include "contraction_kernel.hpp"
@@ -295,9 +299,13 @@ __device__ __forceinline__ float groups_max_valu(float x) {
   return fmaxf(b0, b1);
 }
 
-// A wave's scores of tile t + 1 are computed under the exponentials of tile t, and P V of tile t under the maximum over t + 1, so
-// that K is a tile ahead of V.  SG = 2: two waves share their rows and walk every other tile of 64 keys; their states are joined at the end.  A wave has 16 NQ rows:
-// 32, or 16 for a token or two of some heads, where the empty half would be most of what it waits for.
+// Forward: one pass over the keys with a running reference and sum per row.  A wave's scores of tile t + 1 are computed under the
+// exponentials of tile t, and P V of tile t under the maximum over t + 1, so that K is a tile ahead of V.  SG = 2: two waves share
+// their rows and walk every other tile of 64 keys; their states are joined at the end.  A wave has 16 NQ rows: 32, or 16 for a token
+// or two of some heads, where the empty half would be most of what it waits for.
+// Bound, long rows: vector work (exponential, maximum and conversion of a score cost about as many cycles as its products do) beside
+// the matrix pipe, and power: B4 H32 S4096 bf16 D128 1020 us = 1.08 PFLOP/s, f16 D64 687 us = 0.80.  One query over a long cache: reading K and V,
+// B8 H32:8 D128 over 8192 keys 49 us = 5.5 TB/s with the join (a large copy reaches 4.8; part of it is in the memory-side cache).
 template <int DT, int DL, int DU, int WAVES, int SG, int NQ>
 __global__ void __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 attention_train_forward_kernel(const AttentionTrainArgs a) {
@@ -584,7 +592,7 @@ attention_train_forward_kernel(const AttentionTrainArgs a) {
 }
 
 // Joins the partial results of a split key axis: a row per 32 lanes, which load one part's reference and sum each (at most 32
-// parts) and 4 columns of every part's o.
+// parts) and 4 columns of every part's o.  Bound by the latency of its loads: 3.8 us for 256 rows of 8 parts.
 template <int DT, int DU>
 __global__ void __launch_bounds__(256) attention_train_join_kernel(const AttentionTrainArgs a) {
   const long long id = ((long long)blockIdx.x * 256 + threadIdx.x) / 32;
@@ -617,51 +625,54 @@ __global__ void __launch_bounds__(256) attention_train_join_kernel(const Attenti
 
 // ---- backward ---------------------------------------------------------------------------------------------------
 
-// Per packed row -lse log2(e) and -(dO . O); f16: the largest squared norms of 64 rows of dO, and of 64 keys of V.
+// Per packed row -lse log2(e) and -(dO . O), which both walks need; f16: the largest squared norms of 64 rows of dO, and of 64 keys of V.
+// Bound by reading dO and O: B4 H32 S4096 D128 bf16 51 us = 5.3 TB/s; a launch's 5 us at B1 H12 S197 D64.
 template <int DT>
-__global__ void __launch_bounds__(256) attention_train_rows_kernel(const AttentionTrainArgs a) {
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) attention_train_rows_kernel(const AttentionTrainArgs a) {
   constexpr int LPR = 16;  // lanes per row, 8 columns each
   __shared__ float s_max[4];
   const int c = (threadIdx.x % LPR) * 8, row_blocks = a.rows_pad / TILE;
   const int bh = blockIdx.y, blk = blockIdx.x;
   const Rows w = rows_of(a, bh);
+  const bool of_rows = blk < row_blocks;
+  // (all loads first: a launch of few blocks is as long as the waits one after another)
+  u32x4 xs[TILE / 16], ys[TILE / 16];
+  float lse[TILE / 16];
+#pragma unroll
+  for (int it = 0; it < TILE / 16; ++it) {
+    const int row = it * 16 + (int)threadIdx.x / LPR, r = blk * TILE + row, j = r - row_blocks * TILE;
+    xs[it] = ys[it] = u32x4{0, 0, 0, 0};
+    lse[it] = -INFINITY;
+    if (of_rows && r < a.G * w.lq) {
+      if (c < a.D) {
+        xs[it] = *(const u32x4 *)((const unsigned short *)a.d_o.p + row_at(a, a.d_o, w, r) + c);
+        ys[it] = *(const u32x4 *)((const unsigned short *)a.o.p + row_at(a, a.o, w, r) + c);
+      }
+      const int i = query_of(a, r);
+      lse[it] = a.lse[(long long)w.b * a.lse_sb + (long long)(w.hk * a.G + r - i * a.G) * a.lse_sh + (long long)i * a.lse_ss];
+    } else if (!of_rows && j < w.lk && c < a.D) {
+      xs[it] = *(const u32x4 *)(slice(a.v, w.b, w.hk) + (long long)j * a.v.ss + c);
+    }
+  }
   float big = 0.0f;
 #pragma unroll
   for (int it = 0; it < TILE / 16; ++it) {
-    const int row = it * 16 + (int)threadIdx.x / LPR;
-    float dot = 0.0f, norm = 0.0f;
-    if (blk < row_blocks) {
-      const int r = blk * TILE + row;
-      const bool there = r < a.G * w.lq;
-      if (there && c < a.D) {
-        float x[8], y[8];
-        unpack8<DT>(*(const u32x4 *)((const unsigned short *)a.d_o.p + row_at(a, a.d_o, w, r) + c), x);
-        unpack8<DT>(*(const u32x4 *)((const unsigned short *)a.o.p + row_at(a, a.o, w, r) + c), y);
+    const int r = blk * TILE + it * 16 + (int)threadIdx.x / LPR;
+    float x[8], y[8], dot = 0.0f, norm = 0.0f;
+    unpack8<DT>(xs[it], x);
+    unpack8<DT>(ys[it], y);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          dot = __builtin_fmaf(x[e], y[e], dot);
-          norm = __builtin_fmaf(x[e], x[e], norm);
-        }
-      }
+    for (int e = 0; e < 8; ++e) {
+      dot = __builtin_fmaf(x[e], y[e], dot);
+      norm = __builtin_fmaf(x[e], x[e], norm);
+    }
+    if (of_rows) {
 #pragma unroll
       for (int s = 1; s < LPR; s <<= 1) dot += __shfl_xor(dot, s, 64);
       if (c == 0) {
-        float nl = -INFINITY;
-        if (there) {
-          const int i = query_of(a, r);
-          const float lse = a.lse[(long long)w.b * a.lse_sb + (long long)(w.hk * a.G + r - i * a.G) * a.lse_sh + (long long)i * a.lse_ss];
-          if (lse != -INFINITY) nl = (DT == DT_F16 ? F16_P_SHIFT : 0.0f) - lse * LOG2E;
-        }
-        a.neg_lse2[(long long)bh * a.rows_pad + r] = nl;
-        a.neg_delta[(long long)bh * a.rows_pad + r] = nl == -INFINITY ? 0.0f : -dot;
-      }
-    } else {
-      const int j = (blk - row_blocks) * TILE + row;
-      if (j < w.lk && c < a.D) {
-        float x[8];
-        unpack8<DT>(*(const u32x4 *)(slice(a.v, w.b, w.hk) + (long long)j * a.v.ss + c), x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) norm = __builtin_fmaf(x[e], x[e], norm);
+        const bool sees = lse[it] != -INFINITY;
+        a.neg_lse2[(long long)bh * a.rows_pad + r] = sees ? (DT == DT_F16 ? F16_P_SHIFT : 0.0f) - lse[it] * LOG2E : -INFINITY;
+        a.neg_delta[(long long)bh * a.rows_pad + r] = sees ? -dot : 0.0f;
       }
     }
     if constexpr (DT == DT_F16) {
@@ -678,7 +689,8 @@ __global__ void __launch_bounds__(256) attention_train_rows_kernel(const Attenti
   }
 }
 
-// dQ of a block of packed rows.  SG = 2: two waves share 32 rows, each takes half of every tile of keys.
+// dQ of a block of packed rows: three products and two operands from LDS per tile.  SG = 2: two waves share 32 rows, each takes half of
+// every tile of keys.
 template <int DT, int DL, int DU, int WAVES, int SG>
 __device__ __forceinline__ void dq_block(const AttentionTrainArgs &a, int id, unsigned char *sK) {
   using T = Tile<DL>;
@@ -852,8 +864,8 @@ __device__ __forceinline__ void dq_block(const AttentionTrainArgs &a, int id, un
   }
 }
 
-// dK and dV of a block of keys, or of a part of the rows that see them.  SG = 2: two waves share 32 keys, each takes half of
-// every tile of rows.
+// dK and dV of a block of keys, or of a part of the rows that see them: four products per tile.  SG = 2: two waves share 32 keys,
+// each takes half of every tile of rows.
 template <int DT, int DL, int DU, int WAVES, int SG>
 __device__ __forceinline__ void dkv_block(const AttentionTrainArgs &a, int id, unsigned char *sQ, float *sL, float *sD, u32x4 *parked) {
   using T = Tile<DL>;
@@ -1066,6 +1078,9 @@ __device__ __forceinline__ void dkv_block(const AttentionTrainArgs &a, int id, u
 }
 
 // The workgroups of dK and dV first, then those of dQ: one launch, so that neither waits for the other's last ones.
+// Bound, long rows: matrix pipe and vector work of two waves per SIMD, and power: B4 H32 S4096 D128 bf16 3.0 ms = 1.26 PFLOP/s
+// of the seven products, 0.90 of the five that are needed.  Short rows: the serial walk of a workgroup over its tiles, B1 H12 S1024
+// D64 f16 causal 23 us, S197 11 us.
 template <int DT, int DL, int DU, int WAVES, int SG>
 __global__ void __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 attention_train_backward_kernel(const AttentionTrainArgs a, int dkv_blocks) {
@@ -1076,7 +1091,8 @@ attention_train_backward_kernel(const AttentionTrainArgs a, int dkv_blocks) {
   else dq_block<DT, DL, DU, WAVES, SG>(a, blockIdx.x - dkv_blocks, tiles);
 }
 
-// Adds up the parts of dK and dV where the rows are split over workgroups: 4 columns per thread.
+// Adds up the parts of dK and dV where the rows are split over workgroups, in their order: 4 columns per thread.  Bound by reading the
+// parts: 9.3 us for two parts of B4 H4 S1500 D96 (36.9 MB, 4.0 TB/s).
 template <int DT, int DU>
 __global__ void __launch_bounds__(256) attention_train_sum_kernel(const AttentionTrainArgs a) {
   constexpr int PER = 2 * DU / 4;
