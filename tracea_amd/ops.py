@@ -8,7 +8,7 @@ torch supplies device memory and the current stream; all arithmetic happens in
 ``libtracea.so``.
 """
 import ctypes as C
-import struct
+import math
 
 import torch
 
@@ -340,23 +340,26 @@ def attention(q, k, v, causal=False, scale=0.0, out=None):
 
 
 _LAYOUTS = {}
-_PACK_VIEW = struct.Struct("QIxxxxQQii")  # the bytes of a capi.TensorView
 
 
 def _plain_view(t):
-    """capi.TensorView of a tensor.  The extent and stride arrays it borrows are kept by layout (shape and strides), never by a
-    tensor's address; the view holds them.  (Made from packed bytes: half the time of the structure's constructor.)"""
-    key = (t.shape, t.stride())
+    """capi.TensorView of a tensor.  The extent and stride arrays it borrows, and the bytes of a view without its address, are kept by
+    layout (shape, strides, type and device), never by a tensor's address; the view holds them."""
+    key = (t.shape, t.dtype, t.get_device()) if t.is_contiguous() else (t.shape, t.stride(), t.dtype, t.get_device())
     layout = _LAYOUTS.get(key)
     if layout is None:
+        dtype = _DTYPES.get(t.dtype)
+        if dtype is None:
+            raise TypeError("unsupported dtype %s" % t.dtype)
         if len(_LAYOUTS) >= 1024:
             _LAYOUTS.clear()
-        v = capi.View(None, key[0], key[1], 0, 0)
-        layout = _LAYOUTS[key] = (len(key[0]), C.addressof(v._shape), C.addressof(v._stride), v)
-    dtype = _DTYPES.get(t.dtype)
-    if dtype is None:
-        raise TypeError("unsupported dtype %s" % t.dtype)
-    view = capi.TensorView.from_buffer_copy(_PACK_VIEW.pack(t.data_ptr(), layout[0], layout[1], layout[2], dtype, t.get_device()))
+        strides = t.stride()
+        if t.is_contiguous():  # (whatever stands for the extents of 1: one layout whichever such tensor comes first)
+            strides = [math.prod(max(n, 1) for n in t.shape[i + 1:]) for i in range(t.dim())]
+        v = capi.View(None, t.shape, strides, dtype, t.get_device())
+        layout = _LAYOUTS[key] = (bytes(v.c), v)
+    view = capi.TensorView.from_buffer_copy(layout[0])
+    view.ptr = t.data_ptr()
     view.layout = layout
     return view
 
