@@ -483,8 +483,8 @@ TraceaStatus tracea_rotary(TraceaTensorView q, const TraceaTensorView *k, Tracea
  * The backward pass reads x_out (x where there is no h) and h as the forward pass left them and works out both norms
  * again: dx_out (optional: absent is 0) and dy are the gradients of x_out and y; dx, dh have the type of h, dw_post, dgate
  * [G,C], dw_pre are f32 and are summed in an order that does not change.  Gradients that are not wanted are NULL (dx is
- * required).  It takes a workspace per (device,
- * stream), at most 16 MiB and 8 bytes per channel and batch entry, grown on demand, never under capture. */
+ * required).  It takes a workspace per (device, stream), at most 16 MiB plus 8 bytes per channel and batch entry, grown on
+ * demand, never under capture. */
 typedef struct {
   float eps;
   float residual_scale;
