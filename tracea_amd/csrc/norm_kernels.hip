@@ -10,7 +10,9 @@
 // that they are taken in one go and the threads meet once per row.  Column sums leave as one partial row per workgroup and a second
 // kernel adds these up in their order: no atomics.
 // Measured (GPU time, a large copy reaches 4.8 TB/s): forward C2048 T24960 bf16 89 us = 4.6 TB/s, C4096 T8192 48 us (5.6 TB/s, partly from
-// the memory-side cache), 16 rows of 4096 4.6 us; backward C2048 T24960 118 us = 5.2 TB/s with its column sums.
+// the memory-side cache), 16 rows of 4096 4.6 us; backward C2048 T24960 128 us = 4.8 TB/s with its column sums.
+#include <type_traits>
+
 #include "contraction_kernel.hpp"
 #include "train.hpp"
 
@@ -30,28 +32,51 @@ template <bool VEC>
 __device__ __forceinline__ int channel(int e, int lane, int lanes) {
   return VEC ? lane * V + e : e * lanes + lane;
 }
-// A thread's channels of a row as they lie in memory: the next row's are requested before this one's are worked on.
+// A thread's channels of a row as they lie in memory: the next row's are requested before this one's are worked on.  One by one, every
+// 16-bit value has a register of its own, and hold() keeps the conversions behind all loads: the compiler moves each of them behind
+// its load's test of the channel, where it waits for that load (backward C2047 T24960 bf16 148 us, 452 without; C2048 140).
 template <typename T, bool VEC>
-__device__ __forceinline__ Eight<T> request(const T *row, int lane, int lanes, int C) {
+struct Loaded {
   Eight<T> p;
+};
+template <typename T>
+struct Loaded<T, false> {
+  std::conditional_t<sizeof(T) == 2, unsigned, float> x[V];
+};
+template <typename T, bool VEC>
+__device__ __forceinline__ Loaded<T, VEC> request(const T *row, int lane, int lanes, int C) {
+  Loaded<T, VEC> r;
   if constexpr (VEC) {
     const int c = channel<VEC>(0, lane, lanes);
-    if (c < C) return *(const Eight<T> *)(row + c);
+    if (c < C) return {*(const Eight<T> *)(row + c)};
 #pragma unroll
-    for (int e = 0; e < V; ++e) p.x[e] = (T)0.0f;
+    for (int e = 0; e < V; ++e) r.p.x[e] = (T)0.0f;
   } else {
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       const int c = channel<VEC>(e, lane, lanes);
-      p.x[e] = c < C ? row[c] : (T)0.0f;
+      if constexpr (sizeof(T) == 2) r.x[e] = c < C ? ((const unsigned short *)row)[c] : 0u;
+      else r.x[e] = c < C ? row[c] : 0.0f;
     }
   }
-  return p;
+  return r;
 }
 template <typename T>
-__device__ __forceinline__ void widen(const Eight<T> &p, float (&x)[V]) {
+__device__ __forceinline__ void hold(Loaded<T, false> &r) {
 #pragma unroll
-  for (int e = 0; e < V; ++e) x[e] = (float)p.x[e];
+  for (int e = 0; e < V; ++e) asm volatile("" : "+v"(r.x[e]));
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void widen(const Loaded<T, VEC> &r, float (&x)[V]) {
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    if constexpr (VEC) {
+      x[e] = (float)r.p.x[e];
+    } else {
+      if constexpr (sizeof(T) == 2) x[e] = (float)__builtin_bit_cast(T, (unsigned short)r.x[e]);
+      else x[e] = r.x[e];
+    }
+  }
 }
 template <typename T, bool VEC>
 __device__ __forceinline__ void store(T *row, int lane, int lanes, int C, const float (&x)[V]) {
@@ -79,7 +104,7 @@ __device__ __forceinline__ void load_weights(const float *w, int lane, int lanes
     for (int e = 0; e < V; ++e) x[e] = 1.0f;
     return;
   }
-  widen(request<float, VEC>(w, lane, lanes, C), x);
+  widen<float, VEC>(request<float, VEC>(w, lane, lanes, C), x);
 }
 
 // Sums of N values over the threads that share a row: `lanes` lanes of a wave (a power of two up to 64), then the waves of
@@ -138,7 +163,7 @@ __global__ void __launch_bounds__(1024) norm_forward_kernel(const NormArgs a, in
   const int waves = blockDim.x >> 6;
   RowSum<1> row_sum{buf};
   if (p.first >= p.end) return;
-  Eight<T> next_x, next_h;
+  Loaded<T, VEC> next_x, next_h;
   auto fetch = [&](int t) __attribute__((always_inline)) {
     const int tt = t < p.end ? t : p.first;
     next_x = request<T, VEC>(row_of<const T>(a.x, p.b, tt), p.lane, lanes, a.C);
@@ -159,8 +184,8 @@ __global__ void __launch_bounds__(1024) norm_forward_kernel(const NormArgs a, in
     const int tt = t0 + p.slot;
     const bool there = tt < p.end;
     float x[V], h[V];
-    widen(next_x, x);
-    if constexpr (POST) widen(next_h, h);
+    widen<T, VEC>(next_x, x);
+    if constexpr (POST) widen<T, VEC>(next_h, h);
     if (t0 + p.slots < p.end) fetch(tt + p.slots);
     if constexpr (POST) {
       float sum[1] = {0.0f};
@@ -193,7 +218,7 @@ __global__ void __launch_bounds__(1024) norm_backward_kernel(const NormArgs a, i
   RowSum<6> row_sum{buf};
   const bool has_dx = a.dx_out.p != nullptr;
   constexpr bool AHEAD = VEC && sizeof(T) == 2;  // (else a row more takes the registers beyond the 128 that 1024 threads have)
-  Eight<T> next_x, next_g, next_h, next_d;
+  Loaded<T, VEC> next_x, next_g, next_h, next_d;
   auto fetch = [&](int t) __attribute__((always_inline)) {
     const int tt = t < p.end ? t : p.first;
     if constexpr (PRE) {
@@ -204,7 +229,10 @@ __global__ void __launch_bounds__(1024) norm_backward_kernel(const NormArgs a, i
     if (has_dx) next_d = request<T, VEC>(row_of<const T>(a.dx_out, p.b, tt), p.lane, lanes, a.C);
   };
 #pragma unroll
-  for (int e = 0; e < V; ++e) next_d.x[e] = (T)0.0f;
+  for (int e = 0; e < V; ++e) {
+    if constexpr (VEC) next_d.p.x[e] = (T)0.0f;
+    else next_d.x[e] = 0;
+  }
   if (AHEAD && p.first < p.end) fetch(p.first + p.slot);
   float gw[V], wp[V], sa[V], sp[V];
   if constexpr (POST) {
@@ -223,12 +251,20 @@ __global__ void __launch_bounds__(1024) norm_backward_kernel(const NormArgs a, i
     const bool there = tt < p.end;
     float x[V], g[V], h[V], d[V];
     if constexpr (!AHEAD) fetch(tt);
-    if constexpr (PRE) {
-      widen(next_x, x);
-      widen(next_g, g);
+    if constexpr (!AHEAD && sizeof(T) == 2) {  // (32-bit values have no conversions)
+      if constexpr (PRE) {
+        hold(next_x);
+        hold(next_g);
+      }
+      if constexpr (POST) hold(next_h);
+      hold(next_d);
     }
-    if constexpr (POST) widen(next_h, h);
-    widen(next_d, d);
+    if constexpr (PRE) {
+      widen<T, VEC>(next_x, x);
+      widen<T, VEC>(next_g, g);
+    }
+    if constexpr (POST) widen<T, VEC>(next_h, h);
+    widen<T, VEC>(next_d, d);
     if (AHEAD && t0 + p.slots < p.end) fetch(tt + p.slots);
     // x'.x', g.x', h.h, and (gate w_post h).dx', .g, .x': mean(a h^) follows from the last three
     float s[6] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
