@@ -52,4 +52,5 @@ def test_types_that_no_operator_has_are_refused():
 
 def test_parameter_blocks_have_the_size_of_the_headers():
     assert C.sizeof(capi.NormParams) == 16
-    assert C.sizeof(capi.RotaryParams) == 4 + 4 * capi.MAX_ROTARY_AXES + 4 + 4 + (4 if (12 + 4 * capi.MAX_ROTARY_AXES) % 8 else 0) + 8
+    assert C.sizeof(capi.RotaryParams) == 32  # 4 + 4 * 4, two bytes, padding to 24, a pointer
+    assert (capi.RotaryParams.adjacent.offset, capi.RotaryParams.inverse.offset, capi.RotaryParams.stream.offset) == (20, 21, 24)
