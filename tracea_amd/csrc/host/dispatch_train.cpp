@@ -324,8 +324,9 @@ TraceaStatus check_attention(Attention &c, const TraceaAttentionParams &params, 
     return fail(TRACEA_INVALID_PARAMS, "%s: %lld query heads are not a multiple of %lld key/value heads", op, Hq, Hk);
   if (D < 1 || D > 128) return fail(TRACEA_UNSUPPORTED_CONFIG, "%s: head dim %lld (1 to 128 supported)", op, D);
   const long long G = Hq / Hk;
-  if (G * G * (Sq + 128) >= (1ll << 31) || G * (Sq + Sk + 128) >= (1ll << 31) || B * Hk * ((G * Sq + 127) / 128) >= (1ll << 31) || B * Hk * ((Sk + 127) / 128) >= (1ll << 31) ||
-      B * Hk >= 65536)
+  // (rows are divided by G with a 32-bit product, blocks and heads are grid dimensions)
+  if (G * G * (Sq + 128) >= (1ll << 31) || G * (Sq + Sk + 128) >= (1ll << 31) || B * Hk * ((G * Sq + 127) / 128) >= (1ll << 31) ||
+      B * Hk * ((Sk + 127) / 128) >= (1ll << 31) || B * Hk >= 65536)
     return fail(TRACEA_UNSUPPORTED_CONFIG, "%s: problem too large", op);
   c.scale = params.scale;
   if (c.scale == 0.0f) c.scale = 1.0f / sqrtf((float)D);

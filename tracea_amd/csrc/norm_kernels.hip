@@ -6,9 +6,9 @@
 //
 // Bound by memory: one pass, each row read once and written once.  A row is held in registers by the threads of a
 // workgroup (up to 256 channels: by some lanes of a wave), 8 channels each; a workgroup takes a run of rows of one batch entry,
-// the next one requested ahead, with the weights and, backward, the column sums in registers all along.  The backward pass needs six sums over a row; all are linear in what is loaded, so
-// that they are taken in one go and the threads meet once per row.  Column sums leave as one partial row per workgroup and a second
-// kernel adds these up in their order: no atomics.
+// the next one requested ahead, with the weights and, backward, the column sums in registers all along.  The backward pass needs
+// six sums over a row; all are linear in what is loaded, so that they are taken in one go and the threads meet once per row.
+// Column sums leave as one partial row per workgroup and a second kernel adds these up in their order: no atomics.
 // Measured (GPU time, a large copy reaches 4.8 TB/s): forward C2048 T24960 bf16 89 us = 4.6 TB/s, C4096 T8192 48 us (5.6 TB/s, partly from
 // the memory-side cache), 16 rows of 4096 4.6 us; backward C2048 T24960 128 us = 4.8 TB/s with its column sums.
 #include <type_traits>
