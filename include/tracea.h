@@ -441,8 +441,8 @@ TraceaStatus tracea_conv_coords_device(const TraceaConvParamsBlock *p, int32_t *
  * probabilities and their gradients are rounded once to the operand type for the matrix products.  scale 0 selects
  * 1/sqrt(D); softmax_mode is ignored.  The same call on the same inputs gives the same bits.
  * Read and written in place: D a multiple of 8 and contiguous, other strides multiples of 8 elements (rows and heads not
- * descending), bases on 16 bytes, no result over an operand.  Anything else runs from copies in the padded road's
- * per-(device, stream) buffer (at most 1 GiB, not grown under capture).  Both calls take a workspace per (device,
+ * descending), bases on 16 bytes, no result over an operand.  Anything else runs from padded copies in a buffer of these
+ * two operators' own per (device, stream) (at most 1 GiB, not grown under capture).  Both calls take a workspace per (device,
  * stream), grown on demand, never under capture and never freed: 8 bytes per row for the backward pass; for a forward
  * pass of few rows over many keys, which is split along the keys, the partial results. */
 TraceaStatus tracea_attention_forward(TraceaTensorView q, TraceaTensorView k, TraceaTensorView v,

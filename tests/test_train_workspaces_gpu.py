@@ -1,0 +1,86 @@
+"""Buffers that the operators for training keep per stream: whose they are, what two threads see, what a stream under capture gets."""
+import ctypes as C
+import threading
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+def new_stream():
+    """A stream that no call has been made on."""
+    from tracea_amd import capi
+    handle = C.c_void_p()
+    assert capi.lib().hipStreamCreate(C.byref(handle)) == 0
+    return torch.cuda.ExternalStream(handle.value)
+
+
+def make(*shapes, dtype=torch.bfloat16, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return [torch.randn(*s, device="cuda", generator=g).to(dtype) for s in shapes]
+
+
+def under_capture(stream, call):
+    """What `call` returns or raises on `stream` under capture, and the graph."""
+    from tracea_amd import capi
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    result = None
+    with torch.cuda.stream(stream):
+        with torch.cuda.graph(graph, stream=stream):
+            try:
+                result = call()
+            except capi.TraceaError as e:
+                result = e
+    return result, graph
+
+
+def test_copies_are_not_in_the_buffer_of_other_operators(tracea_gpu):
+    """A stream on which a GEMM has made its padded copies has no buffer for those of attention yet: under capture, where none can be
+    allocated, the call is refused instead of writing over the GEMM's."""
+    from tracea_amd import capi
+    a, b = make((333, 4099), (4099, 65))
+    q, k, v = make((2, 2, 40, 50), (2, 2, 40, 50), (2, 2, 40, 50))
+    out, lse = torch.empty_like(q), torch.empty(2, 2, 40, device="cuda")
+    stream = new_stream()
+    with torch.cuda.stream(stream):
+        tracea_gpu.gemm(a.t().contiguous().t(), b)  # strided along K: from copies
+        torch.cuda.synchronize()
+    result, _ = under_capture(stream, lambda: tracea_gpu.attention_forward(q, k, v, out=out, lse=lse))
+    assert isinstance(result, capi.TraceaError) and result.status == capi.UNSUPPORTED_CONFIG, result
+
+
+def test_two_threads_on_one_stream(tracea_gpu):
+    """Attention and a GEMM, both from copies of their operands, in two threads on the default stream."""
+    a, b = make((333, 1031), (1031, 265), seed=1)
+    a = a.t().contiguous().t()
+    q, k, v, do = make(*[(2, 4, 130, 50)] * 4, seed=2)
+
+    def attend():
+        o, lse = tracea_gpu.attention_forward(q, k, v, causal=True)
+        return (o, lse) + tracea_gpu.attention_backward(q, k, v, o, lse, do, causal=True)
+
+    def multiply():
+        return (tracea_gpu.gemm(a, b),)
+    want = {f: f() for f in (attend, multiply)}
+    torch.cuda.synchronize()
+    got, errors = {attend: [], multiply: []}, []
+
+    def run(f):
+        try:
+            for _ in range(100):
+                got[f].append(f())
+        except Exception as e:  # noqa: BLE001 (reported below)
+            errors.append(e)
+    threads = [threading.Thread(target=run, args=(f,)) for f in got]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors
+    for f in got:
+        for results in got[f]:
+            for x, y in zip(results, want[f]):
+                assert torch.equal(x, y)

@@ -561,7 +561,9 @@ void *splitk_scratch(int device, hipStream_t stream, size_t bytes) {
 // rules: grows on demand up to a cap, never while its stream is being captured, never freed.
 constexpr size_t kPadScratchCap = 1u << 30;
 std::map<std::pair<int, void *>, std::pair<void *, size_t>> g_pad_scratch;
-std::map<std::pair<int, void *>, std::pair<void *, size_t>> g_train_scratch;  // workspaces of the operators for training
+// Of the operators for training: their workspaces, and the padded copies of their operands (not in the buffer above, which calls of
+// other threads on the same stream fill without the lock that keeps the launches of these operators together).
+std::map<std::pair<int, void *>, std::pair<void *, size_t>> g_train_scratch, g_train_copies;
 void *keep_scratch(std::map<std::pair<int, void *>, std::pair<void *, size_t>> &all, int device, hipStream_t stream, size_t bytes) {
   std::lock_guard<std::mutex> lock(g_scratch_mu);
   auto &slot = all[{device, (void *)stream}];
@@ -2879,7 +2881,9 @@ TraceaStatus dispatch_attention(const TraceaTensorView &tq, const TraceaTensorVi
                     attention_variant(vi).launch(a, q.dtype, (hipStream_t)params.stream));
 }
 
-void *padded_scratch(int device, hipStream_t stream, size_t bytes) { return pad_scratch(device, stream, bytes); }
+void *train_copies(int device, hipStream_t stream, size_t bytes) {
+  return bytes > kPadScratchCap ? nullptr : keep_scratch(g_train_copies, device, stream, bytes);
+}
 void *train_scratch(int device, hipStream_t stream, size_t bytes) { return keep_scratch(g_train_scratch, device, stream, bytes); }
 
 TraceaStatus dispatch_clock_probe(void *out, int32_t samples, int32_t gap, void *stream) {

@@ -130,8 +130,9 @@ TraceaStatus dispatch_norm_backward(const TraceaTensorView *dx_out, const Tracea
                                     TraceaTensorView *dw_post, TraceaTensorView *dgate, TraceaTensorView *dw_pre,
                                     const TraceaNormParams &params);
 // Device memory kept per (device, stream): grows on demand, never while the stream is being captured (null then), is never
-// freed.  The first holds padded copies of operands (at most 1 GiB), the second workspaces of the operators for training.
-void *padded_scratch(int device, hipStream_t stream, size_t bytes);
+// freed.  Both belong to the operators for training alone, which use them under one lock: padded copies of operands (at most
+// 1 GiB), workspaces.
+void *train_copies(int device, hipStream_t stream, size_t bytes);
 void *train_scratch(int device, hipStream_t stream, size_t bytes);
 
 // Shader-clock probe (tracea_clock_probe): argument checks, then the one-wave sampling kernel on `stream`.

@@ -10,7 +10,8 @@ namespace tracea_amd {
 
 namespace {
 
-// The launches of a call that pass something on in a workspace stay together on their stream, whichever threads use it.
+// The launches of a call that pass something on in a workspace or in copies stay together on their stream, whichever threads use
+// it: no other operator writes either buffer.
 std::mutex g_launches;
 
 TraceaStatus ready(const char *what) {
@@ -193,7 +194,7 @@ TraceaStatus run_attention(const Attention &c, bool from_copies) {
     const long long Dp = D <= 64 ? 64 : 128;
     const size_t one_q = (size_t)(B * Hq * Sq) * (size_t)Dp * 2, one_k = (size_t)(B * Hk * Sk) * (size_t)Dp * 2;
     const size_t bytes = c.backward ? 4 * one_q + 4 * one_k : 2 * one_q + 2 * one_k;
-    unsigned char *buf = from_copies ? nullptr : (unsigned char *)padded_scratch(c.q.device, c.stream, bytes);
+    unsigned char *buf = from_copies ? nullptr : (unsigned char *)train_copies(c.q.device, c.stream, bytes);
     if (buf == nullptr)
       return fail(TRACEA_UNSUPPORTED_CONFIG,
                   "%s: head dim %lld / these strides need padded copies, and no buffer for them can be had (stream under capture, "
