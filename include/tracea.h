@@ -475,7 +475,7 @@ TraceaStatus tracea_rotary(TraceaTensorView q, const TraceaTensorView *k, Tracea
 /* What stands between two blocks of a network with a norm behind each block and one in front of it:
  *   n = h * rsqrt(mean(h^2) + eps) * w_post      x_out = residual_scale * x + gate * n
  *   y = x_out * rsqrt(mean(x_out^2) + eps) * w_pre                       (means over the channels)
- *   x, h, x_out, y [B,T,C], C contiguous, up to 8192, one type of f32, f16, bf16
+ *   x, h, x_out, y [B,T,C], C contiguous, up to 8192, one type of f32, f16, bf16; B up to 65000, T up to 2^31 - 2^20
  *   w_post, w_pre [C], gate [G,C] with G = 1 or B (absent: 1), contiguous, f32
  * h, w_post, gate and x_out go together: without h (first norm of a network) x_out is x itself, passed as NULL, and
  * residual_scale is not used.  Without y and w_pre (behind the last block) there is no second norm.  x_out may be x or h, y may be

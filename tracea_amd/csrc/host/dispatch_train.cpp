@@ -551,6 +551,8 @@ TraceaStatus norm_call(NormCall &c, const TraceaTensorView &x, const TraceaNormP
   if (!is_float_type(c.dtype)) return fail(TRACEA_UNSUPPORTED_CONFIG, "%s: f32, f16 or bf16 tensors (got %s)", c.op, dtype_name(c.dtype));
   if (c.C < 1 || c.C > kNormMaxChannels) return fail(TRACEA_UNSUPPORTED_CONFIG, "%s: %lld channels (1 to %d supported)", c.op, c.C, kNormMaxChannels);
   if (c.B > 65000) return fail(TRACEA_UNSUPPORTED_CONFIG, "%s: more than 65000 batch entries", c.op);
+  // (rows are counted in 32 bits, up to the end of the last workgroup's run)
+  if (c.T > (1ll << 31) - (1 << 20)) return fail(TRACEA_UNSUPPORTED_CONFIG, "%s: %lld rows (up to 2^31 - 2^20 supported)", c.op, c.T);
   if (!std::isfinite(params.eps) || params.eps < 0.0f || !std::isfinite(params.residual_scale))
     return fail(TRACEA_INVALID_PARAMS, "%s: eps must be finite and not negative, residual_scale finite", c.op);
   return check_device(c.op, c.device);
