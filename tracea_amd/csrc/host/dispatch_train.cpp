@@ -75,6 +75,7 @@ HeadView head_view(const View &v) { return HeadView{v.ptr, v.stride[0], v.stride
 struct Attention {
   const char *op;
   View q, k, v, o, lse, d_o, dq, dk, dv;
+  View q_lengths, k_lengths;  // without elements where absent
   const int *q_len = nullptr, *k_len = nullptr;
   bool backward = false;
   float scale = 0.0f;
@@ -82,9 +83,8 @@ struct Attention {
   hipStream_t stream = nullptr;
 };
 
-TraceaStatus read_lengths(const char *op, const char *name, const TraceaTensorView *t, long long B, int device, const int **out) {
+TraceaStatus read_lengths(const char *op, const char *name, const TraceaTensorView *t, long long B, int device, View &v, const int **out) {
   if (t == nullptr) return TRACEA_SUCCESS;
-  View v;
   TraceaStatus st = read(op, name, *t, 1, &v);
   if (st != TRACEA_SUCCESS) return st;
   if (v.dtype != TRACEA_DTYPE_INT32 || v.shape[0] != B || (B > 1 && v.stride[0] != 1))
@@ -315,8 +315,8 @@ TraceaStatus check_attention(Attention &c, const TraceaAttentionParams &params, 
   if (c.lse.device != c.q.device) return fail(TRACEA_INVALID_PARAMS, "%s: operands live on different devices", op);
   for (int i = 0; i < (c.backward ? 7 : 3); ++i)
     if (halves[i]->device != c.q.device) return fail(TRACEA_INVALID_PARAMS, "%s: operands live on different devices", op);
-  if ((st = read_lengths(op, "q_lengths", q_lengths, B, c.q.device, &c.q_len)) != TRACEA_SUCCESS) return st;
-  if ((st = read_lengths(op, "k_lengths", k_lengths, B, c.q.device, &c.k_len)) != TRACEA_SUCCESS) return st;
+  if ((st = read_lengths(op, "q_lengths", q_lengths, B, c.q.device, c.q_lengths, &c.q_len)) != TRACEA_SUCCESS) return st;
+  if ((st = read_lengths(op, "k_lengths", k_lengths, B, c.q.device, c.k_lengths, &c.k_len)) != TRACEA_SUCCESS) return st;
   if (B == 0 || Hq == 0) {
     *nothing = true;
     return Hk == 0 || B == 0 || Sk == 0 ? TRACEA_SUCCESS : fail(TRACEA_INVALID_PARAMS, "%s: no query heads for %lld key heads", op, Hk);
@@ -341,6 +341,11 @@ TraceaStatus overlapping(const char *op, const char *what) {
   return fail(TRACEA_INVALID_PARAMS, "%s: %s", op, what);
 }
 
+// (the kernels read the lengths while others of their workgroups write)
+bool over_lengths(const Attention &c, const View &result) {
+  return (c.q_len != nullptr && may_overlap(result, c.q_lengths)) || (c.k_len != nullptr && may_overlap(result, c.k_lengths));
+}
+
 }  // namespace
 
 TraceaStatus dispatch_attention_forward(const TraceaTensorView &q, const TraceaTensorView &k, const TraceaTensorView &v,
@@ -360,6 +365,7 @@ TraceaStatus dispatch_attention_forward(const TraceaTensorView &q, const TraceaT
   if (folds(c.o) || folds(c.lse)) return overlapping(op, "elements of a result share an address");
   if (may_overlap(c.lse, c.q) || may_overlap(c.lse, c.k) || may_overlap(c.lse, c.v) || may_overlap(c.lse, c.o))
     return overlapping(op, "lse overlaps another tensor");
+  if (over_lengths(c, c.o) || over_lengths(c, c.lse)) return overlapping(op, "a result overlaps the lengths");
   std::lock_guard<std::mutex> together(g_launches);
   return run_attention(c, false);
 }
@@ -387,6 +393,7 @@ TraceaStatus dispatch_attention_backward(const TraceaTensorView &q, const Tracea
   for (int i = 0; i < 3; ++i) {
     if (folds(*results[i])) return overlapping(op, "elements of a result share an address");
     if (may_overlap(*results[i], c.lse)) return overlapping(op, "a result overlaps lse");
+    if (over_lengths(c, *results[i])) return overlapping(op, "a result overlaps the lengths");
     for (int j = 0; j < i; ++j)
       if (may_overlap(*results[i], *results[j])) return overlapping(op, "results overlap each other");
   }
