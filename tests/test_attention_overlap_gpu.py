@@ -25,3 +25,13 @@ def test_results_over_the_lengths_are_refused(tracea_gpu, which):
         refused(lambda **kw: tracea_gpu.attention_backward(q, q, q, o, lse, q, **n, **kw), **{name: as_half})
     assert (memory == 6).all()
     tracea_gpu.attention_backward(q, q, q, o, lse, q, **n)
+
+
+def test_rotary_over_the_end_of_its_positions_is_refused(tracea_gpu):
+    from tracea_amd import capi
+    memory = torch.zeros(64 + 64 * 64, device="cuda", dtype=torch.int32)
+    pos = memory[:64].view(1, 64, 1)
+    out = memory[63:63 + 64 * 64].view(torch.float32).view(1, 1, 64, 64)  # (over the last position alone)
+    with pytest.raises(capi.TraceaError) as e:
+        tracea_gpu.rotary(torch.randn(1, 1, 64, 64, device="cuda"), None, pos, torch.ones(32, device="cuda"), q_out=out)
+    assert e.value.status == capi.INVALID_PARAMS and "positions" in str(e.value)
