@@ -1,0 +1,39 @@
+"""Sizes, strides and overlaps at the limits of the operators for training: what is taken gives the formulas' results, the rest is refused."""
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+def test_gradients_side_by_side_within_a_head(tracea_gpu):
+    """Operands and gradients as [B,S,H,3,D]: the three share the range of a head's row and no element."""
+    g = torch.Generator(device="cuda").manual_seed(11)
+    qkv = torch.randn(2, 70, 4, 3, 64, device="cuda", generator=g).bfloat16()
+    do = torch.randn(2, 4, 70, 64, device="cuda", generator=g).bfloat16()
+    q, k, v = (qkv[:, :, :, i].transpose(1, 2) for i in range(3))
+    o, lse = tracea_gpu.attention_forward(q, k, v, causal=True)
+    want = tracea_gpu.attention_backward(q, k, v, o, lse, do, causal=True)
+    grad = torch.zeros_like(qkv)
+    part = {n: grad[:, :, :, i].transpose(1, 2) for i, n in enumerate(("dq", "dk", "dv"))}
+    for a, b in zip(tracea_gpu.attention_backward(q, k, v, o, lse, do, causal=True, **part), want):
+        assert torch.equal(a, b)
+    # rotary over them, in place
+    pos = torch.arange(70, dtype=torch.int32, device="cuda").view(1, 70, 1)
+    freq = torch.logspace(0, -3, 32, device="cuda")
+    want = tracea_gpu.rotary(q.contiguous(), k.contiguous(), pos, freq)
+    for a, b in zip(tracea_gpu.rotary(q, k, pos, freq, q_out=q, k_out=k), want):
+        assert torch.equal(a, b)
+
+
+def test_results_that_share_elements_are_refused(tracea_gpu):
+    from tracea_amd import capi
+    q = torch.randn(2, 4, 10, 64, device="cuda").half()
+    lse = torch.zeros(2, 4, 10, device="cuda")
+    wide = torch.empty(2, 10, 4, 160, device="cuda").half()
+    dq, dk, dv = (wide[..., i:i + 64].transpose(1, 2) for i in (0, 56, 96))
+    with pytest.raises(capi.TraceaError) as e:
+        tracea_gpu.attention_backward(q, q, q, q, lse, q, dq=dq, dk=dk, dv=torch.empty_like(q))
+    assert e.value.status == capi.INVALID_PARAMS
+    with pytest.raises(capi.TraceaError) as e:
+        tracea_gpu.attention_backward(q, q, q, q, lse, q, dq=dq, dk=torch.empty_like(q), dv=wide[:, :, :, 1:65].transpose(1, 2))
+    assert e.value.status == capi.INVALID_PARAMS

@@ -25,3 +25,8 @@ def counted(tmp_path_factory):
 
 def test_no_shared_element_is_missed(counted):
     assert counted["missed"] == 0
+
+
+def test_slots_of_one_buffer_are_told_apart(counted):
+    """Tensors in slots of a row or of a head, the slots in any order: no pair without a shared element is taken to overlap."""
+    assert counted["packed_apart"] > 10000 and counted["packed_told"] == counted["packed_apart"]

@@ -57,8 +57,44 @@ inline bool row_form(const View &v, long long *pitch, long long *len) {
   return true;
 }
 
+// Whether no sum of d_i * stride_i, first_i <= d_i <= last_i, strides from the `n`-th on descending, is `rest` (elements).  Gives up (false)
+// where more than a few d_i come into question, which the strides of a tensor's own layout do not allow.
+struct Steps {
+  long long stride, first, last;
+};
+inline bool unreachable(const Steps *s, int n, long long rest) {
+  if (n == 0) return rest != 0;
+  long long low = 0, high = 0;  // what the smaller strides reach
+  for (int i = 1; i < n; ++i) {
+    low += s[i].first * s[i].stride;
+    high += s[i].last * s[i].stride;
+  }
+  auto floor_div = [](long long x, long long y) { return x / y - (x % y < 0); };
+  const long long from = std::max(s->first, -floor_div(high - rest, s->stride)), to = std::min(s->last, floor_div(rest - low, s->stride));
+  if (to - from >= 4) return false;
+  for (long long d = from; d <= to; ++d)
+    if (!unreachable(s + 1, n - 1, rest - d * s->stride)) return false;
+  return true;
+}
+// Two views with the same strides: slots of one buffer, whatever lies between their rows and heads.
+inline bool slots_apart(const View &a, const View &b) {
+  const long long size = elem_size(a.dtype), apart = (long long)((intptr_t)b.ptr - (intptr_t)a.ptr);
+  if (a.rank != b.rank || size != elem_size(b.dtype) || apart % size != 0) return false;
+  Steps s[4];
+  int n = 0;
+  for (int i = 0; i < a.rank; ++i) {
+    if (a.shape[i] == 1 && b.shape[i] == 1) continue;
+    const long long step = a.shape[i] > 1 ? a.stride[i] : b.stride[i];
+    if (a.shape[i] > 1 && b.shape[i] > 1 && a.stride[i] != b.stride[i]) return false;
+    if (step > 0) s[n++] = {step, 1 - b.shape[i], a.shape[i] - 1};
+    else if (step < 0) s[n++] = {-step, 1 - a.shape[i], b.shape[i] - 1};
+  }
+  std::sort(s, s + n, [](const Steps &x, const Steps &y) { return x.stride > y.stride; });
+  return unreachable(s, n, apart / size);
+}
+
 // Whether two views may share an element (columns of one buffer side by side, a query tensor inside a packed
-// [Q K V] row and the like are told apart).
+// [Q K V] row or head and the like are told apart).
 inline bool may_overlap(const View &a, const View &b) {
   auto span = [](const View &v, uintptr_t *lo, uintptr_t *hi) {
     long long first = 0, last = 0;
@@ -73,12 +109,13 @@ inline bool may_overlap(const View &a, const View &b) {
   uintptr_t alo, ahi, blo, bhi;
   if (!span(a, &alo, &ahi) || !span(b, &blo, &bhi) || ahi <= blo || bhi <= alo) return false;
   long long pa, la, pb, lb;
-  if (!row_form(a, &pa, &la) || !row_form(b, &pb, &lb)) return true;
-  pa *= elem_size(a.dtype); la *= elem_size(a.dtype); pb *= elem_size(b.dtype); lb *= elem_size(b.dtype);
-  if (pa != pb) return true;
-  long long d = ((long long)((intptr_t)b.ptr - (intptr_t)a.ptr)) % pa;
-  if (d < 0) d += pa;
-  return d < la || d + lb > pa;
+  if (row_form(a, &pa, &la) && row_form(b, &pb, &lb)) {
+    pa *= elem_size(a.dtype); la *= elem_size(a.dtype); pb *= elem_size(b.dtype); lb *= elem_size(b.dtype);
+    long long d = ((long long)((intptr_t)b.ptr - (intptr_t)a.ptr)) % pa;
+    if (d < 0) d += pa;
+    if (pa == pb && d >= la && d + lb <= pa) return false;
+  }
+  return !slots_apart(a, b);
 }
 
 inline const char *dtype_name(int dt) {
