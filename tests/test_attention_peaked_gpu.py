@@ -59,3 +59,10 @@ def test_one_walk_over_the_keys_lse(one_walk):
     for h in (0, 200, 511):
         for i in range(0, 126, 3):
             within("lse", lse[:, h:h + 1, i:i + 3], want["lse"])
+
+
+def test_one_walk_over_the_keys_o(one_walk):
+    o, _, want = one_walk
+    for h in (0, 200, 511):
+        for i in range(0, 126, 3):
+            within("o", o[:, h:h + 1, i:i + 3], want["o"])

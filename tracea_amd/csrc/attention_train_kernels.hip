@@ -32,8 +32,8 @@ namespace {
 constexpr int TILE = 64;  // rows of a streamed tile
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // Probabilities and their gradients become 16-bit operands.  f16 has no range for either: a row over thousands of keys has
-// probabilities below its smallest normal number.  P is kept as 2^14 P, dS scaled by a power of two from the largest
-// |dP - delta| there can be (see ds_scale); both factors leave with the results.  bf16 needs neither.
+// probabilities below its smallest normal number.  Backward, P is kept as 2^14 P, dS scaled by a power of two from the largest
+// |dP - delta| there can be (see ds_scale); forward, see P_SHIFT.  All factors leave with the results.  bf16 needs none.
 constexpr float F16_P_SHIFT = 14.0f;
 
 template <int DT>
@@ -283,9 +283,14 @@ __device__ __forceinline__ float ds_scale(const AttentionTrainArgs &a, int bh, i
 
 // ---- forward --------------------------------------------------------------------------------------------------
 
-// The running maximum moves only when a tile exceeds it by more than this many powers of two: a row needs one reference for
-// all its keys, not the largest score, and 2^8 is far inside the range of the 16-bit operands.
-constexpr float LAZY_MAX = 8.0f;
+// A row's reference lies P_SHIFT powers of two below a score it has met and moves only when a tile exceeds that score by more than
+// LAZY_MAX: a row needs one reference for all its keys, not the largest score.  Operands are up to 2^(P_SHIFT + LAZY_MAX), in f16
+// 2^15; there the shift keeps what lies 2^25 below the largest probability (2^-25 is 0 in f16, 2^-14 its smallest normal number), of
+// which a long row may have a tail that counts, and each key loses at most 2^-36 of the largest: nothing up to 2^24 keys.
+template <int DT>
+constexpr float P_SHIFT = DT == DT_F16 ? 11.0f : 0.0f;
+template <int DT>
+constexpr float LAZY_MAX = DT == DT_F16 ? 4.0f : 8.0f;
 
 // Over a lane's own value and those of the other three 16-lane groups, by exchanges in the vector ALU: v_permlane16_swap trades the
 // odd 16-lane rows of its first operand for the even ones of its second, v_permlane32_swap the halves; given one value
@@ -402,15 +407,15 @@ attention_train_forward_kernel(const AttentionTrainArgs a) {
       z[qb][kb][e] = (step * SG + kg) * TILE + kb * 16 + g4 * 4 + e > q_last[qb] ? -INFINITY : z[qb][kb][e];
     mx[qb] = fmaxf(mx[qb], z[qb][kb][e]);
   };
-  // A row needs one reference for all its keys, not the largest score: it moves when a tile exceeds it by LAZY_MAX powers of two.
+  // The rows' references, and what is summed up already, where a tile exceeds the scores they stand for by LAZY_MAX powers of two.
   auto move_reference = [&](const float (&mx)[NQ]) __attribute__((always_inline)) {
     bool moved = false;
     float alpha[NQ];
 #pragma unroll
     for (int qb = 0; qb < NQ; ++qb) {
       const float top = groups_max_valu(mx[qb]) * a.scale_log2;
-      const bool mv = top > m[qb] + LAZY_MAX;  // (a first score above -inf always moves it)
-      const float mn = mv ? top : m[qb];
+      const bool mv = top > m[qb] + (P_SHIFT<DT> + LAZY_MAX<DT>);  // (a first score above -inf always moves it)
+      const float mn = mv ? top - P_SHIFT<DT> : m[qb];
       alpha[qb] = mv ? __builtin_amdgcn_exp2f(m[qb] - mn) : 1.0f;
       m[qb] = mn;
       moved |= mv;
