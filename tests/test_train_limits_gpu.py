@@ -5,6 +5,15 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 
+@pytest.mark.parametrize("hq,hk", [(16, 16), (32, 16)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+def test_more_than_65535_problems(tracea_gpu, hq, hk, dtype):
+    # windows of an image: 4100 of them with 16 key/value heads each
+    from test_attention_train_gpu import check
+    check(tracea_gpu, 4100, hq, hk, 3, 5, 8, dtype)
+    check(tracea_gpu, 4100, hq, hk, 3, 3, 16, dtype, True)
+
+
 def test_gradients_side_by_side_within_a_head(tracea_gpu):
     """Operands and gradients as [B,S,H,3,D]: the three share the range of a head's row and no element."""
     g = torch.Generator(device="cuda").manual_seed(11)
@@ -37,3 +46,23 @@ def test_results_that_share_elements_are_refused(tracea_gpu):
     with pytest.raises(capi.TraceaError) as e:
         tracea_gpu.attention_backward(q, q, q, q, lse, q, dq=dq, dk=torch.empty_like(q), dv=wide[:, :, :, 1:65].transpose(1, 2))
     assert e.value.status == capi.INVALID_PARAMS
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+def test_as_many_workgroups_as_a_launch_has(tracea_gpu, dtype):
+    """Up to 2^24 - 1 workgroups of 256 threads (a launch of 2^32 threads and more drops some of them without an error)."""
+    from tracea_amd import capi
+    x = torch.randn(1 << 20, 16, 1, 8, device="cuda").to(dtype)
+    lse = torch.empty(1 << 20, 16, 1, device="cuda")
+    with pytest.raises(capi.TraceaError) as e:
+        tracea_gpu.attention_forward(x, x, x, out=torch.empty_like(x), lse=lse)
+    assert e.value.status == capi.UNSUPPORTED_CONFIG
+    some = x[1:]
+    o, lse = tracea_gpu.attention_forward(some, some, some)  # (one key: o is its value)
+    assert torch.equal(o, some) and torch.isfinite(lse).all()
+    with pytest.raises(capi.TraceaError) as e:
+        tracea_gpu.attention_backward(some, some, some, o, lse, some)
+    assert e.value.status == capi.UNSUPPORTED_CONFIG
+    some, o, lse = some[: (1 << 19) - 1], o[: (1 << 19) - 1], lse[: (1 << 19) - 1]
+    dq, dk, dv = tracea_gpu.attention_backward(some, some, some, o, lse, some)
+    assert (dq == 0).all() and (dk == 0).all() and torch.equal(dv, some)

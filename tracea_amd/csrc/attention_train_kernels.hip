@@ -643,8 +643,8 @@ template <int DT>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) attention_train_rows_kernel(const AttentionTrainArgs a) {
   constexpr int LPR = 16;  // lanes per row, 8 columns each
   __shared__ float s_max[4];
-  const int c = (threadIdx.x % LPR) * 8, row_blocks = a.rows_pad / TILE;
-  const int bh = blockIdx.y, blk = blockIdx.x;
+  const int c = (threadIdx.x % LPR) * 8, row_blocks = a.rows_pad / TILE, blocks = DT == DT_F16 ? a.norm_blocks : row_blocks;
+  const int bh = (int)blockIdx.x / blocks, blk = (int)blockIdx.x - bh * blocks;
   const Rows w = rows_of(a, bh);
   const bool of_rows = blk < row_blocks;
   // (all loads first: a launch of few blocks is as long as the waits one after another)
@@ -1143,7 +1143,7 @@ int backward(const AttentionTrainArgs &a, hipStream_t stream) {
   constexpr int W = 4;
   const unsigned bh = (unsigned)(a.B * a.Hk);
   const unsigned row_blocks = (unsigned)(DT == DT_F16 ? a.norm_blocks : a.rows_pad / TILE);
-  if (row_blocks > 0) hipLaunchKernelGGL((attention_train_rows_kernel<DT>), dim3(row_blocks, bh), dim3(256), 0, stream, a);
+  if (row_blocks > 0) hipLaunchKernelGGL((attention_train_rows_kernel<DT>), dim3(row_blocks * bh), dim3(256), 0, stream, a);
   auto blocks = [&](int n) { return (unsigned)((n + a.block - 1) / a.block) * bh; };
   const unsigned kb = blocks(a.Sk) * (unsigned)a.row_splits, qb = blocks(a.G * a.Sq);
   if (kb + qb > 0) {

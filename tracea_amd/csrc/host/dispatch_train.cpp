@@ -72,6 +72,8 @@ HeadView head_view(const View &v) { return HeadView{v.ptr, v.stride[0], v.stride
 
 // ---- attention ------------------------------------------------------------------------------------------------
 
+constexpr long long kMostBlocks = 1ll << 24;  // workgroups of 256 threads in a launch: fewer than 2^32 threads
+
 struct Attention {
   const char *op;
   View q, k, v, o, lse, d_o, dq, dk, dv;
@@ -165,6 +167,8 @@ BackwardPlan plan_backward(long long heads, long long rows, long long keys, int 
   return best;
 }
 
+TraceaStatus too_many(const char *op) { return fail(TRACEA_UNSUPPORTED_CONFIG, "%s: more workgroups than a launch can have", op); }
+
 TraceaStatus run_attention(const Attention &c, bool from_copies) {
   const long long B = c.q.shape[0], Hq = c.q.shape[1], Sq = c.q.shape[2], D = c.q.shape[3], Hk = c.k.shape[1], Sk = c.k.shape[2];
   const long long G = Hq / Hk, rows_pad = (G * Sq + 63) / 64 * 64;
@@ -255,6 +259,7 @@ TraceaStatus run_attention(const Attention &c, bool from_copies) {
     const int width = D <= 64 ? 64 : D <= 96 ? 96 : 128;
     const ForwardPlan plan = plan_forward(B * Hk, G * Sq, Sk, width, a.causal && Sq == Sk, c.k_len != nullptr, (int)device_limits().cus);
     a.block = plan.block;
+    if (B * Hk * ((G * Sq + a.block - 1) / a.block) >= kMostBlocks) return too_many(c.op);
     if (plan.splits > 1) {
       const long long keys = a.block < 128 ? 128 : 64, steps = (Sk + keys - 1) / keys, per = (steps + plan.splits - 1) / plan.splits;
       const long long splits = (steps + per - 1) / per;
@@ -276,6 +281,10 @@ TraceaStatus run_attention(const Attention &c, bool from_copies) {
   const BackwardPlan plan = plan_backward(B * Hk, G * Sq, Sk, (int)width, a.causal, (int)device_limits().cus);
   a.block = plan.block;
   a.row_splits = plan.row_splits;
+  auto blocks = [&](long long n, long long of) { return B * Hk * ((n + of - 1) / of); };
+  if (blocks(Sk, a.block) * a.row_splits + blocks(G * Sq, a.block) >= kMostBlocks || blocks(rows_pad + Sk + 63, 64) >= kMostBlocks ||
+      (a.row_splits > 1 && blocks(Sk * 2 * (long long)width / 4, 1) / 256 >= kMostBlocks))
+    return too_many(c.op);
   auto workspace = [&]() {
     const size_t parts = a.row_splits > 1 ? (size_t)a.row_splits * (size_t)(B * Hk * Sk) * 2 * width : 0;
     return (float *)train_scratch(c.q.device, c.stream, (2 * stats + norms + parts + 1) * 4);
@@ -325,10 +334,10 @@ TraceaStatus check_attention(Attention &c, const TraceaAttentionParams &params, 
     return fail(TRACEA_INVALID_PARAMS, "%s: %lld query heads are not a multiple of %lld key/value heads", op, Hq, Hk);
   if (D < 1 || D > 128) return fail(TRACEA_UNSUPPORTED_CONFIG, "%s: head dim %lld (1 to 128 supported)", op, D);
   const long long G = Hq / Hk;
-  // (rows are divided by G with a 32-bit product, blocks and heads are grid dimensions)
-  if (G * G * (Sq + 128) >= (1ll << 31) || G * (Sq + Sk + 128) >= (1ll << 31) || B * Hk * ((G * Sq + 127) / 128) >= (1ll << 31) ||
-      B * Hk * ((Sk + 127) / 128) >= (1ll << 31) || B * Hk >= 65536)
-    return fail(TRACEA_UNSUPPORTED_CONFIG, "%s: problem too large", op);
+  // (rows are divided by G with a 32-bit product, rows and keys counted in 32 bits, B * Hk problems are workgroups of a launch)
+  if (G * G * (Sq + 128) >= (1ll << 31) || G * (Sq + Sk + 128) >= (1ll << 31) || B * Hk >= kMostBlocks)
+    return fail(TRACEA_UNSUPPORTED_CONFIG, "%s: %lld x %lld key/value heads of %lld x %lld queries over %lld keys are more than is supported",
+                op, B, Hk, G, Sq, Sk);
   c.scale = params.scale;
   if (c.scale == 0.0f) c.scale = 1.0f / sqrtf((float)D);
   if (!std::isfinite(c.scale)) return fail(TRACEA_INVALID_PARAMS, "%s: scale is not finite", op);
