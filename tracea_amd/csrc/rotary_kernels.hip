@@ -67,8 +67,8 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
     i = (int)(token - entry * (N)a.S);
     b = (long long)entry;
   };
-  if (gridDim.x <= (1u << 24)) split(blockIdx.x * 256u + threadIdx.x);  // (the divisions in 32 bits where they fit)
-  else split((unsigned long long)blockIdx.x * 256u + threadIdx.x);
+  if (gridDim.z == 1) split(blockIdx.x * 256u + threadIdx.x);  // (the divisions in 32 bits where they fit)
+  else split(((unsigned long long)blockIdx.z * gridDim.x + blockIdx.x) * 256u + threadIdx.x);
   if (b >= a.B) return;
   const int h0 = blockIdx.y * a.heads_per_group + slot, h1 = min((int)(blockIdx.y + 1) * a.heads_per_group, a.Hq + a.Hk);
   auto heads = [&](auto &&body) __attribute__((always_inline)) {
@@ -105,7 +105,9 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
 template <typename T, int E>
 int launch(const RotaryArgs &a, hipStream_t stream) {
   const long long threads = (long long)a.B * a.S * a.beside * (a.P / E + (a.D - 2 * a.P) / E);
-  const dim3 grid((unsigned)((threads + 255) / 256), (unsigned)((a.Hq + a.Hk + a.heads_per_group - 1) / a.heads_per_group));
+  // (at most 2^31 threads along x: a launch of 2^32 and more drops some of them without an error)
+  const long long blocks = (threads + 255) / 256, most = 1ll << 23, turns = (blocks + most - 1) / most;
+  const dim3 grid((unsigned)((blocks + turns - 1) / turns), (unsigned)((a.Hq + a.Hk + a.heads_per_group - 1) / a.heads_per_group), (unsigned)turns);
   if (a.adjacent) hipLaunchKernelGGL((rotary_kernel<T, E, true>), grid, dim3(256), 0, stream, a);
   else hipLaunchKernelGGL((rotary_kernel<T, E, false>), grid, dim3(256), 0, stream, a);
   return (int)hipGetLastError();
