@@ -84,3 +84,24 @@ def test_two_threads_on_one_stream(tracea_gpu):
         for results in got[f]:
             for x, y in zip(results, want[f]):
                 assert torch.equal(x, y)
+
+
+def test_the_parts_of_one_query_take_its_rows(tracea_gpu):
+    """One query of 40 heads (8 key heads) over 32768 keys: the partial results of 32 parts at most are 32 x 40 rows of 130 numbers, not of
+    as many as a tile has."""
+    from helpers import launches
+    q, k, v = make((1, 40, 1, 128), (1, 8, 32768, 128), (1, 8, 32768, 128), seed=3)
+    out, lse = torch.empty_like(q), torch.empty(1, 40, 1, device="cuda")
+
+    def call():
+        tracea_gpu.attention_forward(q, k, v, out=out, lse=lse)
+    assert launches(call) == 2  # (the kernels are loaded, too)
+    stream = new_stream()
+    with torch.cuda.stream(stream):
+        out.zero_()
+    torch.cuda.synchronize()
+    before = torch.cuda.mem_get_info()[0]
+    with torch.cuda.stream(stream):
+        call()
+    torch.cuda.synchronize()
+    assert before - torch.cuda.mem_get_info()[0] <= 2 << 20  # (at least 1 MiB by the rule of these buffers, in the device's pieces of 2)

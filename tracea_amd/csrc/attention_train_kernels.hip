@@ -580,7 +580,7 @@ attention_train_forward_kernel(const AttentionTrainArgs a) {
       for (int d = 0; d < DB; ++d) o[qb][d] = f32x4{0, 0, 0, 0};
     }
     if (a.splits > 1) {
-      const long long at = ((long long)blockIdx.y * a.B * a.Hk + bh) * a.rows_pad + r;
+      const long long at = ((long long)blockIdx.y * a.B * a.Hk + bh) * ((long long)a.G * a.Sq) + r;
       if (g4 == 0) {
         a.part_ml[2 * at] = m[qb];
         a.part_ml[2 * at + 1] = sum;
@@ -612,7 +612,7 @@ __global__ void __launch_bounds__(256) attention_train_join_kernel(const Attenti
   if (id >= (long long)a.B * a.Hk * per) return;
   const int bh = (int)(id / per), r = (int)(id - (long long)bh * per);
   const Rows w = rows_of(a, bh);
-  const long long plane = (long long)a.B * a.Hk * a.rows_pad, at = (long long)bh * a.rows_pad + r;
+  const long long plane = (long long)a.B * a.Hk * per, at = (long long)bh * per + r;
   const float own_m = lane < a.splits ? a.part_ml[2 * (lane * plane + at)] : -INFINITY;
   const float own_l = lane < a.splits ? a.part_ml[2 * (lane * plane + at) + 1] : 0.0f;
   float m = own_m;

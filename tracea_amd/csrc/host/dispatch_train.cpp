@@ -263,7 +263,7 @@ TraceaStatus run_attention(const Attention &c, bool from_copies) {
     if (plan.splits > 1) {
       const long long keys = a.block < 128 ? 128 : 64, steps = (Sk + keys - 1) / keys, per = (steps + plan.splits - 1) / plan.splits;
       const long long splits = (steps + per - 1) / per;
-      const size_t n = (size_t)(splits * B * Hk * rows_pad);
+      const size_t n = (size_t)(splits * B * Hk * G * Sq);
       a.part_o = (float *)train_scratch(c.q.device, c.stream, n * (size_t)(width + 2) * 4);
       if (a.part_o != nullptr) {  // (else unsplit: slower, the same result to rounding)
         a.part_ml = a.part_o + n * width;
