@@ -19,6 +19,12 @@ sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 from tracea_amd import capi, ops  # noqa: E402
 
 
+def in_rows(t):
+    """A gradient as the tape brings it: one that was expanded (that of a sum has only strides of zero) is written out, because rotary
+    and the norms read contiguous rows of channels."""
+    return t if t is None or t.stride(-1) == 1 else t.contiguous()
+
+
 class Linear(torch.autograd.Function):
     """y = x w^T for tokens x [..., K] and w [N, K]."""
 
@@ -44,7 +50,7 @@ class Rotary(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dq, dk):
         positions, inv_freq = ctx.saved_tensors
-        return (*ops.rotary(dq, dk, positions, inv_freq, ctx.sections, inverse=True), None, None, None)
+        return (*ops.rotary(in_rows(dq), in_rows(dk), positions, inv_freq, ctx.sections, inverse=True), None, None, None)
 
 
 class Attention(torch.autograd.Function):
@@ -75,7 +81,7 @@ class NormGateResidual(torch.autograd.Function):
         x_out, h, w_post, gate, w_pre = ctx.saved_tensors
         if w_pre is not None and dy is None:
             dy = torch.zeros_like(x_out)
-        return ops.norm_gate_residual_backward(dx_out, dy, x_out, h, w_post, gate, w_pre)
+        return ops.norm_gate_residual_backward(in_rows(dx_out), in_rows(dy), x_out, h, w_post, gate, w_pre)
 
 
 class Block(torch.nn.Module):
