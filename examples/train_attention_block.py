@@ -5,7 +5,7 @@
 
 torch keeps the tape, the optimizer, the memory and the SiLU; the rest of the block's arithmetic is ``tracea_amd.ops``:
 ``norm_gate_residual``, ``rotary``, ``attention_forward`` / ``attention_backward`` and ``gemm`` for the linear layers and their
-two gradients.
+two gradients.  Gradients of gradients are not offered: torch's tape says so where one is asked for.
 
     python examples/train_attention_block.py [--grid 4 8 8] [--steps 20]
 """
@@ -14,6 +14,7 @@ import os
 import sys
 
 import torch
+from torch.autograd.function import once_differentiable
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 from tracea_amd import capi, ops  # noqa: E402
@@ -34,6 +35,7 @@ class Linear(torch.autograd.Function):
         return ops.gemm(x.reshape(-1, x.shape[-1]), w.t()).view(*x.shape[:-1], w.shape[0])
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         x, w = ctx.saved_tensors
         dy = dy.reshape(-1, dy.shape[-1])
@@ -48,6 +50,7 @@ class Rotary(torch.autograd.Function):
         return ops.rotary(q, k, positions, inv_freq, sections)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dq, dk):
         positions, inv_freq = ctx.saved_tensors
         return (*ops.rotary(in_rows(dq), in_rows(dk), positions, inv_freq, ctx.sections, inverse=True), None, None, None)
@@ -62,6 +65,7 @@ class Attention(torch.autograd.Function):
         return o
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_o):
         return (*ops.attention_backward(*ctx.saved_tensors, d_o, q_lengths=ctx.lengths, k_lengths=ctx.lengths), None)
 
@@ -77,6 +81,7 @@ class NormGateResidual(torch.autograd.Function):
         return (x_out.view_as(x) if h is None else x_out), y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dx_out, dy):
         x_out, h, w_post, gate, w_pre = ctx.saved_tensors
         if w_pre is not None and dy is None:

@@ -47,3 +47,10 @@ def test_the_sum_of_the_results(tracea_gpu):
                    ex.Linear.apply(q, block.w_o.detach()[:, :64].bfloat16()), ex.NormGateResidual.apply(x, None, None, None, block.norms[0])[1]):
         result.sum().backward()
     assert torch.isfinite(q.grad).all() and torch.isfinite(k.grad).all()
+
+
+def test_second_derivatives_are_refused_with_the_reason(tracea_gpu):
+    block, x, positions = make()
+    g, = torch.autograd.grad(block(x, positions).float().square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.float().square().sum().backward()
