@@ -66,3 +66,15 @@ def test_one_walk_over_the_keys_o(one_walk):
     for h in (0, 200, 511):
         for i in range(0, 126, 3):
             within("o", o[:, h:h + 1, i:i + 3], want["o"])
+
+
+@pytest.mark.parametrize("shape", [(8, 32, 8, 1, 8192, 128), (2, 8, 2, 1000, 1000, 64), (1, 4, 4, 40, 6000, 96)], ids=str)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+def test_the_forward_pass_repeats_itself(tracea_gpu, shape, dtype):
+    b, hq, hk, sq, sk, d = shape
+    g = torch.Generator(device="cuda").manual_seed(8)
+    q, k, v = (torch.randn(b, h, s, d, device="cuda", generator=g).to(dtype) for h, s in ((hq, sq), (hk, sk), (hk, sk)))
+    o, lse = tracea_gpu.attention_forward(q, k, v, causal=True)
+    for _ in range(5):
+        again = tracea_gpu.attention_forward(q, k, v, causal=True)
+        assert torch.equal(o, again[0]) and torch.equal(lse, again[1])

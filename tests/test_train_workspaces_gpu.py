@@ -105,3 +105,39 @@ def test_the_parts_of_one_query_take_its_rows(tracea_gpu):
         call()
     torch.cuda.synchronize()
     assert before - torch.cuda.mem_get_info()[0] <= 2 << 20  # (at least 1 MiB by the rule of these buffers, in the device's pieces of 2)
+
+
+def test_under_capture_without_a_workspace(tracea_gpu):
+    """On a stream that has made no such call: the forward pass runs unsplit, the backward passes, which cannot do without, are refused."""
+    from helpers import launches
+    from test_attention_train_gpu import reference, within
+    from tracea_amd import capi
+    q, k, v, do = make((1, 8, 2, 64), (1, 2, 5000, 64), (1, 2, 5000, 64), (1, 8, 2, 64), seed=4)
+    want = reference(q, k, v, do, True, 0.0)
+    o, lse = torch.empty_like(q), torch.empty(1, 8, 2, device="cuda")
+    assert launches(lambda: tracea_gpu.attention_forward(q, k, v, causal=True, out=o, lse=lse)) == 2  # split where there is a workspace
+    stream = new_stream()
+    _, graph = under_capture(stream, lambda: tracea_gpu.attention_forward(q, k, v, causal=True, out=o, lse=lse))
+    for _ in range(3):
+        o.fill_(float("nan"))
+        lse.fill_(float("nan"))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        torch.cuda.synchronize()
+        within("o", o, want["o"])
+        within("lse", lse, want["lse"])
+    grads = [torch.empty_like(t) for t in (q, k, v)]
+    result, _ = under_capture(stream, lambda: tracea_gpu.attention_backward(q, k, v, o, lse, do, causal=True, dq=grads[0], dk=grads[1],
+                                                                            dv=grads[2]))
+    assert isinstance(result, capi.TraceaError) and result.status == capi.UNSUPPORTED_CONFIG, result
+    x, h, dx, dy = make(*[(2, 9, 64)] * 4, dtype=torch.float32, seed=5)
+    w = torch.ones(64, device="cuda")
+    result, _ = under_capture(stream, lambda: tracea_gpu.norm_gate_residual_backward(dx, dy, x, h, w, None, w, dx=torch.empty_like(x),
+                                                                                     dh=torch.empty_like(x)))
+    assert isinstance(result, capi.TraceaError) and result.status == capi.UNSUPPORTED_CONFIG, result
+    with torch.cuda.stream(stream):  # and eagerly they have one
+        tracea_gpu.attention_backward(q, k, v, o, lse, do, causal=True, dq=grads[0], dk=grads[1], dv=grads[2])
+        torch.cuda.synchronize()
+    for name, t in zip(("dq", "dk", "dv"), grads):
+        within(name, t, want[name])
