@@ -435,16 +435,19 @@ TraceaStatus tracea_conv_coords_device(const TraceaConvParamsBlock *p, int32_t *
  * Query i of b sees keys j < k_lengths[b]; with params.causal, of those j <= i + k_lengths[b] - q_lengths[b] (the
  * last query sees every key).  lse = log of the sum of exp(scale q.k) over them; a query that sees none, or lies
  * behind its sequence's length, has o = 0, lse = -inf and gradient 0, keys behind the length have gradient 0.
- * (Infinities and NaN within the lengths spread as 0 * inf does: from a key that a causal mask hides, also to queries up to 63
- * positions in front of it.)
+ * (Infinities and NaN within the lengths spread as 0 * inf does: also between a query and a key that a causal mask hides from
+ * it, up to 94 positions apart.)
  * All tensors but lse share one type, f16 or bf16, D from 1 to 128; sums, statistics and probabilities are fp32,
  * probabilities and their gradients are rounded once to the operand type for the matrix products.  scale 0 selects
- * 1/sqrt(D); softmax_mode is ignored.  The same call on the same inputs gives the same bits.
+ * 1/sqrt(D); softmax_mode is ignored.  The same call on the same inputs gives the same bits.  Fewer than 2^31 rows of a group
+ * (Hq / Hk * Sq) and keys; a launch has fewer than 2^24 workgroups, at least one for each of the B Hk problems.
  * Read and written in place: D a multiple of 8 and contiguous, other strides multiples of 8 elements (rows and heads not
- * descending), bases on 16 bytes, no result over an operand.  Anything else runs from padded copies in a buffer of these
- * two operators' own per (device, stream) (at most 1 GiB, not grown under capture).  Both calls take a workspace per (device,
- * stream), grown on demand, never under capture and never freed: 8 bytes per row for the backward pass; for a forward
- * pass of few rows over many keys, which is split along the keys, the partial results. */
+ * descending), bases on 16 bytes.  A result over an operand, and anything else, runs from padded copies in a buffer of these
+ * two operators' own per (device, stream) (at most 1 GiB, not grown under capture); results over lse, the lengths or each other
+ * are refused.  Both calls take a workspace per (device, stream), grown on demand to a power of two, never under capture; what
+ * is outgrown is kept too.  Forward, where few rows over many keys are split along the keys: (D up to 64, 96 or 128, + 2) * 4 bytes
+ * per row and part, at most about 0.5 GiB.  Backward: 8 bytes per row; f16 4 bytes per 64 rows and 64 keys; where few keys are
+ * split along the rows, 8 * (D up to 64, 96 or 128) bytes per key and part, at most 0.5 GiB. */
 TraceaStatus tracea_attention_forward(TraceaTensorView q, TraceaTensorView k, TraceaTensorView v,
                                       const TraceaTensorView *q_lengths, const TraceaTensorView *k_lengths,
                                       TraceaTensorView *o, TraceaTensorView *lse, TraceaAttentionParams params);
@@ -484,7 +487,7 @@ TraceaStatus tracea_rotary(TraceaTensorView q, const TraceaTensorView *k, Tracea
  * again: dx_out (optional: absent is 0) and dy are the gradients of x_out and y; dx, dh have the type of h, dw_post, dgate
  * [G,C], dw_pre are f32 and are summed in an order that does not change.  Gradients that are not wanted are NULL (dx is
  * required).  It takes a workspace per (device, stream), at most 16 MiB plus 8 bytes per channel and batch entry, grown on
- * demand, never under capture. */
+ * demand to a power of two, never under capture. */
 typedef struct {
   float eps;
   float residual_scale;

@@ -5,6 +5,9 @@
 //   lse_i = log sum_j exp(s_ij)      o_i = sum_j exp(s_ij - lse_i) v_j        (no key: lse -inf, o 0)
 //   P_ij = exp(s_ij - lse_i)   delta_i = dO_i . O_i   dS_ij = P_ij (dO_i . v_j - delta_i)
 //   dV_j = sum_i P_ij dO_i     dK_j = scale sum_i dS_ij q_i     dQ_i = scale sum_j dS_ij k_j
+// P and dS are rounded to the operand type for the second products, and delta comes from O as the forward pass rounded it: the price of
+// products at the 16-bit rate and of one pass for delta.  Errors in 2-norm are 1.3 to 1.57 times those of 32-bit arithmetic rounded
+// once, most for dQ and dK of rows with few keys, where the rounding of O averages out least.
 //
 // Three walks of one shape.  A wave owns 32 columns whose operand fragments stay in registers and streams the other
 // side in tiles of 64 through LDS (32: with D = 128 the sums of dK and dV are half of the 256 registers that leave room for two
@@ -309,8 +312,10 @@ __device__ __forceinline__ float groups_max_valu(float x) {
 // their rows and walk every other tile of 64 keys; their states are joined at the end.  A wave has 16 NQ rows: 32, or 16 for a token
 // or two of some heads, where the empty half would be most of what it waits for.
 // Bound, long rows: vector work (exponential, maximum and conversion of a score cost about as many cycles as its products do) beside
-// the matrix pipe, and power: B4 H32 S4096 bf16 D128 1020 us = 1.08 PFLOP/s, f16 D64 687 us = 0.80.  One query over a long cache: reading K and V,
-// B8 H32:8 D128 over 8192 keys 49 us = 5.5 TB/s with the join (a large copy reaches 4.8; part of it is in the memory-side cache).
+// the matrix pipe, and power: B4 H32 S4096 bf16 D128 1030-1100 us by card = 1.00-1.07 PFLOP/s, f16 D64 697-722 us = 0.76-0.79.  One query over a long
+// cache: reading K and V, B8 H32:8 D128 over 8192 keys 47 us = 5.7 TB/s with the join (a large copy reaches 4.8; part of it is in the
+// memory-side cache).  (Two waves a SIMD are what the registers are limited for; the tiles of SG = 2 at D above 64, 128 KB, leave room
+// for one workgroup, and so for one wave.)
 template <int DT, int DL, int DU, int WAVES, int SG, int NQ>
 __global__ void __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 attention_train_forward_kernel(const AttentionTrainArgs a) {
@@ -604,7 +609,7 @@ attention_train_forward_kernel(const AttentionTrainArgs a) {
 }
 
 // Joins the partial results of a split key axis: a row per 32 lanes, which load one part's reference and sum each (at most 32
-// parts) and 4 columns of every part's o.  Bound by the latency of its loads: 3.8 us for 256 rows of 8 parts.
+// parts) and 4 columns of every part's o.  Bound by the latency of its loads: 4 to 5 us for 256 rows of 8 parts.
 template <int DT, int DU>
 __global__ void __launch_bounds__(256) attention_train_join_kernel(const AttentionTrainArgs a) {
   const long long id = ((long long)blockIdx.x * 256 + threadIdx.x) / 32;
@@ -638,7 +643,7 @@ __global__ void __launch_bounds__(256) attention_train_join_kernel(const Attenti
 // ---- backward ---------------------------------------------------------------------------------------------------
 
 // Per packed row -lse log2(e) and -(dO . O), which both walks need; f16: the largest squared norms of 64 rows of dO, and of 64 keys of V.
-// Bound by reading dO and O: B4 H32 S4096 D128 bf16 51 us = 5.3 TB/s; a launch's 5 us at B1 H12 S197 D64.
+// Bound by reading dO and O: B4 H32 S4096 D128 bf16 48.5 us = 5.5 TB/s; a launch's 5 us at B1 H12 S197 D64.
 template <int DT>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) attention_train_rows_kernel(const AttentionTrainArgs a) {
   constexpr int LPR = 16;  // lanes per row, 8 columns each
@@ -1090,9 +1095,10 @@ __device__ __forceinline__ void dkv_block(const AttentionTrainArgs &a, int id, u
 }
 
 // The workgroups of dK and dV first, then those of dQ: one launch, so that neither waits for the other's last ones.
-// Bound, long rows: matrix pipe and vector work of two waves per SIMD, and power: B4 H32 S4096 D128 bf16 3.0 ms = 1.26 PFLOP/s
-// of the seven products, 0.90 of the five that are needed.  Short rows: the serial walk of a workgroup over its tiles, B1 H12 S1024
-// D64 f16 causal 23 us, S197 11 us.
+// Bound, long rows: matrix pipe and vector work of two waves per SIMD, and power: B4 H32 S4096 D128 bf16 3.05-3.15 ms =
+// 1.22-1.26 PFLOP/s of the seven products, 0.87-0.90 of the five that are needed.  Short rows: the walk of a workgroup over its tiles
+// one after another, each waited for whole, B1 H12 S1024 D64 f16 causal 23 us, S197 11 us: 0.95 us a tile of 64 by the plan's fit, of which
+// its products are 0.2 us of the matrix pipe.
 template <int DT, int DL, int DU, int WAVES, int SG>
 __global__ void __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 attention_train_backward_kernel(const AttentionTrainArgs a, int dkv_blocks) {

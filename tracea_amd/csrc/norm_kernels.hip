@@ -9,8 +9,9 @@
 // the next one requested ahead, with the weights and, backward, the column sums in registers all along.  The backward pass needs
 // six sums over a row; all are linear in what is loaded, so that they are taken in one go and the threads meet once per row.
 // Column sums leave as one partial row per workgroup and a second kernel adds these up in their order: no atomics.
-// Measured (GPU time, a large copy reaches 4.8 TB/s): forward C2048 T24960 bf16 89 us = 4.6 TB/s, C4096 T8192 48 us (5.6 TB/s, partly from
-// the memory-side cache), 16 rows of 4096 4.6 us; backward C2048 T24960 128 us = 4.8 TB/s with its column sums.
+// Measured (GPU time of a call, several cards; a large copy reaches 4.8 TB/s): forward C2048 T24960 bf16 89-92 us = 4.5 TB/s, C4096
+// T8192 48-51 us (5.3 TB/s, partly from the memory-side cache), 16 rows of 4096 5 us; backward C2048 T24960 with its column sums
+// 128-141 us = 4.4-4.8 TB/s, of which the column kernel is 8.
 #include <type_traits>
 
 #include "contraction_kernel.hpp"
@@ -34,7 +35,7 @@ __device__ __forceinline__ int channel(int e, int lane, int lanes) {
 }
 // A thread's channels of a row as they lie in memory: the next row's are requested before this one's are worked on.  One by one, every
 // 16-bit value has a register of its own, and hold() keeps the conversions behind all loads: the compiler moves each of them behind
-// its load's test of the channel, where it waits for that load (backward C2047 T24960 bf16 148 us, 452 without; C2048 140).
+// its load's test of the channel, where it waits for that load (backward C2047 T24960 bf16 150 us, 452 without; C2048, in pieces of 16 bytes, 141 on that card).
 template <typename T, bool VEC>
 struct Loaded {
   Eight<T> p;
@@ -415,10 +416,11 @@ int any(const NormArgs &a, bool back, hipStream_t stream) {
 
 }  // namespace
 
-// Workgroups per batch entry: one round of them.  Of waves on a CU, forward 20 (C1152 T8192 f16 19.5 us; 16 20.8, 32 26.8, with 12 23.8),
-// backward 12 where a row takes up to four waves, 16 beyond (C2048 T24960 bf16 118 us; with 16 124, with 8 127; C1152
-// 41; with 16, a round and a bit, 53; C4096 T8192 88; with 12 97).  Backward a workgroup has at least four rows, or its partial
-// column sums are a good part of what it moves (C1001 T999 f32 18 us; one row each 23).
+// Workgroups per batch entry: one round of them.  Of waves on a CU, forward 20 (GPU time of a call, us, one card: C4096 T8192 bf16 51, with 12
+// 75; C1152 T8192 f16 22.1, with 16 23.7, with 32 19.5; C2048 T24960 91-93 with any), backward 12 where a row takes up to four waves,
+// 16 beyond (C2048 T24960 bf16 141, with 16 145, with 8 137; C2047 150, with 8 171; C1152 43.5, with 8 54; C4096 T8192 101, with 12
+// 99).  Backward a workgroup has at least four rows, or its partial column sums are a good part of what it moves (C1001 T999 f32 18.8;
+// one row each 21.7).
 int norm_chunks(int B, int T, int C, int cus, bool backward) {
   const Shape s = shape_of(C);
   const int slots = s.threads / s.lanes;  // rows a workgroup has at a time

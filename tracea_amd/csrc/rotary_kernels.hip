@@ -5,8 +5,8 @@
 // through some heads, so that the sine and cosine of a pair, and the position behind them, are worked out once
 // per group of heads instead of once per element.  Where the heads of a token lie side by side, some neighbouring threads take them in
 // turn, or a wave would touch a short piece of eight tokens at a time.
-// Measured: S24960 H32:8 D128 bf16 98 us = 5.2 TB/s in either layout (a large copy reaches 4.8), B8 H12:12 S1024 D64 f32 25 us = 4.0 TB/s;
-// B1 H12:12 S197 f16 4.9 us, a launch.
+// Measured: S24960 H32:8 D128 bf16 98 us = 5.2 TB/s in either layout (a large copy reaches 4.8), B8 H12:12 S1024 D64 f32 18 us = 5.6 TB/s,
+// with a quarter of the columns copied 21 us; B1 H12:12 S197 f16 5.0 us, a launch.
 #include "contraction_kernel.hpp"
 #include "train.hpp"
 

@@ -402,7 +402,8 @@ def rotary(q, k, positions, inv_freq, sections=None, adjacent=False, inverse=Fal
     """(q, k) with every pair of columns turned by positions[..., axis] * inv_freq[pair].  q [B,Hq,S,D], k [B,Hk,S,D] or
     None; positions [B or 1,S,axes] int32 (or [B or 1,S]: one axis); inv_freq [P] float32, P <= D/2; sections: pairs of
     each axis, together P (default: one axis).  Pair p is columns p and p + P, or 2p and 2p + 1 with ``adjacent``; columns from 2P
-    on stay.  ``inverse`` turns back, which is the gradient: rotary(dq, dk, ..., inverse=True).  q_out may be q, k_out k."""
+    on stay.  ``inverse`` turns back, which is the gradient: rotary(dq, dk, ..., inverse=True).  q_out may be q, k_out k.  D is
+    contiguous in all of them."""
     if positions.dim() == 2:
         positions = positions.unsqueeze(-1)
     sections = [inv_freq.shape[0]] if sections is None else list(sections)
@@ -421,7 +422,7 @@ def rotary(q, k, positions, inv_freq, sections=None, adjacent=False, inverse=Fal
 
 def norm_gate_residual(x, h=None, w_post=None, gate=None, w_pre=None, residual_scale=1.0, eps=1e-6, x_out=None, y=None):
     """(x_out, y) of the sum between two blocks: x_out = residual_scale x + gate norm(h) w_post, y = norm(x_out) w_pre, with
-    norm(t) = t / sqrt(mean(t^2) + eps) over the channels.  x, h [B,T,C]; w_post, w_pre [C], gate [1,C] or [B,C], float32.
+    norm(t) = t / sqrt(mean(t^2) + eps) over the channels.  x, h [B,T,C], channels contiguous; w_post, w_pre [C], gate [1,C] or [B,C], float32.
     Without h (a network's first norm) x_out is x; without w_pre (behind its last block) y is None."""
     if h is not None:
         x_out = torch.empty_like(x) if x_out is None else x_out
@@ -437,7 +438,8 @@ def norm_gate_residual(x, h=None, w_post=None, gate=None, w_pre=None, residual_s
 def norm_gate_residual_backward(dx_out, dy, x_out, h=None, w_post=None, gate=None, w_pre=None, residual_scale=1.0, eps=1e-6,
                                 dx=None, dh=None):
     """(dx, dh, dw_post, dgate, dw_pre) for the gradients dx_out (None: zero) and dy of :func:`norm_gate_residual`'s results, from
-    its x_out (x where there is no h) and h; None for what the call has not."""
+    its x_out (x where there is no h) and h; None for what the call has not.  Channels contiguous: an expanded gradient (that of a
+    sum) is written out first, with contiguous()."""
     dx = torch.empty_like(x_out) if dx is None else dx
     if h is not None:
         dh = torch.empty_like(h) if dh is None else dh
