@@ -66,3 +66,19 @@ def test_as_many_workgroups_as_a_launch_has(tracea_gpu, dtype):
     some, o, lse = some[: (1 << 19) - 1], o[: (1 << 19) - 1], lse[: (1 << 19) - 1]
     dq, dk, dv = tracea_gpu.attention_backward(some, some, some, o, lse, some)
     assert (dq == 0).all() and (dk == 0).all() and torch.equal(dv, some)
+
+
+def test_padded_copies_of_the_next_multiple_of_8(tracea_gpu):
+    """Head dimension 90 off 16 bytes: copies of 96 columns, which fit their buffer where 128 would not; the bits of a call with zeros behind
+    the 90."""
+    g = torch.Generator(device="cuda").manual_seed(21)
+    wide = [torch.randn(4, 32, 4100, 96, device="cuda", generator=g).bfloat16() for _ in range(4)]
+    for t in wide:
+        t[..., 90:] = 0
+    q, k, v, do = (torch.empty(4, 32, 4100, 91, device="cuda", dtype=torch.bfloat16)[..., 1:].copy_(t[..., :90]) for t in wide)
+    o, lse = tracea_gpu.attention_forward(q, k, v, scale=0.1)
+    got = (o, lse) + tracea_gpu.attention_backward(q, k, v, o, lse, do, scale=0.1)
+    o, lse = tracea_gpu.attention_forward(*wide[:3], scale=0.1)
+    want = (o, lse) + tracea_gpu.attention_backward(*wide[:3], o, lse, wide[3], scale=0.1)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b if a.dim() == 3 else b[..., :90])

@@ -195,7 +195,7 @@ TraceaStatus run_attention(const Attention &c, bool from_copies) {
     for (int j = 0; j < n_reads; ++j) in_place = in_place && !may_overlap(*writes[i], *reads[j]);
   }
   if (!in_place) {
-    const long long Dp = D <= 64 ? 64 : 128;
+    const long long Dp = (D + 7) / 8 * 8;
     const size_t one_q = (size_t)(B * Hq * Sq) * (size_t)Dp * 2, one_k = (size_t)(B * Hk * Sk) * (size_t)Dp * 2;
     const size_t bytes = c.backward ? 4 * one_q + 4 * one_k : 2 * one_q + 2 * one_k;
     unsigned char *buf = from_copies ? nullptr : (unsigned char *)train_copies(c.q.device, c.stream, bytes);
