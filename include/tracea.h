@@ -48,7 +48,10 @@ typedef enum {
   TRACEA_DTYPE_FLOAT16 = 1,
   TRACEA_DTYPE_BFLOAT16 = 2,
   TRACEA_DTYPE_INT32 = 3,
-  TRACEA_DTYPE_INT8 = 4
+  TRACEA_DTYPE_INT8 = 4,
+  /* no counterpart in the reference: 1 sign, 4 exponent, 3 mantissa bits, largest value 448, NaN and no infinity; the type of a
+   * key/value cache in 8 bits (tracea_cache_append, tracea_attention_cached) and of nothing else */
+  TRACEA_DTYPE_FLOAT8_E4M3 = 5
 } TraceaDType;
 
 /* reference: include/tracea.hpp:37-47; expansion into operator chains:
@@ -501,6 +504,88 @@ TraceaStatus tracea_norm_gate_residual_backward(const TraceaTensorView *dx_out, 
                                                 const TraceaTensorView *gate, const TraceaTensorView *w_pre, TraceaTensorView *dx,
                                                 TraceaTensorView *dh, TraceaTensorView *dw_post, TraceaTensorView *dgate,
                                                 TraceaTensorView *dw_pre, TraceaNormParams params);
+
+/* ======================================================================== */
+/* Attention with a key/value cache.  None of these has a counterpart in    */
+/* the reference.                                                           */
+/* ======================================================================== */
+
+/* Norms of heads and rotary positions in one pass: every head of q and k becomes
+ *   y = R (x * rsqrt(mean(x^2) + eps) * w)            (mean over the head's D values, R as in tracea_rotary)
+ *   q [B,Hq,S,D], k [B,Hk,S,D] (optional) and their results, f32, f16 or bf16, D contiguous and up to 512, any other strides
+ *   q_weight, k_weight [D] f32, contiguous (absent: 1)
+ *   positions [B,S,A] or [1,S,A] i32 and inv_freq [P] f32 as in tracea_rotary; both NULL (axes 0): no rotation
+ * A result may be its own operand (the same view), and may not otherwise overlap one.  Everything between reading x and
+ * writing y is fp32.
+ * The backward pass takes the gradients of the results (dq_out, dk_out) back through the rotation and the norm, which it works out
+ * again from q and k: dq, dk (required with q, k) have the type of q, dq_weight, dk_weight [D] f32 (optional) are sums over all heads, tokens
+ * and batch entries in an order that does not change; without weights there are no such gradients.  dq may be dq_out or q as the same view, dk likewise.  With weight gradients it takes
+ * a workspace per (device, stream), 8 bytes per value of a head and workgroup, at most 8 MiB, never grown under capture. */
+typedef struct {
+  uint32_t axes;
+  uint32_t sections[TRACEA_MAX_ROTARY_AXES];
+  uint8_t adjacent;
+  float eps;
+  void *stream;
+} TraceaQkNormParams;
+TraceaStatus tracea_qk_norm_rotary(TraceaTensorView q, const TraceaTensorView *k, const TraceaTensorView *q_weight,
+                                   const TraceaTensorView *k_weight, const TraceaTensorView *positions,
+                                   const TraceaTensorView *inv_freq, TraceaTensorView *q_out, TraceaTensorView *k_out,
+                                   TraceaQkNormParams params);
+TraceaStatus tracea_qk_norm_rotary_backward(TraceaTensorView dq_out, const TraceaTensorView *dk_out, TraceaTensorView q,
+                                            const TraceaTensorView *k, const TraceaTensorView *q_weight,
+                                            const TraceaTensorView *k_weight, const TraceaTensorView *positions,
+                                            const TraceaTensorView *inv_freq, TraceaTensorView *dq, TraceaTensorView *dk,
+                                            TraceaTensorView *dq_weight, TraceaTensorView *dk_weight, TraceaQkNormParams params);
+
+/* A cache holds the keys and values of sequences in pages of P tokens:
+ *   k_cache, v_cache [N,Hk,P,D]: N pages, P a multiple of 16, D contiguous and a multiple of 8, other strides multiples of 8
+ *   elements and not negative (the order of heads and tokens is the caller's), bases on 16 bytes, or 8 in 8 bits; of the operands' type, f16 or
+ *   bf16, or TRACEA_DTYPE_FLOAT8_E4M3 with
+ *   k_scale, v_scale [N,Hk] f32, any strides: a value of page n and head h is its code times scale[n,h]
+ *   page_table [B,M] i32, M contiguous: token t of sequence b lies in page page_table[b, t / P], place t % P.  What a sequence does
+ *   not use yet may hold anything; a token whose entry is outside 0..N-1, or that lies behind M P, has no place: it is not written, and no query sees it.
+ *
+ * tracea_cache_append turns new keys (and queries) by their positions and writes keys and values to their places.
+ *   k, v [B,Hk,T,D], q [B,Hq,T,D] and q_out (optional, any Hq), f16 or bf16, D contiguous, any other strides and alignment
+ *   starts [B] i32: tokens that sequence b has already; lengths [B] i32 (optional): how many of the T are new ones of sequence b
+ *   (clamped to 0..T).  Both contiguous, on the device; a negative start counts as 0.
+ *   positions [B,T,A] or [1,T,A] i32 as in tracea_rotary, NULL: starts[b] + t (one axis); inv_freq [P] f32, NULL: no rotation
+ * q_out of a token behind lengths[b] is 0; q_out may be q (the same view).  No other rows of the caches are written than the new tokens'.
+ * In 8 bits the scale of a page and head is the least power of two (2^-126 or more) by which no finite value written to the page so far
+ * exceeds 448; a token at place 0 begins the page anew.  Where new tokens raise it, the older tokens' codes are rescaled, exactly
+ * but for what falls below the normal codes (2^-6 of the scale, 448 2^6 below the largest value), which rounds once more; codes are rounded to
+ * nearest, ties to even, from the fp32 value behind the rotation.  Infinities and NaN become NaN and leave the scale alone.
+ * A page that two sequences share may be read by both, and appended to by neither.  Results overlap no operand but q_out its q. */
+typedef struct {
+  uint32_t axes;
+  uint32_t sections[TRACEA_MAX_ROTARY_AXES];
+  uint8_t adjacent;
+  void *stream;
+} TraceaCacheAppendParams;
+TraceaStatus tracea_cache_append(TraceaTensorView k, TraceaTensorView v, const TraceaTensorView *q, TraceaTensorView *k_cache,
+                                 TraceaTensorView *v_cache, TraceaTensorView *k_scale, TraceaTensorView *v_scale,
+                                 TraceaTensorView page_table, TraceaTensorView starts, const TraceaTensorView *lengths,
+                                 const TraceaTensorView *positions, const TraceaTensorView *inv_freq, TraceaTensorView *q_out,
+                                 TraceaCacheAppendParams params);
+
+/* Attention of queries over a cache, the forward pass that serves a model: one query per sequence, some drafted ones, or a piece of a prompt.
+ *   q, o [B,Hq,Sq,D], f16 or bf16, D a multiple of 8 up to 128 and contiguous, any other strides and alignment; Hq a multiple of Hk
+ *   k_lengths [B] i32: keys of sequence b, with the queries' own; q_lengths [B] i32 (optional): its queries.  Contiguous, on the device,
+ *   clamped to 0..M P and 0..Sq.
+ *   lse [B,Hq,Sq] f32 (optional)
+ * Masks, empty rows, lse and scale as in tracea_attention_forward: with params.causal query i of sequence b sees the keys j <= i +
+ * k_lengths[b] - q_lengths[b]; what lies behind the lengths is never used, whatever it holds.  (Infinities and NaN among the keys
+ * of a sequence spread as 0 * inf does, also to a query that a causal mask hides them from.)
+ * Scores, statistics and sums are fp32 or more; codes are widened exactly, scales multiply scores and probabilities in fp32,
+ * probabilities are rounded once to the type of q.  The same call on the same inputs gives the same bits.  Results overlap no operand
+ * and not each other.  Up to M P = 2^31 - 2^16 keys, M P P < 2^40.
+ * Where few rows meet many keys the keys are shared out over the device: a workspace per (device, stream), at most 80 MiB, grown on
+ * demand, never under capture (without it a call runs unsplit, slower). */
+TraceaStatus tracea_attention_cached(TraceaTensorView q, TraceaTensorView k_cache, TraceaTensorView v_cache,
+                                     const TraceaTensorView *k_scale, const TraceaTensorView *v_scale, TraceaTensorView page_table,
+                                     const TraceaTensorView *q_lengths, TraceaTensorView k_lengths, TraceaTensorView *o,
+                                     TraceaTensorView *lse, TraceaAttentionParams params);
 
 #ifdef __cplusplus
 }

@@ -23,6 +23,7 @@ enum class DType : int {
   BFloat16 = TRACEA_DTYPE_BFLOAT16,
   Int32 = TRACEA_DTYPE_INT32,
   Int8 = TRACEA_DTYPE_INT8,
+  Float8E4M3 = TRACEA_DTYPE_FLOAT8_E4M3,  // key/value caches only
 };
 
 enum class EpilogueKind : int {

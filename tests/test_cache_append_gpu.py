@@ -1,0 +1,175 @@
+"""Appending to a key/value cache in pages against the definition in 64 bits."""
+import pytest
+
+torch = pytest.importorskip("torch")
+from cache_oracle import E4M3, U32, Pool, append, half_step, heads, rotated, table  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+HALVES = [torch.float16, torch.bfloat16]
+
+
+def run(ops, seed, b, hq, hk, t, d, rot, page, dtype, e4m3, starts, lengths=None, adjacent=False, layout="bhsd", order="nhpd", positions=None,
+        spoil=None):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    starts = torch.tensor(starts, dtype=torch.int32, device="cuda")
+    lengths = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    per = max(1, -(-(max(0, int(starts.max())) + t) // page))
+    pool = Pool(g, b * per + 2, hk, page, d, dtype, e4m3, order)
+    pt = table(g, b, per, b * per + 2)
+    q = heads(g, b, hq, t, d, dtype, layout) if hq else None
+    k, v = heads(g, b, hk, t, d, dtype, layout, 2.0), heads(g, b, hk, t, d, dtype, layout, 0.5)
+    if spoil is not None:
+        spoil(pt, k, v)
+    freq = 10000.0 ** (-torch.arange(rot // 2, device="cuda", dtype=torch.float32) / max(rot // 2, 1)) if rot else None
+    if positions is None:
+        angle = (starts.clamp(min=0).double()[:, None] + torch.arange(t, device="cuda"))[..., None] * freq.double() if rot else None
+    else:
+        angle = positions.double() * freq.double()
+    want = append(pool, pt, k, v, starts, lengths, rot, angle, adjacent)
+    before = {n: Pool._u8(getattr(pool, n)).clone() for n in "kv"}
+    turn = dict(inv_freq=freq, positions=positions, adjacent=adjacent) if rot else {}
+    q_out = ops.cache_append(k, v, pool.k, pool.v, pt, starts, lengths=lengths, q=q, **pool.scales(), **turn)
+    for n in "kv":
+        values, allowed, scale, changed = want[n]
+        got = pool.values(n)
+        if e4m3:
+            now = getattr(pool, n + "_scale").double()
+            assert torch.equal(now, scale), n
+        nan = torch.isnan(values) | torch.isinf(values) & e4m3
+        assert torch.equal(torch.isnan(got), nan)
+        fine = torch.isfinite(values)
+        assert ((got - values).abs()[fine] <= allowed[fine] * (1 + 1e-9)).all(), n
+        # nothing else is touched, to the bit: what is neither a new token nor an older one whose page's scale has grown
+        same = ~changed
+        assert torch.equal(Pool._u8(getattr(pool, n))[same], before[n][same])
+    if q is not None:
+        y, made_of = rotated(q, angle, rot, adjacent) if rot else (q.double(), q.double().abs())
+        for i in range(b):
+            n = t if lengths is None else max(0, min(int(lengths[i]), t))
+            off = (q_out[i, :, :n].double() - y[i, :, :n]).abs()
+            assert (off <= half_step(dtype) * y[i, :, :n].abs() * (1 + 1e-6) + 16 * U32 * made_of[i, :, :n] + (2.0 ** -25 if dtype == torch.float16 else 0)).all()
+            assert (q_out[i, :, n:] == 0).all()
+    return pool, q_out
+
+
+CASES = [  # b, hq, hk, t, d, rot, page, starts, lengths, adjacent, layout, order
+    (1, 0, 1, 1, 8, 0, 16, [0], None, False, "bhsd", "nhpd"), (3, 8, 2, 1, 128, 128, 64, [0, 63, 64], None, False, "bshd", "nhpd"),
+    (2, 4, 4, 5, 64, 64, 16, [14, 3], None, False, "bshd", "npHd"), (3, 10, 2, 77, 80, 48, 16, [0, 33, 100], [77, 1, 40], True, "bhsd", "both"),
+    (2, 3, 1, 130, 96, 96, 48, [47, 5], [0, 130], False, "bhsd", "npHd"), (1, 2, 2, 300, 40, 20, 256, [100], None, False, "odd", "nhpd"),
+    (2, 5, 3, 33, 128, 128, 32, [0, 31], None, True, "odd", "both"), (1, 0, 8, 64, 128, 128, 64, [64], None, False, "bshd", "nhpd"),
+    (2, 6, 2, 20, 72, 0, 32, [9, 40], [20, 7], False, "bhsd", "nhpd"), (1, 1, 1, 40, 512, 512, 16, [7], None, False, "bhsd", "nhpd"),
+    (2, 4, 70, 3, 16, 16, 16, [15, 0], None, False, "bhsd", "nhpd"), (1, 2, 1, 600, 64, 64, 512, [500], None, False, "bhsd", "nhpd")]
+
+
+@pytest.mark.parametrize("e4m3", [False, True], ids=["16", "e4m3"])
+@pytest.mark.parametrize("dtype", HALVES, ids=["f16", "bf16"])
+@pytest.mark.parametrize("case", CASES, ids=str)
+def test_append(tracea_gpu, case, dtype, e4m3):
+    b, hq, hk, t, d, rot, page, starts, lengths, adjacent, layout, order = case
+    run(tracea_gpu, 11, b, hq, hk, t, d, rot, page, dtype, e4m3, starts, lengths, adjacent, layout, order)
+
+
+def test_positions_of_the_caller(tracea_gpu):
+    pos = torch.randint(0, 2 ** 31 - 1, (2, 9, 1), dtype=torch.int32, device="cuda")
+    run(tracea_gpu, 12, 2, 4, 2, 9, 64, 64, 16, torch.bfloat16, True, [3, 20], positions=pos)
+
+
+@pytest.mark.parametrize("e4m3", [False, True], ids=["16", "e4m3"])
+def test_tokens_without_a_place(tracea_gpu, e4m3):
+    def spoil(pt, k, v):
+        pt[0, 1], pt[1, 0], pt[1, 2] = -1, 10 ** 6, -(2 ** 31)
+    run(tracea_gpu, 13, 2, 4, 2, 60, 64, 64, 16, torch.float16, e4m3, [5, -9], spoil=spoil)
+    # behind the table, and beyond 32 bits
+    g = torch.Generator(device="cuda").manual_seed(1)
+    pool = Pool(g, 4, 2, 16, 64, torch.float16, e4m3)
+    before = {n: Pool._u8(getattr(pool, n)).clone() for n in "kv"}
+    pt = torch.arange(4, dtype=torch.int32, device="cuda").view(1, 4)
+    k = torch.randn(1, 2, 40, 64, device="cuda").half()
+    for start in (64, 2 ** 31 - 1, 2 ** 31 - 20):
+        tracea_gpu.cache_append(k, k, pool.k, pool.v, pt, torch.tensor([start], dtype=torch.int32, device="cuda"), **pool.scales())
+    assert all(torch.equal(Pool._u8(getattr(pool, n)), before[n]) for n in "kv")
+    tracea_gpu.cache_append(k, k, pool.k, pool.v, pt, torch.tensor([60], dtype=torch.int32, device="cuda"), **pool.scales())
+    assert torch.equal(Pool._u8(pool.k)[:3], before["k"][:3]) and not torch.equal(Pool._u8(pool.k)[3], before["k"][3])
+
+
+@pytest.mark.parametrize("dtype", HALVES, ids=["f16", "bf16"])
+def test_infinities_and_nan(tracea_gpu, dtype):
+    def spoil(pt, k, v):
+        k[0, 0, 3, 5], v[0, 1, 4, 6], v[1, 0, 0, 0], k[1, 1] = float("inf"), float("nan"), -float("inf"), 0
+    for e4m3 in (False, True):
+        run(tracea_gpu, 14, 2, 0, 2, 20, 64, 0, 16, dtype, e4m3, [4, 0], spoil=spoil)
+
+
+def test_extreme_values(tracea_gpu):
+    """The largest and smallest bf16 numbers: scales from 2^-126 to the type's end."""
+    def spoil(pt, k, v):
+        k[0, 0] = torch.finfo(torch.bfloat16).max
+        k[0, 1] = 2.0 ** -133
+        v[0, 0] = 448 * 2.0 ** -20
+        v[0, 1] = 450 * 2.0 ** -20  # (above 448: the next power of two)
+    run(tracea_gpu, 15, 1, 0, 2, 16, 64, 0, 16, torch.bfloat16, True, [0], spoil=spoil)
+
+
+def test_codes_are_those_of_a_rounding_to_nearest_even(tracea_gpu):
+    """Values that are not turned: every f16 number up to 448 that a code or the middle of two is, and its neighbours."""
+    codes = torch.arange(127, dtype=torch.uint8).view(E4M3).float()
+    mids = (codes[1:] + codes[:-1]) / 2
+    x = torch.cat([codes, mids, mids * (1 + 2.0 ** -9), mids * (1 - 2.0 ** -9)]).half()
+    x = torch.cat([x, -x])
+    x = torch.cat([x, torch.full((16 * 64 - x.numel(),), 448.0, dtype=torch.float16)]).view(1, 1, 16, 64).cuda()
+    pool = Pool(torch.Generator(device="cuda").manual_seed(1), 1, 1, 16, 64, torch.float16, True)
+    zero = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    tracea_gpu.cache_append(x, x, pool.k, pool.v, zero, zero[0], **pool.scales())
+    assert pool.k_scale.item() == 1.0 and pool.v_scale.item() == 1.0
+    want = x[0].float().to(E4M3).view(torch.uint8)
+    assert torch.equal(pool.k.view(torch.uint8)[0], want) and torch.equal(pool.v.view(torch.uint8)[0], want)
+
+
+@pytest.mark.parametrize("dtype", HALVES, ids=["f16", "bf16"])
+def test_a_cache_is_the_same_however_its_tokens_were_cut(tracea_gpu, dtype):
+    g = torch.Generator(device="cuda").manual_seed(16)
+    b, hk, t, d, page = 2, 3, 50, 64, 32
+    k, v = (heads(g, b, hk, t, d, dtype) * torch.exp2(torch.randint(-3, 4, (t, 1), device="cuda", generator=g).float()).to(dtype) for _ in range(2))
+    freq = torch.logspace(0, -3, 32, device="cuda")
+    pt = table(g, b, 2, 5)
+    whole, cut = (Pool(torch.Generator(device="cuda").manual_seed(2), 5, hk, page, d, dtype, True) for _ in range(2))
+    zero = torch.zeros(b, dtype=torch.int32, device="cuda")
+    tracea_gpu.cache_append(k, v, whole.k, whole.v, pt, zero, inv_freq=freq, **whole.scales())
+    at = 0
+    for n in (1, 1, 7, 20, 1, 3, 17):
+        tracea_gpu.cache_append(k[:, :, at:at + n], v[:, :, at:at + n], cut.k, cut.v, pt, zero + at, inv_freq=freq, **cut.scales())
+        at += n
+    assert at == t and torch.equal(whole.k_scale, cut.k_scale) and torch.equal(whole.v_scale, cut.v_scale)
+    for n in "kv":
+        x, y = whole.values(n), cut.values(n)
+        scale = getattr(whole, n + "_scale").double()[..., None, None]
+        # codes below the normal ones (2^-6) may have been rounded at up to six scales, each half a step of the last or less
+        assert torch.equal(torch.where(x.abs() >= 2.0 ** -6 * scale, x, y), torch.where(y.abs() > 2.0 ** -6 * scale, y, torch.where(x.abs() >= 2.0 ** -6 * scale, x, y)))
+        assert ((x - y).abs() <= 2.0 ** -9 * scale).all()
+
+
+def test_graph_and_in_place_queries(tracea_gpu):
+    g = torch.Generator(device="cuda").manual_seed(17)
+    b, hq, hk, d, page = 4, 8, 2, 128, 16
+    pool, eager = (Pool(torch.Generator(device="cuda").manual_seed(3), 12, hk, page, d, torch.bfloat16, True) for _ in range(2))
+    pt = table(g, b, 3, 12)
+    q, k, v = heads(g, b, hq, 1, d, torch.bfloat16), heads(g, b, hk, 1, d, torch.bfloat16), heads(g, b, hk, 1, d, torch.bfloat16)
+    starts = torch.tensor([0, 3, 15, 30], dtype=torch.int32, device="cuda")
+    freq = torch.logspace(0, -3, 64, device="cuda")
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            tracea_gpu.cache_append(k, v, pool.k, pool.v, pt, starts, q=q, q_out=q, inv_freq=freq, **pool.scales())
+            starts += 1
+        for i in range(5):
+            for x in (q, k, v):
+                x.normal_(generator=g)
+            want = tracea_gpu.cache_append(k, v, eager.k, eager.v, pt, starts, q=q, inv_freq=freq, **eager.scales())
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(q, want) and starts.tolist() == [i + 1, i + 4, i + 16, i + 31]
+            for n in "kv":
+                assert torch.equal(getattr(pool, n).view(torch.uint8), getattr(eager, n).view(torch.uint8))
+                assert torch.equal(getattr(pool, n + "_scale"), getattr(eager, n + "_scale"))

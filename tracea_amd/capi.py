@@ -13,7 +13,7 @@ LIB_PATH = os.environ.get("TRACEA_LIB") or os.path.join(_HERE, "lib", "libtracea
 # TraceaStatus
 SUCCESS, INVALID_PARAMS, UNSUPPORTED_CONFIG, CUDA_ERROR, CPU_ERROR, UNKNOWN_ERROR = 0, 1, 2, 3, 4, 99
 # TraceaDType
-F32, F16, BF16, I32, I8 = 0, 1, 2, 3, 4
+F32, F16, BF16, I32, I8, E4M3 = 0, 1, 2, 3, 4, 5
 # TraceaEpilogueKind
 (EPI_IDENTITY, EPI_BIAS_ADD, EPI_RELU, EPI_GELU, EPI_SILU, EPI_BIAS_RELU, EPI_BIAS_SILU,
  EPI_RESIDUAL, EPI_RESIDUAL_RELU) = range(9)
@@ -71,6 +71,15 @@ class RotaryParams(C.Structure):
 
 class NormParams(C.Structure):
     _fields_ = [("eps", C.c_float), ("residual_scale", C.c_float), ("stream", C.c_void_p)]
+
+
+class QkNormParams(C.Structure):
+    _fields_ = [("axes", C.c_uint32), ("sections", C.c_uint32 * MAX_ROTARY_AXES), ("adjacent", C.c_uint8), ("eps", C.c_float),
+                ("stream", C.c_void_p)]
+
+
+class CacheAppendParams(C.Structure):
+    _fields_ = [("axes", C.c_uint32), ("sections", C.c_uint32 * MAX_ROTARY_AXES), ("adjacent", C.c_uint8), ("stream", C.c_void_p)]
 
 
 class ConvParamsBlock(C.Structure):
@@ -159,6 +168,13 @@ SIGNATURES = {
     "tracea_norm_gate_residual": (C.c_int, [TensorView] + [C.POINTER(TensorView)] * 6 + [NormParams]),
     "tracea_norm_gate_residual_backward": (C.c_int, [C.POINTER(TensorView)] * 2 + [TensorView] +
                                            [C.POINTER(TensorView)] * 9 + [NormParams]),
+    "tracea_qk_norm_rotary": (C.c_int, [TensorView] + [C.POINTER(TensorView)] * 7 + [QkNormParams]),
+    "tracea_qk_norm_rotary_backward": (C.c_int, [TensorView, C.POINTER(TensorView), TensorView] + [C.POINTER(TensorView)] * 9 +
+                                       [QkNormParams]),
+    "tracea_cache_append": (C.c_int, [TensorView] * 2 + [C.POINTER(TensorView)] * 5 + [TensorView] * 2 +
+                            [C.POINTER(TensorView)] * 4 + [CacheAppendParams]),
+    "tracea_attention_cached": (C.c_int, [TensorView] * 3 + [C.POINTER(TensorView)] * 2 + [TensorView, C.POINTER(TensorView), TensorView] +
+                                [C.POINTER(TensorView)] * 2 + [AttentionParams]),
     "tracea_set_split_k": (None, [C.c_int32]),
     "tracea_set_split_k_one_launch": (None, [C.c_int32]),
     "tracea_last_split_k_launches": (C.c_int32, []),

@@ -173,6 +173,36 @@ TraceaStatus tracea_rotary(TraceaTensorView q, const TraceaTensorView *k, Tracea
   TRACEA_GUARDED(dispatch_rotary(q, k, positions, inv_freq, q_out, k_out, params))
 }
 
+TraceaStatus tracea_qk_norm_rotary(TraceaTensorView q, const TraceaTensorView *k, const TraceaTensorView *q_weight,
+                                   const TraceaTensorView *k_weight, const TraceaTensorView *positions,
+                                   const TraceaTensorView *inv_freq, TraceaTensorView *q_out, TraceaTensorView *k_out,
+                                   TraceaQkNormParams params) {
+  TRACEA_GUARDED(dispatch_qk_norm(q, k, q_weight, k_weight, positions, inv_freq, q_out, k_out, params))
+}
+
+TraceaStatus tracea_qk_norm_rotary_backward(TraceaTensorView dq_out, const TraceaTensorView *dk_out, TraceaTensorView q,
+                                            const TraceaTensorView *k, const TraceaTensorView *q_weight,
+                                            const TraceaTensorView *k_weight, const TraceaTensorView *positions,
+                                            const TraceaTensorView *inv_freq, TraceaTensorView *dq, TraceaTensorView *dk,
+                                            TraceaTensorView *dq_weight, TraceaTensorView *dk_weight, TraceaQkNormParams params) {
+  TRACEA_GUARDED(dispatch_qk_norm_backward(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_freq, dq, dk, dq_weight, dk_weight, params))
+}
+
+TraceaStatus tracea_cache_append(TraceaTensorView k, TraceaTensorView v, const TraceaTensorView *q, TraceaTensorView *k_cache,
+                                 TraceaTensorView *v_cache, TraceaTensorView *k_scale, TraceaTensorView *v_scale,
+                                 TraceaTensorView page_table, TraceaTensorView starts, const TraceaTensorView *lengths,
+                                 const TraceaTensorView *positions, const TraceaTensorView *inv_freq, TraceaTensorView *q_out,
+                                 TraceaCacheAppendParams params) {
+  TRACEA_GUARDED(dispatch_cache_append(k, v, q, k_cache, v_cache, k_scale, v_scale, page_table, starts, lengths, positions, inv_freq, q_out, params))
+}
+
+TraceaStatus tracea_attention_cached(TraceaTensorView q, TraceaTensorView k_cache, TraceaTensorView v_cache,
+                                     const TraceaTensorView *k_scale, const TraceaTensorView *v_scale, TraceaTensorView page_table,
+                                     const TraceaTensorView *q_lengths, TraceaTensorView k_lengths, TraceaTensorView *o,
+                                     TraceaTensorView *lse, TraceaAttentionParams params) {
+  TRACEA_GUARDED(dispatch_attention_cached(q, k_cache, v_cache, k_scale, v_scale, page_table, q_lengths, k_lengths, o, lse, params))
+}
+
 TraceaStatus tracea_norm_gate_residual(TraceaTensorView x, const TraceaTensorView *h, const TraceaTensorView *w_post,
                                        const TraceaTensorView *gate, const TraceaTensorView *w_pre, TraceaTensorView *x_out,
                                        TraceaTensorView *y, TraceaNormParams params) {

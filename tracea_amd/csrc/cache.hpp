@@ -1,0 +1,100 @@
+// Argument blocks and launchers of the operators over a key/value cache in pages: norms of heads with rotary positions, appending, attention.
+#pragma once
+#include "train.hpp"
+
+namespace tracea_amd {
+
+// Element type of a cache in 8 bits (kernels take the other types' DataType).
+constexpr int DT_E4M3 = TRACEA_DTYPE_FLOAT8_E4M3;
+
+// A cache [N, Hk, P, D], D contiguous: strides in bytes.
+struct PageView {
+  unsigned char *p;
+  long long sn, sh, ss;
+};
+struct ScaleView {  // [N, Hk], strides in elements; p null: a cache of 16 bits
+  float *p;
+  long long sn, sh;
+};
+// Page `i` of sequence b: table[b * sb + i], i < M; pages outside 0..N-1 are not there.
+struct PageTable {
+  const int *p;
+  long long sb;
+  int M, N, P;
+};
+
+// The page of tokens slot * P .. + P - 1 of sequence b, or -1: none.
+__host__ __device__ inline int page_of(const PageTable &t, int b, long long slot) {
+  if (slot < 0 || slot >= t.M) return -1;
+  const int page = t.p[(long long)b * t.sb + slot];
+  return page >= 0 && page < t.N ? page : -1;
+}
+
+// Norms of heads and rotary positions; positions and pairs as in RotaryArgs (P 0: no positions).
+struct QkNormArgs {
+  HeadView x[2], out[2], dout[2];  // queries, keys; forward: x -> out, backward: x, dout -> out
+  const float *w[2];               // [D] or null (ones)
+  float *dw[2];                    // backward: [D] or null
+  int H[2];                        // heads; H[1] 0: no keys
+  const int *positions;
+  long long pos_sb, pos_ss;
+  const float *inv_freq;
+  int B, S, D, P, axes;
+  int first[TRACEA_MAX_ROTARY_AXES];
+  int adjacent;
+  int vec;     // pieces of 16 bytes
+  float eps, inv_d;
+  int beside;  // lane groups next to each other that take the heads of a token in turn
+  int lanes;   // of a lane group, which has a row: a power of two
+  int blocks;  // backward: workgroups, which take the tokens in turn
+  float *partial;  // backward: [2][blocks][D] sums over a workgroup's rows
+};
+int launch_qk_norm_forward(const QkNormArgs &a, int dtype, hipStream_t stream);
+int launch_qk_norm_backward(const QkNormArgs &a, int dtype, hipStream_t stream);
+constexpr int kQkNormMaxDim = 512;
+constexpr int kQkNormRuns = 8;  // workgroups a CU of the backward pass, at most
+
+struct CacheAppendArgs {
+  HeadView q, q_out, k, v;  // q.p null: no queries
+  int Hq, Hk;
+  PageView kc, vc;
+  ScaleView ks, vs;
+  PageTable table;
+  const int *starts, *lengths;  // [B]; lengths null: T
+  const int *positions;         // null: the token's place in its sequence, one axis
+  long long pos_sb, pos_ss;
+  const float *inv_freq;
+  int B, T, D, P, axes;  // P pairs
+  int first[TRACEA_MAX_ROTARY_AXES];
+  int adjacent;
+  int vec;           // pieces of 8 elements
+  int pages;         // that the T tokens of a sequence can touch
+  int groups;        // of key/value heads, each with as large a part of the query heads
+};
+constexpr int kAppendHeads = 64;  // key/value heads of a workgroup, at most
+int launch_cache_append(const CacheAppendArgs &a, int dtype, hipStream_t stream);
+
+struct AttentionCachedArgs {
+  HeadView q, o;
+  float *lse;  // null: not wanted
+  long long lse_sb, lse_sh, lse_ss;
+  PageView k, v;
+  ScaleView ks, vs;
+  PageTable table;
+  unsigned page_magic;  // ceil(2^32 / (P / 16)), 0 for P = 16
+  const int *q_len, *k_len;
+  int B, Hk, G, Sq, D;
+  unsigned g_magic;  // as in AttentionTrainArgs
+  float scale_log2;  // magnitude
+  int negate, causal;
+  int q_vec, o_vec;  // 16-byte pieces
+  int row_blocks;    // blocks of rows of a (batch entry, key/value head)
+  int two;           // blocks of 32 rows, else 16
+  int workgroups;    // 0: one for each block of rows; else the steps of all of them are shared out evenly
+  int least;         // steps of a workgroup, at least
+  float *part_o, *part_ml;  // [2 * workgroups][rows of a block][width], [..][2]
+};
+int launch_attention_cached(const AttentionCachedArgs &a, int dtype, bool e4m3, hipStream_t stream);
+constexpr int kCachedStep = 128;  // keys of a step of a workgroup
+
+}  // namespace tracea_amd

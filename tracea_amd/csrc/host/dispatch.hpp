@@ -129,8 +129,26 @@ TraceaStatus dispatch_norm_backward(const TraceaTensorView *dx_out, const Tracea
                                     const TraceaTensorView *w_pre, TraceaTensorView *dx, TraceaTensorView *dh,
                                     TraceaTensorView *dw_post, TraceaTensorView *dgate, TraceaTensorView *dw_pre,
                                     const TraceaNormParams &params);
+TraceaStatus dispatch_qk_norm(const TraceaTensorView &q, const TraceaTensorView *k, const TraceaTensorView *q_weight,
+                              const TraceaTensorView *k_weight, const TraceaTensorView *positions, const TraceaTensorView *inv_freq,
+                              TraceaTensorView *q_out, TraceaTensorView *k_out, const TraceaQkNormParams &params);
+TraceaStatus dispatch_qk_norm_backward(const TraceaTensorView &dq_out, const TraceaTensorView *dk_out, const TraceaTensorView &q,
+                                       const TraceaTensorView *k, const TraceaTensorView *q_weight, const TraceaTensorView *k_weight,
+                                       const TraceaTensorView *positions, const TraceaTensorView *inv_freq, TraceaTensorView *dq,
+                                       TraceaTensorView *dk, TraceaTensorView *dq_weight, TraceaTensorView *dk_weight,
+                                       const TraceaQkNormParams &params);
+TraceaStatus dispatch_cache_append(const TraceaTensorView &k, const TraceaTensorView &v, const TraceaTensorView *q,
+                                   TraceaTensorView *k_cache, TraceaTensorView *v_cache, TraceaTensorView *k_scale,
+                                   TraceaTensorView *v_scale, const TraceaTensorView &page_table, const TraceaTensorView &starts,
+                                   const TraceaTensorView *lengths, const TraceaTensorView *positions, const TraceaTensorView *inv_freq,
+                                   TraceaTensorView *q_out, const TraceaCacheAppendParams &params);
+TraceaStatus dispatch_attention_cached(const TraceaTensorView &q, const TraceaTensorView &k_cache, const TraceaTensorView &v_cache,
+                                       const TraceaTensorView *k_scale, const TraceaTensorView *v_scale,
+                                       const TraceaTensorView &page_table, const TraceaTensorView *q_lengths,
+                                       const TraceaTensorView &k_lengths, TraceaTensorView *o, TraceaTensorView *lse,
+                                       const TraceaAttentionParams &params);
 // Device memory kept per (device, stream): grows on demand, never while the stream is being captured (null then), is never
-// freed.  Both belong to the operators for training alone, which use them under one lock: padded copies of operands (at most
+// freed.  Both belong to the operators for training and over a key/value cache, which use them under one lock: padded copies of operands (at most
 // 1 GiB), workspaces.
 void *train_copies(int device, hipStream_t stream, size_t bytes);
 void *train_scratch(int device, hipStream_t stream, size_t bytes);

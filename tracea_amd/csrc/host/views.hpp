@@ -40,7 +40,7 @@ inline TraceaStatus read_view(const char *what, const TraceaTensorView &t, int w
 
 inline bool is_half(int dt) { return dt == TRACEA_DTYPE_FLOAT16 || dt == TRACEA_DTYPE_BFLOAT16; }
 inline bool is_float_type(int dt) { return dt == TRACEA_DTYPE_FLOAT32 || is_half(dt); }
-inline int elem_size(int dt) { return dt == TRACEA_DTYPE_FLOAT32 || dt == TRACEA_DTYPE_INT32 ? 4 : dt == TRACEA_DTYPE_INT8 ? 1 : 2; }
+inline int elem_size(int dt) { return dt == TRACEA_DTYPE_FLOAT32 || dt == TRACEA_DTYPE_INT32 ? 4 : dt == TRACEA_DTYPE_INT8 || dt == TRACEA_DTYPE_FLOAT8_E4M3 ? 1 : 2; }
 inline bool aligned(const void *p, size_t a) { return (((uintptr_t)p) & (a - 1)) == 0; }
 
 // Rows of equal length on one pitch, the form of most views: element rows `pitch` apart, `len` elements of each used.
@@ -125,6 +125,7 @@ inline const char *dtype_name(int dt) {
     case TRACEA_DTYPE_BFLOAT16: return "bf16";
     case TRACEA_DTYPE_INT32: return "i32";
     case TRACEA_DTYPE_INT8: return "i8";
+    case TRACEA_DTYPE_FLOAT8_E4M3: return "e4m3";
     default: return "?";
   }
 }

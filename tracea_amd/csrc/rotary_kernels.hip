@@ -8,6 +8,7 @@
 // Measured: S24960 H32:8 D128 bf16 98 us = 5.2 TB/s in either layout (a large copy reaches 4.8), B8 H12:12 S1024 D64 f32 18 us = 5.6 TB/s,
 // with a quarter of the columns copied 21 us; B1 H12:12 S197 f16 5.0 us, a launch.
 #include "contraction_kernel.hpp"
+#include "rotation.hpp"
 #include "train.hpp"
 
 namespace tracea_amd {
@@ -18,15 +19,6 @@ template <typename T, int E>
 struct alignas(sizeof(T) * E) Piece {
   T x[E];
 };
-
-// The angle is formed and reduced in 64 bits: the product of a 31-bit position and a 24-bit frequency has up to 55 bits,
-// and what counts is its remainder of a whole turn.  32 bits would be off by 2^-24 of the ANGLE: 0.004 rad at position 65536.
-// The sine and cosine of the remainder are fp32.
-__device__ __forceinline__ void turn(int position, float freq, float sign, float &c, float &s) {
-  const double turns = (double)position * (double)freq * 0.15915494309189535;
-  sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
-  s *= sign;
-}
 
 template <typename T, int E, bool ADJ>
 __device__ __forceinline__ void rotate(const T *in, T *out, int at_u, int at_v, const float (&c)[E], const float (&s)[E]) {

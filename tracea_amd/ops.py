@@ -15,7 +15,7 @@ import torch
 from . import capi
 
 _DTYPES = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF16,
-           torch.int32: capi.I32, torch.int8: capi.I8}
+           torch.int32: capi.I32, torch.int8: capi.I8, torch.float8_e4m3fn: capi.E4M3}
 
 
 _VIEW_CACHE = {}
@@ -452,3 +452,81 @@ def norm_gate_residual_backward(dx_out, dy, x_out, h=None, w_post=None, gate=Non
                                                        _ref(dgate), _ref(dw_pre), params)
     capi.check("tracea_norm_gate_residual_backward", st)
     return dx, dh, dw_post, dgate, dw_pre
+
+
+def _rotation(positions, inv_freq, sections):
+    """positions with an axis for the axes, their number and the pairs of each, as the parameter blocks take them."""
+    if positions is not None and positions.dim() == 2:
+        positions = positions.unsqueeze(-1)
+    if inv_freq is None:
+        sections = [] if sections is None else list(sections)
+    else:
+        sections = [inv_freq.shape[0]] if sections is None else list(sections)
+    if len(sections) > capi.MAX_ROTARY_AXES or any(n < 0 for n in sections):
+        raise ValueError("sections: the pairs of 1 to %d axes, got %r" % (capi.MAX_ROTARY_AXES, sections))
+    return positions, len(sections), (C.c_uint32 * capi.MAX_ROTARY_AXES)(*sections)
+
+
+def qk_norm_rotary(q, k, q_weight=None, k_weight=None, positions=None, inv_freq=None, sections=None, adjacent=False, eps=1e-6,
+                   q_out=None, k_out=None):
+    """(q, k) with every head normed and turned in one pass: x / sqrt(mean(x^2) + eps) * weight, then as :func:`rotary`.  q [B,Hq,S,D], k
+    [B,Hk,S,D] or None; q_weight, k_weight [D] float32 (None: ones); positions, inv_freq, sections, adjacent as in :func:`rotary` (both None: no
+    rotation).  q_out may be q, k_out k.  D is contiguous in all of them."""
+    positions, axes, pairs = _rotation(positions, inv_freq, sections)
+    q_out = torch.empty_like(q) if q_out is None else q_out
+    if k is not None:
+        k_out = torch.empty_like(k) if k_out is None else k_out
+    params = capi.QkNormParams(axes, pairs, 1 if adjacent else 0, float(eps), _stream(q))
+    st = capi.lib().tracea_qk_norm_rotary(_plain_view(q), _ref(k), _ref(q_weight), _ref(k_weight), _ref(positions), _ref(inv_freq),
+                                          _ref(q_out), _ref(k_out), params)
+    capi.check("tracea_qk_norm_rotary", st)
+    return q_out, k_out
+
+
+def qk_norm_rotary_backward(dq_out, dk_out, q, k, q_weight=None, k_weight=None, positions=None, inv_freq=None, sections=None,
+                            adjacent=False, eps=1e-6, dq=None, dk=None):
+    """(dq, dk, dq_weight, dk_weight) for the gradients of :func:`qk_norm_rotary`'s results, from its operands; None for what the call has not."""
+    positions, axes, pairs = _rotation(positions, inv_freq, sections)
+    dq = torch.empty_like(q) if dq is None else dq
+    if k is not None:
+        dk = torch.empty_like(k) if dk is None else dk
+    dq_weight = None if q_weight is None else torch.empty_like(q_weight)
+    dk_weight = None if k_weight is None else torch.empty_like(k_weight)
+    params = capi.QkNormParams(axes, pairs, 1 if adjacent else 0, float(eps), _stream(q))
+    st = capi.lib().tracea_qk_norm_rotary_backward(_plain_view(dq_out), _ref(dk_out), _plain_view(q), _ref(k), _ref(q_weight), _ref(k_weight),
+                                                   _ref(positions), _ref(inv_freq), _ref(dq), _ref(dk), _ref(dq_weight), _ref(dk_weight),
+                                                   params)
+    capi.check("tracea_qk_norm_rotary_backward", st)
+    return dq, dk, dq_weight, dk_weight
+
+
+def cache_append(k, v, k_cache, v_cache, page_table, starts, lengths=None, k_scale=None, v_scale=None, q=None, positions=None, inv_freq=None,
+                 sections=None, adjacent=False, q_out=None):
+    """Writes new keys, turned by their positions, and values [B,Hk,T,D] into the pages of k_cache and v_cache [N,Hk,P,D], of k's type or
+    float8_e4m3fn with k_scale, v_scale [N,Hk] float32, which the call keeps up.  Token t of sequence b goes to place starts[b] + t: page
+    page_table[b, place // P] (int32 [B,M]); lengths [B] int32: how many of the T tokens a sequence has.  positions [B or 1,T,axes] int32
+    (None: the place), inv_freq (None: no rotation), sections, adjacent as in :func:`rotary`.  Returns q [B,Hq,T,D] turned by the same positions
+    (zeros behind lengths; q_out may be q), or None without q."""
+    positions, axes, pairs = _rotation(positions, inv_freq, sections)
+    if q is not None:
+        q_out = torch.empty_like(q) if q_out is None else q_out
+    params = capi.CacheAppendParams(axes, pairs, 1 if adjacent else 0, _stream(k))
+    st = capi.lib().tracea_cache_append(_plain_view(k), _plain_view(v), _ref(q), _ref(k_cache), _ref(v_cache), _ref(k_scale), _ref(v_scale),
+                                        _plain_view(page_table), _plain_view(starts), _ref(lengths), _ref(positions), _ref(inv_freq),
+                                        _ref(q_out), params)
+    capi.check("tracea_cache_append", st)
+    return q_out
+
+
+def attention_cached(q, k_cache, v_cache, page_table, k_lengths, q_lengths=None, causal=True, scale=0.0, k_scale=None, v_scale=None,
+                     out=None, lse=None):
+    """softmax(scale q k^T) v over the keys and values that :func:`cache_append` keeps.  q [B,Hq,Sq,D]; k_lengths [B] int32: the keys of each
+    sequence, those of the queries among them; q_lengths [B] int32: its queries; causal: the last query sees every key, the one before it
+    all but one, and so on.  scale 0 means 1/sqrt(D).  lse: [B,Hq,Sq] float32, gets the log-sum-exp of the scores.  Rows that see no
+    key: o 0, lse -inf."""
+    out = torch.empty_like(q) if out is None else out
+    params = capi.AttentionParams(1 if causal else 0, 0, float(scale), _stream(q))
+    st = capi.lib().tracea_attention_cached(_plain_view(q), _plain_view(k_cache), _plain_view(v_cache), _ref(k_scale), _ref(v_scale),
+                                            _plain_view(page_table), _ref(q_lengths), _plain_view(k_lengths), _ref(out), _ref(lse), params)
+    capi.check("tracea_attention_cached", st)
+    return out
