@@ -91,8 +91,9 @@ def gathered(pool, name, page_table, length):
     return torch.where(there[:, None, None], x, torch.zeros_like(x)), there
 
 
-def attention(q, pool, page_table, k_lengths, q_lengths=None, causal=True, scale=None):
-    """(o, lse, allowed) in 64 bits; allowed: how far a kernel's o may be off, without its last rounding."""
+def attention(q, pool, page_table, k_lengths, q_lengths=None, causal=True, scale=None, rounded=False):
+    """(o, lse, allowed, lse_off) in 64 bits; allowed: how far a kernel's o may be off, without its last rounding.  rounded: keys and values are
+    rounded to the type of q (scales that are no powers of two)."""
     b, hq, sq, d = q.shape
     hk = pool.k.shape[1]
     scale = d ** -0.5 if scale is None else scale
@@ -119,10 +120,12 @@ def attention(q, pool, page_table, k_lengths, q_lengths=None, causal=True, scale
             # a score is a sum of D products in fp32, its exponent and the scales some roundings more
             made_of = abs(scale) * (q[i, h, :lq].double().abs() @ kk.abs().t())
             off = U32 * ((d + 8) * torch.where(seen, made_of, torch.zeros_like(x)).amax(-1) + 40 if lk else torch.zeros(lq, device=q.device))
+            if rounded and lk:
+                off = off + half_step(q.dtype) * torch.where(seen, made_of, torch.zeros_like(x)).amax(-1)
             weight = p @ vv.abs()
             # a probability is rounded to the operand type; f16 loses what is 2^36 below a row's largest
             lost = (2.0 ** -36) * vv.abs().sum(0) if q.dtype == torch.float16 and lk else 0.0
-            allowed[i, h, :lq] = (half_step(q.dtype) + 2 * off[:, None] + 64 * U32) * weight + lost
+            allowed[i, h, :lq] = (half_step(q.dtype) * (2 if rounded else 1) + 2 * off[:, None] + 64 * U32) * weight + lost
             lse_off[i, h, :lq] = off + 8 * U32 * torch.where(some, lse[i, h, :lq].abs(), torch.zeros_like(off))
     return o, lse, allowed, lse_off
 

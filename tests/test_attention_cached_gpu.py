@@ -11,7 +11,7 @@ HALVES = [torch.float16, torch.bfloat16]
 
 
 def run(ops, seed, b, hq, hk, sq, k_lengths, d, page, dtype, e4m3, causal=True, q_lengths=None, layout="bhsd", order="nhpd", scale=None, extra=0, spoil=None,
-        garbage=True):
+        garbage=True, rounded=False):
     g = torch.Generator(device="cuda").manual_seed(seed)
     per = max(1, -(-max(k_lengths) // page)) + extra
     pool = Pool(g, b * per + 1, hk, page, d, dtype, e4m3, order)
@@ -21,7 +21,7 @@ def run(ops, seed, b, hq, hk, sq, k_lengths, d, page, dtype, e4m3, causal=True, 
     ql = None if q_lengths is None else torch.tensor(q_lengths, dtype=torch.int32, device="cuda")
     if spoil is not None:
         spoil(pt, pool)
-    want, want_lse, allowed, lse_off = attention(q, pool, pt, k_lengths, q_lengths, causal, scale)
+    want, want_lse, allowed, lse_off = attention(q, pool, pt, k_lengths, q_lengths, causal, scale, rounded)
     if garbage:  # what lies behind the lengths may be anything
         for i in range(b):
             for slot in range(per):
@@ -75,7 +75,7 @@ def test_a_table_far_wider_than_the_sequences(tracea_gpu, dtype):
 
 
 @pytest.mark.parametrize("e4m3", [False, True], ids=["16", "e4m3"])
-@pytest.mark.parametrize("sq", [1, 50])
+@pytest.mark.parametrize("sq", [1, 50, 100])
 def test_pages_that_are_not_there(tracea_gpu, sq, e4m3):
     def spoil(pt, pool):
         pt[0, 1], pt[0, 3], pt[1, 0], pt[1, 1], pt[2] = -1, 10 ** 6, 2 ** 31 - 1, -(2 ** 31), -7
@@ -119,6 +119,28 @@ def test_pages_of_very_different_scales(tracea_gpu, dtype):
         pool.v_scale[pt[0, 2].long()] = 2.0 ** -126
         pool.k_scale[pt[0, 4].long()] = 2.0 ** -126
     run(tracea_gpu, 27, 2, 4, 2, 2, [3000, 555], 128, 16, dtype, True, spoil=spoil, garbage=False)
+
+
+@pytest.mark.parametrize("dtype", HALVES, ids=["f16", "bf16"])
+@pytest.mark.parametrize("sq", [1, 9, 70])
+def test_scales_that_are_no_powers_of_two(tracea_gpu, sq, dtype):
+    def spoil(pt, pool):
+        g = torch.Generator(device="cuda").manual_seed(6)
+        for t in (pool.k_scale, pool.v_scale):
+            t.copy_(0.002 + 0.01 * torch.rand(t.shape, device="cuda", generator=g))
+    run(tracea_gpu, 34, 2, 4, 2, sq, [1100, 333], 128, 16, dtype, True, spoil=spoil, rounded=True)
+    run(tracea_gpu, 35, 2, 4, 2, sq, [1100, 333], 64, 64, dtype, True, spoil=spoil, rounded=True)
+
+
+@pytest.mark.parametrize("sq", [1, 40])
+def test_f16_values_at_the_ends_of_the_type(tracea_gpu, sq):
+    """Codes times scales beyond f16's largest number and below its smallest: only the results have to fit."""
+    def spoil(pt, pool):
+        pool.k_scale.fill_(2.0 ** -8)
+        pool.k_scale[pt[0, :2].long()] = 2.0 ** -26
+        pool.v_scale.fill_(2.0 ** -22)
+        pool.v_scale[pt[1].long()] = 2.0 ** 5
+    run(tracea_gpu, 36, 2, 4, 2, sq, [200, 200], 64, 16, torch.float16, True, spoil=spoil, garbage=False)
 
 
 @pytest.mark.parametrize("dtype", HALVES, ids=["f16", "bf16"])

@@ -37,7 +37,7 @@ HOST_SOURCES = ["abi.cpp", "tuner_abi.cpp", "graph_abi.cpp", "plan_abi.cpp", "tt
                 "host/graph_fusion.cpp"]
 DEVICE_SOURCES = ["support_kernels.hip", "gemm_rows_kernels.hip", "gemm_ragged_kernels.hip", "conv_transpose_kernels.hip", "graph_kernels.hip", "attention_kernels.hip",
                   "attention_train_kernels.hip", "rotary_kernels.hip", "norm_kernels.hip", "qk_norm_kernels.hip", "cache_append_kernels.hip",
-                  "attention_cached_kernels.hip"]
+                  "attention_cached_kernels.hip", "attention_cached_tiles_kernels.hip"]
 
 
 def hipcc():

@@ -17,118 +17,62 @@
 // A wave walks every fourth block of 32 keys, the next one requested before it works on the last; a workgroup's four waves join through LDS.
 // Where blocks of rows are few, all steps of 128 keys of all sequences are one line that the workgroups share out evenly, whatever the
 // lengths; a problem cut between workgroups is joined by a second launch, parts in their order.
+#include <algorithm>
 #include <type_traits>
 
-#include "cache.hpp"
-#include "contraction_kernel.hpp"
+#include "attention_cached_share.hpp"
 
 namespace tracea_amd {
 
 namespace {
 
-constexpr float LN2 = 0.6931471805599453f;
 constexpr int WAVES = 4;
 
-// As in the attention for training: a row's reference lies P_SHIFT powers of two below a score it has met and moves only when a step exceeds
-// that score by more than LAZY_MAX.  f16 has no range below 2^-24: the shift keeps the tails of long rows.
-template <int DT>
-constexpr float P_SHIFT = DT == DT_F16 ? 11.0f : 0.0f;
-template <int DT>
-constexpr float LAZY_MAX = DT == DT_F16 ? 4.0f : 8.0f;
+// Of a cache in 8 bits, what the scales of the groups of 16 keys in Places make of scores and probabilities:
+//   c     scale log2(e) ks: scores times c are exponents of 2 (above 0, so that -inf of a key that is not seen stays that)
+//   lift  log2(vs / ref), ref the largest scale of values that the wave has met: what is summed up is in units of ref, so that f16
+//         probabilities times a scale keep their range; the scale joins the probability in its exponent, p vs / ref = 2^(x - m + lift), and the sum
+//         of probabilities takes it back, 2^-lift times a group's four.  -60 at least: less is nothing beside the largest.
+constexpr float LEAST_LIFT = -60.0f;
+struct Scales {
+  float c, lift, ref = 0.0f;
+  float lift_before;  // of the 64 groups before
 
-template <int DT>
-__device__ __forceinline__ unsigned pack2(float a, float b) {
-  if constexpr (DT == DT_F16) {
-    typedef _Float16 half2 __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(unsigned, half2{(_Float16)a, (_Float16)b});
-  } else {
-    typedef __bf16 pair __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(unsigned, pair{(__bf16)a, (__bf16)b});
+  // The factor by which what is summed up so far changes.
+  __device__ __forceinline__ float load(const AttentionCachedArgs &a, int hk, int page, bool there) {
+    c = fmaxf(a.scale_log2 * a.ks.p[page * a.ks.sn + hk * a.ks.sh], 1.17549435e-38f);
+    const float vs = a.vs.p[page * a.vs.sn + hk * a.vs.sh], top = wave_max(there ? vs : 0.0f);
+    float f = 1.0f;
+    lift_before = lift;
+    if (top > ref) {  // (lifts from before, in its terms)
+      f = ref / top;
+      ref = top;
+      lift_before = fmaxf(lift + fmaxf(__builtin_amdgcn_logf(f), LEAST_LIFT), LEAST_LIFT);
+    }
+    lift = fmaxf(__builtin_amdgcn_logf(vs / fmaxf(ref, 1.17549435e-38f)), LEAST_LIFT);
+    return f;
   }
-}
-// Two e4m3 codes of a register (its upper half: HI) in 16 bits, exactly: e4m3 has no value that f16 or bf16 lacks.
-template <int DT, bool HI>
-__device__ __forceinline__ unsigned widen2(unsigned codes) {
-  if constexpr (DT == DT_F16) return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)codes, 1.0f, HI));
-  else return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)codes, 1.0f, HI));
-}
-
-// max over a lane's own value and those of the other three 16-lane groups (see attention_train_kernels.hip)
-__device__ __forceinline__ float groups_max(float x) {
-  float a0 = x, a1 = x;
-  asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a0), "+v"(a1));
-  float b0 = fmaxf(a0, a1), b1 = b0;
-  asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(b0), "+v"(b1));
-  return fmaxf(b0, b1);
-}
-__device__ __forceinline__ float groups_sum(float x) {
-  x += __shfl_xor(x, 16, 64);
-  return x + __shfl_xor(x, 32, 64);
-}
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) x = fmaxf(x, __shfl_xor(x, m, 64));
-  return x;
-}
-
-__device__ __forceinline__ int query_of(const AttentionCachedArgs &a, int r) {
-  return a.G == 1 ? r : (int)__umulhi((unsigned)r, a.g_magic);
-}
-__device__ __forceinline__ int keys_of(const AttentionCachedArgs &a, int b) {
-  return min(max(a.k_len[b], 0), a.table.M * a.table.P);
-}
-// Steps of a block of rows of sequence b: at least one, which writes what rows without keys get.
-__device__ __forceinline__ int steps_of(const AttentionCachedArgs &a, int b) {
-  return max(1, (keys_of(a, b) + kCachedStep - 1) / kCachedStep);
-}
-
-// Steps of all blocks of rows in front of those of sequence b (b a multiple of 64) for lane l: those in front of b + l, and of all 64 together.
-__device__ __forceinline__ long long scan_steps(const AttentionCachedArgs &a, int b, int lane, long long &total, int &own) {
-  own = b + lane < a.B ? steps_of(a, b + lane) : 0;
-  long long x = (long long)own * (a.Hk * a.row_blocks);
-  const long long mine = x;
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const long long y = __shfl_up(x, m, 64);
-    if (lane >= m) x += y;
-  }
-  total = __shfl(x, 63, 64);
-  return x - mine;
-}
-__device__ __forceinline__ long long uniform(long long x) {
-  return (long long)(unsigned)__builtin_amdgcn_readfirstlane((int)x) | (long long)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
-}
-// Steps of a workgroup where all of them are shared out.
-__device__ __forceinline__ long long share_of(const AttentionCachedArgs &a, int lane, long long &all) {
-  all = 0;
-  for (int b = 0; b < a.B; b += 64) {
-    long long total;
-    int own;
-    (void)scan_steps(a, b, lane, total, own);
-    all += total;
-  }
-  all = uniform(all);
-  const long long per = (all + a.workgroups - 1) / a.workgroups;
-  return per < a.least ? a.least : per;
-}
+  __device__ __forceinline__ float unit() const { return fmaxf(ref, 1.17549435e-38f); }
+};
 
 template <int DT, bool C8, int DU, int NQ, bool FULL>
 struct Stream {
   static constexpr int KS = DU / 32, VC = DU / 16, ES = C8 ? 1 : 2, ROWS = 16 * NQ;
   static constexpr int KW = 2 * ES, VW = VC * ES / 4;  // registers of 8 columns of a key, of a chunk of a row of values
 
-  // What a step loads: 32 keys.
-  struct Loads {
+  // Whether a step's loads have registers of their own beside those of the step before: else K of the next step is requested when the scores
+  // are there, V when its products are done.  Without, the 16-bit form with 32 rows needs more than half of the registers.
+  static constexpr bool DEEP = C8 || NQ == 1 || DU == 64;
+
+  struct Keys {  // of a step: 32 keys
     unsigned k[2][KS][KW];
-    unsigned v[8][VW];
-    float ks[2], vs[2];
-    unsigned valid;  // of the two groups of 16
   };
-  // Where the wave's next groups of 16 keys lie, one per lane.
-  struct Places {
-    unsigned k_lo, k_hi, v_lo, v_hi;
-    float ks, vs;
-    unsigned long long valid;
+  struct Values {
+    unsigned v[8][VW];
+  };
+  struct Tags {
+    unsigned valid;  // of the two groups of 16
+    float c[2], lift[2];
   };
 };
 
@@ -144,8 +88,7 @@ __device__ __forceinline__ void load_words(const unsigned char *base, unsigned o
 }
 
 template <int DT, bool C8, int DU, int NQ, bool FULL>
-// (two waves a SIMD, but for the form whose loads in flight and sums fill more than half of the registers)
-__global__ void __launch_bounds__(WAVES * 64, NQ == 2 && !C8 && DU == 128 ? 1 : 2) attention_cached_kernel(const AttentionCachedArgs a) {
+__global__ void __launch_bounds__(WAVES * 64, 2) attention_cached_kernel(const AttentionCachedArgs a) {
   using S = Stream<DT, C8, DU, NQ, FULL>;
   constexpr int KS = S::KS, VC = S::VC, ES = S::ES, KW = S::KW, VW = S::VW, ROWS = S::ROWS, PITCH = DU + 4;
   __shared__ __attribute__((aligned(16))) float s_o[WAVES][ROWS][PITCH];
@@ -153,64 +96,32 @@ __global__ void __launch_bounds__(WAVES * 64, NQ == 2 && !C8 && DU == 128 ? 1 : 
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, g4 = lane >> 4;
-  const int per_b = a.Hk * a.row_blocks;
 
-  // the workgroup's share: `left` steps from step s0 of problem `inner` of sequence b
-  int b, inner, s0, sb;
-  long long left;
-  bool fresh_start = true;
+  Share w;
+  bool begins = true;
   if (a.workgroups == 0) {
-    b = (int)blockIdx.x / per_b;
-    inner = (int)blockIdx.x - b * per_b;
-    s0 = 0;
-    sb = steps_of(a, b);
-    left = sb;
-  } else {
-    long long all;
-    const long long per = share_of(a, lane, all), first = (long long)blockIdx.x * per;
-    if (first >= all) return;
-    left = min(per, all - first);
-    long long before = 0;
-    b = 0;
-    for (int b0 = 0;; b0 += 64) {
-      long long total;
-      int own;
-      const long long mine = scan_steps(a, b0, lane, total, own);
-      if (uniform(before + total) > first) {
-        const unsigned long long here = __ballot(before + mine <= first && own > 0);
-        const int at = 63 - __clzll(here);
-        b = b0 + at;
-        sb = __builtin_amdgcn_readlane(own, at);
-        const long long u = first - (before + uniform(__shfl(mine, at, 64)));
-        inner = (int)(u / sb);
-        s0 = (int)(u - (long long)inner * sb);
-        break;
-      }
-      before += total;
-    }
-    b = __builtin_amdgcn_readfirstlane(b);
-    inner = __builtin_amdgcn_readfirstlane(inner);
-    s0 = __builtin_amdgcn_readfirstlane(s0);
-    left = uniform(left);
+    w.b = (int)blockIdx.x / (a.Hk * a.row_blocks);
+    w.inner = (int)blockIdx.x - w.b * (a.Hk * a.row_blocks);
+    w.s0 = w.first = 0;
+    w.sb = w.per = w.left = steps_of(a, w.b);
+  } else if (!share_of(a, lane, w)) {
+    return;
   }
+  int line = w.first;
 
-  while (left > 0) {
-    const int n = (int)min((long long)(sb - s0), left);  // steps of this problem
-    const int hk = inner / a.row_blocks, rb = inner - hk * a.row_blocks;
-    const int lk = keys_of(a, b), lq = a.q_len != nullptr ? min(max(a.q_len[b], 0), a.Sq) : a.Sq;
+  while (w.left > 0) {
+    const int b = w.b, s0 = w.s0, n = min(w.sb - s0, w.left);  // steps of this problem
+    const int hk = w.inner / a.row_blocks, rb = w.inner - hk * a.row_blocks;
+    const int lk = keys_of(a, b), lq = queries_of(a, b);
     const int rows = a.G * lq, off = lk - lq, r_first = rb * ROWS;
-
-    const unsigned char *k_head = a.k.p + hk * a.k.sh, *v_head = a.v.p + hk * a.v.sh;
-    const float *ks_head = C8 ? a.ks.p + hk * a.ks.sh : nullptr, *vs_head = C8 ? a.vs.p + hk * a.vs.sh : nullptr;
 
     // keys in front of which the wave's steps begin: it has those with any key
     const int key0 = s0 * kCachedStep + wave * 32;
     const int end = min(lk, (s0 + n) * kCachedStep);
     const int steps = end > key0 ? (end - key0 + kCachedStep - 1) / kCachedStep : 0;
 
-    typename S::Places at;
-    float v_ref = 0.0f;  // the largest scale of values met
-    float v_inv = 1.0f;
+    Places at;
+    Scales scales;
     f32x4 o[NQ][VC];
     float m[NQ];
     double total[NQ];
@@ -223,31 +134,16 @@ __global__ void __launch_bounds__(WAVES * 64, NQ == 2 && !C8 && DU == 128 ? 1 : 
     }
     // the places of the wave's steps t .. t + 31, two groups of 16 keys each
     auto locate = [&](int t) __attribute__((always_inline)) {
-      const int key = key0 + (t + lane / 2) * kCachedStep + (lane & 1) * 16, group = key >> 4;
-      const int slot_page = a.page_magic == 0 ? group : (int)__umulhi((unsigned)group, a.page_magic);
-      int page = key < end ? page_of(a.table, b, slot_page) : -1;
-      const bool there = page >= 0;
-      const int place = there ? key - slot_page * a.table.P : 0;
-      page = there ? page : 0;  // (something to load)
-      const unsigned long long k = (unsigned long long)(k_head + page * a.k.sn + place * a.k.ss);
-      const unsigned long long v = (unsigned long long)(v_head + page * a.v.sn + place * a.v.ss);
-      at.k_lo = (unsigned)k; at.k_hi = (unsigned)(k >> 32);
-      at.v_lo = (unsigned)v; at.v_hi = (unsigned)(v >> 32);
-      at.valid = __ballot(there);
-      if constexpr (C8) {
-        at.ks = ks_head[page * a.ks.sn];
-        at.vs = vs_head[page * a.vs.sn];
-        const float top = wave_max(there ? fabsf(at.vs) : 0.0f);
-        if (top > v_ref) {
-          const float f = v_ref / top;
-          v_ref = top;
-          v_inv = 1.0f / fmaxf(v_ref, 1.17549435e-38f);
+      bool there;
+      const int page = at.locate(a, b, hk, key0 + (t + lane / 2) * kCachedStep + (lane & 1) * 16, end, there);
+      const float f = C8 ? scales.load(a, hk, page, there) : 1.0f;
+      if (C8 && f != 1.0f) {
 #pragma unroll
-          for (int qb = 0; qb < NQ; ++qb)
+        for (int qb = 0; qb < NQ; ++qb)
 #pragma unroll
-            for (int j = 0; j < VC; ++j) o[qb][j] *= f;
-        }
+          for (int j = 0; j < VC; ++j) o[qb][j] *= f;
       }
+      return f;
     };
 
     unsigned k_off[KS], v_off[4];
@@ -259,41 +155,55 @@ __global__ void __launch_bounds__(WAVES * 64, NQ == 2 && !C8 && DU == 128 ? 1 : 
 #pragma unroll
     for (int i = 0; i < 4; ++i) v_off[i] = (unsigned)((g4 * 4 + i) * (int)a.v.ss + (FULL || r16 * VC < a.D ? r16 * VC : 0) * ES);
 
-    auto request = [&](int t, typename S::Loads &l) __attribute__((always_inline)) {
+    auto request_k = [&](int t, typename S::Keys &l) __attribute__((always_inline)) {
       const int e = (t & 31) * 2;
-      l.valid = (unsigned)(at.valid >> e) & 3u;
 #pragma unroll
       for (int blk = 0; blk < 2; ++blk) {
-        const unsigned char *k = (const unsigned char *)((unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)at.k_lo, e + blk) |
-                                                         (unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)at.k_hi, e + blk) << 32);
-        const unsigned char *v = (const unsigned char *)((unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)at.v_lo, e + blk) |
-                                                         (unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)at.v_hi, e + blk) << 32);
+        const unsigned char *k = at.k(e + blk);
         if constexpr (FULL) {  // a run of 8 KS columns, 16 bytes at a time
           constexpr int PER = 4 / KW;  // pieces of 8 columns in 16 bytes
 #pragma unroll
           for (int s = 0; s < KS; s += PER) {
-            unsigned w[4];
-            load_words<4>(k, k_off[s], w);
+            unsigned x[4];
+            load_words<4>(k, k_off[s], x);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) l.k[blk][s + i / KW][i % KW] = w[i];
+            for (int i = 0; i < 4; ++i) l.k[blk][s + i / KW][i % KW] = x[i];
           }
         } else {
 #pragma unroll
           for (int s = 0; s < KS; ++s) load_words<KW>(k, k_off[s], l.k[blk][s]);
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) load_words<VW>(v, v_off[i], l.v[blk * 4 + i]);
-        if constexpr (C8) {
-          l.ks[blk] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, at.ks), e + blk));
-          l.vs[blk] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, at.vs), e + blk));
-        }
       }
     };
+    auto request_v = [&](int t, typename S::Values &l) __attribute__((always_inline)) {
+      const int e = (t & 31) * 2;
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk) {
+        const unsigned char *v = at.v(e + blk);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load_words<VW>(v, v_off[i], l.v[blk * 4 + i]);
+      }
+    };
+    auto tags_of = [&](int t) __attribute__((always_inline)) {
+      const int e = (t & 31) * 2;
+      typename S::Tags x;
+      x.valid = (unsigned)(at.valid >> e) & 3u;
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk) {
+        x.c[blk] = C8 ? of_lane(scales.c, e + blk) : a.scale_log2;
+        x.lift[blk] = C8 ? of_lane(scales.lift, e + blk) : 0.0f;
+      }
+      return x;
+    };
 
-    typename S::Loads now, next;
+    typename S::Keys k_now, k_next;
+    typename S::Values v_now, v_next;
+    typename S::Tags tags, tags_next;
     if (steps > 0) {
-      locate(0);
-      request(0, now);
+      (void)locate(0);
+      request_k(0, k_now);
+      request_v(0, v_now);
+      tags = tags_of(0);
     }
 
     int q_last[NQ];  // the last key that the lane's row sees
@@ -306,27 +216,24 @@ __global__ void __launch_bounds__(WAVES * 64, NQ == 2 && !C8 && DU == 128 ? 1 : 
       const unsigned short *p =
           (const unsigned short *)a.q.p + (there ? (long long)b * a.q.sb + (long long)(hk * a.G + r - i * a.G) * a.q.sh + (long long)i * a.q.ss : 0);
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const int c = (g4 * KS + s) * 8;
-        qf[qb][s] = u32x4{0, 0, 0, 0};
-        if (there && c < a.D) {
-          if (a.q_vec) {
-            qf[qb][s] = *(const u32x4 *)(p + c);
-          } else {
-#pragma unroll
-            for (int w = 0; w < 4; ++w) qf[qb][s][w] = (unsigned)p[c + 2 * w] | (unsigned)p[c + 2 * w + 1] << 16;
-          }
-        }
-        if (a.negate) qf[qb][s] ^= 0x80008000u;
-      }
+      for (int s = 0; s < KS; ++s) qf[qb][s] = query_columns(a, p, there, (g4 * KS + s) * 8);
     }
     // keys that every row of the block sees, those past the last row aside (what they hold is dropped)
     int all_see = lk;
     if (a.causal && r_first < rows) all_see = min(lk, query_of(a, r_first) + off + 1);
 
-    auto work = [&](int t, typename S::Loads &l) __attribute__((always_inline)) {
+    // Places of step t, where it is the first of 32, while the step before is not done.
+    auto locate_ahead = [&](int t) __attribute__((always_inline)) {
+      if ((t & 31) != 0) return;
+      const float f = locate(t);
+      if (C8 && f != 1.0f) {
+#pragma unroll
+        for (int blk = 0; blk < 2; ++blk) tags.lift[blk] = of_lane(scales.lift_before, 62 + blk);
+      }
+    };
+    auto work = [&](int t, typename S::Keys &keys, typename S::Values &values, auto &&between) __attribute__((always_inline)) {
       const int key = key0 + t * kCachedStep;
-      const bool edge = key + 32 > all_see || l.valid != 3u;
+      const bool edge = key + 32 > all_see || tags.valid != 3u;
       f32x4 z[NQ][2];
 #pragma unroll
       for (int blk = 0; blk < 2; ++blk)
@@ -334,9 +241,9 @@ __global__ void __launch_bounds__(WAVES * 64, NQ == 2 && !C8 && DU == 128 ? 1 : 
         for (int s = 0; s < KS; ++s) {
           u32x4 f;
           if constexpr (C8) {
-            f = u32x4{widen2<DT, false>(l.k[blk][s][0]), widen2<DT, true>(l.k[blk][s][0]), widen2<DT, false>(l.k[blk][s][1]), widen2<DT, true>(l.k[blk][s][1])};
+            f = u32x4{widen2<DT, false>(keys.k[blk][s][0]), widen2<DT, true>(keys.k[blk][s][0]), widen2<DT, false>(keys.k[blk][s][1]), widen2<DT, true>(keys.k[blk][s][1])};
           } else {
-            f = u32x4{l.k[blk][s][0], l.k[blk][s][1], l.k[blk][s][2], l.k[blk][s][3]};
+            f = u32x4{keys.k[blk][s][0], keys.k[blk][s][1], keys.k[blk][s][2], keys.k[blk][s][3]};
           }
           if constexpr (!FULL) {  // columns from D on: the queries have zeros there, which a NaN would outlive
             if ((g4 * KS + s) * 8 >= a.D) f = u32x4{0, 0, 0, 0};
@@ -344,11 +251,12 @@ __global__ void __launch_bounds__(WAVES * 64, NQ == 2 && !C8 && DU == 128 ? 1 : 
 #pragma unroll
           for (int qb = 0; qb < NQ; ++qb) z[qb][blk] = Mfma16<DT>::run(f, qf[qb][s], s == 0 ? f32x4{0, 0, 0, 0} : z[qb][blk]);
         }
+      between();
       if (edge) {
         // a query does not see what lies behind its last key, nor a group without a page
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk) {
-          const bool there = (l.valid >> blk) & 1u;
+          const bool there = (tags.valid >> blk) & 1u;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int j = key + blk * 16 + g4 * 4 + i;
@@ -356,35 +264,24 @@ __global__ void __launch_bounds__(WAVES * 64, NQ == 2 && !C8 && DU == 128 ? 1 : 
             for (int qb = 0; qb < NQ; ++qb) z[qb][blk][i] = !there || j > q_last[qb] ? -INFINITY : z[qb][blk][i];
             if (!there || j >= lk) {  // what has no key may hold anything
 #pragma unroll
-              for (int w = 0; w < VW; ++w) l.v[blk * 4 + i][w] = 0;
+              for (int x = 0; x < VW; ++x) values.v[blk * 4 + i][x] = 0;
             }
           }
         }
       }
       u32x4 pf[NQ];
       bool moved = false;
-      float alpha[NQ], c[2], ratio[2];
+      float alpha[NQ], back[2];
+      const float(&c)[2] = tags.c, (&lift)[2] = tags.lift;
 #pragma unroll
-      for (int blk = 0; blk < 2; ++blk) {
-        c[blk] = C8 ? a.scale_log2 * l.ks[blk] : a.scale_log2;
-        ratio[blk] = C8 ? l.vs[blk] * v_inv : 1.0f;
-      }
+      for (int blk = 0; blk < 2; ++blk) back[blk] = C8 ? __builtin_amdgcn_exp2f(-lift[blk]) : 1.0f;
 #pragma unroll
       for (int qb = 0; qb < NQ; ++qb) {
         float mx = -INFINITY;
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if constexpr (C8) {
-              // (-inf stays what it is whatever the scale)
-              z[qb][blk][i] = z[qb][blk][i] == -INFINITY ? -INFINITY : z[qb][blk][i] * c[blk];
-            } else {
-              z[qb][blk][i] *= c[blk];
-            }
-            mx = fmaxf(mx, z[qb][blk][i]);
-          }
-        mx = groups_max(mx);
+          mx = fmaxf(mx, c[blk] * fmaxf(fmaxf(z[qb][blk][0], z[qb][blk][1]), fmaxf(z[qb][blk][2], z[qb][blk][3])));
+        mx = groups_max_valu(mx);
         const bool mv = mx > m[qb] + (P_SHIFT<DT> + LAZY_MAX<DT>);  // (a first score above -inf always moves it)
         const float mn = mv ? mx - P_SHIFT<DT> : m[qb];
         alpha[qb] = mv ? __builtin_amdgcn_exp2f(m[qb] - mn) : 1.0f;
@@ -404,10 +301,12 @@ __global__ void __launch_bounds__(WAVES * 64, NQ == 2 && !C8 && DU == 128 ? 1 : 
         const float ref = m[qb] == -INFINITY ? 0.0f : m[qb];  // (nothing visible yet: exp2(-inf) = 0)
         float p[8], sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          p[i] = __builtin_amdgcn_exp2f(z[qb][i / 4][i % 4] - ref);
-          sum += p[i];
-          if constexpr (C8) p[i] *= ratio[i / 4];
+        for (int blk = 0; blk < 2; ++blk) {
+          const float r = lift[blk] - ref;
+          float four = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) four += p[blk * 4 + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[qb][blk][i], c[blk], r));
+          sum += C8 ? four * back[blk] : four;
         }
         total[qb] += (double)sum;
         pf[qb] = u32x4{pack2<DT>(p[0], p[1]), pack2<DT>(p[2], p[3]), pack2<DT>(p[4], p[5]), pack2<DT>(p[6], p[7])};
@@ -417,8 +316,8 @@ __global__ void __launch_bounds__(WAVES * 64, NQ == 2 && !C8 && DU == 128 ? 1 : 
         unsigned x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          if constexpr (C8) x[i] = j % 4 == 0 ? widen2<DT, false>(l.v[i][j / 4]) : widen2<DT, true>(l.v[i][j / 4]);
-          else x[i] = l.v[i][j / 2];
+          if constexpr (C8) x[i] = j % 4 == 0 ? widen2<DT, false>(values.v[i][j / 4]) : widen2<DT, true>(values.v[i][j / 4]);
+          else x[i] = values.v[i][j / 2];
         }
         u32x4 lo, hi;
 #pragma unroll
@@ -434,17 +333,34 @@ __global__ void __launch_bounds__(WAVES * 64, NQ == 2 && !C8 && DU == 128 ? 1 : 
       }
     };
 
-    auto ahead = [&](int t, typename S::Loads &l) __attribute__((always_inline)) {
-      if (t >= steps) return;
-      if ((t & 31) == 0) locate(t);
-      request(t, l);
-    };
-    for (int t = 0; t < steps; t += 2) {
-      ahead(t + 1, next);
-      work(t, now);
-      if (t + 1 >= steps) break;
-      ahead(t + 2, now);
-      work(t + 1, next);
+    if constexpr (S::DEEP) {
+      auto ahead = [&](int t, typename S::Keys &k, typename S::Values &v) __attribute__((always_inline)) {
+        if (t >= steps) return;
+        locate_ahead(t);
+        request_k(t, k);
+        request_v(t, v);
+        tags_next = tags_of(t);
+      };
+      for (int t = 0; t < steps; t += 2) {
+        ahead(t + 1, k_next, v_next);
+        work(t, k_now, v_now, [] {});
+        tags = tags_next;
+        if (t + 1 >= steps) break;
+        ahead(t + 2, k_now, v_now);
+        work(t + 1, k_next, v_next, [] {});
+        tags = tags_next;
+      }
+    } else {
+      for (int t = 0; t < steps; ++t) {
+        work(t, k_now, v_now, [&]() __attribute__((always_inline)) {
+          if (t + 1 >= steps) return;
+          locate_ahead(t + 1);
+          request_k(t + 1, k_now);
+          tags_next = tags_of(t + 1);
+        });
+        if (t + 1 < steps) request_v(t + 1, v_now);
+        tags = tags_next;
+      }
     }
 
     // the four waves' states meet
@@ -460,30 +376,31 @@ __global__ void __launch_bounds__(WAVES * 64, NQ == 2 && !C8 && DU == 128 ? 1 : 
 #pragma unroll
         for (int j = 0; j < VC; j += 4) {
           f32x4 x = {o[qb][j][i], o[qb][j + 1][i], o[qb][j + 2][i], o[qb][j + 3][i]};
-          if constexpr (C8) x *= fmaxf(v_ref, 1.17549435e-38f);
+          if constexpr (C8) x *= scales.unit();
           *(f32x4 *)&s_o[wave][qb * 16 + r16][(g4 * 4 + i) * VC + j] = x;
         }
     }
     __syncthreads();
-    const bool whole = n == sb;
-    const long long slot = 2ll * blockIdx.x + (fresh_start ? 0 : 1);
+    const bool whole = n == w.sb;
+    const long long slot = 2ll * blockIdx.x + (begins ? 0 : 1);
+    if (a.workgroups > 0 && s0 == 0 && threadIdx.x == 0) write_meta(a, w, line, n, begins);
 #pragma unroll
     for (int qb = 0; qb < NQ; ++qb) {
       const int row = qb * 16 + (int)threadIdx.x / 16, col = (threadIdx.x & 15) * VC, r = r_first + row;
       float top = s_m[0][row];
 #pragma unroll
-      for (int w = 1; w < WAVES; ++w) top = fmaxf(top, s_m[w][row]);
+      for (int x = 1; x < WAVES; ++x) top = fmaxf(top, s_m[x][row]);
       const float ref = top == -INFINITY ? 0.0f : top;
       float sum = 0.0f, x[VC];
 #pragma unroll
       for (int j = 0; j < VC; ++j) x[j] = 0.0f;
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) {
-        const float f = __builtin_amdgcn_exp2f(s_m[w][row] - ref);
-        sum += f * s_l[w][row];
+      for (int from = 0; from < WAVES; ++from) {
+        const float f = __builtin_amdgcn_exp2f(s_m[from][row] - ref);
+        sum += f * s_l[from][row];
 #pragma unroll
         for (int j = 0; j < VC; j += 4) {
-          const f32x4 y = *(const f32x4 *)&s_o[w][row][col + j];
+          const f32x4 y = *(const f32x4 *)&s_o[from][row][col + j];
 #pragma unroll
           for (int i = 0; i < 4; ++i) x[j + i] += f * y[i];
         }
@@ -518,74 +435,51 @@ __global__ void __launch_bounds__(WAVES * 64, NQ == 2 && !C8 && DU == 128 ? 1 : 
       if (col == 0 && a.lse != nullptr)
         a.lse[(long long)b * a.lse_sb + (long long)h * a.lse_sh + (long long)i * a.lse_ss] = there ? (top + __builtin_amdgcn_logf(sum)) * LN2 : -INFINITY;
     }
-    left -= n;
-    if (left > 0) {
+    line += n;
+    w.left -= n;
+    if (w.left > 0) {
       __syncthreads();  // (before the next problem's states)
-      fresh_start = false;
-      s0 = 0;
-      if (++inner == per_b) {
-        inner = 0;
-        ++b;
-        sb = steps_of(a, b);
-      }
+      begins = false;
+      next_problem(a, w);
     }
   }
 }
 
 // Joins the parts of problems that were cut between workgroups: a workgroup for each row of a problem, its four waves
 // taking the parts in turn.
-template <int DT, int DU, int NQ>
+template <int DT, int DU>
 __global__ void __launch_bounds__(256) attention_cached_join_kernel(const AttentionCachedArgs a) {
-  constexpr int ROWS = 16 * NQ, C = DU / 64;
+  constexpr int C = DU / 64;
+  typedef float Columns __attribute__((ext_vector_type(C)));
   __shared__ float s_o[4][DU], s_l[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, per_b = a.Hk * a.row_blocks;
-  const int b = (int)blockIdx.y / per_b, inner = (int)blockIdx.y - b * per_b, row = blockIdx.x;
-  const int hk = inner / a.row_blocks, rb = inner - hk * a.row_blocks, r = rb * ROWS + row;
-  if (r >= a.G * a.Sq) return;
-  long long all, before = 0;
-  const long long per = share_of(a, lane, all);
-  int sb = 0;
-  for (int b0 = 0; b0 <= b; b0 += 64) {
-    long long total;
-    int own;
-    const long long mine = scan_steps(a, b0, lane, total, own);
-    if (b < b0 + 64) {
-      before += __shfl(mine, b - b0, 64);
-      sb = __shfl(own, b - b0, 64);
-    } else {
-      before += total;
-    }
-  }
-  const long long first = uniform(before) + (long long)inner * sb, last = first + sb - 1;
-  const long long w0 = first / per, w1 = last / per;
-  if (w0 == w1) return;  // (not cut)
-  auto slot_of = [&](long long w) { return 2 * w + (w == w0 && w0 * per != first ? 1 : 0); };  // (a workgroup's second part begins behind its start)
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, per_b = a.Hk * a.row_blocks, row = blockIdx.x;
+  const int s0 = a.meta[2 * blockIdx.y], parts = a.meta[2 * blockIdx.y + 1];
+  const int b = (int)blockIdx.y / per_b, inner = (int)blockIdx.y - b * per_b;
+  const int hk = inner / a.row_blocks, rb = inner - hk * a.row_blocks, r = rb * a.rows + row;
+  if (s0 < 0 || r >= a.G * a.Sq) return;  // (not cut)
+  auto at = [&](int i) { return (long long)(i == 0 ? s0 : (s0 & -a.slots) + a.slots * i) * a.rows + row; };
 
   float m = -INFINITY;
-  for (long long w = w0 + lane; w <= w1; w += 64) m = fmaxf(m, a.part_ml[2 * (slot_of(w) * ROWS + row)]);
+  for (int i = lane; i < parts; i += 64) m = fmaxf(m, a.part_ml[2 * at(i)]);
   m = wave_max(m);
   const float ref = m == -INFINITY ? 0.0f : m;
-  float sum = 0.0f, x[C];
-#pragma unroll
-  for (int c = 0; c < C; ++c) x[c] = 0.0f;
+  float sum = 0.0f;
+  Columns x = {};
 #pragma unroll 4
-  for (long long w = w0 + wave; w <= w1; w += 4) {
-    const long long at = slot_of(w) * ROWS + row;
-    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - ref);
-    sum += f * a.part_ml[2 * at + 1];
-#pragma unroll
-    for (int c = 0; c < C; ++c) x[c] += f * a.part_o[at * DU + lane * C + c];
+  for (int i = wave; i < parts; i += 4) {
+    const long long p = at(i);
+    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * p] - ref);
+    sum += f * a.part_ml[2 * p + 1];
+    x += f * *(const Columns *)(a.part_o + p * DU + lane * C);
   }
-#pragma unroll
-  for (int c = 0; c < C; ++c) s_o[wave][lane * C + c] = x[c];
+  *(Columns *)&s_o[wave][lane * C] = x;
   if (lane == 0) s_l[wave] = sum;
   __syncthreads();
   const int col = threadIdx.x;
   if (col >= a.D) return;
   sum = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
   const int i = query_of(a, r), h = hk * a.G + r - i * a.G;
-  const int lq = a.q_len != nullptr ? min(max(a.q_len[b], 0), a.Sq) : a.Sq;
-  const bool there = r < a.G * lq && sum != 0.0f;
+  const bool there = r < a.G * queries_of(a, b) && sum != 0.0f;
   const float inv = sum > 0.0f ? 1.0f / sum : sum;
   const float y = there ? ((s_o[0][col] + s_o[1][col]) + (s_o[2][col] + s_o[3][col])) * inv : 0.0f;
   ((unsigned short *)a.o.p)[(long long)b * a.o.sb + (long long)h * a.o.sh + (long long)i * a.o.ss + col] = (unsigned short)pack2<DT>(y, 0.0f);
@@ -594,30 +488,35 @@ __global__ void __launch_bounds__(256) attention_cached_join_kernel(const Attent
 }
 
 template <int DT, int DU, int NQ>
-int launch_rows(const AttentionCachedArgs &a, bool e4m3, hipStream_t stream) {
-  const int problems = a.B * a.Hk * a.row_blocks;
-  const dim3 grid((unsigned)(a.workgroups > 0 ? a.workgroups : problems)), block(WAVES * 64);
+void launch_rows(const AttentionCachedArgs &a, bool e4m3, hipStream_t stream) {
+  const dim3 grid((unsigned)(a.workgroups > 0 ? a.workgroups : a.B * a.Hk * a.row_blocks)), block(WAVES * 64);
   const bool full = a.D == DU;
   if (e4m3 && full) hipLaunchKernelGGL((attention_cached_kernel<DT, true, DU, NQ, true>), grid, block, 0, stream, a);
   else if (e4m3) hipLaunchKernelGGL((attention_cached_kernel<DT, true, DU, NQ, false>), grid, block, 0, stream, a);
   else if (full) hipLaunchKernelGGL((attention_cached_kernel<DT, false, DU, NQ, true>), grid, block, 0, stream, a);
   else hipLaunchKernelGGL((attention_cached_kernel<DT, false, DU, NQ, false>), grid, block, 0, stream, a);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.workgroups == 0) return (int)e;
-  const int rows = a.G * a.Sq < 16 * NQ ? a.G * a.Sq : 16 * NQ;
-  hipLaunchKernelGGL((attention_cached_join_kernel<DT, DU, NQ>), dim3((unsigned)rows, (unsigned)problems), dim3(256), 0, stream, a);
-  return (int)hipGetLastError();
 }
-template <int DT>
-int launch_type(const AttentionCachedArgs &a, bool e4m3, hipStream_t stream) {
-  if (a.D <= 64) return a.two ? launch_rows<DT, 64, 2>(a, e4m3, stream) : launch_rows<DT, 64, 1>(a, e4m3, stream);
-  return a.two ? launch_rows<DT, 128, 2>(a, e4m3, stream) : launch_rows<DT, 128, 1>(a, e4m3, stream);
+template <int DT, int DU>
+int launch_width(const AttentionCachedArgs &a, bool e4m3, hipStream_t stream) {
+  hipError_t e;
+  if (a.rows > 32) {
+    e = (hipError_t)launch_attention_cached_tiles(a, DT, e4m3, stream);
+  } else {
+    if (a.rows == 32) launch_rows<DT, DU, 2>(a, e4m3, stream);
+    else launch_rows<DT, DU, 1>(a, e4m3, stream);
+    e = hipGetLastError();
+  }
+  if (e != hipSuccess || a.meta == nullptr) return (int)e;
+  const dim3 grid((unsigned)std::min(a.G * a.Sq, a.rows), (unsigned)(a.B * a.Hk * a.row_blocks));
+  hipLaunchKernelGGL((attention_cached_join_kernel<DT, DU>), grid, dim3(256), 0, stream, a);
+  return (int)hipGetLastError();
 }
 
 }  // namespace
 
 int launch_attention_cached(const AttentionCachedArgs &a, int dtype, bool e4m3, hipStream_t stream) {
-  return dtype == DT_F16 ? launch_type<DT_F16>(a, e4m3, stream) : launch_type<DT_BF16>(a, e4m3, stream);
+  if (a.D <= 64) return dtype == DT_F16 ? launch_width<DT_F16, 64>(a, e4m3, stream) : launch_width<DT_BF16, 64>(a, e4m3, stream);
+  return dtype == DT_F16 ? launch_width<DT_F16, 128>(a, e4m3, stream) : launch_width<DT_BF16, 128>(a, e4m3, stream);
 }
 
 }  // namespace tracea_amd

@@ -88,13 +88,18 @@ struct AttentionCachedArgs {
   float scale_log2;  // magnitude
   int negate, causal;
   int q_vec, o_vec;  // 16-byte pieces
-  int row_blocks;    // blocks of rows of a (batch entry, key/value head)
-  int two;           // blocks of 32 rows, else 16
-  int workgroups;    // 0: one for each block of rows; else the steps of all of them are shared out evenly
-  int least;         // steps of a workgroup, at least
-  float *part_o, *part_ml;  // [2 * workgroups][rows of a block][width], [..][2]
+  int rows;        // of a block: 16 or 32 (waves share the keys), 128 (they share tiles of them)
+  int row_blocks;  // blocks of rows of a (sequence, key/value head)
+  int step, step_log2;  // keys of a workgroup's step
+  int workgroups;  // up to 32 rows; 0: one for each block of rows; else the steps of all of them are shared out evenly
+  int splits;      // 128 rows: parts of a block's steps
+  int least;       // steps of a workgroup, at least
+  int *meta;       // [problems][2]: first slot of its parts or -1, their number; null: no problem is cut
+  int slots;       // from one part to the next: 2 (up to 32 rows) or 1
+  float *part_o, *part_ml;  // [slot][rows][64 or 128], [..][2]
 };
+constexpr int kCachedStep = 128, kCachedTile = 64;
 int launch_attention_cached(const AttentionCachedArgs &a, int dtype, bool e4m3, hipStream_t stream);
-constexpr int kCachedStep = 128;  // keys of a step of a workgroup
+int launch_attention_cached_tiles(const AttentionCachedArgs &a, int dtype, bool e4m3, hipStream_t stream);
 
 }  // namespace tracea_amd

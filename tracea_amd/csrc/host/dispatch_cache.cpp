@@ -498,23 +498,41 @@ TraceaStatus dispatch_attention_cached(const TraceaTensorView &tq, const TraceaT
   a.q_vec = rows_on(q, 16);
   a.o_vec = rows_on(o, 16);
   const long long rows = G * Sq;
-  a.two = rows > 16;
-  const long long block = a.two ? 32 : 16;
-  a.row_blocks = (int)((rows + block - 1) / block);
+  // Blocks of 128 rows share tiles of keys through LDS, blocks of 16 or 32 read them straight into registers.
+  a.rows = rows > 64 ? 128 : rows > 16 ? 32 : 16;
+  const bool tiles = a.rows == 128;
+  a.step = tiles ? kCachedTile : kCachedStep;
+  a.step_log2 = tiles ? 6 : 7;
+  a.row_blocks = (int)((rows + a.rows - 1) / a.rows);
+  a.splits = 1;
   const long long problems = B * Hk * a.row_blocks;
   if (problems >= (1ll << 24)) return fail(TRACEA_UNSUPPORTED_CONFIG, "%s: more workgroups than a launch can have", op);
   DeviceScope scope(device);
   if (scope.err != hipSuccess) return hip_status("hipSetDevice", (int)scope.err);
   hipStream_t stream = (hipStream_t)params.stream;
   std::lock_guard<std::mutex> together(g_launches);
-  const long long wgs = 2 * (long long)device_limits().cus, most = std::max(1ll, ((long long)a.table.M * c.pages.P + kCachedStep - 1) / kCachedStep);
-  a.least = 2;
-  if (problems < 2 * wgs && most > a.least && problems * most < (1ll << 31)) {
-    const size_t n = (size_t)(2 * wgs * block), width = D <= 64 ? 64 : 128;
-    a.part_o = (float *)train_scratch(device, stream, n * (width + 2) * 4);
-    if (a.part_o != nullptr) {  // (else unsplit: slower, the same result to rounding)
+  const long long wgs = 2 * (long long)device_limits().cus, most = std::max(1ll, ((long long)a.table.M * c.pages.P + a.step - 1) / a.step);
+  a.least = tiles ? 4 : 2;
+  long long slots = 0;
+  if (!tiles && problems < 2 * wgs && most > a.least && problems * most < (1ll << 30)) {
+    slots = 2 * wgs;
+    a.slots = 2;
+    a.workgroups = (int)wgs;
+  }
+  if (tiles && problems < wgs && most >= 2 * a.least) {
+    a.splits = (int)std::min({wgs / problems, most / a.least, 32ll});
+    slots = a.splits > 1 ? problems * a.splits : 0;
+    a.slots = 1;
+  }
+  if (slots > 0) {
+    const size_t n = (size_t)(slots * a.rows), width = D <= 64 ? 64 : 128;
+    a.part_o = (float *)train_scratch(device, stream, n * (width + 2) * 4 + (size_t)problems * 8);
+    if (a.part_o != nullptr) {
       a.part_ml = a.part_o + n * width;
-      a.workgroups = (int)wgs;
+      a.meta = (int *)(a.part_ml + 2 * n);
+    } else {  // (slower, the same result to rounding)
+      a.workgroups = 0;
+      a.splits = 1;
     }
   }
   return hip_status("attention over a cache launch", launch_attention_cached(a, q.dtype, c.e4m3, stream));
