@@ -60,10 +60,6 @@ struct Stream {
   static constexpr int KS = DU / 32, VC = DU / 16, ES = C8 ? 1 : 2, ROWS = 16 * NQ;
   static constexpr int KW = 2 * ES, VW = VC * ES / 4;  // registers of 8 columns of a key, of a chunk of a row of values
 
-  // Whether a step's loads have registers of their own beside those of the step before: else K of the next step is requested when the scores
-  // are there, V when its products are done.  Without, the 16-bit form with 32 rows needs more than half of the registers.
-  static constexpr bool DEEP = C8 || NQ == 1 || DU == 64;
-
   struct Keys {  // of a step: 32 keys
     unsigned k[2][KS][KW];
   };
@@ -196,8 +192,8 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attention_cached_kernel(const A
       return x;
     };
 
-    typename S::Keys k_now, k_next;
-    typename S::Values v_now, v_next;
+    typename S::Keys k_now;
+    typename S::Values v_now;
     typename S::Tags tags, tags_next;
     if (steps > 0) {
       (void)locate(0);
@@ -333,34 +329,17 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attention_cached_kernel(const A
       }
     };
 
-    if constexpr (S::DEEP) {
-      auto ahead = [&](int t, typename S::Keys &k, typename S::Values &v) __attribute__((always_inline)) {
-        if (t >= steps) return;
-        locate_ahead(t);
-        request_k(t, k);
-        request_v(t, v);
-        tags_next = tags_of(t);
-      };
-      for (int t = 0; t < steps; t += 2) {
-        ahead(t + 1, k_next, v_next);
-        work(t, k_now, v_now, [] {});
-        tags = tags_next;
-        if (t + 1 >= steps) break;
-        ahead(t + 2, k_now, v_now);
-        work(t + 1, k_next, v_next, [] {});
-        tags = tags_next;
-      }
-    } else {
-      for (int t = 0; t < steps; ++t) {
-        work(t, k_now, v_now, [&]() __attribute__((always_inline)) {
-          if (t + 1 >= steps) return;
-          locate_ahead(t + 1);
-          request_k(t + 1, k_now);
-          tags_next = tags_of(t + 1);
-        });
-        if (t + 1 < steps) request_v(t + 1, v_now);
-        tags = tags_next;
-      }
+    // K of the next step is requested when the scores are there, V when its products are done: registers of their own for the next step's
+    // loads gained nothing (8 x 8192 keys of 8 bits 27.0 us, without 26.0).
+    for (int t = 0; t < steps; ++t) {
+      work(t, k_now, v_now, [&]() __attribute__((always_inline)) {
+        if (t + 1 >= steps) return;
+        locate_ahead(t + 1);
+        request_k(t + 1, k_now);
+        tags_next = tags_of(t + 1);
+      });
+      if (t + 1 < steps) request_v(t + 1, v_now);
+      tags = tags_next;
     }
 
     // the four waves' states meet
@@ -445,18 +424,20 @@ __global__ void __launch_bounds__(WAVES * 64, 2) attention_cached_kernel(const A
   }
 }
 
-// Joins the parts of problems that were cut between workgroups: a workgroup for each row of a problem, its four waves
-// taking the parts in turn.
-template <int DT, int DU>
+// Joins the parts of problems that were cut between workgroups.  Blocks of up to 32 rows have up to a part from every workgroup: a workgroup
+// for each row of a problem, its four waves taking the parts in turn (TOGETHER).  Blocks of 128 rows have few parts and many rows: a wave
+// for each.  Bound by the latency of three loads one after another, 3.5 us for 64 rows of some parts; 128 problems of 128 rows in two parts TODO us.
+template <int DT, int DU, bool TOGETHER>
 __global__ void __launch_bounds__(256) attention_cached_join_kernel(const AttentionCachedArgs a) {
   constexpr int C = DU / 64;
   typedef float Columns __attribute__((ext_vector_type(C)));
   __shared__ float s_o[4][DU], s_l[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, per_b = a.Hk * a.row_blocks, row = blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), per_b = a.Hk * a.row_blocks;
+  const int row = TOGETHER ? (int)blockIdx.x : (int)blockIdx.x * 4 + wave;
   const int s0 = a.meta[2 * blockIdx.y], parts = a.meta[2 * blockIdx.y + 1];
   const int b = (int)blockIdx.y / per_b, inner = (int)blockIdx.y - b * per_b;
   const int hk = inner / a.row_blocks, rb = inner - hk * a.row_blocks, r = rb * a.rows + row;
-  if (s0 < 0 || r >= a.G * a.Sq) return;  // (not cut)
+  if (s0 < 0 || r >= a.G * a.Sq) return;  // (not cut; a workgroup whose waves share a row leaves as a whole)
   auto at = [&](int i) { return (long long)(i == 0 ? s0 : (s0 & -a.slots) + a.slots * i) * a.rows + row; };
 
   float m = -INFINITY;
@@ -466,24 +447,30 @@ __global__ void __launch_bounds__(256) attention_cached_join_kernel(const Attent
   float sum = 0.0f;
   Columns x = {};
 #pragma unroll 4
-  for (int i = wave; i < parts; i += 4) {
+  for (int i = TOGETHER ? wave : 0; i < parts; i += TOGETHER ? 4 : 1) {
     const long long p = at(i);
     const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * p] - ref);
     sum += f * a.part_ml[2 * p + 1];
-    x += f * *(const Columns *)(a.part_o + p * DU + lane * C);
+    x += f * *(const Columns *)(a.part_o + p * DU + lane * C);  // (columns from D on are never written, nor used)
   }
-  *(Columns *)&s_o[wave][lane * C] = x;
-  if (lane == 0) s_l[wave] = sum;
-  __syncthreads();
-  const int col = threadIdx.x;
-  if (col >= a.D) return;
-  sum = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
+  if constexpr (TOGETHER) {
+    *(Columns *)&s_o[wave][lane * C] = x;
+    if (lane == 0) s_l[wave] = sum;
+    __syncthreads();
+    if (wave != 0) return;
+    sum = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
+    x = Columns{};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) x += *(const Columns *)&s_o[w][lane * C];
+  }
   const int i = query_of(a, r), h = hk * a.G + r - i * a.G;
   const bool there = r < a.G * queries_of(a, b) && sum != 0.0f;
-  const float inv = sum > 0.0f ? 1.0f / sum : sum;
-  const float y = there ? ((s_o[0][col] + s_o[1][col]) + (s_o[2][col] + s_o[3][col])) * inv : 0.0f;
-  ((unsigned short *)a.o.p)[(long long)b * a.o.sb + (long long)h * a.o.sh + (long long)i * a.o.ss + col] = (unsigned short)pack2<DT>(y, 0.0f);
-  if (col == 0 && a.lse != nullptr)
+  const float inv = sum > 0.0f ? 1.0f / sum : sum;  // (NaN stays)
+  unsigned short *o = (unsigned short *)a.o.p + (long long)b * a.o.sb + (long long)h * a.o.sh + (long long)i * a.o.ss;
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+    if (lane * C + c < a.D) o[lane * C + c] = there ? (unsigned short)pack2<DT>(x[c] * inv, 0.0f) : (unsigned short)0;
+  if (lane == 0 && a.lse != nullptr)
     a.lse[(long long)b * a.lse_sb + (long long)h * a.lse_sh + (long long)i * a.lse_ss] = there ? (m + __builtin_amdgcn_logf(sum)) * LN2 : -INFINITY;
 }
 
@@ -507,8 +494,9 @@ int launch_width(const AttentionCachedArgs &a, bool e4m3, hipStream_t stream) {
     e = hipGetLastError();
   }
   if (e != hipSuccess || a.meta == nullptr) return (int)e;
-  const dim3 grid((unsigned)std::min(a.G * a.Sq, a.rows), (unsigned)(a.B * a.Hk * a.row_blocks));
-  hipLaunchKernelGGL((attention_cached_join_kernel<DT, DU>), grid, dim3(256), 0, stream, a);
+  const unsigned rows = (unsigned)std::min(a.G * a.Sq, a.rows), problems = (unsigned)(a.B * a.Hk * a.row_blocks);
+  if (a.rows <= 32) hipLaunchKernelGGL((attention_cached_join_kernel<DT, DU, true>), dim3(rows, problems), dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((attention_cached_join_kernel<DT, DU, false>), dim3((rows + 3) / 4, problems), dim3(256), 0, stream, a);
   return (int)hipGetLastError();
 }
 

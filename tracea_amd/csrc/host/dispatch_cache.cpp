@@ -157,6 +157,35 @@ TraceaStatus read_cache(const char *op, const TraceaTensorView &tk, const Tracea
   return TRACEA_SUCCESS;
 }
 
+// Whether few problems (blocks of up to 32 rows) of up to `most` steps share their steps out.  Unshared, a workgroup walks its problem at 0.74
+// to 1.1 us a step until the cache's bytes bound it; shared, the line is worked out and parts are joined by a second launch, 4.4 us more.  us
+// unshared / shared, one query, Hk 8, D128 e4m3: B1 512 keys 8.8 / 10.9, 1024 11.7 / 10.8, 4096 29.5 / 11.0; B16 1024 15.1 / 15.6, 4096 39.6 / 29.9;
+// B48 512 14.5 / 21.2, 4096 85 / 91 (lengths alike; of unlike lengths the shares gain: 0.9).
+bool shares_pay(long long problems, long long most, bool e4m3, double width, int rows) {
+  if (most <= 2 || problems * most >= (1ll << 30) || problems > 65535) return false;
+  const double bytes = (e4m3 ? 6.2e-3 : 12.4e-3) * width * problems, step = (rows > 16 ? 1.1 : 1.0) * (e4m3 ? 1.0 : 1.1);
+  return 6.0 + most * std::max(step, bytes) > 10.4 + 0.9 * most * bytes;
+}
+
+// Parts of the steps (tiles of 64 keys) of blocks of 128 rows, by the least of this estimate (us).  A workgroup alone on its CU takes 1.8 us a
+// tile, two 2.5 each; parts cost a launch that joins them and their way through memory, 66 KB each.  us, one part / best, 8 heads, D128
+// e4m3: B1 32 queries over 8192 keys 251 / 31 (32 parts), B4 128 queries over 4096 132 / 63 (4), over 512 24 / 24 (1), B16 32 over 2048 74 / 46 (4).
+int plan_tiles(long long problems, long long most, bool e4m3, double width, long long cus) {
+  int best = 1;
+  double least = 1e300;
+  for (int parts : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+    if (parts > 1 && (parts > most || problems * parts > 4 * cus || problems > 65535)) break;
+    const double n = (double)(problems * parts), walk = (double)((most + parts - 1) / parts);
+    const double tile = (e4m3 ? 1.0 : 0.85) * (0.3 + 0.7 * width) * std::max(1.8, n > cus ? 2.5 * std::ceil(n / (2.0 * cus)) : 0.0);
+    const double time = walk * tile + (parts > 1 ? 4.5 + 0.035 * width * n : 0.0);
+    if (time < least) {
+      least = time;
+      best = parts;
+    }
+  }
+  return best;
+}
+
 }  // namespace
 
 // ---- norms of heads with rotary positions ---------------------------------------------------------------------
@@ -511,18 +540,19 @@ TraceaStatus dispatch_attention_cached(const TraceaTensorView &tq, const TraceaT
   if (scope.err != hipSuccess) return hip_status("hipSetDevice", (int)scope.err);
   hipStream_t stream = (hipStream_t)params.stream;
   std::lock_guard<std::mutex> together(g_launches);
-  const long long wgs = 2 * (long long)device_limits().cus, most = std::max(1ll, ((long long)a.table.M * c.pages.P + a.step - 1) / a.step);
-  a.least = tiles ? 4 : 2;
+  const long long cus = (long long)device_limits().cus, most = std::max(1ll, ((long long)a.table.M * c.pages.P + a.step - 1) / a.step);
+  const double width_of = D <= 64 ? 0.5 : 1.0;
   long long slots = 0;
-  if (!tiles && problems < 2 * wgs && most > a.least && problems * most < (1ll << 30)) {
-    slots = 2 * wgs;
-    a.slots = 2;
-    a.workgroups = (int)wgs;
-  }
-  if (tiles && problems < wgs && most >= 2 * a.least) {
-    a.splits = (int)std::min({wgs / problems, most / a.least, 32ll});
+  a.least = tiles ? 1 : 2;
+  a.slots = tiles ? 1 : 2;
+  if (tiles) {
+    a.splits = plan_tiles(problems, most, c.e4m3, width_of, cus);
     slots = a.splits > 1 ? problems * a.splits : 0;
-    a.slots = 1;
+  } else if (shares_pay(problems, most, c.e4m3, width_of, a.rows)) {
+    // One workgroup a CU leaves half the parts of two: 8 x 8192 keys of 8 bits 26.0 / 27.0 us, of 16 bits 40.0 / 40.7; of 64 columns, with half
+    // as much in flight, 21.4 / 20.0.
+    a.workgroups = (int)(D <= 64 ? 2 * cus : cus);
+    slots = 2 * a.workgroups;
   }
   if (slots > 0) {
     const size_t n = (size_t)(slots * a.rows), width = D <= 64 ? 64 : 128;
