@@ -68,8 +68,10 @@ struct CacheAppendArgs {
   int first[TRACEA_MAX_ROTARY_AXES];
   int adjacent;
   int vec;           // pieces of 8 elements
+  int near;          // offsets between the tokens of a page are 31-bit
   int pages;         // that the T tokens of a sequence can touch
-  int groups;        // of key/value heads, each with as large a part of the query heads
+  int groups;        // of heads
+  int heads, queries;  // key/value and query heads of a group
 };
 constexpr int kAppendHeads = 64;  // key/value heads of a workgroup, at most
 int launch_cache_append(const CacheAppendArgs &a, int dtype, hipStream_t stream);

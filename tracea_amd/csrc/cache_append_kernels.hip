@@ -10,6 +10,8 @@
 // A workgroup has the tokens of one sequence that fall into one page, for some of the heads: no other writes that page and head, so that scales
 // need no atomics across workgroups.  Sines and cosines of its tokens are kept in LDS for its heads.  In 8 bits it reads its
 // operands twice, for the largest value and for the codes; the second time they come from the caches.
+#include <type_traits>
+
 #include "cache.hpp"
 #include "contraction_kernel.hpp"
 #include "rotation.hpp"
@@ -29,31 +31,45 @@ struct alignas(E) Codes {
   unsigned char x[E];
 };
 
-__device__ __forceinline__ float coded(float x, float inv) {  // an infinity becomes NaN: e4m3 has none
-  return __builtin_isfinite(x) ? x * inv : __builtin_nanf("");
-}
 // The least power of two by which `largest` (finite) is at most 448 = 1.75 2^8, at least 2^-126.
 __device__ __forceinline__ float scale_for(float largest) {
   const unsigned bits = __builtin_bit_cast(unsigned, largest);
   const int e = (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u);
   return __builtin_bit_cast(float, (unsigned)(e < 1 ? 1 : e) << 23);
 }
-// e4m3 codes of two values up to 448, rounded to nearest, ties to even
+// e4m3 codes of two values up to 448, rounded to nearest, ties to even; infinities and NaN become NaN
 __device__ __forceinline__ unsigned encode2(float a, float b) { return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false) & 0xffffu; }
 template <int E>
 __device__ __forceinline__ Codes<E> encode(const float (&x)[E], float inv) {
   Codes<E> c;
   if constexpr (E == 1) {
-    c.x[0] = (unsigned char)encode2(coded(x[0], inv), 0.0f);
+    c.x[0] = (unsigned char)encode2(x[0] * inv, 0.0f);
   } else {
 #pragma unroll
     for (int e = 0; e < E; e += 2) {
-      const unsigned two = encode2(coded(x[e], inv), coded(x[e + 1], inv));
+      const unsigned two = encode2(x[e] * inv, x[e + 1] * inv);
       c.x[e] = (unsigned char)two;
       c.x[e + 1] = (unsigned char)(two >> 8);
     }
   }
   return c;
+}
+
+// Codes of `rows` rows of a head of a page, times f (a power of two below 1), by the first threads of a workgroup.
+__device__ __forceinline__ void rescale(unsigned char *head, long long apart, int rows, int D, float f, int threads) {
+  for (int i = threadIdx.x; i < rows * (D / 8); i += threads) {
+    const int row = i / (D / 8), at = (i - row * (D / 8)) * 8;
+    u32x2 *p = (u32x2 *)(head + row * apart + at);
+    const u32x2 x = *p;
+    u32x2 y;
+#pragma unroll
+    for (int d = 0; d < 2; ++d) {
+      const unsigned lo = encode2(__builtin_amdgcn_cvt_f32_fp8((int)x[d], 0) * f, __builtin_amdgcn_cvt_f32_fp8((int)x[d], 1) * f);
+      const unsigned hi = encode2(__builtin_amdgcn_cvt_f32_fp8((int)x[d], 2) * f, __builtin_amdgcn_cvt_f32_fp8((int)x[d], 3) * f);
+      y[d] = lo | hi << 16;
+    }
+    *p = y;
+  }
 }
 
 template <typename T, bool C8, int E, bool ADJ>
@@ -64,11 +80,10 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const CacheAppendArgs
   const int b = blockIdx.y, j = (int)blockIdx.x / a.groups, grp = (int)blockIdx.x - j * a.groups, PT = a.table.P;
   const long long start = a.starts[b] > 0 ? a.starts[b] : 0;
   const int n = a.lengths != nullptr ? min(max(a.lengths[b], 0), a.T) : a.T;
-  const long long slot = start / PT + j, base = slot * PT - start;  // of the page, in new tokens
+  const long long slot = (unsigned)start / (unsigned)PT + j, base = slot * PT - start;  // of the page, in new tokens
   const int lo = base > 0 ? (int)min(base, (long long)a.T) : 0, hi = (int)min(base + PT, (long long)a.T), end = min(hi, n);  // (from `end` on: queries' zeros)
   if (lo >= hi) return;
-  const int h0 = (int)((long long)a.Hk * grp / a.groups), h1 = (int)((long long)a.Hk * (grp + 1) / a.groups);
-  const int q0 = (int)((long long)a.Hq * grp / a.groups), q1 = (int)((long long)a.Hq * (grp + 1) / a.groups);
+  const int h0 = min(a.Hk, grp * a.heads), h1 = min(a.Hk, h0 + a.heads), q0 = min(a.Hq, grp * a.queries), q1 = min(a.Hq, q0 + a.queries);
   const int page = page_of(a.table, b, slot);
   const bool there = page >= 0 && end > lo;
   const int heads = h1 - h0;
@@ -142,23 +157,34 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const CacheAppendArgs
       const int to = min(end, from + chunk);
       __syncthreads();
       angles(from, to);
-      for (int i = threadIdx.x; i < heads * (to - from) * pieces; i += 256) {
-        const int row = i / pieces, piece = i - row * pieces, h = row / (to - from), t = from + row - h * (to - from);
-        int at_u, at_v;
-        float u[E], v[E];
-        columns(piece, at_u, at_v);
-      turned((const T *)a.k.p + b * a.k.sb + (h0 + h) * a.k.sh + t * a.k.ss, (t - from) * a.P + piece * E, at_u, at_v, u, v);
-        float top = largest(u, 0.0f);
-        if (at_v >= 0) top = largest(v, top);
-        atomicMax(&s_max[0][h], __builtin_bit_cast(unsigned, top));
-      }
-      for (int i = threadIdx.x; i < heads * (to - from) * all; i += 256) {
-        const int row = i / all, piece = i - row * all, h = row / (to - from), t = from + row - h * (to - from);
-        const Piece<T, E> x = *(const Piece<T, E> *)((const T *)a.v.p + b * a.v.sb + (h0 + h) * a.v.sh + t * a.v.ss + piece * E);
-        float u[E];
+      for (int h = 0; h < heads; ++h) {
+        float k_top = 0.0f, v_top = 0.0f;
+        for (int i = threadIdx.x; i < (to - from) * pieces; i += 256) {
+          const int row = i / pieces, piece = i - row * pieces, t = from + row;
+          int at_u, at_v;
+          float u[E], v[E];
+          columns(piece, at_u, at_v);
+          turned((const T *)a.k.p + b * a.k.sb + (h0 + h) * a.k.sh + t * a.k.ss, row * a.P + piece * E, at_u, at_v, u, v);
+          k_top = largest(u, k_top);
+          if (at_v >= 0) k_top = largest(v, k_top);
+        }
+        for (int i = threadIdx.x; i < (to - from) * all; i += 256) {
+          const int row = i / all, piece = i - row * all, t = from + row;
+          const Piece<T, E> x = *(const Piece<T, E> *)((const T *)a.v.p + b * a.v.sb + (h0 + h) * a.v.sh + t * a.v.ss + piece * E);
+          float u[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) u[e] = (float)x.x[e];
-        atomicMax(&s_max[1][h], __builtin_bit_cast(unsigned, largest(u, 0.0f)));
+          for (int e = 0; e < E; ++e) u[e] = (float)x.x[e];
+          v_top = largest(u, v_top);
+        }
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) {
+          k_top = fmaxf(k_top, __shfl_xor(k_top, m, 64));
+          v_top = fmaxf(v_top, __shfl_xor(v_top, m, 64));
+        }
+        if ((threadIdx.x & 63) == 0) {  // (magnitudes compare as their bits do)
+          atomicMax(&s_max[0][h], __builtin_bit_cast(unsigned, k_top));
+          atomicMax(&s_max[1][h], __builtin_bit_cast(unsigned, v_top));
+        }
       }
     }
     __syncthreads();
@@ -178,21 +204,8 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const CacheAppendArgs
         for (int h = 0; h < heads; ++h) {
           const float f = s_move[w][h];
           if (f == 1.0f) continue;
-          unsigned char *rows = w == 0 ? a.kc.p + page * a.kc.sn + (h0 + h) * a.kc.sh : a.vc.p + page * a.vc.sn + (h0 + h) * a.vc.sh;
-          const long long apart = w == 0 ? a.kc.ss : a.vc.ss;
-          for (int i = threadIdx.x; i < older * (a.D / 8); i += 256) {
-            const int row = i / (a.D / 8), at = (i - row * (a.D / 8)) * 8;
-            u32x2 *p = (u32x2 *)(rows + row * apart + at);
-            const u32x2 x = *p;
-            u32x2 y;
-#pragma unroll
-            for (int d = 0; d < 2; ++d) {
-              const unsigned lo2 = encode2(__builtin_amdgcn_cvt_f32_fp8((int)x[d], 0) * f, __builtin_amdgcn_cvt_f32_fp8((int)x[d], 1) * f);
-              const unsigned hi2 = encode2(__builtin_amdgcn_cvt_f32_fp8((int)x[d], 2) * f, __builtin_amdgcn_cvt_f32_fp8((int)x[d], 3) * f);
-              y[d] = lo2 | hi2 << 16;
-            }
-            *p = y;
-          }
+          if (w == 0) rescale(a.kc.p + page * a.kc.sn + (h0 + h) * a.kc.sh, a.kc.ss, older, a.D, f, 256);
+          else rescale(a.vc.p + page * a.vc.sn + (h0 + h) * a.vc.sh, a.vc.ss, older, a.D, f, 256);
         }
   }
 
@@ -245,9 +258,292 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const CacheAppendArgs
   }
 }
 
+// The same where a workgroup's tokens are few enough for their angles to be kept all at once and their operands in registers between the largest value
+// and the codes: every byte is read once.  Pieces of 8 columns only.  Half of the workgroup's threads, SIDE, have the keys and values, the
+// other half the queries, so that neither waits behind the other's loads.  A thread has up to HK pieces of a head's keys, 2 HK of its values.
+
+template <typename T, bool C8, bool ADJ, int SIDE, int HK>
+__global__ void __launch_bounds__(2 * SIDE) __attribute__((amdgpu_waves_per_eu(4))) cache_append_held_kernel(const CacheAppendArgs a) {
+  constexpr int WAVES = SIDE / 64, HV = 2 * HK, PAIRS = SIDE * HK * 8;
+  typedef float f4 __attribute__((ext_vector_type(4)));
+  __shared__ f4 s_cos[PAIRS / 4], s_sin[PAIRS / 4];
+  __shared__ float s_max[2][2][WAVES];
+  const int b = blockIdx.y, j = (int)blockIdx.x / a.groups, grp = (int)blockIdx.x - j * a.groups, PT = a.table.P;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, id = threadIdx.x & (SIDE - 1);
+  const bool of_keys = __builtin_amdgcn_readfirstlane((int)threadIdx.x) < SIDE;
+  const long long start = a.starts[b] > 0 ? a.starts[b] : 0;
+  const int n = a.lengths != nullptr ? min(max(a.lengths[b], 0), a.T) : a.T;
+  const long long slot = (unsigned)start / (unsigned)PT + j, base = slot * PT - start;  // of the page, in new tokens
+  const int lo = base > 0 ? (int)min(base, (long long)a.T) : 0, hi = (int)min(base + PT, (long long)a.T), end = min(hi, n);  // (from `end` on: queries' zeros)
+  if (lo >= hi) return;
+  const int h0 = min(a.Hk, grp * a.heads), h1 = min(a.Hk, h0 + a.heads), q0 = min(a.Hq, grp * a.queries), q1 = min(a.Hq, q0 + a.queries);
+  const int page = page_of(a.table, b, slot);
+  const int tokens = page >= 0 && end > lo ? end - lo : 0;  // with a place
+  const int turned_pieces = a.P / 8, pieces = (a.D + 8) / 16, all = a.D / 8;
+
+  // A thread's pieces are the same in every head: token (from lo) and two times 8 columns, partners that are turned by the angles from
+  // `angle` on, or columns side by side that are not (angle < 0; v < 0: there is no second).
+  struct Couple {
+    int t, u, v, angle;
+  };
+  // (worked out where they are used, a few instructions: kept for a loop over heads they would fill the registers)
+  const unsigned by_pieces = 0xffffffffu / (unsigned)pieces + 1, by_all = 0xffffffffu / (unsigned)all + 1;  // 0: divided by 1
+  auto place_in = [&](int s, unsigned magic, int per, int &t, int &piece) __attribute__((always_inline)) {
+    unsigned i = (unsigned)id;
+    asm volatile("" : "+v"(i));
+    i += (unsigned)(s * SIDE);
+    t = magic == 0 ? (int)i : (int)__umulhi(i, magic);
+    piece = (int)i - t * per;
+  };
+  auto couple = [&](int s) __attribute__((always_inline)) {
+    Couple p;
+    int piece;
+    place_in(s, by_pieces, pieces, p.t, piece);
+    const bool pair = piece < turned_pieces;
+    p.u = !pair ? 2 * a.P + (piece - turned_pieces) * 16 : ADJ ? 16 * piece : 8 * piece;
+    p.v = pair && !ADJ ? p.u + a.P : p.u + 8 < a.D ? p.u + 8 : -1;
+    p.angle = pair ? (p.t * a.P + piece * 8) / 4 : -1;
+    return p;
+  };
+  using X = Piece<T, 8>;
+  // What a thread holds: couples of keys, then pieces of values; or couples of two heads' queries.
+  u32x4 held[4 * HK];
+  // The compiler takes them for new values: it would keep all of them widened and turned from the largest value to the codes.
+  auto anew = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4 * HK; ++i) asm volatile("" : "+v"(held[i]));
+  };
+  auto piece_of = [&](int i) { return __builtin_bit_cast(X, held[i]); };
+  auto load_row = [&](const HeadView &x, int h, int count, auto first) __attribute__((always_inline)) {
+    const char *at = (const char *)((const T *)x.p + b * x.sb + h * x.sh + lo * x.ss);
+#pragma unroll
+    for (int s = 0; s < HK; ++s) {
+      const Couple p = couple(s);
+      if (p.t >= count) continue;
+      const unsigned row = (unsigned)p.t * (unsigned)x.ss;
+      held[first() + s] = *(const u32x4 *)(at + (row + (unsigned)p.u) * 2);
+      held[first() + HK + s] = *(const u32x4 *)(at + (row + (unsigned)(p.v < 0 ? p.u : p.v)) * 2);
+    }
+  };
+  auto turned = [&](const Couple &p, const X &x, const X &y, float (&u)[8], float (&v)[8]) __attribute__((always_inline)) {
+    const bool pair = p.angle >= 0;
+    const int angle = pair ? p.angle : 0;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const f4 c = s_cos[angle + half], sn = s_sin[angle + half];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int e = half * 4 + i;
+        const float f = (float)(!ADJ ? x.x[e] : half == 0 ? x.x[2 * i] : y.x[2 * i]), g = (float)(!ADJ ? y.x[e] : half == 0 ? x.x[2 * i + 1] : y.x[2 * i + 1]);
+        const float first = pair ? f * c[i] - g * sn[i] : f, second = pair ? g * c[i] + f * sn[i] : g;
+        if constexpr (!ADJ) {
+          u[e] = first;
+          v[e] = second;
+        } else if (half == 0) {
+          u[2 * i] = first;
+          u[2 * i + 1] = second;
+        } else {
+          v[2 * i] = first;
+          v[2 * i + 1] = second;
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // ... of any value but NaN; a head that has an infinity is looked through again for its finite ones
+  auto largest = [](const float (&x)[8], float top, bool finite) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float y = fabsf(x[e]);
+      top = fmaxf(top, finite && !(y < INFINITY) ? 0.0f : y);
+    }
+    return top;
+  };
+  auto store16 = [](void *at, const float (&x)[8]) __attribute__((always_inline)) {
+    X y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y.x[e] = (T)x[e];
+    *(X *)at = y;
+  };
+  auto wide = [](const X &x, float (&y)[8]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = (float)x.x[e];
+  };
+
+  float k_old = 0.0f, v_old = 0.0f;
+  auto load_head = [&](int h) __attribute__((always_inline)) {
+    load_row(a.k, h, tokens, std::integral_constant<int, 0>{});
+    const char *at = (const char *)((const T *)a.v.p + b * a.v.sb + h * a.v.sh + lo * a.v.ss);
+#pragma unroll
+    for (int s = 0; s < HV; ++s) {
+      int t, piece;
+      place_in(s, by_all, all, t, piece);
+      if (t < tokens) held[2 * HK + s] = *(const u32x4 *)(at + ((unsigned)t * (unsigned)a.v.ss + (unsigned)piece * 8) * 2);
+    }
+    if (C8 && tokens > 0 && base < 0) {
+      k_old = a.ks.p[page * a.ks.sn + h * a.ks.sh];
+      v_old = a.vs.p[page * a.vs.sn + h * a.vs.sh];
+    }
+  };
+  auto load_queries = [&](int h) __attribute__((always_inline)) {
+    load_row(a.q, h, hi - lo, std::integral_constant<int, 0>{});
+    if (h + 1 < q1) load_row(a.q, h + 1, hi - lo, std::integral_constant<int, 2 * HK>{});
+  };
+  // (on their way while the angles are worked out)
+  if (of_keys && h0 < h1) load_head(h0);
+  if (!of_keys && q0 < q1) load_queries(q0);
+#pragma unroll 1
+  for (int i = threadIdx.x; i < (hi - lo) * a.P; i += 2 * SIDE) {
+    const int t = i / a.P, p = i - t * a.P;
+    int axis = 0;
+    for (int x = 1; x < a.axes; ++x) axis += p >= a.first[x];
+    const int position = a.positions != nullptr ? a.positions[b * a.pos_sb + (lo + t) * a.pos_ss + axis] : (int)(start + lo + t);
+    float c, s;
+    turn(position, a.inv_freq[p], 1.0f, c, s);
+    ((float *)s_cos)[i] = c;
+    ((float *)s_sin)[i] = s;
+  }
+  __syncthreads();
+
+  if (!of_keys) {
+    for (int h = q0; h < q1; h += 2) {
+      if (h > q0) load_queries(h);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (h + i >= q1) continue;
+        char *at = (char *)((T *)a.q_out.p + b * a.q_out.sb + (h + i) * a.q_out.sh + lo * a.q_out.ss);
+#pragma unroll
+        for (int s = 0; s < HK; ++s) {
+          const Couple p = couple(s);
+          if (p.t >= hi - lo) continue;
+          float u[8], v[8];
+          turned(p, piece_of(2 * HK * i + s), piece_of(2 * HK * i + HK + s), u, v);
+          if (lo + p.t >= n) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) u[e] = v[e] = 0.0f;
+          }
+          const unsigned row = (unsigned)p.t * (unsigned)a.q_out.ss;
+          store16(at + (row + (unsigned)p.u) * 2, u);
+          if (p.v >= 0) store16(at + (row + (unsigned)p.v) * 2, v);
+        }
+      }
+    }
+    if (C8 && tokens > 0)
+      for (int h = h0; h < h1; ++h) __syncthreads();  // (those of the other half)
+    return;
+  }
+  for (int h = h0; h < h1 && tokens > 0; ++h) {
+    if (h > h0) load_head(h);
+    // of the page, and of token lo in it
+    unsigned char *k_page = a.kc.p + page * a.kc.sn + h * a.kc.sh, *v_page = a.vc.p + page * a.vc.sn + h * a.vc.sh;
+    unsigned char *k_rows = k_page + (lo - base) * a.kc.ss, *v_rows = v_page + (lo - base) * a.vc.ss;
+    float k_inv = 1.0f, v_inv = 1.0f;
+    if constexpr (C8) {
+      float k_top, v_top;
+      auto tops_of = [&](bool finite) __attribute__((always_inline)) {
+        k_top = v_top = 0.0f;
+#pragma unroll
+        for (int s = 0; s < HK; ++s) {
+          const Couple p = couple(s);
+          if (p.t >= tokens) continue;
+          float u[8], v[8];
+          turned(p, piece_of(s), piece_of(HK + s), u, v);
+          k_top = largest(u, k_top, finite);
+          if (p.v >= 0) k_top = largest(v, k_top, finite);
+        }
+#pragma unroll
+        for (int s = 0; s < HV; ++s) {
+          int t, piece;
+          place_in(s, by_all, all, t, piece);
+          if (t >= tokens) continue;
+          float u[8];
+          wide(piece_of(2 * HK + s), u);
+          v_top = largest(u, v_top, finite);
+        }
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) {
+          k_top = fmaxf(k_top, __shfl_xor(k_top, m, 64));
+          v_top = fmaxf(v_top, __shfl_xor(v_top, m, 64));
+        }
+      };
+      tops_of(false);
+      if (__builtin_amdgcn_readfirstlane((int)(k_top == INFINITY || v_top == INFINITY))) {
+        anew();
+        tops_of(true);
+      }
+      anew();
+      float(&tops)[2][WAVES] = s_max[h & 1];
+      if (lane == 0) {
+        tops[0][wave] = k_top;
+        tops[1][wave] = v_top;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        k_top = fmaxf(k_top, tops[0][w]);
+        v_top = fmaxf(v_top, tops[1][w]);
+      }
+      const float k_now = fmaxf(k_old, scale_for(k_top)), v_now = fmaxf(v_old, scale_for(v_top));
+      if (threadIdx.x == 0) {
+        a.ks.p[page * a.ks.sn + h * a.ks.sh] = k_now;
+        a.vs.p[page * a.vs.sn + h * a.vs.sh] = v_now;
+      }
+      k_inv = 1.0f / k_now;
+      v_inv = 1.0f / v_now;
+      // older codes of the page, where the scale has grown
+      if (base < 0 && k_now > k_old) rescale(k_page, a.kc.ss, (int)-base, a.D, k_old / k_now, SIDE);
+      if (base < 0 && v_now > v_old) rescale(v_page, a.vc.ss, (int)-base, a.D, v_old / v_now, SIDE);
+    }
+#pragma unroll
+    for (int s = 0; s < HK; ++s) {
+      const Couple p = couple(s);
+      if (p.t >= tokens) continue;
+      float u[8], v[8];
+      turned(p, piece_of(s), piece_of(HK + s), u, v);
+      unsigned char *row = k_rows + (unsigned)p.t * (unsigned)a.kc.ss;
+      if constexpr (C8) {
+        *(Codes<8> *)(row + p.u) = encode<8>(u, k_inv);
+        if (p.v >= 0) *(Codes<8> *)(row + p.v) = encode<8>(v, k_inv);
+      } else {
+        store16(row + p.u * 2, u);
+        if (p.v >= 0) store16(row + p.v * 2, v);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < HV; ++s) {
+      int t, piece;
+      place_in(s, by_all, all, t, piece);
+      if (t >= tokens) continue;
+      unsigned char *row = v_rows + ((unsigned)t * (unsigned)a.vc.ss + (unsigned)piece * (C8 ? 8 : 16));
+      if constexpr (C8) {
+        float u[8];
+        wide(piece_of(2 * HK + s), u);
+        *(Codes<8> *)row = encode<8>(u, v_inv);
+      } else {
+        *(u32x4 *)row = held[2 * HK + s];
+      }
+    }
+  }
+}
+
 template <typename T, bool C8>
 int launch(const CacheAppendArgs &a, hipStream_t stream) {
   const dim3 grid((unsigned)(a.pages * a.groups), (unsigned)a.B);
+  const int tokens = a.T < a.table.P ? a.T : a.table.P, pieces = (a.D + 8) / 16;
+  auto holds = [&](int side, int held) {
+    return a.vec && a.near && tokens * a.P <= side * held * 8 && tokens * pieces <= side * held && tokens * (a.D / 8) <= 2 * side * held;
+  };
+#define HELD(SIDE, HK)                                                                                                                     \
+  if (holds(SIDE, HK)) {                                                                                                                   \
+    if (a.adjacent) hipLaunchKernelGGL((cache_append_held_kernel<T, C8, true, SIDE, HK>), grid, dim3(2 * SIDE), 0, stream, a);             \
+    else hipLaunchKernelGGL((cache_append_held_kernel<T, C8, false, SIDE, HK>), grid, dim3(2 * SIDE), 0, stream, a);                       \
+    return (int)hipGetLastError();                                                                                                         \
+  }
+  HELD(64, 2)
+  HELD(128, 2)
+  HELD(256, 2)
+  HELD(512, 2)
+#undef HELD
   if (a.vec && a.adjacent) hipLaunchKernelGGL((cache_append_kernel<T, C8, 8, true>), grid, dim3(256), 0, stream, a);
   else if (a.vec) hipLaunchKernelGGL((cache_append_kernel<T, C8, 8, false>), grid, dim3(256), 0, stream, a);
   else if (a.adjacent) hipLaunchKernelGGL((cache_append_kernel<T, C8, 1, true>), grid, dim3(256), 0, stream, a);

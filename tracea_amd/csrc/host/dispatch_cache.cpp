@@ -443,15 +443,25 @@ TraceaStatus dispatch_cache_append(const TraceaTensorView &tk, const TraceaTenso
   a.adjacent = params.adjacent != 0;
   a.vec = a.P % 8 == 0;
   for (const View *t : operands) a.vec = a.vec && rows_on(*t, 16);
+  a.near = 1;
+  for (const View *t : operands) a.near = a.near && t->stride[2] >= 0 && (t->stride[2] * std::min(T, (long long)c.pages.P) + D) * 2 < (1ll << 31);
+  for (const View *t : {&c.k, &c.v}) a.near = a.near && (t->stride[2] * c.pages.P + D) * 2 < (1ll << 31);
   const long long pages = (T + c.pages.P - 2) / c.pages.P + 1;
   if (B > 65535 || pages >= (1 << 22)) return fail(TRACEA_UNSUPPORTED_CONFIG, "%s: %lld sequences of %lld new tokens are more than is supported", op, B, T);
   a.pages = (int)pages;
   DeviceScope scope(device);
   if (scope.err != hipSuccess) return hip_status("hipSetDevice", (int)scope.err);
-  // Workgroups for the heads of a page: the angles of a token are worked out once for the heads of a workgroup, and few pages leave CUs idle.
-  const long long cus = (long long)device_limits().cus, heads = std::max(1ll, Hk);
-  a.groups = (int)std::min(heads, std::max((heads + kAppendHeads - 1) / kAppendHeads, 8 * cus / (B * pages)));
-  if (pages * a.groups >= (1ll << 22)) return fail(TRACEA_UNSUPPORTED_CONFIG, "%s: %lld heads of %lld new tokens are more than is supported", op, Hk, T);
+  // Workgroups for the heads of a page: a token's angles are worked out once for the heads of a workgroup, and a CU wants four with 64 tokens of
+  // 128 columns, more of smaller ones.  Two prompts of 4096 tokens in pages of 64, workgroups for 8 / 4 / 2 heads: 61 / 52 / 52 us; of 16, for 8 /
+  // 2: 111 / 50.
+  const long long cus = (long long)device_limits().cus, heads = std::max(1ll, Hk), couples = std::min(T, (long long)c.pages.P) * ((D + 8) / 16);
+  const long long smaller = couples <= 128 ? 4 : couples <= 256 ? 2 : 1;
+  long long groups = std::min(heads, std::max((heads + kAppendHeads - 1) / kAppendHeads, 4 * smaller * cus / (B * pages)));
+  a.heads = (int)((heads + groups - 1) / groups);
+  groups = (heads + a.heads - 1) / a.heads;
+  a.queries = (int)((a.Hq + groups - 1) / groups);
+  if (pages * groups >= (1ll << 22)) return fail(TRACEA_UNSUPPORTED_CONFIG, "%s: %lld heads of %lld new tokens are more than is supported", op, Hk, T);
+  a.groups = (int)groups;
   return hip_status("cache append launch", launch_cache_append(a, k.dtype, (hipStream_t)params.stream));
 }
 
