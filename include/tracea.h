@@ -520,7 +520,7 @@ TraceaStatus tracea_norm_gate_residual_backward(const TraceaTensorView *dx_out, 
  * The backward pass takes the gradients of the results (dq_out, dk_out) back through the rotation and the norm, which it works out
  * again from q and k: dq, dk (required with q, k) have the type of q, dq_weight, dk_weight [D] f32 (optional) are sums over all heads, tokens
  * and batch entries in an order that does not change; without weights there are no such gradients.  dq may be dq_out or q as the same view, dk likewise.  With weight gradients it takes
- * a workspace per (device, stream), 8 bytes per value of a head and workgroup, at most 8 MiB, never grown under capture. */
+ * a workspace per (device, stream), 8 bytes per value of a head and workgroup, at most 4 MiB, never grown under capture. */
 typedef struct {
   uint32_t axes;
   uint32_t sections[TRACEA_MAX_ROTARY_AXES];

@@ -52,7 +52,7 @@ struct QkNormArgs {
 int launch_qk_norm_forward(const QkNormArgs &a, int dtype, hipStream_t stream);
 int launch_qk_norm_backward(const QkNormArgs &a, int dtype, hipStream_t stream);
 constexpr int kQkNormMaxDim = 512;
-constexpr int kQkNormRuns = 8;  // workgroups a CU of the backward pass, at most
+constexpr int kQkNormRuns = 4;  // workgroups a CU of the backward pass, at most
 
 struct CacheAppendArgs {
   HeadView q, q_out, k, v;  // q.p null: no queries

@@ -230,7 +230,7 @@ TraceaStatus qk_norm_call(const TraceaTensorView &q, bool two, const TraceaQkNor
   if (columns_apart(*v)) return fail(TRACEA_UNSUPPORTED_CONFIG, "%s: the head dimension must be contiguous (q)", c->op);
   return check_device(c->op, c->device);
 }
-void set_qk_norm(const QkNorm &c, const Rotation &r, const View *const *tensors, int n, const TraceaQkNormParams &params, QkNormArgs *a) {
+void set_qk_norm(const QkNorm &c, const Rotation &r, const View *const *tensors, int n, bool backward, const TraceaQkNormParams &params, QkNormArgs *a) {
   a->B = (int)c.B; a->S = (int)c.S; a->D = (int)c.D;
   set_rotation(r, a);
   a->adjacent = params.adjacent != 0;
@@ -245,11 +245,12 @@ void set_qk_norm(const QkNorm &c, const Rotation &r, const View *const *tensors,
   if (a->vec)
     while (a->lanes / 2 * 2 * e >= c.D && a->lanes > 1) a->lanes /= 2;
   const long long heads = a->H[0] + a->H[1], tokens = c.B * c.S, groups = 256 / a->lanes;
-  // Lane groups that share a token's angles take its heads in turn: as many as fill the device with 8 waves a CU where tokens are few, 8
-  // where heads lie side by side (pieces of a row's neighbours), else one.
+  // Lane groups that share a token's angles take its heads in turn: as many as fill the device with 8 waves a CU where tokens are few; else,
+  // where heads lie side by side, 8 forward (pieces next to each other: S24960 H32:8 D128 bf16, by 8 / 4 / 2 groups 99 / 104 / 120 us) and 2 backward, where
+  // angles cost more, being worked out for queries and keys apart (4 x 2048 tokens 74 / 70 / 65 us); where they are a sequence apart, one.
   const long long want = ((long long)device_limits().cus * 8 * (64 / a->lanes) + tokens - 1) / std::max(1ll, tokens);
   const bool side_by_side = a->H[0] > 1 && std::llabs(a->x[0].sh) < std::llabs(c.S > 1 ? a->x[0].ss : a->x[0].sb);
-  a->beside = (int)std::max(1ll, std::min(heads, std::max(want, side_by_side ? 8ll : 1ll)));
+  a->beside = (int)std::max(1ll, std::min(heads, std::max(want, !side_by_side ? 1ll : backward ? 2ll : 8ll)));
   a->blocks = (int)std::max(1ll, std::min((long long)device_limits().cus * kQkNormRuns, (tokens * a->beside + groups - 1) / groups));
 }
 
@@ -291,7 +292,7 @@ TraceaStatus dispatch_qk_norm(const TraceaTensorView &tq, const TraceaTensorView
     tensors[n++] = &out[i];
   }
   if (c.n == 2 && may_overlap(out[0], out[1])) return overlapping(op, "results overlap each other");
-  set_qk_norm(c, r, tensors, n, params, &a);
+  set_qk_norm(c, r, tensors, n, false, params, &a);
   if (c.B * c.S * a.beside >= (1ll << 40)) return fail(TRACEA_UNSUPPORTED_CONFIG, "%s: problem too large", op);
   DeviceScope scope(c.device);
   if (scope.err != hipSuccess) return hip_status("hipSetDevice", (int)scope.err);
@@ -360,7 +361,7 @@ TraceaStatus dispatch_qk_norm_backward(const TraceaTensorView &tdq_out, const Tr
     a.H[0] = a.H[1] = 0;
     c.B = c.S = 1;
   }
-  set_qk_norm(c, r, tensors, n, params, &a);
+  set_qk_norm(c, r, tensors, n, true, params, &a);
   if (nothing) a.positions = nullptr;
   DeviceScope scope(c.device);
   if (scope.err != hipSuccess) return hip_status("hipSetDevice", (int)scope.err);

@@ -25,17 +25,22 @@ inline long long count_of(const View &v) {
 
 // As read_view; a tensor without elements may have no address.
 inline TraceaStatus read(const char *op, const char *name, const TraceaTensorView &t, int rank, View *v) {
-  char what[96];
-  snprintf(what, sizeof(what), "%s: %s", op, name);
-  TraceaTensorView u = t;
-  static char nothing;
-  if (u.ptr == nullptr && u.shape != nullptr && (int)u.rank == rank)
-    for (int i = 0; i < rank; ++i)
-      if (u.shape[i] == 0) u.ptr = &nothing;
-  const TraceaStatus st = read_view(what, u, rank, v);
-  if (st != TRACEA_SUCCESS) return st;
+  if (t.ptr != nullptr && t.shape != nullptr && (int)t.rank == rank) {  // (what can be read at all: no message has to be made up)
+    const TraceaStatus st = read_view(name, t, rank, v);
+    if (st != TRACEA_SUCCESS) return st;
+  } else {
+    char what[96];
+    snprintf(what, sizeof(what), "%s: %s", op, name);
+    TraceaTensorView u = t;
+    static char nothing;
+    if (u.ptr == nullptr && u.shape != nullptr && (int)u.rank == rank)
+      for (int i = 0; i < rank; ++i)
+        if (u.shape[i] == 0) u.ptr = &nothing;
+    const TraceaStatus st = read_view(what, u, rank, v);
+    if (st != TRACEA_SUCCESS) return st;
+  }
   for (int i = 0; i < rank; ++i)
-    if (t.shape[i] >= (1ull << 31)) return fail(TRACEA_UNSUPPORTED_CONFIG, "%s: extents of 2^31 and more are not supported", what);
+    if (t.shape[i] >= (1ull << 31)) return fail(TRACEA_UNSUPPORTED_CONFIG, "%s: %s: extents of 2^31 and more are not supported", op, name);
   return TRACEA_SUCCESS;
 }
 

@@ -103,6 +103,27 @@ struct Lane {
       }
     }
   }
+  // A row as it lies in memory: requested before the one ahead of it is worked on (in pieces; one by one, rows are not requested ahead).
+  struct Raw {
+    Piece<T, VEC ? E : 1> a, b;
+  };
+  __device__ __forceinline__ void request(const T *row, Raw &r) const {
+    if constexpr (VEC) {
+      if (there) {
+        r.a = *(const Piece<T, E> *)(row + at_u);
+        r.b = *(const Piece<T, E> *)(row + at_v);
+      }
+    }
+  }
+  __device__ __forceinline__ void take(const T *row, const Raw &r, float (&u)[N], float (&v)[N]) const {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) u[e] = v[e] = 0.0f;
+      if (there) couple(r.a.x, r.b.x, u, v);
+    } else {
+      load(row, u, v);
+    }
+  }
   template <typename F>
   __device__ __forceinline__ void store(F *row, const float (&u)[N], const float (&v)[N]) const {
     if constexpr (VEC) {
@@ -222,12 +243,21 @@ __global__ void __launch_bounds__(256) qk_norm_backward_kernel(const QkNormArgs 
       for (long long item = (long long)blockIdx.x * groups + group; item < items; item += (long long)gridDim.x * groups) {
         const long long token = item / a.beside;
         const int slot = (int)(item - token * a.beside), b = (int)(token / a.S), s = (int)(token - (long long)b * a.S);
+        typename L::Raw x, dy, x_next, dy_next;
+        if (slot < a.H[t]) {  // (on their way while the angles are worked out)
+          me.request(row_of<const T>(a.x[t], b, slot, s), x);
+          me.request(row_of<const T>(a.dout[t], b, slot, s), dy);
+        }
         float c[N], sn[N];
         me.angles(a, b, s, c, sn);
-        for (int h = slot; h < a.H[t]; h += a.beside) {
+        for (int h = slot; h < a.H[t]; h += a.beside, x = x_next, dy = dy_next) {
+          if (h + a.beside < a.H[t]) {
+            me.request(row_of<const T>(a.x[t], b, h + a.beside, s), x_next);
+            me.request(row_of<const T>(a.dout[t], b, h + a.beside, s), dy_next);
+          }
           float u[N], v[N], p[N], q[N];
-          me.load(row_of<const T>(a.x[t], b, h, s), u, v);
-          me.load(row_of<const T>(a.dout[t], b, h, s), p, q);
+          me.take(row_of<const T>(a.x[t], b, h, s), x, u, v);
+          me.take(row_of<const T>(a.dout[t], b, h, s), dy, p, q);
           float ss = 0.0f, gx = 0.0f;
 #pragma unroll
           for (int k = 0; k < N; ++k) {
@@ -265,21 +295,23 @@ __global__ void __launch_bounds__(256) qk_norm_backward_kernel(const QkNormArgs 
   }
 }
 
-// Sums over the workgroups: 16 columns of one weight, 16 runs of workgroups.
-__global__ void __launch_bounds__(256) qk_norm_weights_kernel(const QkNormArgs a) {
-  __shared__ float s_sum[16][17];
+// Sums over the workgroups: 16 columns of one weight, 64 runs of workgroups, whose loads are what it waits for (2048 workgroups, D128: 16 runs 8.3 us).
+__global__ void __launch_bounds__(1024) qk_norm_weights_kernel(const QkNormArgs a) {
+  constexpr int RUNS = 64;
+  __shared__ float s_sum[RUNS][17];
   const int t = blockIdx.y, c16 = threadIdx.x & 15, run = threadIdx.x >> 4, col = blockIdx.x * 16 + c16;
   if (a.dw[t] == nullptr) return;
   float sum = 0.0f;
   if (col < a.D) {
 #pragma unroll 8
-    for (int i = run; i < a.blocks; i += 16) sum += a.partial[((long long)t * a.blocks + i) * a.D + col];
+    for (int i = run; i < a.blocks; i += RUNS) sum += a.partial[((long long)t * a.blocks + i) * a.D + col];
   }
   s_sum[run][c16] = sum;
-  __syncthreads();
-  if (run != 0 || col >= a.D) return;
-  for (int i = 1; i < 16; ++i) sum += s_sum[i][c16];
-  a.dw[t][col] = sum;
+  for (int half = RUNS / 2; half > 0; half >>= 1) {
+    __syncthreads();
+    if (run < half) s_sum[run][c16] += s_sum[run + half][c16];
+  }
+  if (run == 0 && col < a.D) a.dw[t][col] = s_sum[0][c16];
 }
 
 template <typename T, bool VEC, bool ADJ>
@@ -295,7 +327,7 @@ int launch(const QkNormArgs &a, bool backward, hipStream_t stream) {
   hipLaunchKernelGGL((qk_norm_backward_kernel<T, VEC, ADJ>), dim3((unsigned)a.blocks), dim3(256), (unsigned)(groups * a.D * 4), stream, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || (a.dw[0] == nullptr && a.dw[1] == nullptr)) return (int)e;
-  hipLaunchKernelGGL(qk_norm_weights_kernel, dim3((unsigned)((a.D + 15) / 16), 2), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL(qk_norm_weights_kernel, dim3((unsigned)((a.D + 15) / 16), 2), dim3(1024), 0, stream, a);
   return (int)hipGetLastError();
 }
 template <typename T>
