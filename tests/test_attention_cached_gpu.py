@@ -22,6 +22,10 @@ def run(ops, seed, b, hq, hk, sq, k_lengths, d, page, dtype, e4m3, causal=True, 
     if spoil is not None:
         spoil(pt, pool)
     want, want_lse, allowed, lse_off = attention(q, pool, pt, k_lengths, q_lengths, causal, scale, rounded)
+    if garbage and e4m3:  # pages in no table, the first of the pool too
+        used = torch.zeros(b * per + 1, dtype=torch.bool, device="cuda")
+        used[pt[(pt >= 0) & (pt <= b * per)].long()] = True
+        pool.k_scale[~used], pool.v_scale[~used] = float("inf"), float("nan")
     if garbage:  # what lies behind the lengths may be anything
         for i in range(b):
             for slot in range(per):
@@ -31,6 +35,9 @@ def run(ops, seed, b, hq, hk, sq, k_lengths, d, page, dtype, e4m3, causal=True, 
                     for t in (pool.k, pool.v):
                         if e4m3:
                             Pool._u8(t)[page_id, :, first:] = 0x7f
+                            if first == 0:  # (a page that nobody uses)
+                                pool.k_scale[page_id] = float("nan")
+                                pool.v_scale[page_id] = float("inf")
                         else:
                             t[page_id, :, first:] = float("nan")
     lse = torch.full((b, hq, sq), 7.0, device="cuda")

@@ -40,8 +40,10 @@ struct Scales {
 
   // The factor by which what is summed up so far changes.
   __device__ __forceinline__ float load(const AttentionCachedArgs &a, int hk, int page, bool there) {
-    c = fmaxf(a.scale_log2 * a.ks.p[page * a.ks.sn + hk * a.ks.sh], 1.17549435e-38f);
-    const float vs = a.vs.p[page * a.vs.sn + hk * a.vs.sh], top = wave_max(there ? vs : 0.0f);
+    // (a group without a page: nothing of a scale that may be anything)
+    const float ks = there ? a.ks.p[page * a.ks.sn + hk * a.ks.sh] : 1.0f, vs = there ? a.vs.p[page * a.vs.sn + hk * a.vs.sh] : 0.0f;
+    c = fmaxf(a.scale_log2 * ks, 1.17549435e-38f);
+    const float top = wave_max(vs);
     float f = 1.0f;
     lift_before = lift;
     if (top > ref) {  // (lifts from before, in its terms)

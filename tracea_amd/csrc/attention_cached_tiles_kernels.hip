@@ -181,8 +181,9 @@ __global__ void __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu
     bool there;
     const int page = at.locate(a, b, hk, located * TILE + lane * 16, lk, there);
     if constexpr (C8) {
-      ks = a.ks.p[page * a.ks.sn + hk * a.ks.sh] / k_unit;
-      vs = a.vs.p[page * a.vs.sn + hk * a.vs.sh] / v_unit;
+      // (a group without a page: 1, as its zeros stay zeros only with a finite scale, and that of a page that nobody uses may be anything)
+      ks = there ? a.ks.p[page * a.ks.sn + hk * a.ks.sh] / k_unit : 1.0f;
+      vs = there ? a.vs.p[page * a.vs.sn + hk * a.vs.sh] / v_unit : 1.0f;
     }
   };
   // Which groups of a tile in LDS have pages: the others' keys are zeros that nobody sees.
