@@ -58,7 +58,9 @@ CASES = [  # b, hq, hk, t, d, rot, page, starts, lengths, adjacent, layout, orde
     (2, 3, 1, 130, 96, 96, 48, [47, 5], [0, 130], False, "bhsd", "npHd"), (1, 2, 2, 300, 40, 20, 256, [100], None, False, "odd", "nhpd"),
     (2, 5, 3, 33, 128, 128, 32, [0, 31], None, True, "odd", "both"), (1, 0, 8, 64, 128, 128, 64, [64], None, False, "bshd", "nhpd"),
     (2, 6, 2, 20, 72, 0, 32, [9, 40], [20, 7], False, "bhsd", "nhpd"), (1, 1, 1, 40, 512, 512, 16, [7], None, False, "bhsd", "nhpd"),
-    (2, 4, 70, 3, 16, 16, 16, [15, 0], None, False, "bhsd", "nhpd"), (1, 2, 1, 600, 64, 64, 512, [500], None, False, "bhsd", "nhpd")]
+    (2, 4, 70, 3, 16, 16, 16, [15, 0], None, False, "bhsd", "nhpd"), (1, 2, 1, 600, 64, 64, 512, [500], None, False, "bhsd", "nhpd"),
+    (2, 5, 3, 300, 128, 128, 256, [200, 0], [300, 131], True, "bshd", "npHd"), (1, 3, 3, 300, 128, 64, 256, [131], None, False, "bhsd", "both"),
+    (1, 2, 2, 270, 128, 128, 512, [300], None, False, "bhsd", "nhpd")]
 
 
 @pytest.mark.parametrize("e4m3", [False, True], ids=["16", "e4m3"])

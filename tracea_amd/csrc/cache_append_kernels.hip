@@ -8,8 +8,12 @@
 // exact except below the normal codes, and so a cache is the same, up to these, however its tokens were cut into calls.
 //
 // A workgroup has the tokens of one sequence that fall into one page, for some of the heads: no other writes that page and head, so that scales
-// need no atomics across workgroups.  Sines and cosines of its tokens are kept in LDS for its heads.  In 8 bits it reads its
-// operands twice, for the largest value and for the codes; the second time they come from the caches.
+// need no atomics across workgroups.  Sines and cosines of its tokens are kept in LDS for its heads.  Two kernels: cache_append_held_kernel where
+// rows are in whole pieces of 8 and a workgroup's tokens fit its registers, cache_append_kernel for everything else.
+//
+// Two prompts of 4096 tokens, 32 heads of queries and 8 of keys, 128 columns, bf16 into pages of 64 tokens in 8 bits: 52 us, 3.5 TB/s of 5.06 that
+// a copy reaches, bound by the vector work beside the loads (a sine and cosine per token and pair, each operand turned twice, codes) and by a
+// workgroup's chain of loads, largest value and stores; in 16 bits 50 us, 4.0 TB/s.  One token of 16 sequences: 7 us, latency only.
 #include <type_traits>
 
 #include "cache.hpp"
@@ -72,6 +76,8 @@ __device__ __forceinline__ void rescale(unsigned char *head, long long apart, in
   }
 }
 
+// Any sizes, E columns at a time (8, or 1 where rows are not aligned): angles of up to ANGLES pairs at once, and in 8 bits operands are read
+// twice, for the largest value and for the codes; the second time they come from the caches.
 template <typename T, bool C8, int E, bool ADJ>
 __global__ void __launch_bounds__(256) cache_append_kernel(const CacheAppendArgs a) {
   __shared__ float s_cos[ANGLES], s_sin[ANGLES];
@@ -258,13 +264,14 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const CacheAppendArgs
   }
 }
 
-// The same where a workgroup's tokens are few enough for their angles to be kept all at once and their operands in registers between the largest value
-// and the codes: every byte is read once.  Pieces of 8 columns only.  Half of the workgroup's threads, SIDE, have the keys and values, the
-// other half the queries, so that neither waits behind the other's loads.  A thread has up to HK pieces of a head's keys, 2 HK of its values.
-
+// The same where a workgroup's tokens are few enough for their angles to be kept all at once and their operands in registers between the largest
+// value and the codes: every byte is read once.  Pieces of 8 columns only.  Half of the workgroup's threads, SIDE, have the keys and values, the
+// other half the queries, so that neither waits behind the other's loads.  A thread has up to HK couples of pieces of a head: with 2, keys and values
+// are held together and queries by two heads, with 4 one after the other.  The smallest workgroup that holds a page is taken: measured with the prompts
+// above, pages of 64 52 us (64 by the kernel before), of 16 52 (78), of 128 57, of 256 57 (131).
 template <typename T, bool C8, bool ADJ, int SIDE, int HK>
 __global__ void __launch_bounds__(2 * SIDE) __attribute__((amdgpu_waves_per_eu(4))) cache_append_held_kernel(const CacheAppendArgs a) {
-  constexpr int WAVES = SIDE / 64, HV = 2 * HK, PAIRS = SIDE * HK * 8;
+  constexpr int WAVES = SIDE / 64, PAIRS = SIDE * HK * 8, SETS = HK == 2 ? 2 : 1;
   typedef float f4 __attribute__((ext_vector_type(4)));
   __shared__ f4 s_cos[PAIRS / 4], s_sin[PAIRS / 4];
   __shared__ float s_max[2][2][WAVES];
@@ -279,7 +286,7 @@ __global__ void __launch_bounds__(2 * SIDE) __attribute__((amdgpu_waves_per_eu(4
   const int h0 = min(a.Hk, grp * a.heads), h1 = min(a.Hk, h0 + a.heads), q0 = min(a.Hq, grp * a.queries), q1 = min(a.Hq, q0 + a.queries);
   const int page = page_of(a.table, b, slot);
   const int tokens = page >= 0 && end > lo ? end - lo : 0;  // with a place
-  const int turned_pieces = a.P / 8, pieces = (a.D + 8) / 16, all = a.D / 8;
+  const int turned_pieces = a.P / 8, pieces = (a.D + 8) / 16;
 
   // A thread's pieces are the same in every head: token (from lo) and two times 8 columns, partners that are turned by the angles from
   // `angle` on, or columns side by side that are not (angle < 0; v < 0: there is no second).
@@ -287,38 +294,34 @@ __global__ void __launch_bounds__(2 * SIDE) __attribute__((amdgpu_waves_per_eu(4
     int t, u, v, angle;
   };
   // (worked out where they are used, a few instructions: kept for a loop over heads they would fill the registers)
-  const unsigned by_pieces = 0xffffffffu / (unsigned)pieces + 1, by_all = 0xffffffffu / (unsigned)all + 1;  // 0: divided by 1
-  auto place_in = [&](int s, unsigned magic, int per, int &t, int &piece) __attribute__((always_inline)) {
+  const unsigned by_pieces = 0xffffffffu / (unsigned)pieces + 1;  // 0: divided by 1
+  auto couple = [&](int s, int turned_of) __attribute__((always_inline)) {  // turned_of: how many of a token's couples are turned
+    Couple p;
     unsigned i = (unsigned)id;
     asm volatile("" : "+v"(i));
     i += (unsigned)(s * SIDE);
-    t = magic == 0 ? (int)i : (int)__umulhi(i, magic);
-    piece = (int)i - t * per;
-  };
-  auto couple = [&](int s) __attribute__((always_inline)) {
-    Couple p;
-    int piece;
-    place_in(s, by_pieces, pieces, p.t, piece);
-    const bool pair = piece < turned_pieces;
-    p.u = !pair ? 2 * a.P + (piece - turned_pieces) * 16 : ADJ ? 16 * piece : 8 * piece;
+    p.t = by_pieces == 0 ? (int)i : (int)__umulhi(i, by_pieces);
+    const int piece = (int)i - p.t * pieces;
+    const bool pair = piece < turned_of;
+    p.u = !pair ? 16 * turned_of + (piece - turned_of) * 16 : ADJ ? 16 * piece : 8 * piece;
     p.v = pair && !ADJ ? p.u + a.P : p.u + 8 < a.D ? p.u + 8 : -1;
     p.angle = pair ? (p.t * a.P + piece * 8) / 4 : -1;
     return p;
   };
   using X = Piece<T, 8>;
-  // What a thread holds: couples of keys, then pieces of values; or couples of two heads' queries.
-  u32x4 held[4 * HK];
+  // What a thread holds: couples of keys and of values, or of two heads' queries.
+  u32x4 held[SETS * 2 * HK];
   // The compiler takes them for new values: it would keep all of them widened and turned from the largest value to the codes.
   auto anew = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < 4 * HK; ++i) asm volatile("" : "+v"(held[i]));
+    for (int i = 0; i < SETS * 2 * HK; ++i) asm volatile("" : "+v"(held[i]));
   };
   auto piece_of = [&](int i) { return __builtin_bit_cast(X, held[i]); };
-  auto load_row = [&](const HeadView &x, int h, int count, auto first) __attribute__((always_inline)) {
+  auto load_row = [&](const HeadView &x, int h, int count, int turned_of, auto first) __attribute__((always_inline)) {
     const char *at = (const char *)((const T *)x.p + b * x.sb + h * x.sh + lo * x.ss);
 #pragma unroll
     for (int s = 0; s < HK; ++s) {
-      const Couple p = couple(s);
+      const Couple p = couple(s, turned_of);
       if (p.t >= count) continue;
       const unsigned row = (unsigned)p.t * (unsigned)x.ss;
       held[first() + s] = *(const u32x4 *)(at + (row + (unsigned)p.u) * 2);
@@ -365,29 +368,20 @@ __global__ void __launch_bounds__(2 * SIDE) __attribute__((amdgpu_waves_per_eu(4
     for (int e = 0; e < 8; ++e) y.x[e] = (T)x[e];
     *(X *)at = y;
   };
-  auto wide = [](const X &x, float (&y)[8]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = (float)x.x[e];
-  };
-
+  constexpr std::integral_constant<int, 0> FIRST{};
+  constexpr std::integral_constant<int, SETS == 2 ? 2 * HK : 0> SECOND{};
   float k_old = 0.0f, v_old = 0.0f;
   auto load_head = [&](int h) __attribute__((always_inline)) {
-    load_row(a.k, h, tokens, std::integral_constant<int, 0>{});
-    const char *at = (const char *)((const T *)a.v.p + b * a.v.sb + h * a.v.sh + lo * a.v.ss);
-#pragma unroll
-    for (int s = 0; s < HV; ++s) {
-      int t, piece;
-      place_in(s, by_all, all, t, piece);
-      if (t < tokens) held[2 * HK + s] = *(const u32x4 *)(at + ((unsigned)t * (unsigned)a.v.ss + (unsigned)piece * 8) * 2);
-    }
+    load_row(a.k, h, tokens, turned_pieces, FIRST);
+    if constexpr (SETS == 2) load_row(a.v, h, tokens, 0, SECOND);
     if (C8 && tokens > 0 && base < 0) {
       k_old = a.ks.p[page * a.ks.sn + h * a.ks.sh];
       v_old = a.vs.p[page * a.vs.sn + h * a.vs.sh];
     }
   };
   auto load_queries = [&](int h) __attribute__((always_inline)) {
-    load_row(a.q, h, hi - lo, std::integral_constant<int, 0>{});
-    if (h + 1 < q1) load_row(a.q, h + 1, hi - lo, std::integral_constant<int, 2 * HK>{});
+    load_row(a.q, h, hi - lo, turned_pieces, FIRST);
+    if (SETS == 2 && h + 1 < q1) load_row(a.q, h + 1, hi - lo, turned_pieces, SECOND);
   };
   // (on their way while the angles are worked out)
   if (of_keys && h0 < h1) load_head(h0);
@@ -406,15 +400,15 @@ __global__ void __launch_bounds__(2 * SIDE) __attribute__((amdgpu_waves_per_eu(4
   __syncthreads();
 
   if (!of_keys) {
-    for (int h = q0; h < q1; h += 2) {
+    for (int h = q0; h < q1; h += SETS) {
       if (h > q0) load_queries(h);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < SETS; ++i) {
         if (h + i >= q1) continue;
         char *at = (char *)((T *)a.q_out.p + b * a.q_out.sb + (h + i) * a.q_out.sh + lo * a.q_out.ss);
 #pragma unroll
         for (int s = 0; s < HK; ++s) {
-          const Couple p = couple(s);
+          const Couple p = couple(s, turned_pieces);
           if (p.t >= hi - lo) continue;
           float u[8], v[8];
           turned(p, piece_of(2 * HK * i + s), piece_of(2 * HK * i + HK + s), u, v);
@@ -429,100 +423,68 @@ __global__ void __launch_bounds__(2 * SIDE) __attribute__((amdgpu_waves_per_eu(4
       }
     }
     if (C8 && tokens > 0)
-      for (int h = h0; h < h1; ++h) __syncthreads();  // (those of the other half)
+      for (int h = h0; h < h1; ++h) {  // (those of the other half)
+        __syncthreads();
+        __syncthreads();
+      }
     return;
   }
-  for (int h = h0; h < h1 && tokens > 0; ++h) {
-    if (h > h0) load_head(h);
-    // of the page, and of token lo in it
-    unsigned char *k_page = a.kc.p + page * a.kc.sn + h * a.kc.sh, *v_page = a.vc.p + page * a.vc.sn + h * a.vc.sh;
-    unsigned char *k_rows = k_page + (lo - base) * a.kc.ss, *v_rows = v_page + (lo - base) * a.vc.ss;
-    float k_inv = 1.0f, v_inv = 1.0f;
+  // Keys or values of a head, from where they are held to their places.
+  auto leave = [&](int h, const PageView &cache, const ScaleView &scales, float old, int turned_of, float (&tops)[WAVES], auto first) __attribute__((always_inline)) {
+    unsigned char *head = cache.p + page * cache.sn + h * cache.sh, *rows = head + (lo - base) * cache.ss;  // of the page; of token lo in it
+    float inv = 1.0f;
     if constexpr (C8) {
-      float k_top, v_top;
-      auto tops_of = [&](bool finite) __attribute__((always_inline)) {
-        k_top = v_top = 0.0f;
+      float top;
+      auto top_of = [&](bool finite) __attribute__((always_inline)) {
+        top = 0.0f;
 #pragma unroll
         for (int s = 0; s < HK; ++s) {
-          const Couple p = couple(s);
+          const Couple p = couple(s, turned_of);
           if (p.t >= tokens) continue;
           float u[8], v[8];
-          turned(p, piece_of(s), piece_of(HK + s), u, v);
-          k_top = largest(u, k_top, finite);
-          if (p.v >= 0) k_top = largest(v, k_top, finite);
+          turned(p, piece_of(first() + s), piece_of(first() + HK + s), u, v);
+          top = largest(u, top, finite);
+          if (p.v >= 0) top = largest(v, top, finite);
         }
 #pragma unroll
-        for (int s = 0; s < HV; ++s) {
-          int t, piece;
-          place_in(s, by_all, all, t, piece);
-          if (t >= tokens) continue;
-          float u[8];
-          wide(piece_of(2 * HK + s), u);
-          v_top = largest(u, v_top, finite);
-        }
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
-          k_top = fmaxf(k_top, __shfl_xor(k_top, m, 64));
-          v_top = fmaxf(v_top, __shfl_xor(v_top, m, 64));
-        }
+        for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
       };
-      tops_of(false);
-      if (__builtin_amdgcn_readfirstlane((int)(k_top == INFINITY || v_top == INFINITY))) {
+      top_of(false);
+      if (__builtin_amdgcn_readfirstlane((int)(top == INFINITY))) {
         anew();
-        tops_of(true);
+        top_of(true);
       }
       anew();
-      float(&tops)[2][WAVES] = s_max[h & 1];
-      if (lane == 0) {
-        tops[0][wave] = k_top;
-        tops[1][wave] = v_top;
-      }
+      if (lane == 0) tops[wave] = top;
       __syncthreads();
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) {
-        k_top = fmaxf(k_top, tops[0][w]);
-        v_top = fmaxf(v_top, tops[1][w]);
-      }
-      const float k_now = fmaxf(k_old, scale_for(k_top)), v_now = fmaxf(v_old, scale_for(v_top));
-      if (threadIdx.x == 0) {
-        a.ks.p[page * a.ks.sn + h * a.ks.sh] = k_now;
-        a.vs.p[page * a.vs.sn + h * a.vs.sh] = v_now;
-      }
-      k_inv = 1.0f / k_now;
-      v_inv = 1.0f / v_now;
-      // older codes of the page, where the scale has grown
-      if (base < 0 && k_now > k_old) rescale(k_page, a.kc.ss, (int)-base, a.D, k_old / k_now, SIDE);
-      if (base < 0 && v_now > v_old) rescale(v_page, a.vc.ss, (int)-base, a.D, v_old / v_now, SIDE);
+      for (int w = 0; w < WAVES; ++w) top = fmaxf(top, tops[w]);
+      const float now = fmaxf(old, scale_for(top));
+      if (threadIdx.x == 0) scales.p[page * scales.sn + h * scales.sh] = now;
+      inv = 1.0f / now;
+      if (base < 0 && now > old) rescale(head, cache.ss, (int)-base, a.D, old / now, SIDE);  // older codes of the page
     }
 #pragma unroll
     for (int s = 0; s < HK; ++s) {
-      const Couple p = couple(s);
+      const Couple p = couple(s, turned_of);
       if (p.t >= tokens) continue;
       float u[8], v[8];
-      turned(p, piece_of(s), piece_of(HK + s), u, v);
-      unsigned char *row = k_rows + (unsigned)p.t * (unsigned)a.kc.ss;
+      turned(p, piece_of(first() + s), piece_of(first() + HK + s), u, v);
+      unsigned char *row = rows + (unsigned)p.t * (unsigned)cache.ss;
       if constexpr (C8) {
-        *(Codes<8> *)(row + p.u) = encode<8>(u, k_inv);
-        if (p.v >= 0) *(Codes<8> *)(row + p.v) = encode<8>(v, k_inv);
+        *(Codes<8> *)(row + p.u) = encode<8>(u, inv);
+        if (p.v >= 0) *(Codes<8> *)(row + p.v) = encode<8>(v, inv);
       } else {
         store16(row + p.u * 2, u);
         if (p.v >= 0) store16(row + p.v * 2, v);
       }
     }
-#pragma unroll
-    for (int s = 0; s < HV; ++s) {
-      int t, piece;
-      place_in(s, by_all, all, t, piece);
-      if (t >= tokens) continue;
-      unsigned char *row = v_rows + ((unsigned)t * (unsigned)a.vc.ss + (unsigned)piece * (C8 ? 8 : 16));
-      if constexpr (C8) {
-        float u[8];
-        wide(piece_of(2 * HK + s), u);
-        *(Codes<8> *)row = encode<8>(u, v_inv);
-      } else {
-        *(u32x4 *)row = held[2 * HK + s];
-      }
-    }
+  };
+  for (int h = h0; h < h1 && tokens > 0; ++h) {
+    if (h > h0) load_head(h);
+    leave(h, a.kc, a.ks, k_old, turned_pieces, s_max[h & 1][0], FIRST);
+    if constexpr (SETS == 1) load_row(a.v, h, tokens, 0, SECOND);
+    leave(h, a.vc, a.vs, v_old, 0, s_max[h & 1][1], SECOND);
   }
 }
 
@@ -531,7 +493,7 @@ int launch(const CacheAppendArgs &a, hipStream_t stream) {
   const dim3 grid((unsigned)(a.pages * a.groups), (unsigned)a.B);
   const int tokens = a.T < a.table.P ? a.T : a.table.P, pieces = (a.D + 8) / 16;
   auto holds = [&](int side, int held) {
-    return a.vec && a.near && tokens * a.P <= side * held * 8 && tokens * pieces <= side * held && tokens * (a.D / 8) <= 2 * side * held;
+    return a.vec && a.near && tokens * a.P <= side * held * 8 && tokens * pieces <= side * held;
   };
 #define HELD(SIDE, HK)                                                                                                                     \
   if (holds(SIDE, HK)) {                                                                                                                   \
@@ -543,6 +505,7 @@ int launch(const CacheAppendArgs &a, hipStream_t stream) {
   HELD(128, 2)
   HELD(256, 2)
   HELD(512, 2)
+  HELD(512, 4)
 #undef HELD
   if (a.vec && a.adjacent) hipLaunchKernelGGL((cache_append_kernel<T, C8, 8, true>), grid, dim3(256), 0, stream, a);
   else if (a.vec) hipLaunchKernelGGL((cache_append_kernel<T, C8, 8, false>), grid, dim3(256), 0, stream, a);
