@@ -551,11 +551,12 @@ TraceaStatus tracea_qk_norm_rotary_backward(TraceaTensorView dq_out, const Trace
  *   starts [B] i32: tokens that sequence b has already; lengths [B] i32 (optional): how many of the T are new ones of sequence b
  *   (clamped to 0..T).  Both contiguous, on the device; a negative start counts as 0.
  *   positions [B,T,A] or [1,T,A] i32 as in tracea_rotary, NULL: starts[b] + t (one axis); inv_freq [P] f32, NULL: no rotation
- * q_out of a token behind lengths[b] is 0; q_out may be q (the same view).  No other rows of the caches are written than the new tokens'.
+ * q_out of a token behind lengths[b] is 0; q_out may be q (the same view).  In 16 bits no other rows of the caches are written than the new
+ * tokens'.
  * In 8 bits the scale of a page and head is the least power of two (2^-126 or more) by which no finite value written to the page so far
- * exceeds 448; a token at place 0 begins the page anew.  Where new tokens raise it, the older tokens' codes are rescaled, exactly
- * but for what falls below the normal codes (2^-6 of the scale, 448 2^6 below the largest value), which rounds once more; codes are rounded to
- * nearest, ties to even, from the fp32 value behind the rotation.  Infinities and NaN become NaN and leave the scale alone.
+ * exceeds 448; a token at place 0 begins the page anew.  Where new tokens raise it, the codes of all other places of that
+ * page and head are rescaled, exactly but for what falls below the normal codes (2^-6 of the scale, 448 2^6 below the largest value), which rounds
+ * once more; where they do not, no other row is written.  Codes are rounded to nearest, ties to even, from the fp32 value behind the rotation.  Infinities and NaN become NaN and leave the scale alone.
  * A page that two sequences share may be read by both, and appended to by neither.  Results overlap no operand but q_out its q. */
 typedef struct {
   uint32_t axes;

@@ -141,13 +141,9 @@ def check_attention(got, lse, want, want_lse, allowed, lse_off):
         assert ((lse.double() - want_lse).abs()[fine] <= lse_off[fine] + 1e-6).all()
 
 
-def rows_before(lo, slot, p):
-    return slice(0, lo - slot * p)
-
-
 def append(pool, page_table, k, v, starts, lengths=None, rot=0, angle=None, adjacent=False):
-    """What the caches hold afterwards: {name: (values [N,Hk,P,D], allowed, scales or None, changed)} in 64 bits.  Sequence by sequence.  Places
-    behind the new tokens keep their codes, whatever the scale: `changed` leaves them out, and `allowed` says nothing of their value."""
+    """What the caches hold afterwards: {name: (values [N,Hk,P,D], allowed, scales or None, changed)} in 64 bits.  Sequence by sequence.
+    changed [N,Hk,P]: the new tokens' places, and all others of a page and head whose scale has grown."""
     out = {}
     for name, x in (("k", k), ("v", v)):
         y, made_of = rotated(x, angle, rot, adjacent) if name == "k" and rot else (x.double(), x.double().abs())
@@ -177,9 +173,11 @@ def append(pool, page_table, k, v, starts, lengths=None, rot=0, angle=None, adja
                 old = torch.zeros_like(need) if lo == slot * p else scale[page]
                 now = torch.maximum(old, need)
                 grown = (now > old) & (old > 0)
-                written[page, :, rows_before(lo, slot, p)] |= grown[:, None]
-                allowed[page, :, hi - slot * p:] = math.inf
-                rows = rows_before(lo, slot, p)
+                written[page] |= grown[:, None]
+                rows = torch.ones(p, dtype=torch.bool, device=values.device)  # (the other places)
+                rows[at] = False
+                if lo == slot * p:  # (begun anew: what its other codes stand for is nobody's)
+                    allowed[page, :, rows] = math.inf
                 step = torch.maximum(2.0 ** -10 * now[:, None, None].expand_as(values[page, :, rows]), torch.zeros(1, device=values.device).double())
                 allowed[page, :, rows] += torch.where(grown[:, None, None], step, torch.zeros_like(step))  # (below the normal codes)
                 scale[page] = now

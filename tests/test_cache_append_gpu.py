@@ -39,7 +39,7 @@ def run(ops, seed, b, hq, hk, t, d, rot, page, dtype, e4m3, starts, lengths=None
         assert torch.equal(torch.isnan(got), nan)
         fine = torch.isfinite(values)
         assert ((got - values).abs()[fine] <= allowed[fine] * (1 + 1e-9)).all(), n
-        # nothing else is touched, to the bit: what is neither a new token nor an older one whose page's scale has grown
+        # nothing else is touched, to the bit: what is neither a new token nor in a page whose scale has grown
         same = ~changed
         assert torch.equal(Pool._u8(getattr(pool, n))[same], before[n][same])
     if q is not None:
@@ -143,8 +143,10 @@ def test_a_cache_is_the_same_however_its_tokens_were_cut(tracea_gpu, dtype):
         at += n
     assert at == t and torch.equal(whole.k_scale, cut.k_scale) and torch.equal(whole.v_scale, cut.v_scale)
     for n in "kv":
-        x, y = whole.values(n), cut.values(n)
-        scale = getattr(whole, n + "_scale").double()[..., None, None]
+        # the tokens' places (what lies behind them is no token's, and moves with the scale as often as it grows)
+        of = pt.long()
+        x, y = (p.values(n)[of].transpose(2, 3).flatten(1, 2)[:, :t] for p in (whole, cut))  # [B,T,Hk,D]
+        scale = getattr(whole, n + "_scale").double()[of].repeat_interleave(page, 1)[:, :t, :, None]
         # codes below the normal ones (2^-6) may have been rounded at up to six scales, each half a step of the last or less
         assert torch.equal(torch.where(x.abs() >= 2.0 ** -6 * scale, x, y), torch.where(y.abs() > 2.0 ** -6 * scale, y, torch.where(x.abs() >= 2.0 ** -6 * scale, x, y)))
         assert ((x - y).abs() <= 2.0 ** -9 * scale).all()

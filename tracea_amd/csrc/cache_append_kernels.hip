@@ -3,8 +3,8 @@
 //   16 bits  cache[page, h, place] = R x                       q' = R q
 //   8 bits   need = least power of two with max|R x| <= 448 need over the new tokens of the page and head (finite ones, 2^-126 or more)
 //            scale = max(old, need), old = 0 where the page begins with a new token
-//            code = e4m3(R x / scale), older codes e4m3(code old / scale)
-// A scale that is a power of two moves codes by whole exponents: it costs no mantissa bit whatever the values are, rescaling older codes is
+//            code = e4m3(R x / scale), the page's other codes e4m3(code old / scale)
+// A scale that is a power of two moves codes by whole exponents: it costs no mantissa bit whatever the values are, rescaling other codes is
 // exact except below the normal codes, and so a cache is the same, up to these, however its tokens were cut into calls.
 //
 // A workgroup has the tokens of one sequence that fall into one page, for some of the heads: no other writes that page and head, so that scales
@@ -59,10 +59,13 @@ __device__ __forceinline__ Codes<E> encode(const float (&x)[E], float inv) {
   return c;
 }
 
-// Codes of `rows` rows of a head of a page, times f (a power of two below 1), by the first threads of a workgroup.
-__device__ __forceinline__ void rescale(unsigned char *head, long long apart, int rows, int D, float f, int threads) {
-  for (int i = threadIdx.x; i < rows * (D / 8); i += threads) {
-    const int row = i / (D / 8), at = (i - row * (D / 8)) * 8;
+// Codes of a head of a page of PT rows but for `count` new ones from `first` on, times f (a power of two below 1), by the first threads of a
+// workgroup.  (Rows behind the new ones as well: they may hold tokens, where a call writes again what a sequence had.)
+__device__ __forceinline__ void rescale(unsigned char *head, long long apart, int PT, int first, int count, int D, float f, int threads) {
+  for (int i = threadIdx.x; i < (PT - count) * (D / 8); i += threads) {
+    int row = i / (D / 8);
+    const int at = (i - row * (D / 8)) * 8;
+    row += row >= first ? count : 0;
     u32x2 *p = (u32x2 *)(head + row * apart + at);
     const u32x2 x = *p;
     u32x2 y;
@@ -203,15 +206,15 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const CacheAppendArgs
       s_move[w][h] = old < now ? old / now : 1.0f;
     }
     __syncthreads();
-    // older codes of the page, where the scale has grown
-    const int older = base < 0 ? (int)-base : 0;
-    if (older > 0)
+    // the page's other codes, where the scale has grown
+    const int first = (int)(lo - base);
+    if (base < 0)
       for (int w = 0; w < 2; ++w)
         for (int h = 0; h < heads; ++h) {
           const float f = s_move[w][h];
           if (f == 1.0f) continue;
-          if (w == 0) rescale(a.kc.p + page * a.kc.sn + (h0 + h) * a.kc.sh, a.kc.ss, older, a.D, f, 256);
-          else rescale(a.vc.p + page * a.vc.sn + (h0 + h) * a.vc.sh, a.vc.ss, older, a.D, f, 256);
+          if (w == 0) rescale(a.kc.p + page * a.kc.sn + (h0 + h) * a.kc.sh, a.kc.ss, PT, first, end - lo, a.D, f, 256);
+          else rescale(a.vc.p + page * a.vc.sn + (h0 + h) * a.vc.sh, a.vc.ss, PT, first, end - lo, a.D, f, 256);
         }
   }
 
@@ -462,7 +465,7 @@ __global__ void __launch_bounds__(2 * SIDE) __attribute__((amdgpu_waves_per_eu(4
       const float now = fmaxf(old, scale_for(top));
       if (threadIdx.x == 0) scales.p[page * scales.sn + h * scales.sh] = now;
       inv = 1.0f / now;
-      if (base < 0 && now > old) rescale(head, cache.ss, (int)-base, a.D, old / now, SIDE);  // older codes of the page
+      if (base < 0 && now > old) rescale(head, cache.ss, PT, (int)(lo - base), tokens, a.D, old / now, SIDE);  // the page's other codes
     }
 #pragma unroll
     for (int s = 0; s < HK; ++s) {
