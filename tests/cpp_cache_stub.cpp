@@ -63,7 +63,8 @@ long long stub_value(const char *what) {
   if (is("row_blocks")) return g_attention.row_blocks;
   if (is("workgroups")) return g_attention.workgroups;
   if (is("splits")) return g_attention.splits;
-  if (is("least")) return g_attention.least;
+  if (is("shares")) return g_attention.shares;
+  if (is("apart")) return g_attention.apart;
   if (is("step")) return g_attention.step;
   if (is("slots")) return g_attention.slots;
   if (is("meta")) return (long long)(intptr_t)g_attention.meta;

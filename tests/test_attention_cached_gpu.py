@@ -68,12 +68,12 @@ def test_attention(tracea_gpu, case, dtype, e4m3):
 
 
 @pytest.mark.parametrize("e4m3", [False, True], ids=["16", "e4m3"])
-@pytest.mark.parametrize("sq", [1, 6, 40])
-def test_long_and_short_sequences_together(tracea_gpu, sq, e4m3):
-    """One line of steps over 70 sequences, most of them short: parts that begin and end anywhere."""
+@pytest.mark.parametrize("sq, long", [(1, 20000), (6, 20000), (40, 20000), (1, 100000), (6, 100000)])
+def test_long_and_short_sequences_together(tracea_gpu, sq, long, e4m3):
+    """70 sequences, most of them short, cut one by one (20000 keys) or as one line of steps, parts of which begin and end anywhere."""
     lengths = [(i * 37) % 90 for i in range(70)]
-    lengths[3], lengths[66] = 20000, 3001
-    run(tracea_gpu, 22, 70, 4, 2, sq, lengths, 64, 32, torch.bfloat16, e4m3)
+    lengths[3], lengths[66] = long, 3001
+    run(tracea_gpu, 22, 70, 4, 2, sq, lengths, 64, 32 if long < 50000 else 1024, torch.bfloat16, e4m3)
 
 
 @pytest.mark.parametrize("dtype", HALVES, ids=["f16", "bf16"])

@@ -2,8 +2,11 @@
 //
 // A problem is a block of rows of a (sequence, key/value head); its steps are runs of a.step keys.  Where problems are few, the steps of all of
 // them, in the order (sequence, head, block), are one line, of which every workgroup has the same number whatever the lengths are: worked out
-// from the lengths on the device, in 32 bits (the host sees to that).  A problem cut between workgroups leaves parts in the workspace: slot
-// 2 w for a part that workgroup w begins with, 2 w + 1 for one that it comes to later; meta[problem] says which they are.
+// from the lengths on the device, in 32 bits (the host sees to that).  Where that number is small (a.apart or less), a workgroup with the
+// end of one problem and the beginning of the next would spend more on the second beginning than on its steps: every problem is cut into
+// parts of that many steps by itself, for which there are as many workgroups more as there are problems.  A problem cut between workgroups
+// leaves parts in the workspace: slot 2 w for a part that workgroup w begins with, 2 w + 1 for one that it comes to later; meta[problem] says
+// which they are.
 #pragma once
 #include "attention_tile.hpp"
 #include "cache.hpp"
@@ -26,48 +29,53 @@ __device__ __forceinline__ int steps_of(const AttentionCachedArgs &a, int b) {
   return max(1, (keys_of(a, b) + a.step - 1) >> a.step_log2);
 }
 
-// A workgroup's share of the line: `left` steps from step s0 of `inner` (head and block of rows) of sequence b, whose problems have sb steps.
+// A workgroup's share: `left` steps from step s0 of `inner` (head and block of rows) of sequence b, whose problems have sb steps.
 struct Share {
   int b, inner, s0, sb, left;
-  int first, per;  // of the line
+  int first, per;  // where it begins in the line, or -1: a part of a problem cut by itself; steps of a share
 };
 __device__ __forceinline__ bool share_of(const AttentionCachedArgs &a, int lane, Share &w) {
-  const int per_b = a.Hk * a.row_blocks;
-  auto scan = [&](int b0, int &own, int &total) __attribute__((always_inline)) {  // steps in front of lane l's sequence
-    own = b0 + lane < a.B ? steps_of(a, b0 + lane) : 0;
+  const int per_b = a.Hk * a.row_blocks, here = lane < a.B ? steps_of(a, lane) : 0;
+  int steps, own, total, before = 0, mine;  // of lane l's sequence: steps and units of a problem, units in front of it
+  auto scan = [&](int b0, int unit) __attribute__((always_inline)) {
+    steps = b0 == 0 ? here : b0 + lane < a.B ? steps_of(a, b0 + lane) : 0;
+    own = unit == 1 ? steps : (int)((unsigned)(steps + unit - 1) / (unsigned)unit);
     int x = own * per_b;
-    const int mine = x;
+    mine = -x;
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
       const int y = __shfl_up(x, m, 64);
       x += lane >= m ? y : 0;
     }
     total = __builtin_amdgcn_readlane(x, 63);
-    return x - mine;
+    mine += x;
   };
-  int own, total, all = 0, before = 0, mine = scan(0, own, total);
-  all = total;
+  scan(0, 1);
+  int all = total;
   for (int b0 = 64; b0 < a.B; b0 += 64) {
-    int o, t;
-    (void)scan(b0, o, t);
-    all += t;
+    scan(b0, 1);
+    all += total;
   }
-  w.per = max(a.least, (int)(((unsigned)all + (unsigned)a.workgroups - 1) / (unsigned)a.workgroups));
-  if ((long long)blockIdx.x * w.per >= all) return false;
-  w.first = (int)blockIdx.x * w.per;
-  w.left = min(w.per, all - w.first);
+  w.per = (int)(((unsigned)all + (unsigned)a.shares - 1) / (unsigned)a.shares);
+  const bool apart = w.per <= a.apart;
+  if (!apart && (long long)blockIdx.x * w.per >= all) return false;
+  const int at_unit = apart ? (int)blockIdx.x : (int)blockIdx.x * w.per, unit = apart ? w.per : 1;
   int b0 = 0;
-  while (before + total <= w.first) {
+  if (apart || a.B > 64) scan(0, unit);
+  while (before + total <= at_unit) {
     before += total;
     b0 += 64;
-    mine = scan(b0, own, total);
+    if (b0 >= a.B) return false;
+    scan(b0, unit);
   }
-  const int at = 63 - __clzll(__ballot(before + mine <= w.first && own > 0));
+  const int at = 63 - __clzll(__ballot(before + mine <= at_unit && own > 0));
   w.b = b0 + at;
-  w.sb = __builtin_amdgcn_readlane(own, at);
-  const int u = w.first - (before + __builtin_amdgcn_readlane(mine, at));
-  w.inner = __builtin_amdgcn_readfirstlane((int)((unsigned)u / (unsigned)w.sb));
-  w.s0 = u - w.inner * w.sb;
+  w.sb = __builtin_amdgcn_readlane(steps, at);
+  const int u = at_unit - (before + __builtin_amdgcn_readlane(mine, at)), units = __builtin_amdgcn_readlane(own, at);
+  w.inner = __builtin_amdgcn_readfirstlane((int)((unsigned)u / (unsigned)units));
+  w.s0 = (u - w.inner * units) * unit;
+  w.first = apart ? -1 : at_unit;
+  w.left = apart ? min(w.per, w.sb - w.s0) : min(w.per, all - at_unit);
   return true;
 }
 // The next problem of the line.
@@ -83,7 +91,7 @@ __device__ __forceinline__ void next_problem(const AttentionCachedArgs &a, Share
 __device__ __forceinline__ void write_meta(const AttentionCachedArgs &a, const Share &w, int at, int n, bool begins) {
   const long long problem = (long long)w.b * a.Hk * a.row_blocks + w.inner;
   a.meta[2 * problem] = n == w.sb ? -1 : 2 * (int)blockIdx.x + (begins ? 0 : 1);
-  a.meta[2 * problem + 1] = (at + w.sb - 1) / w.per - (int)blockIdx.x + 1;
+  a.meta[2 * problem + 1] = w.first < 0 ? (w.sb + w.per - 1) / w.per : (at + w.sb - 1) / w.per - (int)blockIdx.x + 1;
 }
 
 __device__ __forceinline__ float wave_max(float x) {

@@ -66,7 +66,7 @@ __global__ void __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu
   const long long problem = ((long long)b * a.Hk + hk) * a.row_blocks + rb;
   bool cut = false;
   if (gridDim.y > 1) {  // the problem's steps in even parts
-    const int per = max(a.least, (steps + (int)gridDim.y - 1) / (int)gridDim.y), parts = max(1, (steps + per - 1) / per);
+    const int per = max(1, (steps + (int)gridDim.y - 1) / (int)gridDim.y), parts = max(1, (steps + per - 1) / per);
     cut = parts > 1;
     if (blockIdx.y == 0 && threadIdx.x == 0) {
       a.meta[2 * problem] = cut ? (int)(problem * gridDim.y) : -1;

@@ -93,9 +93,10 @@ struct AttentionCachedArgs {
   int rows;        // of a block: 16 or 32 (waves share the keys), 128 (they share tiles of them)
   int row_blocks;  // blocks of rows of a (sequence, key/value head)
   int step, step_log2;  // keys of a workgroup's step
-  int workgroups;  // up to 32 rows; 0: one for each block of rows; else the steps of all of them are shared out evenly
+  int workgroups;  // up to 32 rows; 0: one for each block of rows; else the steps of all of them are shared out evenly,
+  int shares;      // to so many of them,
+  int apart;       // or every problem by itself where a share has no more steps than this
   int splits;      // 128 rows: parts of a block's steps
-  int least;       // steps of a workgroup, at least
   int *meta;       // [problems][2]: first slot of its parts or -1, their number; null: no problem is cut
   int slots;       // from one part to the next: 2 (up to 32 rows) or 1
   float *part_o, *part_ml;  // [slot][rows][64 or 128], [..][2]

@@ -157,14 +157,15 @@ TraceaStatus read_cache(const char *op, const TraceaTensorView &tk, const Tracea
   return TRACEA_SUCCESS;
 }
 
-// Whether few problems (blocks of up to 32 rows) of up to `most` steps share their steps out.  Unshared, a workgroup walks its problem at 0.74
-// to 1.1 us a step until the cache's bytes bound it; shared, the line is worked out and parts are joined by a second launch, 4.4 us more.  us
-// unshared / shared, one query, Hk 8, D128 e4m3: B1 512 keys 8.8 / 10.9, 1024 11.7 / 10.8, 4096 29.5 / 11.0; B16 1024 15.1 / 15.6, 4096 39.6 / 29.9;
-// B48 512 14.5 / 21.2, 4096 85 / 91 (lengths alike; of unlike lengths the shares gain: 0.9).
+// Whether few problems (blocks of up to 32 rows) of up to `most` steps share their steps out.  Unshared, a workgroup walks its problem at 0.75
+// to 1.1 us a step, more slowly the more walk beside it, until the cache's bytes bound it; shared, the lengths are worked through and parts are
+// joined by a second launch, 4.2 us more.  us unshared / shared, one query, Hk 8, D128 e4m3: B1 512 keys 8.5 / 9.8, 800 10.5 / 10.2; B4 640 9.3 /
+// 10.3, 1000 11.6 / 10.4; B16 800 13.5 / 15.2, 1200 16.5 / 16.5, 4096 39.6 / 29.9; B48 2000 46.7 / 53.4; 5 queries of 4 heads, Hk 4, D96 f16: B16 700 14.7 /
+// 14.8, 1000 17.2 / 15.9 (lengths alike; of unlike lengths the shares gain: 0.9).
 bool shares_pay(long long problems, long long most, bool e4m3, double width, int rows) {
   if (most <= 2 || problems * most >= (1ll << 30) || problems > 65535) return false;
-  const double bytes = (e4m3 ? 6.2e-3 : 12.4e-3) * width * problems, step = (rows > 16 ? 1.1 : 1.0) * (e4m3 ? 1.0 : 1.1);
-  return 6.0 + most * std::max(step, bytes) > 10.4 + 0.9 * most * bytes;
+  const double bytes = (e4m3 ? 6.2e-3 : 12.4e-3) * width * problems, more = rows > 16 ? 1.1 : 1.0;
+  return 5.5 * more + most * std::max(more * ((e4m3 ? 0.75 : 1.0) + 0.002 * problems), bytes) > 9.7 + 0.9 * most * bytes;
 }
 
 // Parts of the steps (tiles of 64 keys) of blocks of 128 rows, by the least of this estimate (us).  A workgroup alone on its CU takes 1.8 us a
@@ -554,7 +555,6 @@ TraceaStatus dispatch_attention_cached(const TraceaTensorView &tq, const TraceaT
   const long long cus = (long long)device_limits().cus, most = std::max(1ll, ((long long)a.table.M * c.pages.P + a.step - 1) / a.step);
   const double width_of = D <= 64 ? 0.5 : 1.0;
   long long slots = 0;
-  a.least = tiles ? 1 : 2;
   a.slots = tiles ? 1 : 2;
   if (tiles) {
     a.splits = plan_tiles(problems, most, c.e4m3, width_of, cus);
@@ -562,7 +562,14 @@ TraceaStatus dispatch_attention_cached(const TraceaTensorView &tq, const TraceaT
   } else if (shares_pay(problems, most, c.e4m3, width_of, a.rows)) {
     // One workgroup a CU leaves half the parts of two: 8 x 8192 keys of 8 bits 26.0 / 27.0 us, of 16 bits 40.0 / 40.7; of 64 columns, with half
     // as much in flight, 21.4 / 20.0.
-    a.workgroups = (int)(D <= 64 ? 2 * cus : cus);
+    a.workgroups = a.shares = (int)(D <= 64 ? 2 * cus : cus);
+    // Shares of up to 6 steps are cut problem by problem, us in a line / by themselves: 16 x 2000 keys of 96 columns, 20 rows (shares of 3) 20.3 /
+    // 18.4, 2 x 20000 (5) 22.9 / 20.0; of 10 steps and more nothing is gained, and where parts come out uneven much is lost: 8 x 8192 keys of
+    // 16 bits 40 / 46.
+    if (problems <= a.shares) {
+      a.apart = 6;
+      a.workgroups += (int)problems;
+    }
     slots = 2 * a.workgroups;
   }
   if (slots > 0) {
