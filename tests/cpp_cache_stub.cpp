@@ -54,7 +54,7 @@ long long stub_value(const char *what) {
   if (is("qk.beside")) return g_qk.beside;
   if (is("qk.blocks")) return g_qk.blocks;
   if (is("append.vec")) return g_append.vec;
-  if (is("append.near")) return g_append.near;
+  if (is("append.held")) return g_append.held;
   if (is("append.pages")) return g_append.pages;
   if (is("append.groups")) return g_append.groups;
   if (is("append.heads")) return g_append.heads;

@@ -60,7 +60,13 @@ CASES = [  # b, hq, hk, t, d, rot, page, starts, lengths, adjacent, layout, orde
     (2, 6, 2, 20, 72, 0, 32, [9, 40], [20, 7], False, "bhsd", "nhpd"), (1, 1, 1, 40, 512, 512, 16, [7], None, False, "bhsd", "nhpd"),
     (2, 4, 70, 3, 16, 16, 16, [15, 0], None, False, "bhsd", "nhpd"), (1, 2, 1, 600, 64, 64, 512, [500], None, False, "bhsd", "nhpd"),
     (2, 5, 3, 300, 128, 128, 256, [200, 0], [300, 131], True, "bshd", "npHd"), (1, 3, 3, 300, 128, 64, 256, [131], None, False, "bhsd", "both"),
-    (1, 2, 2, 270, 128, 128, 512, [300], None, False, "bhsd", "nhpd")]
+    (1, 2, 2, 270, 128, 128, 512, [300], None, False, "bhsd", "nhpd"),
+    # pairs in fours and twos
+    (2, 5, 2, 70, 80, 40, 16, [0, 33], [70, 9], False, "bhsd", "npHd"), (2, 5, 2, 70, 80, 40, 64, [0, 33], [70, 9], True, "bshd", "npHd"),
+    (2, 3, 3, 130, 40, 40, 64, [5, 64], None, False, "bshd", "nhpd"), (2, 3, 3, 130, 40, 40, 256, [5, 64], None, True, "bhsd", "nhpd"),
+    (1, 2, 2, 50, 40, 20, 32, [3], None, False, "bhsd", "nhpd"), (1, 2, 2, 50, 40, 20, 32, [3], None, True, "bhsd", "nhpd"),
+    (1, 4, 1, 33, 88, 24, 48, [7], None, False, "bshd", "nhpd"), (2, 1, 1, 9, 72, 8, 16, [0, 9], None, True, "bhsd", "nhpd"),
+    (1, 2, 2, 300, 80, 40, 512, [9], None, False, "bhsd", "nhpd"), (1, 2, 2, 300, 80, 40, 512, [9], None, True, "bhsd", "nhpd")]
 
 
 @pytest.mark.parametrize("e4m3", [False, True], ids=["16", "e4m3"])

@@ -301,17 +301,23 @@ def test_heads_of_appending_workgroups(stub):
 
 def test_pieces_are_taken_where_rows_allow_them(stub):
     a = norm_args()
-    assert norm(stub, a) == OK and stub.stub_value(b"qk.vec") == 1 and stub.stub_value(b"qk.lanes") == 4
+    assert norm(stub, a) == OK and stub.stub_value(b"qk.vec") == 8 and stub.stub_value(b"qk.lanes") == 4
     assert norm(stub, dict(a, q=a["q"].at(2))) == OK and stub.stub_value(b"qk.vec") == 0 and stub.stub_value(b"qk.lanes") == 64
     assert norm(stub, dict(a, q=a["q"].but(stride=[2604, 651, 65, 1]))) == OK and stub.stub_value(b"qk.vec") == 0
-    assert norm(stub, norm_args(p=30)) == OK and stub.stub_value(b"qk.vec") == 0
+    assert norm(stub, dict(a, q=a["q"].at(4))) == OK and stub.stub_value(b"qk.vec") == 2 and stub.stub_value(b"qk.lanes") == 16
+    assert norm(stub, dict(a, q=a["q"].at(8))) == OK and stub.stub_value(b"qk.vec") == 4 and stub.stub_value(b"qk.lanes") == 8
+    for p, pieces in ((32, 8), (30, 2), (28, 4), (16, 8), (15, 0), (0, 8)):
+        assert norm(stub, norm_args(p=p)) == OK and stub.stub_value(b"qk.vec") == pieces, p
     a = append_args()
-    assert append(stub, a) == OK and stub.stub_value(b"append.vec") == 1 and stub.stub_value(b"append.near") == 1
-    assert append(stub, dict(a, k=a["k"].at(2))) == OK and stub.stub_value(b"append.vec") == 0
+    assert append(stub, a) == OK and stub.stub_value(b"append.vec") == 8 and stub.stub_value(b"append.held") == 1
+    assert append(stub, dict(a, k=a["k"].at(2))) == OK and stub.stub_value(b"append.vec") == 1 and stub.stub_value(b"append.held") == 0
+    assert append(stub, dict(a, q=a["q"].at(8))) == OK and stub.stub_value(b"append.vec") == 4 and stub.stub_value(b"append.held") == 0
+    for p, pieces in ((32, 8), (30, 2), (28, 4), (15, 1), (0, 8)):
+        assert append(stub, append_args(p=p)) == OK and stub.stub_value(b"append.vec") == pieces and stub.stub_value(b"append.held") == (p % 4 == 0), p
     flipped = a["v"].but(stride=[640, 320, -64, 1], ptr=1 << 50)
-    assert append(stub, dict(a, v=flipped)) == OK and stub.stub_value(b"append.near") == 0
+    assert append(stub, dict(a, v=flipped)) == OK and stub.stub_value(b"append.held") == 0
     far = a["v"].but(stride=[1 << 33, 1 << 32, 1 << 28, 1], ptr=1 << 50)
-    assert append(stub, dict(a, v=far)) == OK and stub.stub_value(b"append.near") == 0
+    assert append(stub, dict(a, v=far)) == OK and stub.stub_value(b"append.held") == 0
 
 
 def test_pages_outside_a_table_or_a_cache(stub):

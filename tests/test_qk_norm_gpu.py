@@ -35,7 +35,10 @@ CASES = [  # b, hq, hk, s, d, rot, sections, adjacent, layout
     (3, 5, 1, 19, 96, 96, [16, 0, 32], False, "bshd"), (1, 12, 12, 197, 64, 64, [32], True, "bshd"), (2, 3, 2, 33, 80, 40, [20], False, "bhsd"),
     (2, 2, 1, 11, 40, 40, [20], True, "bhsd"), (1, 3, 2, 50, 128, 64, [32], False, "odd"), (1, 2, 2, 9, 33, 20, [5, 5], True, "odd"),
     (1, 2, 1, 21, 512, 256, [128], False, "bshd"), (1, 2, 1, 5, 511, 511 // 2 * 2, [255], False, "bhsd"), (1, 1, 1, 3, 1, 0, [], False, "bhsd"),
-    (1, 4, 4, 700, 256, 256, [128], True, "bshd")]
+    (1, 4, 4, 700, 256, 256, [128], True, "bshd"),
+    # pairs in fours and twos
+    (2, 3, 1, 17, 40, 20, [10], False, "bshd"), (1, 3, 1, 70, 40, 20, [4, 6], True, "bhsd"), (2, 2, 2, 9, 88, 24, [12], True, "bhsd"),
+    (2, 2, 2, 9, 88, 24, [12], False, "bshd"), (1, 2, 1, 9, 12, 4, [2], False, "bhsd"), (1, 40, 8, 300, 80, 40, [20], True, "bshd")]
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "f16", "bf16"])

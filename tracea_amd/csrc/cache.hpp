@@ -42,7 +42,7 @@ struct QkNormArgs {
   int B, S, D, P, axes;
   int first[TRACEA_MAX_ROTARY_AXES];
   int adjacent;
-  int vec;     // pieces of 16 bytes
+  int vec;     // elements of a piece: 16, 8 or 4 bytes; 0: one by one
   float eps, inv_d;
   int beside;  // lane groups next to each other that take the heads of a token in turn
   int lanes;   // of a lane group, which has a row: a power of two
@@ -67,8 +67,8 @@ struct CacheAppendArgs {
   int B, T, D, P, axes;  // P pairs
   int first[TRACEA_MAX_ROTARY_AXES];
   int adjacent;
-  int vec;           // pieces of 8 elements
-  int near;          // offsets between the tokens of a page are 31-bit
+  int vec;           // elements of a piece: 8, 4, 2 or 1
+  int held;          // rows on 16 bytes, pairs in fours, offsets between the tokens of a page in 31 bits
   int pages;         // that the T tokens of a sequence can touch
   int groups;        // of heads
   int heads, queries;  // key/value and query heads of a group

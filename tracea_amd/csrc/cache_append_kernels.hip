@@ -79,7 +79,7 @@ __device__ __forceinline__ void rescale(unsigned char *head, long long apart, in
   }
 }
 
-// Any sizes, E columns at a time (8, or 1 where rows are not aligned): angles of up to ANGLES pairs at once, and in 8 bits operands are read
+// Any sizes, E columns at a time (8, or 4, 2 or 1 where pairs, strides or addresses do not go into that): angles of up to ANGLES pairs at once, and in 8 bits operands are read
 // twice, for the largest value and for the codes; the second time they come from the caches.
 template <typename T, bool C8, int E, bool ADJ>
 __global__ void __launch_bounds__(256) cache_append_kernel(const CacheAppendArgs a) {
@@ -268,13 +268,17 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const CacheAppendArgs
 }
 
 // The same where a workgroup's tokens are few enough for their angles to be kept all at once and their operands in registers between the largest
-// value and the codes: every byte is read once.  Pieces of 8 columns only.  Half of the workgroup's threads, SIDE, have the keys and values, the
+// value and the codes: every byte is read once.  Rows on 16 bytes, pairs in fours.  Half of the workgroup's threads, SIDE, have the keys and values, the
 // other half the queries, so that neither waits behind the other's loads.  A thread has up to HK couples of pieces of a head: with 2, keys and values
 // are held together and queries by two heads, with 4 one after the other.  The smallest workgroup that holds a page is taken: measured with the prompts
-// above, pages of 64 52 us (64 by the kernel before), of 16 52 (78), of 128 57, of 256 57 (131).
-template <typename T, bool C8, bool ADJ, int SIDE, int HK>
+// above, pages of 64 52 us (64 by the kernel before), of 16 52 (78), of 128 57, of 256 57 (131).// Pairs of halves whose number is not a multiple of 8 go by fours: two prompts of 4096 tokens of 80 columns, 40 of them turned, 36 us
+// (129 one by one).
+enum { HALVES, HALVES_IN_FOURS, SIDE_BY_SIDE };
+
+template <typename T, bool C8, int PAIRING, int SIDE, int HK>
 __global__ void __launch_bounds__(2 * SIDE) __attribute__((amdgpu_waves_per_eu(4))) cache_append_held_kernel(const CacheAppendArgs a) {
   constexpr int WAVES = SIDE / 64, PAIRS = SIDE * HK * 8, SETS = HK == 2 ? 2 : 1;
+  constexpr bool ADJ = PAIRING == SIDE_BY_SIDE, FOURS = PAIRING == HALVES_IN_FOURS;
   typedef float f4 __attribute__((ext_vector_type(4)));
   __shared__ f4 s_cos[PAIRS / 4], s_sin[PAIRS / 4];
   __shared__ float s_max[2][2][WAVES];
@@ -289,26 +293,39 @@ __global__ void __launch_bounds__(2 * SIDE) __attribute__((amdgpu_waves_per_eu(4
   const int h0 = min(a.Hk, grp * a.heads), h1 = min(a.Hk, h0 + a.heads), q0 = min(a.Hq, grp * a.queries), q1 = min(a.Hq, q0 + a.queries);
   const int page = page_of(a.table, b, slot);
   const int tokens = page >= 0 && end > lo ? end - lo : 0;  // with a place
-  const int turned_pieces = a.P / 8, pieces = (a.D + 8) / 16;
+  const int turned_fours = a.P / 4, pieces = (a.D + 8) / 16;
 
-  // A thread's pieces are the same in every head: token (from lo) and two times 8 columns, partners that are turned by the angles from
-  // `angle` on, or columns side by side that are not (angle < 0; v < 0: there is no second).
+  // A thread's pieces are the same in every head: token (from lo) and two times 8 columns, in two halves of 4 and 4: partners that are turned by
+  // the angles from 4 angle, 4 angle + 4 on (pair), or columns that are not.  u and v begin 8 columns each (v < 0: there are none); by fours, u and v
+  // the first half's, u1 and v1 the second's (u1 < 0: there are none).
   struct Couple {
-    int t, u, v, angle;
+    int t, u, v, u1, v1, angle;
+    bool pair[2];
   };
   // (worked out where they are used, a few instructions: kept for a loop over heads they would fill the registers)
   const unsigned by_pieces = 0xffffffffu / (unsigned)pieces + 1;  // 0: divided by 1
-  auto couple = [&](int s, int turned_of) __attribute__((always_inline)) {  // turned_of: how many of a token's couples are turned
+  auto couple = [&](int s, int turned_of) __attribute__((always_inline)) {  // turned_of: how many of a token's halves are turned
     Couple p;
     unsigned i = (unsigned)id;
     asm volatile("" : "+v"(i));
     i += (unsigned)(s * SIDE);
     p.t = by_pieces == 0 ? (int)i : (int)__umulhi(i, by_pieces);
     const int piece = (int)i - p.t * pieces;
-    const bool pair = piece < turned_of;
-    p.u = !pair ? 16 * turned_of + (piece - turned_of) * 16 : ADJ ? 16 * piece : 8 * piece;
-    p.v = pair && !ADJ ? p.u + a.P : p.u + 8 < a.D ? p.u + 8 : -1;
-    p.angle = pair ? (p.t * a.P + piece * 8) / 4 : -1;
+    p.pair[0] = 2 * piece < turned_of;
+    p.pair[1] = 2 * piece + 1 < turned_of;
+    if constexpr (FOURS) {
+      auto half = [&](int i, bool pair, int &u, int &v) __attribute__((always_inline)) {
+        u = pair ? 4 * i : 8 * i;
+        v = pair ? u + a.P : u + 4;
+      };
+      half(2 * piece, p.pair[0], p.u, p.v);
+      half(2 * piece + 1, p.pair[1], p.u1, p.v1);
+      if (p.v1 >= a.D) p.u1 = -1;
+    } else {
+      p.u = ADJ || !p.pair[0] ? 16 * piece : 8 * piece;
+      p.v = p.pair[0] && !ADJ ? p.u + a.P : p.u + 8 < a.D ? p.u + 8 : -1;
+    }
+    p.angle = p.pair[0] ? p.t * turned_fours + 2 * piece : 0;
     return p;
   };
   using X = Piece<T, 8>;
@@ -327,16 +344,22 @@ __global__ void __launch_bounds__(2 * SIDE) __attribute__((amdgpu_waves_per_eu(4
       const Couple p = couple(s, turned_of);
       if (p.t >= count) continue;
       const unsigned row = (unsigned)p.t * (unsigned)x.ss;
-      held[first() + s] = *(const u32x4 *)(at + (row + (unsigned)p.u) * 2);
-      held[first() + HK + s] = *(const u32x4 *)(at + (row + (unsigned)(p.v < 0 ? p.u : p.v)) * 2);
+      if constexpr (FOURS) {
+        auto four = [&](int c) { return *(const u32x2 *)(at + (row + (unsigned)c) * 2); };
+        const u32x2 u = four(p.u), v = four(p.v), u1 = four(p.u1 < 0 ? p.u : p.u1), v1 = four(p.u1 < 0 ? p.v : p.v1);
+        held[first() + s] = u32x4{u[0], u[1], u1[0], u1[1]};
+        held[first() + HK + s] = u32x4{v[0], v[1], v1[0], v1[1]};
+      } else {
+        held[first() + s] = *(const u32x4 *)(at + (row + (unsigned)p.u) * 2);
+        held[first() + HK + s] = *(const u32x4 *)(at + (row + (unsigned)(p.v < 0 ? p.u : p.v)) * 2);
+      }
     }
   };
   auto turned = [&](const Couple &p, const X &x, const X &y, float (&u)[8], float (&v)[8]) __attribute__((always_inline)) {
-    const bool pair = p.angle >= 0;
-    const int angle = pair ? p.angle : 0;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const f4 c = s_cos[angle + half], sn = s_sin[angle + half];
+      const bool pair = p.pair[half];
+      const f4 c = s_cos[p.angle + half], sn = s_sin[p.angle + half];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int e = half * 4 + i;
@@ -365,17 +388,43 @@ __global__ void __launch_bounds__(2 * SIDE) __attribute__((amdgpu_waves_per_eu(4
     }
     return top;
   };
-  auto store16 = [](void *at, const float (&x)[8]) __attribute__((always_inline)) {
-    X y;
+  // A couple to a row in 16 bits or, times inv, in codes.
+  auto store = [](auto *row, const Couple &p, const float (&u)[8], const float (&v)[8], float inv) __attribute__((always_inline)) {
+    constexpr bool CODES = sizeof(*row) == 1;
+    auto piece = [&](int at, const float(&x)[8], auto from, auto count) __attribute__((always_inline)) {
+      constexpr int N = decltype(count)::value;
+      if constexpr (CODES) {
+        float y[N];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y.x[e] = (T)x[e];
-    *(X *)at = y;
+        for (int e = 0; e < N; ++e) y[e] = x[from() + e];
+        *(Codes<N> *)(row + at) = encode<N>(y, inv);
+      } else {
+        Piece<T, N> y;
+#pragma unroll
+        for (int e = 0; e < N; ++e) y.x[e] = (T)x[from() + e];
+        *(Piece<T, N> *)(row + at) = y;
+      }
+    };
+    constexpr std::integral_constant<int, 0> ZERO{};
+    constexpr std::integral_constant<int, 4> FOUR{};
+    if constexpr (FOURS) {
+      piece(p.u, u, ZERO, FOUR);
+      piece(p.v, v, ZERO, FOUR);
+      if (p.u1 >= 0) {
+        piece(p.u1, u, FOUR, FOUR);
+        piece(p.v1, v, FOUR, FOUR);
+      }
+    } else {
+      constexpr std::integral_constant<int, 8> EIGHT{};
+      piece(p.u, u, ZERO, EIGHT);
+      if (p.v >= 0) piece(p.v, v, ZERO, EIGHT);
+    }
   };
   constexpr std::integral_constant<int, 0> FIRST{};
   constexpr std::integral_constant<int, SETS == 2 ? 2 * HK : 0> SECOND{};
   float k_old = 0.0f, v_old = 0.0f;
   auto load_head = [&](int h) __attribute__((always_inline)) {
-    load_row(a.k, h, tokens, turned_pieces, FIRST);
+    load_row(a.k, h, tokens, turned_fours, FIRST);
     if constexpr (SETS == 2) load_row(a.v, h, tokens, 0, SECOND);
     if (C8 && tokens > 0 && base < 0) {
       k_old = a.ks.p[page * a.ks.sn + h * a.ks.sh];
@@ -383,8 +432,8 @@ __global__ void __launch_bounds__(2 * SIDE) __attribute__((amdgpu_waves_per_eu(4
     }
   };
   auto load_queries = [&](int h) __attribute__((always_inline)) {
-    load_row(a.q, h, hi - lo, turned_pieces, FIRST);
-    if (SETS == 2 && h + 1 < q1) load_row(a.q, h + 1, hi - lo, turned_pieces, SECOND);
+    load_row(a.q, h, hi - lo, turned_fours, FIRST);
+    if (SETS == 2 && h + 1 < q1) load_row(a.q, h + 1, hi - lo, turned_fours, SECOND);
   };
   // (on their way while the angles are worked out)
   if (of_keys && h0 < h1) load_head(h0);
@@ -408,10 +457,10 @@ __global__ void __launch_bounds__(2 * SIDE) __attribute__((amdgpu_waves_per_eu(4
 #pragma unroll
       for (int i = 0; i < SETS; ++i) {
         if (h + i >= q1) continue;
-        char *at = (char *)((T *)a.q_out.p + b * a.q_out.sb + (h + i) * a.q_out.sh + lo * a.q_out.ss);
+        T *at = (T *)a.q_out.p + b * a.q_out.sb + (h + i) * a.q_out.sh + lo * a.q_out.ss;
 #pragma unroll
         for (int s = 0; s < HK; ++s) {
-          const Couple p = couple(s, turned_pieces);
+          const Couple p = couple(s, turned_fours);
           if (p.t >= hi - lo) continue;
           float u[8], v[8];
           turned(p, piece_of(2 * HK * i + s), piece_of(2 * HK * i + HK + s), u, v);
@@ -419,9 +468,7 @@ __global__ void __launch_bounds__(2 * SIDE) __attribute__((amdgpu_waves_per_eu(4
 #pragma unroll
             for (int e = 0; e < 8; ++e) u[e] = v[e] = 0.0f;
           }
-          const unsigned row = (unsigned)p.t * (unsigned)a.q_out.ss;
-          store16(at + (row + (unsigned)p.u) * 2, u);
-          if (p.v >= 0) store16(at + (row + (unsigned)p.v) * 2, v);
+          store(at + (unsigned)p.t * (unsigned)a.q_out.ss, p, u, v, 1.0f);
         }
       }
     }
@@ -447,7 +494,7 @@ __global__ void __launch_bounds__(2 * SIDE) __attribute__((amdgpu_waves_per_eu(4
           float u[8], v[8];
           turned(p, piece_of(first() + s), piece_of(first() + HK + s), u, v);
           top = largest(u, top, finite);
-          if (p.v >= 0) top = largest(v, top, finite);
+          top = largest(v, top, finite);  // (what is not there repeats what is)
         }
 #pragma unroll
         for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
@@ -474,18 +521,13 @@ __global__ void __launch_bounds__(2 * SIDE) __attribute__((amdgpu_waves_per_eu(4
       float u[8], v[8];
       turned(p, piece_of(first() + s), piece_of(first() + HK + s), u, v);
       unsigned char *row = rows + (unsigned)p.t * (unsigned)cache.ss;
-      if constexpr (C8) {
-        *(Codes<8> *)(row + p.u) = encode<8>(u, inv);
-        if (p.v >= 0) *(Codes<8> *)(row + p.v) = encode<8>(v, inv);
-      } else {
-        store16(row + p.u * 2, u);
-        if (p.v >= 0) store16(row + p.v * 2, v);
-      }
+      if constexpr (C8) store(row, p, u, v, inv);
+      else store((T *)row, p, u, v, 1.0f);
     }
   };
   for (int h = h0; h < h1 && tokens > 0; ++h) {
     if (h > h0) load_head(h);
-    leave(h, a.kc, a.ks, k_old, turned_pieces, s_max[h & 1][0], FIRST);
+    leave(h, a.kc, a.ks, k_old, turned_fours, s_max[h & 1][0], FIRST);
     if constexpr (SETS == 1) load_row(a.v, h, tokens, 0, SECOND);
     leave(h, a.vc, a.vs, v_old, 0, s_max[h & 1][1], SECOND);
   }
@@ -496,12 +538,13 @@ int launch(const CacheAppendArgs &a, hipStream_t stream) {
   const dim3 grid((unsigned)(a.pages * a.groups), (unsigned)a.B);
   const int tokens = a.T < a.table.P ? a.T : a.table.P, pieces = (a.D + 8) / 16;
   auto holds = [&](int side, int held) {
-    return a.vec && a.near && tokens * a.P <= side * held * 8 && tokens * pieces <= side * held;
+    return a.held && tokens * a.P <= side * held * 8 && tokens * pieces <= side * held;
   };
 #define HELD(SIDE, HK)                                                                                                                     \
   if (holds(SIDE, HK)) {                                                                                                                   \
-    if (a.adjacent) hipLaunchKernelGGL((cache_append_held_kernel<T, C8, true, SIDE, HK>), grid, dim3(2 * SIDE), 0, stream, a);             \
-    else hipLaunchKernelGGL((cache_append_held_kernel<T, C8, false, SIDE, HK>), grid, dim3(2 * SIDE), 0, stream, a);                       \
+    if (a.adjacent) hipLaunchKernelGGL((cache_append_held_kernel<T, C8, SIDE_BY_SIDE, SIDE, HK>), grid, dim3(2 * SIDE), 0, stream, a);       \
+    else if (a.P % 8 == 0) hipLaunchKernelGGL((cache_append_held_kernel<T, C8, HALVES, SIDE, HK>), grid, dim3(2 * SIDE), 0, stream, a);      \
+    else hipLaunchKernelGGL((cache_append_held_kernel<T, C8, HALVES_IN_FOURS, SIDE, HK>), grid, dim3(2 * SIDE), 0, stream, a);               \
     return (int)hipGetLastError();                                                                                                         \
   }
   HELD(64, 2)
@@ -510,10 +553,16 @@ int launch(const CacheAppendArgs &a, hipStream_t stream) {
   HELD(512, 2)
   HELD(512, 4)
 #undef HELD
-  if (a.vec && a.adjacent) hipLaunchKernelGGL((cache_append_kernel<T, C8, 8, true>), grid, dim3(256), 0, stream, a);
-  else if (a.vec) hipLaunchKernelGGL((cache_append_kernel<T, C8, 8, false>), grid, dim3(256), 0, stream, a);
-  else if (a.adjacent) hipLaunchKernelGGL((cache_append_kernel<T, C8, 1, true>), grid, dim3(256), 0, stream, a);
-  else hipLaunchKernelGGL((cache_append_kernel<T, C8, 1, false>), grid, dim3(256), 0, stream, a);
+#define PIECES(E)                                                                                                      \
+  if (a.vec == E) {                                                                                                    \
+    if (a.adjacent) hipLaunchKernelGGL((cache_append_kernel<T, C8, E, true>), grid, dim3(256), 0, stream, a);          \
+    else hipLaunchKernelGGL((cache_append_kernel<T, C8, E, false>), grid, dim3(256), 0, stream, a);                    \
+  }
+  PIECES(8)
+  PIECES(4)
+  PIECES(2)
+  PIECES(1)
+#undef PIECES
   return (int)hipGetLastError();
 }
 

@@ -237,14 +237,17 @@ void set_qk_norm(const QkNorm &c, const Rotation &r, const View *const *tensors,
   a->adjacent = params.adjacent != 0;
   a->eps = params.eps;
   a->inv_d = 1.0f / (float)c.D;
-  const int e = 16 / elem_size(c.dtype);
-  // (the D - 2P columns that are not turned go two pieces to a thread)
-  a->vec = a->P % e == 0 && (c.D - 2 * a->P) % (2 * e) == 0 && c.D / (2 * e) <= 64;
-  for (int i = 0; i < n; ++i)
-    if (!rows_on(*tensors[i], 16)) a->vec = 0;
+  // Pieces of 16 bytes, or of 8 or 4 where pairs, columns that are not turned (they go two pieces to a thread), strides or addresses do not go into
+  // them; else single elements.  S24960 H32:8 bf16, D80 of which 40 turned (8 bytes) 84 us, D40 of which 20 (4 bytes) 74; one by one 371, 351.
+  const int size = elem_size(c.dtype);
+  for (int e = 16 / size; e >= 2 && a->vec == 0; e /= 2) {
+    a->vec = a->P % e == 0 && (c.D - 2 * a->P) % (2 * e) == 0 && c.D / (2 * e) <= 64 ? e : 0;
+    for (int i = 0; i < n; ++i)
+      if (!rows_on(*tensors[i], (size_t)(e * size))) a->vec = 0;
+  }
   a->lanes = 64;
   if (a->vec)
-    while (a->lanes / 2 * 2 * e >= c.D && a->lanes > 1) a->lanes /= 2;
+    while (a->lanes * a->vec >= c.D && a->lanes > 1) a->lanes /= 2;
   const long long heads = a->H[0] + a->H[1], tokens = c.B * c.S, groups = 256 / a->lanes;
   // Lane groups that share a token's angles take its heads in turn: as many as fill the device with 8 waves a CU where tokens are few; else,
   // where heads lie side by side, 8 forward (pieces next to each other: S24960 H32:8 D128 bf16, by 8 / 4 / 2 groups 99 / 104 / 120 us) and 2 backward, where
@@ -443,11 +446,15 @@ TraceaStatus dispatch_cache_append(const TraceaTensorView &tk, const TraceaTenso
   set_rotation(r, &a);
   a.B = (int)B; a.T = (int)T; a.D = (int)D;
   a.adjacent = params.adjacent != 0;
-  a.vec = a.P % 8 == 0;
-  for (const View *t : operands) a.vec = a.vec && rows_on(*t, 16);
-  a.near = 1;
-  for (const View *t : operands) a.near = a.near && t->stride[2] >= 0 && (t->stride[2] * std::min(T, (long long)c.pages.P) + D) * 2 < (1ll << 31);
-  for (const View *t : {&c.k, &c.v}) a.near = a.near && (t->stride[2] * c.pages.P + D) * 2 < (1ll << 31);
+  for (a.vec = 8; a.vec > 1; a.vec /= 2) {
+    bool fits = a.P % a.vec == 0;
+    for (const View *t : operands) fits = fits && rows_on(*t, (size_t)(2 * a.vec));
+    if (fits) break;
+  }
+  a.held = a.P % 4 == 0;
+  for (const View *t : operands)
+    a.held = a.held && rows_on(*t, 16) && t->stride[2] >= 0 && (t->stride[2] * std::min(T, (long long)c.pages.P) + D) * 2 < (1ll << 31);
+  for (const View *t : {&c.k, &c.v}) a.held = a.held && (t->stride[2] * c.pages.P + D) * 2 < (1ll << 31);
   const long long pages = (T + c.pages.P - 2) / c.pages.P + 1;
   if (B > 65535 || pages >= (1 << 22)) return fail(TRACEA_UNSUPPORTED_CONFIG, "%s: %lld sequences of %lld new tokens are more than is supported", op, B, T);
   a.pages = (int)pages;

@@ -3,8 +3,8 @@
 //   backward  dn = R^T dy, g = dn w, dx = r (g - x^ mean(g x^)), x^ = x r; dw = sum over all rows of dn x^
 //
 // Bound by memory: every element is read once and written once.  A row (a head of a token) is held by a group of lanes, each
-// with the two pieces of 16 bytes that hold the partners of a pair, so that the rotation needs no exchange and the norm one sum over
-// the group.  The sine and cosine of a pair are worked out once for the heads that a lane group has of a token.
+// with the two pieces of 16 bytes (8 or 4 where the sizes ask for it) that hold the partners of a pair, so that the rotation needs no exchange and
+// the norm one sum over the group.  The sine and cosine of a pair are worked out once for the heads that a lane group has of a token.
 // The backward pass recomputes r, takes both sums of a row at once, keeps the weights' gradients of its rows in registers, joins
 // them per workgroup, and a second kernel adds the workgroups' up in their order.
 #include "cache.hpp"
@@ -24,11 +24,12 @@ struct __attribute__((packed, aligned(4))) Floats {  // of a weight, wherever it
   float x[E];
 };
 
-// What a lane holds of a row: N pairs (u, v) of columns.  In pieces: N = 16 bytes of u and of v; else, one by one, up to 4 pairs that are turned
-// and 4 couples of columns that are not.
-template <typename T, bool VEC, bool ADJ>
+// What a lane holds of a row: N pairs (u, v) of columns.  In pieces: N = E elements of u and of v; else (E 0), one by one, up to 4 pairs that are
+// turned and 4 couples of columns that are not.
+template <typename T, int E, bool ADJ>
 struct Lane {
-  static constexpr int E = 16 / sizeof(T), N = VEC ? E : 8;
+  static constexpr bool VEC = E > 0;
+  static constexpr int N = VEC ? E : 8;
   int at_u, at_v;  // pieces
   bool there, turned;
   int lane, D, P;
@@ -184,9 +185,9 @@ __device__ __forceinline__ T *row_of(const HeadView &t, int b, int h, int s) {
   return (T *)t.p + b * t.sb + h * t.sh + s * t.ss;
 }
 
-template <typename T, bool VEC, bool ADJ>
+template <typename T, int E, bool ADJ>
 __global__ void __launch_bounds__(256) qk_norm_forward_kernel(const QkNormArgs a) {
-  using L = Lane<T, VEC, ADJ>;
+  using L = Lane<T, E, ADJ>;
   constexpr int N = L::N;
   const int groups = 256 / a.lanes, lane = threadIdx.x & (a.lanes - 1);
   const L me(lane, a.D, a.P);
@@ -222,9 +223,9 @@ __global__ void __launch_bounds__(256) qk_norm_forward_kernel(const QkNormArgs a
   }
 }
 
-template <typename T, bool VEC, bool ADJ>
+template <typename T, int E, bool ADJ>
 __global__ void __launch_bounds__(256) qk_norm_backward_kernel(const QkNormArgs a) {
-  using L = Lane<T, VEC, ADJ>;
+  using L = Lane<T, E, ADJ>;
   constexpr int N = L::N;
   extern __shared__ float s_dw[];  // [lane groups][D]
   const int groups = 256 / a.lanes, lane = threadIdx.x & (a.lanes - 1), group = threadIdx.x / a.lanes;
@@ -314,17 +315,17 @@ __global__ void __launch_bounds__(1024) qk_norm_weights_kernel(const QkNormArgs 
   if (run == 0 && col < a.D) a.dw[t][col] = s_sum[0][c16];
 }
 
-template <typename T, bool VEC, bool ADJ>
+template <typename T, int E, bool ADJ>
 int launch(const QkNormArgs &a, bool backward, hipStream_t stream) {
   const int groups = 256 / a.lanes;
   if (!backward) {
     // (at most 2^31 threads along x: a launch of 2^32 and more drops some of them without an error)
     const long long blocks = ((long long)a.B * a.S * a.beside + groups - 1) / groups, most = 1ll << 23, turns = (blocks + most - 1) / most;
     if (turns > 65535) return (int)hipErrorInvalidValue;
-    hipLaunchKernelGGL((qk_norm_forward_kernel<T, VEC, ADJ>), dim3((unsigned)((blocks + turns - 1) / turns), (unsigned)turns), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((qk_norm_forward_kernel<T, E, ADJ>), dim3((unsigned)((blocks + turns - 1) / turns), (unsigned)turns), dim3(256), 0, stream, a);
     return (int)hipGetLastError();
   }
-  hipLaunchKernelGGL((qk_norm_backward_kernel<T, VEC, ADJ>), dim3((unsigned)a.blocks), dim3(256), (unsigned)(groups * a.D * 4), stream, a);
+  hipLaunchKernelGGL((qk_norm_backward_kernel<T, E, ADJ>), dim3((unsigned)a.blocks), dim3(256), (unsigned)(groups * a.D * 4), stream, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || (a.dw[0] == nullptr && a.dw[1] == nullptr)) return (int)e;
   hipLaunchKernelGGL(qk_norm_weights_kernel, dim3((unsigned)((a.D + 15) / 16), 2), dim3(1024), 0, stream, a);
@@ -332,8 +333,15 @@ int launch(const QkNormArgs &a, bool backward, hipStream_t stream) {
 }
 template <typename T>
 int launch_type(const QkNormArgs &a, bool backward, hipStream_t stream) {
-  if (a.vec) return a.adjacent ? launch<T, true, true>(a, backward, stream) : launch<T, true, false>(a, backward, stream);
-  return a.adjacent ? launch<T, false, true>(a, backward, stream) : launch<T, false, false>(a, backward, stream);
+#define PIECES(E) \
+  if (a.vec == E) return a.adjacent ? launch<T, E, true>(a, backward, stream) : launch<T, E, false>(a, backward, stream);
+  if constexpr (sizeof(T) == 2) {
+    PIECES(8)
+  }
+  PIECES(4)
+  PIECES(2)
+#undef PIECES
+  return a.adjacent ? launch<T, 0, true>(a, backward, stream) : launch<T, 0, false>(a, backward, stream);
 }
 int launch_any(const QkNormArgs &a, int dtype, bool backward, hipStream_t stream) {
   if (dtype == DT_F32) return launch_type<float>(a, backward, stream);
