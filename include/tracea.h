@@ -519,8 +519,9 @@ TraceaStatus tracea_norm_gate_residual_backward(const TraceaTensorView *dx_out, 
  * writing y is fp32.
  * The backward pass takes the gradients of the results (dq_out, dk_out) back through the rotation and the norm, which it works out
  * again from q and k: dq, dk (required with q, k) have the type of q, dq_weight, dk_weight [D] f32 (optional) are sums over all heads, tokens
- * and batch entries in an order that does not change; without weights there are no such gradients.  dq may be dq_out or q as the same view, dk likewise.  With weight gradients it takes
- * a workspace per (device, stream), 8 bytes per value of a head and workgroup, at most 4 MiB, never grown under capture. */
+ * and batch entries in an order that does not change; without weights there are no such gradients.  dq may be dq_out or q as the same view,
+ * dk likewise.  With weight gradients it takes a workspace per (device, stream), 8 bytes per value of a head and workgroup, at most 4 MiB,
+ * never grown under capture. */
 typedef struct {
   uint32_t axes;
   uint32_t sections[TRACEA_MAX_ROTARY_AXES];
@@ -542,7 +543,7 @@ TraceaStatus tracea_qk_norm_rotary_backward(TraceaTensorView dq_out, const Trace
  *   k_cache, v_cache [N,Hk,P,D]: N pages, P a multiple of 16, D contiguous and a multiple of 8, other strides multiples of 8
  *   elements and not negative (the order of heads and tokens is the caller's), bases on 16 bytes, or 8 in 8 bits; of the operands' type, f16 or
  *   bf16, or TRACEA_DTYPE_FLOAT8_E4M3 with
- *   k_scale, v_scale [N,Hk] f32, any strides: a value of page n and head h is its code times scale[n,h]
+ *   k_scale, v_scale [N,Hk] f32, any strides, finite and not negative where a page is used: a value of page n and head h is its code times scale[n,h]
  *   page_table [B,M] i32, M contiguous: token t of sequence b lies in page page_table[b, t / P], place t % P.  What a sequence does
  *   not use yet may hold anything; a token whose entry is outside 0..N-1, or that lies behind M P, has no place: it is not written, and no query sees it.
  *
@@ -578,8 +579,10 @@ TraceaStatus tracea_cache_append(TraceaTensorView k, TraceaTensorView v, const T
  * Masks, empty rows, lse and scale as in tracea_attention_forward: with params.causal query i of sequence b sees the keys j <= i +
  * k_lengths[b] - q_lengths[b]; what lies behind the lengths is never used, whatever it holds.  (Infinities and NaN among the keys
  * of a sequence spread as 0 * inf does, also to a query that a causal mask hides them from.)
- * Scores, statistics and sums are fp32 or more; codes are widened exactly, scales multiply scores and probabilities in fp32,
- * probabilities are rounded once to the type of q.  The same call on the same inputs gives the same bits.  Results overlap no operand
+ * Scores, statistics and sums are fp32 or more, probabilities are rounded once to the type of q.  In 8 bits scales multiply scores and
+ * probabilities, in fp32, and in calls with more than 64 rows (Hq / Hk Sq) the keys and values, in their widening to the type of q: exactly
+ * where they are powers of two, as tracea_cache_append leaves them (in f16 as far as it reaches below the largest of them), else with one
+ * rounding more.  The same call on the same inputs gives the same bits.  Results overlap no operand
  * and not each other.  Up to M P = 2^31 - 2^16 keys, M P P < 2^40.
  * Where few rows meet many keys the keys are shared out over the device: a workspace per (device, stream), at most 80 MiB, grown on
  * demand, never under capture (without it a call runs unsplit, slower). */

@@ -4,6 +4,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 from cache_oracle import E4M3, U32, Pool, attention, check_attention, half_step, rotated  # noqa: E402
+from tracea_amd.capi import TraceaError  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 EPS = 1e-6
@@ -175,3 +176,15 @@ def test_training_step_through_norms_and_attention(tracea_gpu):
     for a, w in zip(got, want):
         # some ten roundings to 11 bits one after another, of gradients of a few times the result's size; in 2-norm
         assert (a.double() - w).norm() <= 40 * 2.0 ** -11 * w.norm()
+
+
+def test_other_operators_refuse_codes(tracea_gpu):
+    """Codes of 8 bits are a type of caches only."""
+    x = torch.randn(2, 4, 16, 64, device="cuda").to(E4M3)
+    a, pos, freq = x[0, 0], torch.zeros(2, 16, 1, dtype=torch.int32, device="cuda"), torch.ones(32, device="cuda")
+    w = torch.ones(64, device="cuda")
+    for call in (lambda: tracea_gpu.gemm(a, a.t()), lambda: tracea_gpu.attention(x, x, x), lambda: tracea_gpu.softmax(a),
+                 lambda: tracea_gpu.attention_forward(x, x, x), lambda: tracea_gpu.rotary(x, x, pos, freq),
+                 lambda: tracea_gpu.qk_norm_rotary(x, x, w, w, pos, freq), lambda: tracea_gpu.norm_gate_residual(x[0], x[0], w, None, w)):
+        with pytest.raises((TraceaError, TypeError)):
+            call()

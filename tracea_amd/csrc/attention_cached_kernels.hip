@@ -14,9 +14,14 @@
 //                 permutation per two values.  The result has row l & 15 and, over the VC products, VC columns in a run for each of 4 lanes' chunks.
 // Codes of 8 bits become f16 or bf16 exactly on the way (two per instruction).
 //
-// A wave walks every fourth block of 32 keys, the next one requested before it works on the last; a workgroup's four waves join through LDS.
-// Where blocks of rows are few, all steps of 128 keys of all sequences are one line that the workgroups share out evenly, whatever the
+// A wave walks every fourth block of 32 keys, the next one requested while it works on the last; a workgroup's four waves join through LDS.
+// Where blocks of rows are few, all steps of 128 keys of all sequences are shared out evenly (attention_cached_share.hpp), whatever the
 // lengths; a problem cut between workgroups is joined by a second launch, parts in their order.
+//
+// One query of 40:8 heads over 131072 keys of 128 columns in 8 bits (269 MB): 55 to 62 us, 4.3 to 4.9 TB/s (a copy: 5.06), 4 to 5 of them the second
+// launch; 8 sequences of up to 8192 keys, 32:8 heads, 26 us (a copy: 18), of which 5 are a chain of dependent loads (lengths, table, keys, values)
+// before the first result and 4 the second launch; 5 queries of 16:4 heads of 96 columns over 16 sequences of up to 2000 keys in 16 bits 18 us
+// (a copy: 6.4), the same chain and three steps; one query of 12 heads over 197 keys 5.5 us.
 #include <algorithm>
 #include <type_traits>
 
