@@ -9,6 +9,7 @@ torch supplies device memory and the current stream; all arithmetic happens in
 """
 import ctypes as C
 import math
+import struct
 
 import torch
 
@@ -342,9 +343,9 @@ def attention(q, k, v, causal=False, scale=0.0, out=None):
 _LAYOUTS = {}
 
 
-def _plain_view(t):
-    """capi.TensorView of a tensor.  The extent and stride arrays it borrows, and the bytes of a view without its address, are kept by
-    layout (shape, strides, type and device), never by a tensor's address; the view holds them."""
+def _layout(t):
+    """What a view of the tensor holds apart from its address: (the view's bytes, its owner, the bytes behind the address).  Kept by shape, strides,
+    type and device, never by a tensor's address."""
     key = (t.shape, t.dtype, t.get_device()) if t.is_contiguous() else (t.shape, t.stride(), t.dtype, t.get_device())
     layout = _LAYOUTS.get(key)
     if layout is None:
@@ -357,11 +358,52 @@ def _plain_view(t):
         if t.is_contiguous():  # (whatever stands for the extents of 1: one layout whichever such tensor comes first)
             strides = [math.prod(max(n, 1) for n in t.shape[i + 1:]) for i in range(t.dim())]
         v = capi.View(None, t.shape, strides, dtype, t.get_device())
-        layout = _LAYOUTS[key] = (bytes(v.c), v)
+        layout = _LAYOUTS[key] = (bytes(v.c), v, bytes(v.c)[8:])
+    return layout
+
+
+def _plain_view(t):
+    """capi.TensorView of a tensor.  The extent and stride arrays it borrows, and the bytes of a view without its address, are kept by
+    layout; the view holds them."""
+    layout = _layout(t)
     view = capi.TensorView.from_buffer_copy(layout[0])
     view.ptr = t.data_ptr()
     view.layout = layout
     return view
+
+
+class _Frame:
+    """The views of a call's operands, side by side: filled in one go, taken by one call at a time."""
+
+    def __init__(self):
+        self.buffer = (capi.TensorView * 16)()
+        self.views = [self.buffer[i] for i in range(16)]
+
+
+_FRAMES = []
+_FILLS = [struct.Struct("P32s" * n) for n in range(17)]  # an address and the rest of a view
+
+
+def _call(name, params, *operands):
+    """The entry point of that name on the operands (None: left out), views in the order of its arguments."""
+    try:
+        frame = _FRAMES.pop()
+    except IndexError:
+        frame = _Frame()
+    fields, layouts, args = [], [], []  # (layouts: what the views point to lives as long as the call)
+    for t, view in zip(operands, frame.views):
+        if t is None:
+            fields += (0, b"")
+            args.append(None)
+            continue
+        layout = _layout(t)
+        layouts.append(layout)
+        fields += (t.data_ptr(), layout[2])
+        args.append(view)
+    _FILLS[len(operands)].pack_into(frame.buffer, 0, *fields)
+    st = getattr(capi.lib(), name)(*args, params)
+    _FRAMES.append(frame)
+    capi.check(name, st)
 
 
 def _ref(t):
@@ -477,9 +519,7 @@ def qk_norm_rotary(q, k, q_weight=None, k_weight=None, positions=None, inv_freq=
     if k is not None:
         k_out = torch.empty_like(k) if k_out is None else k_out
     params = capi.QkNormParams(axes, pairs, 1 if adjacent else 0, float(eps), _stream(q))
-    st = capi.lib().tracea_qk_norm_rotary(_plain_view(q), _ref(k), _ref(q_weight), _ref(k_weight), _ref(positions), _ref(inv_freq),
-                                          _ref(q_out), _ref(k_out), params)
-    capi.check("tracea_qk_norm_rotary", st)
+    _call("tracea_qk_norm_rotary", params, q, k, q_weight, k_weight, positions, inv_freq, q_out, k_out)
     return q_out, k_out
 
 
@@ -493,10 +533,7 @@ def qk_norm_rotary_backward(dq_out, dk_out, q, k, q_weight=None, k_weight=None, 
     dq_weight = None if q_weight is None else torch.empty_like(q_weight)
     dk_weight = None if k_weight is None else torch.empty_like(k_weight)
     params = capi.QkNormParams(axes, pairs, 1 if adjacent else 0, float(eps), _stream(q))
-    st = capi.lib().tracea_qk_norm_rotary_backward(_plain_view(dq_out), _ref(dk_out), _plain_view(q), _ref(k), _ref(q_weight), _ref(k_weight),
-                                                   _ref(positions), _ref(inv_freq), _ref(dq), _ref(dk), _ref(dq_weight), _ref(dk_weight),
-                                                   params)
-    capi.check("tracea_qk_norm_rotary_backward", st)
+    _call("tracea_qk_norm_rotary_backward", params, dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_freq, dq, dk, dq_weight, dk_weight)
     return dq, dk, dq_weight, dk_weight
 
 
@@ -511,10 +548,7 @@ def cache_append(k, v, k_cache, v_cache, page_table, starts, lengths=None, k_sca
     if q is not None:
         q_out = torch.empty_like(q) if q_out is None else q_out
     params = capi.CacheAppendParams(axes, pairs, 1 if adjacent else 0, _stream(k))
-    st = capi.lib().tracea_cache_append(_plain_view(k), _plain_view(v), _ref(q), _ref(k_cache), _ref(v_cache), _ref(k_scale), _ref(v_scale),
-                                        _plain_view(page_table), _plain_view(starts), _ref(lengths), _ref(positions), _ref(inv_freq),
-                                        _ref(q_out), params)
-    capi.check("tracea_cache_append", st)
+    _call("tracea_cache_append", params, k, v, q, k_cache, v_cache, k_scale, v_scale, page_table, starts, lengths, positions, inv_freq, q_out)
     return q_out
 
 
@@ -526,7 +560,5 @@ def attention_cached(q, k_cache, v_cache, page_table, k_lengths, q_lengths=None,
     key: o 0, lse -inf."""
     out = torch.empty_like(q) if out is None else out
     params = capi.AttentionParams(1 if causal else 0, 0, float(scale), _stream(q))
-    st = capi.lib().tracea_attention_cached(_plain_view(q), _plain_view(k_cache), _plain_view(v_cache), _ref(k_scale), _ref(v_scale),
-                                            _plain_view(page_table), _ref(q_lengths), _plain_view(k_lengths), _ref(out), _ref(lse), params)
-    capi.check("tracea_attention_cached", st)
+    _call("tracea_attention_cached", params, q, k_cache, v_cache, k_scale, v_scale, page_table, q_lengths, k_lengths, out, lse)
     return out
