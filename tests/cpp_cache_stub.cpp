@@ -65,6 +65,7 @@ long long stub_value(const char *what) {
   if (is("splits")) return g_attention.splits;
   if (is("shares")) return g_attention.shares;
   if (is("apart")) return g_attention.apart;
+  if (is("line")) return g_attention.line;
   if (is("step")) return g_attention.step;
   if (is("slots")) return g_attention.slots;
   if (is("meta")) return (long long)(intptr_t)g_attention.meta;

@@ -279,8 +279,8 @@ def test_workspaces_hold_what_the_kernels_write(stub, d, cache):
                     assert v("workspace") == v("meta") - v("part_o") + problems * 8 and v("part_o") % 16 == 0
                     assert v("workspace") <= 80 << 20
                     assert problems <= 65535 and problems * -(-m * 64 // v("step")) < 1 << 30
-                    if rows < 128:  # parts of problems cut by themselves: at most one more for each than the shares
-                        assert v("workgroups") >= v("shares") + (problems if v("apart") > 0 else 0)
+                    if rows < 128:  # a line's shares have workgroups, as parts for one a share and a last one for each problem have
+                        assert v("workgroups") >= v("line") and (v("apart") == 0 or v("workgroups") >= v("shares") + problems)
     a = backward_args(b=4, hq=32, hk=8, s=2048, d=128, p=64)
     assert norm_backward(stub, a) == OK and stub.stub_value(b"workspace") == 2 * stub.stub_value(b"qk.blocks") * 128 * 4 <= 4 << 20
 

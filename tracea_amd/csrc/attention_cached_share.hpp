@@ -1,12 +1,11 @@
 // What the kernels of attention over a cache share: how steps over keys are shared out between workgroups, and where pages lie.
 //
-// A problem is a block of rows of a (sequence, key/value head); its steps are runs of a.step keys.  Where problems are few, the steps of all of
-// them, in the order (sequence, head, block), are one line, of which every workgroup has the same number whatever the lengths are: worked out
-// from the lengths on the device, in 32 bits (the host sees to that).  Where that number is small (a.apart or less), a workgroup with the
-// end of one problem and the beginning of the next would spend more on the second beginning than on its steps: every problem is cut into
-// parts of that many steps by itself, for which there are as many workgroups more as there are problems.  A problem cut between workgroups
-// leaves parts in the workspace: slot 2 w for a part that workgroup w begins with, 2 w + 1 for one that it comes to later; meta[problem] says
-// which they are.
+// A problem is a block of rows of a (sequence, key/value head); its steps are runs of a.step keys.  What the workgroups have of them is worked
+// out from the lengths on the device, in 32 bits (the host sees to that), whatever the lengths are.  Either every problem is cut into parts of
+// the same number of steps by itself, a workgroup for each, where such parts are short (a.apart) and not more than the workgroups; or the
+// steps of all problems, in the order (sequence, head, block), are one line, of which every workgroup has the same number.  A problem cut
+// between workgroups leaves parts in the workspace: slot 2 w for a part that workgroup w begins with, 2 w + 1 for one that it comes to later;
+// meta[problem] says which they are.
 #pragma once
 #include "attention_tile.hpp"
 #include "cache.hpp"
@@ -50,22 +49,32 @@ __device__ __forceinline__ bool share_of(const AttentionCachedArgs &a, int lane,
     total = __builtin_amdgcn_readlane(x, 63);
     mine += x;
   };
-  scan(0, 1);
-  int all = total;
-  for (int b0 = 64; b0 < a.B; b0 += 64) {
-    scan(b0, 1);
-    all += total;
+  auto count = [&](int unit) __attribute__((always_inline)) {  // of all sequences; own, mine and total are left as the first 64 have them
+    int n = 0;
+    for (int b0 = (a.B - 1) & -64; b0 >= 0; b0 -= 64) {
+      scan(b0, unit);
+      n += total;
+    }
+    return n;
+  };
+  const int all = count(1);
+  auto per_of = [&](int shares) { return (int)(((unsigned)all + (unsigned)shares - 1) / (unsigned)shares); };
+  w.per = per_of(a.shares);
+  if (w.per > a.twice) w.per = per_of(2 * a.shares);
+  bool apart = w.per <= a.apart;
+  if (apart) {
+    const int parts = count(w.per);
+    if ((int)blockIdx.x >= parts && parts <= a.workgroups) return false;
+    apart = parts <= a.workgroups;
+    if (!apart) (void)count(1);
   }
-  w.per = (int)(((unsigned)all + (unsigned)a.shares - 1) / (unsigned)a.shares);
-  const bool apart = w.per <= a.apart;
+  if (!apart) w.per = per_of(a.line);
   if (!apart && (long long)blockIdx.x * w.per >= all) return false;
   const int at_unit = apart ? (int)blockIdx.x : (int)blockIdx.x * w.per, unit = apart ? w.per : 1;
   int b0 = 0;
-  if (apart || a.B > 64) scan(0, unit);
   while (before + total <= at_unit) {
     before += total;
     b0 += 64;
-    if (b0 >= a.B) return false;
     scan(b0, unit);
   }
   const int at = 63 - __clzll(__ballot(before + mine <= at_unit && own > 0));

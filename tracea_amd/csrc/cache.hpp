@@ -94,8 +94,9 @@ struct AttentionCachedArgs {
   int row_blocks;  // blocks of rows of a (sequence, key/value head)
   int step, step_log2;  // keys of a workgroup's step
   int workgroups;  // up to 32 rows; 0: one for each block of rows; else the steps of all of them are shared out evenly,
-  int shares;      // to so many of them,
-  int apart;       // or every problem by itself where a share has no more steps than this
+  int shares, apart;  // every problem by itself, in parts of 1 / shares of all steps if these have no more than `apart`
+  int twice;       // (of half as many where they have more than this) and if the workgroups are enough for the parts,
+  int line;        // or all problems in a line, to so many
   int splits;      // 128 rows: parts of a block's steps
   int *meta;       // [problems][2]: first slot of its parts or -1, their number; null: no problem is cut
   int slots;       // from one part to the next: 2 (up to 32 rows) or 1

@@ -157,15 +157,18 @@ TraceaStatus read_cache(const char *op, const TraceaTensorView &tk, const Tracea
   return TRACEA_SUCCESS;
 }
 
-// Whether few problems (blocks of up to 32 rows) of up to `most` steps share their steps out.  Unshared, a workgroup walks its problem at 0.75
-// to 1.1 us a step, more slowly the more walk beside it, until the cache's bytes bound it; shared, the lengths are worked through and parts are
-// joined by a second launch, 4.2 us more.  us unshared / shared, one query, Hk 8, D128 e4m3: B1 512 keys 8.5 / 9.8, 800 10.5 / 10.2; B4 640 9.3 /
-// 10.3, 1000 11.6 / 10.4; B16 800 13.5 / 15.2, 1200 16.5 / 16.5, 4096 39.6 / 29.9; B48 2000 46.7 / 53.4; 5 queries of 4 heads, Hk 4, D96 f16: B16 700 14.7 /
-// 14.8, 1000 17.2 / 15.9 (lengths alike; of unlike lengths the shares gain: 0.9).
+// Whether problems (blocks of up to 32 rows) of up to `most` steps share their steps out.  Unshared, a workgroup walks its problem at 0.75 to
+// 1.1 us a step, more slowly the more walk beside it; shared, the lengths are worked through and parts are joined by a second launch, 4.2 us more
+// and up to 1.8 where many shares begin inside a problem; then all workgroups read at what the caches' bytes allow.  us unshared / shared, one
+// query, Hk 8, D128, lengths from a quarter of the longest up, 8 bits: B1 512 keys 8.5 / 9.8, 800 10.5 / 10.2; B16 800 12.6 / 13.6, 2000 21.3 / 17.4; B30 2000
+// 22.0 / 27.5; B32 4096 51 / 46; B100 4096 121 / 118; 16 bits: B4 1000 13.7 / 10.5; B16 1200 18.6 / 21.6, 2000 26 / 21; B12 4096 49 / 28; B48 4096 118 / 101; 20 rows,
+// Hk 4, D96, 16 bits: B16 700 14.1 / 14.4, 1000 16.4 / 14.6; B160 2000 73 / 87.
 bool shares_pay(long long problems, long long most, bool e4m3, double width, int rows) {
   if (most <= 2 || problems * most >= (1ll << 30) || problems > 65535) return false;
-  const double bytes = (e4m3 ? 6.2e-3 : 12.4e-3) * width * problems, more = rows > 16 ? 1.1 : 1.0;
-  return 5.5 * more + most * std::max(more * ((e4m3 ? 0.75 : 1.0) + 0.002 * problems), bytes) > 9.7 + 0.9 * most * bytes;
+  const double n = (double)problems, more = rows > 16 ? 1.1 : 1.0;
+  const double alone = 5.5 * more + most * std::max(more * (e4m3 ? 0.75 + 0.002 * n : 1.0 + 0.004 * n), (e4m3 ? 5.0e-3 : 8.2e-3) * width * n);
+  const double shared = 9.7 + 1.8 * std::min(1.0, n / 128) + (rows > 16 ? 1.15 : 1.0) * most * (e4m3 ? 4.1e-3 : 7.0e-3) * width * n;
+  return alone > shared;
 }
 
 // Parts of the steps (tiles of 64 keys) of blocks of 128 rows, by the least of this estimate (us).  A workgroup alone on its CU takes 1.8 us a
@@ -567,15 +570,20 @@ TraceaStatus dispatch_attention_cached(const TraceaTensorView &tq, const TraceaT
     a.splits = plan_tiles(problems, most, c.e4m3, width_of, cus);
     slots = a.splits > 1 ? problems * a.splits : 0;
   } else if (shares_pay(problems, most, c.e4m3, width_of, a.rows)) {
-    // One workgroup a CU leaves half the parts of two: 8 x 8192 keys of 8 bits 26.0 / 27.0 us, of 16 bits 40.0 / 40.7; of 64 columns, with half
-    // as much in flight, 21.4 / 20.0.
-    a.workgroups = a.shares = (int)(D <= 64 ? 2 * cus : cus);
-    // Shares of up to 6 steps are cut problem by problem, us in a line / by themselves: 16 x 2000 keys of 96 columns, 20 rows (shares of 3) 20.3 /
-    // 18.4, 2 x 20000 (5) 22.9 / 20.0; of 10 steps and more nothing is gained, and where parts come out uneven much is lost: 8 x 8192 keys of
-    // 16 bits 40 / 46.
+    // Every problem by itself, where shares are of few steps and their parts fill the device about evenly: in a line many workgroups
+    // would have the end of one problem and the beginning of the next, which costs more than a step.  Parts for one workgroup a CU (two of 64
+    // columns), or for two where there are problems enough to keep the join short.  us in a line / by themselves: B16, 20 rows, 2000 keys of 96
+    // columns (parts of 3 steps) 20.3 / 18.4; B2 20000 (5) 22.9 / 20.1; one query, D128, B8 4096 keys (two of 3 steps a CU) 19.2 / 17.3 in 8 bits, 26.0 /
+    // 21.0 in 16.  In parts of 6 and more what is uneven costs more: B8 8192 keys of 16 bits 40 / 46.
+    // In a line, two workgroups a CU where most have more than one problem: B32 4096 keys of 8 bits 51.8 / 45.8 us; else one, which leaves half
+    // the parts: B8 8192 26.5 / 25.7, of 16 bits 41.5 / 40.5.
+    a.shares = (int)(D <= 64 ? 2 * cus : cus);
+    a.line = (int)(D <= 64 || 2 * problems > cus ? 2 * cus : cus);
+    a.workgroups = a.line;
     if (problems <= a.shares) {
-      a.apart = 6;
-      a.workgroups += (int)problems;
+      a.apart = 5;
+      a.twice = D > 64 && 8 * problems >= cus ? 3 : a.apart;
+      a.workgroups = 2 * a.shares;
     }
     slots = 2 * a.workgroups;
   }
