@@ -253,11 +253,12 @@ void set_qk_norm(const QkNorm &c, const Rotation &r, const View *const *tensors,
     while (a->lanes * a->vec >= c.D && a->lanes > 1) a->lanes /= 2;
   const long long heads = a->H[0] + a->H[1], tokens = c.B * c.S, groups = 256 / a->lanes;
   // Lane groups that share a token's angles take its heads in turn: as many as fill the device with 8 waves a CU where tokens are few; else,
-  // where heads lie side by side, 8 forward (pieces next to each other: S24960 H32:8 D128 bf16, by 8 / 4 / 2 groups 99 / 104 / 120 us) and 2 backward, where
-  // angles cost more, being worked out for queries and keys apart (4 x 2048 tokens 74 / 70 / 65 us); where they are a sequence apart, one.
+  // where heads lie side by side, a group for 4 heads forward, 8 at most (pieces next to each other: S24960 D128 bf16, 40 heads by 8 / 4 / 2 groups 99 /
+  // 104 / 120 us, 24 by 8 / 6 / 2 69 / 62 / 71, 8 by 8 / 2 40 / 23) and 2 backward, where angles cost more, being worked out for queries and keys apart (4 x
+  // 2048 tokens of 40 heads by 2 / 4 65 / 70 us, of 8 20 / 25); where they are a sequence apart, one.
   const long long want = ((long long)device_limits().cus * 8 * (64 / a->lanes) + tokens - 1) / std::max(1ll, tokens);
   const bool side_by_side = a->H[0] > 1 && std::llabs(a->x[0].sh) < std::llabs(c.S > 1 ? a->x[0].ss : a->x[0].sb);
-  a->beside = (int)std::max(1ll, std::min(heads, std::max(want, !side_by_side ? 1ll : backward ? 2ll : 8ll)));
+  a->beside = (int)std::max(1ll, std::min(heads, std::max(want, !side_by_side ? 1ll : backward ? 2ll : std::min(8ll, heads / 4))));
   a->blocks = (int)std::max(1ll, std::min((long long)device_limits().cus * kQkNormRuns, (tokens * a->beside + groups - 1) / groups));
 }
 
