@@ -584,6 +584,7 @@ TraceaStatus tracea_cache_append(TraceaTensorView k, TraceaTensorView v, const T
  * where they are powers of two, as tracea_cache_append leaves them (in f16 as far as it reaches below the largest of them), else with one
  * rounding more.  The same call on the same inputs gives the same bits.  Results overlap no operand
  * and not each other.  Up to M P = 2^31 - 2^16 keys, M P P < 2^40.
+ * The lengths are read more than once: while a call runs nobody may write them (results are undefined then, nothing else is touched).
  * Where few rows meet many keys the keys are shared out over the device: a workspace per (device, stream), at most 80 MiB, grown on
  * demand, never under capture (without it a call runs unsplit, slower). */
 TraceaStatus tracea_attention_cached(TraceaTensorView q, TraceaTensorView k_cache, TraceaTensorView v_cache,

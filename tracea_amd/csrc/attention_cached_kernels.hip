@@ -445,6 +445,8 @@ __global__ void __launch_bounds__(256) attention_cached_join_kernel(const Attent
   const int b = (int)blockIdx.y / per_b, inner = (int)blockIdx.y - b * per_b;
   const int hk = inner / a.row_blocks, rb = inner - hk * a.row_blocks, r = rb * a.rows + row;
   if (s0 < 0 || r >= a.G * a.Sq) return;  // (not cut; a workgroup whose waves share a row leaves as a whole)
+  // (nobody may have written them, where lengths were changed while they were read)
+  if (parts < 1 || parts > a.all_slots || s0 + (long long)a.slots * (parts - 1) >= a.all_slots) return;
   auto at = [&](int i) { return (long long)(i == 0 ? s0 : (s0 & -a.slots) + a.slots * i) * a.rows + row; };
 
   float m = -INFINITY;

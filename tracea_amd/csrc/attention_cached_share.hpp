@@ -75,6 +75,7 @@ __device__ __forceinline__ bool share_of(const AttentionCachedArgs &a, int lane,
   while (before + total <= at_unit) {
     before += total;
     b0 += 64;
+    if (b0 >= a.B) return false;  // (lengths that somebody writes while they are read: the walk has to end)
     scan(b0, unit);
   }
   const int at = 63 - __clzll(__ballot(before + mine <= at_unit && own > 0));
@@ -92,7 +93,7 @@ __device__ __forceinline__ void next_problem(const AttentionCachedArgs &a, Share
   w.s0 = 0;
   if (++w.inner == a.Hk * a.row_blocks) {
     w.inner = 0;
-    ++w.b;
+    w.b = min(w.b + 1, a.B - 1);  // (the last only where lengths were changed meanwhile)
     w.sb = steps_of(a, w.b);
   }
 }

@@ -100,6 +100,7 @@ struct AttentionCachedArgs {
   int splits;      // 128 rows: parts of a block's steps
   int *meta;       // [problems][2]: first slot of its parts or -1, their number; null: no problem is cut
   int slots;       // from one part to the next: 2 (up to 32 rows) or 1
+  int all_slots;   // of the workspace
   float *part_o, *part_ml;  // [slot][rows][64 or 128], [..][2]
 };
 constexpr int kCachedStep = 128, kCachedTile = 64;

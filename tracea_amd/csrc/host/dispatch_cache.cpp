@@ -588,6 +588,7 @@ TraceaStatus dispatch_attention_cached(const TraceaTensorView &tq, const TraceaT
     }
     slots = 2 * a.workgroups;
   }
+  a.all_slots = (int)slots;
   if (slots > 0) {
     const size_t n = (size_t)(slots * a.rows), width = D <= 64 ? 64 : 128;
     a.part_o = (float *)train_scratch(device, stream, n * (width + 2) * 4 + (size_t)problems * 8);
