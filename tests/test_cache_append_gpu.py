@@ -183,3 +183,47 @@ def test_graph_and_in_place_queries(tracea_gpu):
             for n in "kv":
                 assert torch.equal(getattr(pool, n).view(torch.uint8), getattr(eager, n).view(torch.uint8))
                 assert torch.equal(getattr(pool, n + "_scale"), getattr(eager, n + "_scale"))
+
+
+@pytest.mark.parametrize("dtype", HALVES, ids=["f16", "bf16"])
+@pytest.mark.parametrize("adjacent", [False, True], ids=["halves", "side"])
+@pytest.mark.parametrize("t, page", [(20, 16), (70, 64), (300, 256)])
+@pytest.mark.parametrize("d", [8, 24, 40, 72, 88, 104])
+def test_scales_are_those_of_turned_keys(tracea_gpu, d, t, page, adjacent, dtype):
+    """Heads that are turned as a whole and end in half a couple of pieces: the last pair of some tokens is (450, 0), turned by 45 degrees or so.  What
+    is written stays below 448, what was given does not."""
+    def spoil(pt, k, v):
+        k *= 2.0 ** -6
+        k[:, :, ::7, d - 2 if adjacent else d // 2 - 1] = 450
+        k[:, :, ::7, d - 1] = 0
+    slowest = 10000.0 ** (-(d // 2 - 1) / (d // 2))
+    pos = torch.full((2, t, 1), round(0.785 / slowest), dtype=torch.int32, device="cuda")
+    run(tracea_gpu, 18, 2, 3, 2, t, d, d, page, dtype, True, [0, 33], None, adjacent, "bshd", positions=pos, spoil=spoil)
+
+
+@pytest.mark.parametrize("dtype", HALVES, ids=["f16", "bf16"])
+@pytest.mark.parametrize("adjacent", [False, True], ids=["halves", "side"])
+@pytest.mark.parametrize("d, page", [(40, 64), (72, 64), (24, 512), (128, 512)])
+def test_heads_of_any_width_are_the_same_however_their_tokens_were_cut(tracea_gpu, d, page, adjacent, dtype):
+    """The scales of pages that a call, or several (whose pages the other kernel may take), have written; codes up to what was rounded more than once."""
+    g = torch.Generator(device="cuda").manual_seed(20)
+    b, hk, t = 4, 4, 600
+    k, v = (heads(g, b, hk, t, d, dtype, "bshd") for _ in range(2))
+    freq = torch.logspace(0, -3, d // 2, device="cuda")
+    per = -(-t // page)
+    pt = table(g, b, per, b * per)
+    whole, cut = (Pool(torch.Generator(device="cuda").manual_seed(2), b * per, hk, page, d, dtype, True) for _ in range(2))
+    zero = torch.zeros(b, dtype=torch.int32, device="cuda")
+    turn = dict(inv_freq=freq, adjacent=adjacent)
+    tracea_gpu.cache_append(k, v, whole.k, whole.v, pt, zero, **whole.scales(), **turn)
+    at = 0
+    for n in (1, 1, 7, 300, 1, 3, 20, 267):
+        tracea_gpu.cache_append(k[:, :, at:at + n], v[:, :, at:at + n], cut.k, cut.v, pt, zero + at, **cut.scales(), **turn)
+        at += n
+    assert at == t and torch.equal(whole.k_scale, cut.k_scale) and torch.equal(whole.v_scale, cut.v_scale)
+    for n in "kv":
+        of = pt.long()
+        x, y = (p.values(n)[of].transpose(2, 3).flatten(1, 2)[:, :t] for p in (whole, cut))
+        scale = getattr(whole, n + "_scale").double()[of].repeat_interleave(page, 1)[:, :t, :, None]
+        normal = torch.maximum(x.abs(), y.abs()) > 2.0 ** -6 * scale
+        assert torch.equal(x[normal], y[normal]) and ((x - y).abs() <= 2.0 ** -9 * scale).all()

@@ -379,17 +379,30 @@ __global__ void __launch_bounds__(2 * SIDE) __attribute__((amdgpu_waves_per_eu(4
       __builtin_amdgcn_sched_barrier(0);
     }
   };
+  constexpr std::integral_constant<int, 0> ZERO{};
+  constexpr std::integral_constant<int, 4> FOUR{};
+  constexpr std::integral_constant<int, 8> EIGHT{};
   // ... of any value but NaN; a head that has an infinity is looked through again for its finite ones
-  auto largest = [](const float (&x)[8], float top, bool finite) __attribute__((always_inline)) {
+  auto largest = [](const float (&x)[8], auto from, auto count, float top, bool finite) __attribute__((always_inline)) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float y = fabsf(x[e]);
+    for (int e = 0; e < decltype(count)::value; ++e) {
+      const float y = fabsf(x[from() + e]);
       top = fmaxf(top, finite && !(y < INFINITY) ? 0.0f : y);
     }
     return top;
   };
+  // ... of a couple: of what is written.  The part that is not there repeats columns that are, but as they were given, not turned.
+  auto largest_of = [&](const Couple &p, const float (&u)[8], const float (&v)[8], bool finite) __attribute__((always_inline)) {
+    if constexpr (FOURS) {
+      const float first = largest(v, ZERO, FOUR, largest(u, ZERO, FOUR, 0.0f, finite), finite), second = largest(v, FOUR, FOUR, largest(u, FOUR, FOUR, 0.0f, finite), finite);
+      return p.u1 >= 0 ? fmaxf(first, second) : first;
+    } else {
+      const float first = largest(u, ZERO, EIGHT, 0.0f, finite), second = largest(v, ZERO, EIGHT, 0.0f, finite);
+      return p.v >= 0 ? fmaxf(first, second) : first;
+    }
+  };
   // A couple to a row in 16 bits or, times inv, in codes.
-  auto store = [](auto *row, const Couple &p, const float (&u)[8], const float (&v)[8], float inv) __attribute__((always_inline)) {
+  auto store = [=](auto *row, const Couple &p, const float (&u)[8], const float (&v)[8], float inv) __attribute__((always_inline)) {
     constexpr bool CODES = sizeof(*row) == 1;
     auto piece = [&](int at, const float(&x)[8], auto from, auto count) __attribute__((always_inline)) {
       constexpr int N = decltype(count)::value;
@@ -405,8 +418,6 @@ __global__ void __launch_bounds__(2 * SIDE) __attribute__((amdgpu_waves_per_eu(4
         *(Piece<T, N> *)(row + at) = y;
       }
     };
-    constexpr std::integral_constant<int, 0> ZERO{};
-    constexpr std::integral_constant<int, 4> FOUR{};
     if constexpr (FOURS) {
       piece(p.u, u, ZERO, FOUR);
       piece(p.v, v, ZERO, FOUR);
@@ -415,7 +426,6 @@ __global__ void __launch_bounds__(2 * SIDE) __attribute__((amdgpu_waves_per_eu(4
         piece(p.v1, v, FOUR, FOUR);
       }
     } else {
-      constexpr std::integral_constant<int, 8> EIGHT{};
       piece(p.u, u, ZERO, EIGHT);
       if (p.v >= 0) piece(p.v, v, ZERO, EIGHT);
     }
@@ -493,8 +503,7 @@ __global__ void __launch_bounds__(2 * SIDE) __attribute__((amdgpu_waves_per_eu(4
           if (p.t >= tokens) continue;
           float u[8], v[8];
           turned(p, piece_of(first() + s), piece_of(first() + HK + s), u, v);
-          top = largest(u, top, finite);
-          top = largest(v, top, finite);  // (what is not there repeats what is)
+          top = fmaxf(top, largest_of(p, u, v, finite));
         }
 #pragma unroll
         for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
