@@ -59,6 +59,8 @@ long long stub_value(const char *what) {
   if (is("append.groups")) return g_append.groups;
   if (is("append.heads")) return g_append.heads;
   if (is("append.queries")) return g_append.queries;
+  if (is("append.tokens_at_once")) return append_tokens_at_once(g_append.P);
+  if (is("append.queries_at_once")) return kAppendQueries;
   if (is("rows")) return g_attention.rows;
   if (is("row_blocks")) return g_attention.row_blocks;
   if (is("workgroups")) return g_attention.workgroups;

@@ -227,3 +227,27 @@ def test_heads_of_any_width_are_the_same_however_their_tokens_were_cut(tracea_gp
         scale = getattr(whole, n + "_scale").double()[of].repeat_interleave(page, 1)[:, :t, :, None]
         normal = torch.maximum(x.abs(), y.abs()) > 2.0 ** -6 * scale
         assert torch.equal(x[normal], y[normal]) and ((x - y).abs() <= 2.0 ** -9 * scale).all()
+
+
+@pytest.mark.parametrize("e4m3", [False, True], ids=["16", "e4m3"])
+def test_more_query_heads_than_are_taken_at_once(tracea_gpu, e4m3):
+    run(tracea_gpu, 23, 2, 1100, 1, 5, 24, 16, 16, torch.float16, e4m3, [0, 14], [5, 3], layout="odd")
+
+
+def test_long_pages_without_a_rotation(tracea_gpu):
+    """More tokens of a page than a workgroup takes at once."""
+    run(tracea_gpu, 24, 1, 3, 2, 9000, 40, 0, 16384, torch.bfloat16, True, [100], layout="odd")
+    run(tracea_gpu, 25, 1, 3, 2, 9000, 40, 0, 16384, torch.bfloat16, False, [100], [8195])
+
+
+def test_more_than_31_bits_of_pieces_in_a_page(tracea_gpu):
+    """131072 tokens of 128 heads and 128 columns in one page, rows that begin anywhere: 2^31 pieces, all of them one workgroup's (5 s)."""
+    t, h, d = 131072, 128, 128
+    g = torch.Generator(device="cuda").manual_seed(26)
+    at = lambda n: torch.randn(1, n, t, d + 1, device="cuda", dtype=torch.bfloat16, generator=g)[..., 1:]  # noqa: E731
+    q, k, v = at(h), at(1), at(1)
+    out = torch.full((1, h, t, d + 1), 7.0, device="cuda", dtype=torch.bfloat16)[..., 1:]
+    k_cache, v_cache = (torch.zeros(1, 1, t, d, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    zero = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    tracea_gpu.cache_append(k, v, k_cache, v_cache, zero, zero[0], q=q, q_out=out)
+    assert torch.equal(k_cache, k) and torch.equal(v_cache, v) and all(torch.equal(q[0, i], out[0, i]) for i in range(h))

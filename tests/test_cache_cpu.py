@@ -299,6 +299,35 @@ def test_heads_of_appending_workgroups(stub):
                 assert v("append.pages") == (t + page - 2) // page + 1
 
 
+def test_pieces_of_appending_are_counted_in_32_bits(stub):
+    """Whatever pages, heads and rotations a call has, what a workgroup takes at once (heads x tokens x pieces of single columns) stays below 2^31."""
+    for t, page in ((1, 16), (4096, 64), (131072, 131072), (1 << 20, (1 << 20) - 16), (1 << 22, 16), ((1 << 31) - (1 << 16), (1 << 20) - 16)):
+        for hq, hk in ((1, 1), (128, 1), (200, 65), (1 << 20, 1)):
+            for d, p in ((128, 0), (512, 0), (512, 1), (128, 5), (512, 256), (512, 255)):
+                if hq * t > 1 << 42:
+                    continue
+                a = append_args(b=1, hq=1, hk=1, t=t, d=d, p=max(p, 1), page=page, m=1)
+                for n, h in (("q", hq), ("qo", hq), ("k", hk), ("v", hk)):  # (rows that begin anywhere)
+                    a[n] = T([1, h, t, d], BF16, stride=[0, (d + 1) * t, d + 1, 1]).at(2)
+                for n in ("kc", "vc"):
+                    a[n] = T([9, hk, page, d], E4M3)
+                for n in ("ks", "vs"):
+                    a[n] = T([9, hk], F32)
+                if p == 0:
+                    a.update(pos=None, freq=None, axes=0, sections=[])
+                v = lambda n: stub.stub_value(n.encode())  # noqa: E731
+                assert append(stub, a) == OK and v("append.vec") == 1, stub.stub_message()
+                tokens = min(t, page, v("append.tokens_at_once"))
+                assert tokens > 0 and tokens * p <= 4096
+                for heads in (v("append.heads"), min(v("append.queries"), v("append.queries_at_once"))):
+                    assert heads > 0 and heads * tokens * d < (1 << 31) - 256
+
+
+def test_more_new_tokens_than_are_counted(stub):
+    a = append_args(b=1, t=(1 << 31) - (1 << 16) + 1, page=1 << 19, m=1)
+    assert append(stub, a) == UNSUPPORTED and b"new tokens" in stub.stub_message()
+
+
 def test_pieces_are_taken_where_rows_allow_them(stub):
     a = norm_args()
     assert norm(stub, a) == OK and stub.stub_value(b"qk.vec") == 8 and stub.stub_value(b"qk.lanes") == 4

@@ -74,6 +74,10 @@ struct CacheAppendArgs {
   int heads, queries;  // key/value and query heads of a group
 };
 constexpr int kAppendHeads = 64;  // key/value heads of a workgroup, at most
+// What the kernel for any sizes works on at once, so that its pieces (up to 512 a row) are counted in 32 bits, whatever pages and heads there
+// are: tokens whose sines and cosines fit 32 KB, as many where nothing is turned, and heads of queries.
+constexpr int kAppendAngles = 4096, kAppendQueries = 512;
+__host__ __device__ inline int append_tokens_at_once(int P) { return P > 0 ? kAppendAngles / P : kAppendAngles; }
 int launch_cache_append(const CacheAppendArgs &a, int dtype, hipStream_t stream);
 
 struct AttentionCachedArgs {

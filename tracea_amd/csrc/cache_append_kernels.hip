@@ -24,8 +24,6 @@ namespace tracea_amd {
 
 namespace {
 
-constexpr int ANGLES = 4096;  // pairs whose sine and cosine are kept, 32 KB
-
 template <typename T, int E>
 struct alignas(sizeof(T) * E) Piece {
   T x[E];
@@ -79,11 +77,11 @@ __device__ __forceinline__ void rescale(unsigned char *head, long long apart, in
   }
 }
 
-// Any sizes, E columns at a time (8, or 4, 2 or 1 where pairs, strides or addresses do not go into that): angles of up to ANGLES pairs at once, and in 8 bits operands are read
-// twice, for the largest value and for the codes; the second time they come from the caches.
+// Any sizes, E columns at a time (8, or 4, 2 or 1 where pairs, strides or addresses do not go into that): angles of up to kAppendAngles pairs at
+// once, and in 8 bits operands are read twice, for the largest value and for the codes; the second time they come from the caches.
 template <typename T, bool C8, int E, bool ADJ>
 __global__ void __launch_bounds__(256) cache_append_kernel(const CacheAppendArgs a) {
-  __shared__ float s_cos[ANGLES], s_sin[ANGLES];
+  __shared__ float s_cos[kAppendAngles], s_sin[kAppendAngles];
   __shared__ unsigned s_max[2][kAppendHeads];   // largest finite magnitudes, as bits
   __shared__ float s_inv[2][kAppendHeads], s_move[2][kAppendHeads];
   const int b = blockIdx.y, j = (int)blockIdx.x / a.groups, grp = (int)blockIdx.x - j * a.groups, PT = a.table.P;
@@ -98,7 +96,7 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const CacheAppendArgs
   const int heads = h1 - h0;
 
   const int pair_pieces = a.P / E, straight = (a.D - 2 * a.P) / E, pieces = pair_pieces + straight, all = a.D / E;
-  const int chunk = a.P > 0 ? max(1, ANGLES / a.P) : PT;
+  const int chunk = append_tokens_at_once(a.P);
 
   auto angles = [&](int from, int to) __attribute__((always_inline)) {
     for (int i = threadIdx.x; i < (to - from) * a.P; i += 256) {
@@ -250,19 +248,22 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const CacheAppendArgs
         *(Piece<T, E> *)((T *)to_row + piece * E) = x;
       }
     }
-    for (int i = threadIdx.x; i < (q1 - q0) * (to - from) * pieces; i += 256) {
-      const int row = i / pieces, piece = i - row * pieces, h = row / (to - from), t = from + row - h * (to - from);
-      int at_u, at_v;
-      float u[E], v[E];
-      columns(piece, at_u, at_v);
-      turned((const T *)a.q.p + b * a.q.sb + (q0 + h) * a.q.sh + t * a.q.ss, (t - from) * a.P + piece * E, at_u, at_v, u, v);
-      T *out = (T *)a.q_out.p + b * a.q_out.sb + (q0 + h) * a.q_out.sh + t * a.q_out.ss;
-      if (t >= n) {
+    for (int g0 = q0, count; g0 < q1; g0 += count) {
+      count = min(q1 - g0, kAppendQueries);
+      for (int i = threadIdx.x; i < count * (to - from) * pieces; i += 256) {
+        const int row = i / pieces, piece = i - row * pieces, h = row / (to - from), t = from + row - h * (to - from);
+        int at_u, at_v;
+        float u[E], v[E];
+        columns(piece, at_u, at_v);
+        turned((const T *)a.q.p + b * a.q.sb + (g0 + h) * a.q.sh + t * a.q.ss, (t - from) * a.P + piece * E, at_u, at_v, u, v);
+        T *out = (T *)a.q_out.p + b * a.q_out.sb + (g0 + h) * a.q_out.sh + t * a.q_out.ss;
+        if (t >= n) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) u[e] = v[e] = 0.0f;
+          for (int e = 0; e < E; ++e) u[e] = v[e] = 0.0f;
+        }
+        store16(out, at_u, u);
+        if (at_v >= 0) store16(out, at_v, v);
       }
-      store16(out, at_u, u);
-      if (at_v >= 0) store16(out, at_v, v);
     }
   }
 }
@@ -547,7 +548,7 @@ int launch(const CacheAppendArgs &a, hipStream_t stream) {
   const dim3 grid((unsigned)(a.pages * a.groups), (unsigned)a.B);
   const int tokens = a.T < a.table.P ? a.T : a.table.P, pieces = (a.D + 8) / 16;
   auto holds = [&](int side, int held) {
-    return a.held && tokens * a.P <= side * held * 8 && tokens * pieces <= side * held;
+    return a.held && (long long)tokens * a.P <= side * held * 8 && (long long)tokens * pieces <= side * held;
   };
 #define HELD(SIDE, HK)                                                                                                                     \
   if (holds(SIDE, HK)) {                                                                                                                   \

@@ -460,7 +460,7 @@ TraceaStatus dispatch_cache_append(const TraceaTensorView &tk, const TraceaTenso
     a.held = a.held && rows_on(*t, 16) && t->stride[2] >= 0 && (t->stride[2] * std::min(T, (long long)c.pages.P) + D) * 2 < (1ll << 31);
   for (const View *t : {&c.k, &c.v}) a.held = a.held && (t->stride[2] * c.pages.P + D) * 2 < (1ll << 31);
   const long long pages = (T + c.pages.P - 2) / c.pages.P + 1;
-  if (B > 65535 || pages >= (1 << 22)) return fail(TRACEA_UNSUPPORTED_CONFIG, "%s: %lld sequences of %lld new tokens are more than is supported", op, B, T);
+  if (B > 65535 || pages >= (1 << 22) || T > (1ll << 31) - (1 << 16)) return fail(TRACEA_UNSUPPORTED_CONFIG, "%s: %lld sequences of %lld new tokens are more than is supported", op, B, T);
   a.pages = (int)pages;
   DeviceScope scope(device);
   if (scope.err != hipSuccess) return hip_status("hipSetDevice", (int)scope.err);
