@@ -392,14 +392,16 @@ __global__ void __launch_bounds__(2 * SIDE) __attribute__((amdgpu_waves_per_eu(4
     }
     return top;
   };
-  // ... of a couple: of what is written.  The part that is not there repeats columns that are, but as they were given, not turned.
-  auto largest_of = [&](const Couple &p, const float (&u)[8], const float (&v)[8], bool finite) __attribute__((always_inline)) {
+  // ... of a couple: of what is written.  The part that is not there repeats columns that are, but as they were given: not turned where they are.
+  auto largest_of = [&](const Couple &p, const float (&u)[8], const float (&v)[8], float top, bool finite) __attribute__((always_inline)) {
     if constexpr (FOURS) {
-      const float first = largest(v, ZERO, FOUR, largest(u, ZERO, FOUR, 0.0f, finite), finite), second = largest(v, FOUR, FOUR, largest(u, FOUR, FOUR, 0.0f, finite), finite);
-      return p.u1 >= 0 ? fmaxf(first, second) : first;
+      top = largest(v, ZERO, FOUR, largest(u, ZERO, FOUR, top, finite), finite);
+      const float both = largest(v, FOUR, FOUR, largest(u, FOUR, FOUR, top, finite), finite);
+      return p.u1 >= 0 ? both : top;
     } else {
-      const float first = largest(u, ZERO, EIGHT, 0.0f, finite), second = largest(v, ZERO, EIGHT, 0.0f, finite);
-      return p.v >= 0 ? fmaxf(first, second) : first;
+      top = largest(u, ZERO, EIGHT, top, finite);
+      const float both = largest(v, ZERO, EIGHT, top, finite);
+      return !ADJ || p.v >= 0 ? both : top;  // (a half of pairs of halves that is not there is not turned either)
     }
   };
   // A couple to a row in 16 bits or, times inv, in codes.
@@ -504,7 +506,7 @@ __global__ void __launch_bounds__(2 * SIDE) __attribute__((amdgpu_waves_per_eu(4
           if (p.t >= tokens) continue;
           float u[8], v[8];
           turned(p, piece_of(first() + s), piece_of(first() + HK + s), u, v);
-          top = fmaxf(top, largest_of(p, u, v, finite));
+          top = largest_of(p, u, v, top, finite);
         }
 #pragma unroll
         for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
