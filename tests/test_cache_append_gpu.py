@@ -229,6 +229,20 @@ def test_heads_of_any_width_are_the_same_however_their_tokens_were_cut(tracea_gp
         assert torch.equal(x[normal], y[normal]) and ((x - y).abs() <= 2.0 ** -9 * scale).all()
 
 
+@pytest.mark.parametrize("layout", ["bshd", "odd"])
+def test_queries_at_places_beyond_31_bits(tracea_gpu, layout):
+    """starts + t reaches 2^31: such tokens have no place, their queries are turned like all others."""
+    g = torch.Generator(device="cuda").manual_seed(22)
+    t, d = 40, 64
+    starts = torch.tensor([2 ** 31 - 1, 2 ** 31 - 20, 3], dtype=torch.int32, device="cuda")
+    freq = torch.logspace(0, -3, 32, device="cuda")
+    pool = Pool(g, 9, 2, 16, d, torch.bfloat16, False)
+    q, k, v = (heads(g, 3, h, t, d, torch.bfloat16, layout) for h in (4, 2, 2))
+    q_out = tracea_gpu.cache_append(k, v, pool.k, pool.v, table(g, 3, 3, 9), starts, q=q, inv_freq=freq)
+    y, made_of = rotated(q, (starts.double()[:, None] + torch.arange(t, device="cuda"))[..., None] * freq.double(), d, False)
+    assert ((q_out.double() - y).abs() <= half_step(torch.bfloat16) * y.abs() * (1 + 1e-6) + 16 * U32 * made_of).all()
+
+
 @pytest.mark.parametrize("e4m3", [False, True], ids=["16", "e4m3"])
 def test_more_query_heads_than_are_taken_at_once(tracea_gpu, e4m3):
     run(tracea_gpu, 23, 2, 1100, 1, 5, 24, 16, 16, torch.float16, e4m3, [0, 14], [5, 3], layout="odd")

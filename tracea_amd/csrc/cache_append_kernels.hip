@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const CacheAppendArgs
       const int t = from + i / a.P, p = i - (t - from) * a.P;
       int axis = 0;
       for (int x = 1; x < a.axes; ++x) axis += p >= a.first[x];
-      const int position = a.positions != nullptr ? a.positions[b * a.pos_sb + t * a.pos_ss + axis] : (int)(start + t);
+      const double position = a.positions != nullptr ? (double)a.positions[b * a.pos_sb + t * a.pos_ss + axis] : (double)((unsigned)start + (unsigned)t);
       float c, sn;
       turn(position, a.inv_freq[p], 1.0f, c, sn);
       s_cos[i] = c;
@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(2 * SIDE) __attribute__((amdgpu_waves_per_eu(4
     const int t = i / a.P, p = i - t * a.P;
     int axis = 0;
     for (int x = 1; x < a.axes; ++x) axis += p >= a.first[x];
-    const int position = a.positions != nullptr ? a.positions[b * a.pos_sb + (lo + t) * a.pos_ss + axis] : (int)(start + lo + t);
+    const double position = a.positions != nullptr ? (double)a.positions[b * a.pos_sb + (lo + t) * a.pos_ss + axis] : (double)((unsigned)start + (unsigned)(lo + t));
     float c, s;
     turn(position, a.inv_freq[p], 1.0f, c, s);
     ((float *)s_cos)[i] = c;
