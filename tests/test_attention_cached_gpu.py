@@ -282,3 +282,19 @@ def test_agrees_with_the_attention_over_dense_keys(tracea_gpu):
     assert torch.equal(lse == -math.inf, want_lse == -math.inf)
     fine = lse > -math.inf
     assert ((lse - want_lse).abs()[fine] <= 1e-5 * lse[fine].abs() + 1e-5).all()
+
+
+@pytest.mark.parametrize("e4m3", [False, True], ids=["16", "e4m3"])
+@pytest.mark.parametrize("dtype", HALVES, ids=["f16", "bf16"])
+@pytest.mark.parametrize("hq, hk, sq", [(33, 1, 1), (8, 1, 5), (16, 2, 6), (64, 1, 1), (32, 2, 4)])  # 33, 40, 48, 64, 64 rows a key/value head
+@pytest.mark.parametrize("k_lengths, page", [([70, 6, 256], 16), ([3000, 5, 700], 64), ([20000, 1030, 6], 64)])
+def test_two_blocks_of_32_rows(tracea_gpu, k_lengths, page, hq, hk, sq, dtype, e4m3):
+    """Heads that share keys, times drafted tokens, beyond one block: keys uncut, cut problem by problem, and cut as one line."""
+    run(tracea_gpu, 37, 3, hq, hk, sq, k_lengths, 128 if sq < 6 else 96, page, dtype, e4m3, True, [sq, max(1, sq - 2), sq])
+
+
+@pytest.mark.parametrize("e4m3", [False, True], ids=["16", "e4m3"])
+@pytest.mark.parametrize("hq, sq", [(8, 1), (8, 5), (8, 10), (8, 100)])  # rows a key/value head: 4, 20, 40, 400
+def test_tables_far_wider_than_the_sequences(tracea_gpu, hq, sq, e4m3):
+    """The plan is that of the longest sequences that the table could hold: parts of one step, shares of nothing."""
+    run(tracea_gpu, 38, 3, hq, 2, sq, [197, 0, 700], 128, 16, torch.bfloat16, e4m3, extra=2000, q_lengths=[sq, 0, max(1, sq - 1)], layout="bshd")

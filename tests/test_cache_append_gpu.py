@@ -2,7 +2,7 @@
 import pytest
 
 torch = pytest.importorskip("torch")
-from cache_oracle import E4M3, U32, Pool, append, half_step, heads, rotated, table  # noqa: E402
+from cache_oracle import E4M3, U32, Pool, angles, append, half_step, heads, rotated, table  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 HALVES = [torch.float16, torch.bfloat16]
@@ -203,6 +203,27 @@ def test_scales_are_those_of_turned_keys(tracea_gpu, d, t, page, adjacent, dtype
 
 @pytest.mark.parametrize("dtype", HALVES, ids=["f16", "bf16"])
 @pytest.mark.parametrize("adjacent", [False, True], ids=["halves", "side"])
+@pytest.mark.parametrize("d, rot, page", [(40, 40, 64), (72, 72, 32), (24, 24, 256), (128, 128, 64), (80, 40, 48), (64, 32, 16)])
+def test_every_layout_of_keys_gives_the_same_cache(tracea_gpu, d, rot, page, adjacent, dtype):
+    """Rows on 16 bytes and rows that begin anywhere are taken by different kernels: the same scales and codes.  (Queries in 16 bits may be rounded
+    once or, behind fp32, twice.)"""
+    b, hq, hk, t = 2, 3, 2, 300
+    freq = torch.logspace(0, -3, rot // 2, device="cuda")
+    starts = torch.tensor([5, 1000], dtype=torch.int32, device="cuda")
+    got = []
+    for layout in ("bshd", "odd"):
+        g = torch.Generator(device="cuda").manual_seed(19)
+        pool = Pool(g, 2 * (1300 // page + 1), hk, page, d, dtype, True)
+        pt = table(g, b, 1300 // page + 1, 2 * (1300 // page + 1))
+        q, k, v = (heads(g, b, h, t, d, dtype, layout) for h in (hq, hk, hk))
+        tracea_gpu.cache_append(k, v, pool.k, pool.v, pt, starts, q=q, inv_freq=freq, adjacent=adjacent, **pool.scales())
+        got.append([pool.k_scale, pool.v_scale, pool.k.view(torch.uint8), pool.v.view(torch.uint8)])
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", HALVES, ids=["f16", "bf16"])
+@pytest.mark.parametrize("adjacent", [False, True], ids=["halves", "side"])
 @pytest.mark.parametrize("d, page", [(40, 64), (72, 64), (24, 512), (128, 512)])
 def test_heads_of_any_width_are_the_same_however_their_tokens_were_cut(tracea_gpu, d, page, adjacent, dtype):
     """The scales of pages that a call, or several (whose pages the other kernel may take), have written; codes up to what was rounded more than once."""
@@ -227,6 +248,30 @@ def test_heads_of_any_width_are_the_same_however_their_tokens_were_cut(tracea_gp
         scale = getattr(whole, n + "_scale").double()[of].repeat_interleave(page, 1)[:, :t, :, None]
         normal = torch.maximum(x.abs(), y.abs()) > 2.0 ** -6 * scale
         assert torch.equal(x[normal], y[normal]) and ((x - y).abs() <= 2.0 ** -9 * scale).all()
+
+
+@pytest.mark.parametrize("e4m3", [False, True], ids=["16", "e4m3"])
+@pytest.mark.parametrize("layout", ["bshd", "odd"])
+@pytest.mark.parametrize("batches", [1, 3])
+def test_positions_along_several_axes(tracea_gpu, batches, layout, e4m3):
+    """Positions [1,T,A] and [B,T,A], sections of unlike length, one of them empty."""
+    g = torch.Generator(device="cuda").manual_seed(21)
+    b, hq, hk, t, d, page, sections = 3, 4, 2, 50, 96, 32, [20, 0, 17, 7]
+    pos = torch.randint(0, 5000, (batches, t, 4), dtype=torch.int32, device="cuda", generator=g)
+    freq = torch.cat([10000.0 ** (-torch.arange(n, device="cuda", dtype=torch.float32) / max(n, 1)) for n in sections])
+    angle = angles(pos, freq, sections).expand(b, -1, -1)
+    starts = torch.tensor([0, 40, 7], dtype=torch.int32, device="cuda")
+    pool = Pool(g, 12, hk, page, d, torch.bfloat16, e4m3)
+    pt = table(g, b, 3, 12)
+    q, k, v = (heads(g, b, h, t, d, torch.bfloat16, layout) for h in (hq, hk, hk))
+    want = append(pool, pt, k, v, starts, None, 88, angle, False)
+    q_out = tracea_gpu.cache_append(k, v, pool.k, pool.v, pt, starts, q=q, positions=pos, inv_freq=freq, sections=sections, **pool.scales())
+    for n in "kv":
+        values, allowed, scale, _ = want[n]
+        assert ((pool.values(n) - values).abs() <= allowed * (1 + 1e-9)).all(), n
+        assert not e4m3 or torch.equal(getattr(pool, n + "_scale").double(), scale), n
+    y, made_of = rotated(q, angle, 88, False)
+    assert ((q_out.double() - y).abs() <= half_step(torch.bfloat16) * y.abs() * (1 + 1e-6) + 16 * U32 * made_of).all()
 
 
 @pytest.mark.parametrize("layout", ["bshd", "odd"])
