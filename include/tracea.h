@@ -550,7 +550,7 @@ TraceaStatus tracea_qk_norm_rotary_backward(TraceaTensorView dq_out, const Trace
  * tracea_cache_append turns new keys (and queries) by their positions and writes keys and values to their places.
  *   k, v [B,Hk,T,D], q [B,Hq,T,D] and q_out (optional, any Hq), f16 or bf16, D contiguous, any other strides and alignment
  *   starts [B] i32: tokens that sequence b has already; lengths [B] i32 (optional): how many of the T are new ones of sequence b
- *   (clamped to 0..T).  Both contiguous, on the device; a negative start counts as 0.
+ *   (clamped to 0..T, T up to 2^31 - 2^16).  Both contiguous, on the device; a negative start counts as 0.
  *   positions [B,T,A] or [1,T,A] i32 as in tracea_rotary, NULL: starts[b] + t (one axis); inv_freq [P] f32, NULL: no rotation
  * q_out of a token behind lengths[b] is 0; q_out may be q (the same view).  In 16 bits no other rows of the caches are written than the new
  * tokens'.
@@ -582,8 +582,9 @@ TraceaStatus tracea_cache_append(TraceaTensorView k, TraceaTensorView v, const T
  * Scores, statistics and sums are fp32 or more, probabilities are rounded once to the type of q.  In 8 bits scales multiply scores and
  * probabilities, in fp32, and in calls with more than 64 rows (Hq / Hk Sq) the keys and values, in their widening to the type of q: exactly
  * where they are powers of two, as tracea_cache_append leaves them (in f16 as far as it reaches below the largest of them), else with one
- * rounding more.  The same call on the same inputs gives the same bits.  Results overlap no operand
- * and not each other.  Up to M P = 2^31 - 2^16 keys, M P P < 2^40.
+ * rounding more.  In f16 with up to 64 rows a probability is rounded behind its value scale, so that each key's part of a result is off by
+ * half a step of f16 or, if that is more, by 2^-36 of its code times the largest value scale that the sequence has in the head.  The same call
+ * on the same inputs gives the same bits.  Results overlap no operand and not each other.  Up to M P = 2^31 - 2^16 keys, M P P < 2^40.
  * The lengths are read more than once: while a call runs nobody may write them (results are undefined then, nothing else is touched).
  * Where few rows meet many keys the keys are shared out over the device: a workspace per (device, stream), at most 80 MiB, grown on
  * demand, never under capture (without it a call runs unsplit, slower). */

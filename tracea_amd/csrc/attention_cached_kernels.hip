@@ -4,7 +4,9 @@
 //   s_ij = scale q_i . k_j  over the keys a row sees     o_i = sum_j exp(s_ij - lse_i) v_j     lse_i = log sum_j exp(s_ij)
 //   k_j = ks[page of j] code_j, v_j = vs[page of j] code_j: ks multiplies the score, vs the probability, both in fp32.
 //
-// Bound by reading the cache, once for all heads that share it: rows r = query G + head of the group are packed as in the attention for training.
+// Bound by reading the cache, once for each block of up to 32 rows: rows r = query G + head of the group are packed as in the attention for
+// training, so that up to 32 heads and queries share a walk over the keys.  33 to 64 rows are two blocks, each with a walk of its own: 64:8 heads over 16
+// sequences of 4096 keys, 4 queries (32 rows) 35 us in 8 bits, 5 to 8 queries 56; in 16 bits 52 and 81, where the tiles of 128 rows take 57 for 9.
 // Nothing passes through LDS on its way: the products are v_mfma_f32_16x16x32, whose first operand is 8 values a lane, and which values these are
 // is free as long as both operands agree.
 //   S^T = K Q^T   of 16 keys: lane l has key l & 15 and the columns 8 KS (l >> 4) .. + 8 KS - 1, a run of the key's row; the resident
@@ -21,7 +23,8 @@
 // One query of 40:8 heads over 131072 keys of 128 columns in 8 bits (269 MB): 55 to 62 us, 4.3 to 4.9 TB/s (a copy: 5.06), 4 to 5 of them the second
 // launch; 8 sequences of up to 8192 keys, 32:8 heads, 26 us (a copy: 18), of which 5 are a chain of dependent loads (lengths, table, keys, values)
 // before the first result and 4 the second launch; 5 queries of 16:4 heads of 96 columns over 16 sequences of up to 2000 keys in 16 bits 18 us
-// (a copy: 6.4), the same chain and three steps; one query of 12 heads over 197 keys 5.5 us.
+// (a copy: 6.4), the same chain and three steps; one query of 12 heads over 197 keys 5.5 us, 8.6 where the table has room for 800 keys or more,
+// as the plan is made for those.
 #include <algorithm>
 #include <type_traits>
 
@@ -37,7 +40,8 @@ constexpr int WAVES = 4;
 //   c     scale log2(e) ks: scores times c are exponents of 2 (above 0, so that -inf of a key that is not seen stays that)
 //   lift  log2(vs / ref), ref the largest scale of values that the wave has met: what is summed up is in units of ref, so that f16
 //         probabilities times a scale keep their range; the scale joins the probability in its exponent, p vs / ref = 2^(x - m + lift), and the sum
-//         of probabilities takes it back, 2^-lift times a group's four.  -60 at least: less is nothing beside the largest.
+//         of probabilities takes it back, 2^-lift times a group's four.  -60 at least: less is nothing beside the largest.  The product is what is
+//         rounded: below f16's normal numbers (a row's largest probability: lifts below -25) it is off by 2^-36 of ref.
 constexpr float LEAST_LIFT = -60.0f;
 struct Scales {
   float c, lift, ref = 0.0f;

@@ -9,8 +9,8 @@
 //
 // Bound by the matrix pipe (busy for a third of the time) and the vector work beside it (exponentials, maxima, packing: half of the time), which
 // two waves a SIMD overlap only in part.  1024 queries of 32:8 heads of 128 columns over 8192 keys, two sequences: 315 us in 8 bits (0.82
-// PFLOP/s; the library's largest product reaches 1.27), 283 us in 16 (0.91); of unlike lengths (8192 and about 5000) 254 us in 8 bits, as
-// the shorter one leaves its places empty.
+// PFLOP/s; the library's largest product reaches 1.27), 279 us in 16 (0.92); of unlike lengths (8192 and about 5000) 255 us in 8 bits on one set
+// of operands, 280 to 286 on two in turn, and 217 in 16, as the shorter one leaves its places empty.
 #include <type_traits>
 
 #include "attention_cached_share.hpp"
